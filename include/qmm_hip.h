@@ -280,6 +280,145 @@ int qmm_lm_head_scan_rmsnorm(qmm_context *ctx, const float *x, const float *gamm
                              const uint32_t *draft_ids, float *best_val, uint32_t *best_id,
                              int32_t *scan_state);
 
+/* ------------------------------------------------------- attention, cache */
+/* What a layer does between its q / k / v projections and its output
+ * projection: append the new tokens to a paged key-value cache, and attend to
+ * it. A call works on a batch of sequences, each with any number of new tokens
+ * (1 while it decodes, a few draft tokens, a prompt or a part of one).
+ *
+ * These operators add to the numeric contract above: norms, rotations, scores
+ * and softmax sums are fp32, angles are reduced in 64 bits, and q_out, the
+ * fp16 cache, the softmax weights before their product with the values, and
+ * the attention's outputs are rounded to fp16 (nearest even).
+ *
+ * Device arrays are bounds-checked where they are used, not trusted: row_start
+ * is clamped to [0, n_rows], kv_len to [0, max_pages * page_tokens], and the
+ * cells of a page id outside [0, n_pages) are neither read nor written and are
+ * visible to no row. Rows that no sequence holds (past row_start[n_seqs]) keep
+ * their outputs as they were. */
+
+/* One layer's cache: n_pages pages of page_tokens tokens (a power of two,
+ * 16..1024), n_heads key-value heads of head_dim (64, 128 or 256) values.
+ *   k: [n_pages][n_heads][page_tokens][head_dim]
+ *   v: [n_pages][n_heads][head_dim][page_tokens]  (a value's tokens side by
+ *      side: both products of the attention then read their operands in order)
+ * QMM_KV_F16: fp16. QMM_KV_Q8: int8 codes, and one fp32 scale for each token's
+ * head in k_scale / v_scale [n_pages][n_heads][page_tokens]: value = code *
+ * scale, scale = max|x| / 127, code = rint(x * (127 / max|x|)); where max|x| is
+ * below 2^-100 both are 0. k and v 16-B aligned, scales 16-B aligned. */
+#define QMM_KV_F16 1
+#define QMM_KV_Q8 2
+typedef struct {
+    uint32_t type; /* QMM_KV_* */
+    int page_tokens;
+    int n_pages;
+    int n_heads;
+    int head_dim;
+    void *k, *v;              /* device */
+    float *k_scale, *v_scale; /* device; QMM_KV_Q8 only */
+} qmm_kv_cache;
+
+/* The sequences of one call. Sequence s holds kv_len[s] tokens, the new ones
+ * included; its new tokens are rows row_start[s] .. row_start[s + 1] of the
+ * row tensors and sit at its last positions: row row_start[s] + i at position
+ * kv_len[s] - (row_start[s + 1] - row_start[s]) + i. Token j is in page
+ * pages[s][j / page_tokens], slot j % page_tokens. */
+typedef struct {
+    int n_seqs;
+    int n_rows;               /* rows of the row tensors */
+    const int32_t *row_start; /* device [n_seqs + 1], ascending */
+    const int32_t *kv_len;    /* device [n_seqs] */
+    const int32_t *pages;     /* device [n_seqs][max_pages]; entries past a sequence's end are not read */
+    int max_pages;
+    /* What the host knows of the device arrays, for choosing a launch: the
+     * most new rows of a sequence and the largest kv_len (0: not known). A
+     * captured graph may be replayed with others: they change no result. */
+    int max_new;
+    int max_kv;
+} qmm_kv_batch;
+
+/* Position rotation of a head's first rot_dim values. Pair j < rot_dim / 2 is
+ * (x[j], x[j + rot_dim / 2]) in QMM_ROPE_HALF style, (x[2j], x[2j + 1]) in
+ * QMM_ROPE_PAIRS style, and turns by pos[axis(j)] * freq(j) radians; the turned
+ * values are multiplied by `scale`. */
+#define QMM_ROPE_HALF 0
+#define QMM_ROPE_PAIRS 1
+typedef struct {
+    int rot_dim;              /* a multiple of 8, 8..256 */
+    int style;                /* QMM_ROPE_* */
+    double base;              /* freq(j) = base^(-2j / rot_dim); > 0 */
+    const double *pair_freq;  /* host [rot_dim / 2]: these frequencies instead, or NULL */
+    int n_axes;               /* 1..3 position axes (time, height, width) */
+    const uint8_t *pair_axis; /* host [rot_dim / 2]: the axis of each pair, or NULL (all 0) */
+    float scale;              /* 0 means 1 */
+} qmm_rope_params;
+typedef struct qmm_rope qmm_rope;
+/* The device table of one rotation; kept by the program, used by any stream
+ * and graph of the context's device. Not during a capture. */
+int qmm_rope_create(qmm_context *ctx, const qmm_rope_params *params, qmm_rope **out);
+/* Calls on the context's stream are waited for; memory that a living graph may
+ * hold is kept until the last graph is destroyed. Calls that run on another
+ * stream must have ended. */
+int qmm_rope_destroy(qmm_context *ctx, qmm_rope *rope);
+
+/* The rows of one append: fp32 projections, each with its own row stride (in
+ * values), so that parts of one fused projection can be given in place. */
+typedef struct {
+    const float *q; /* device [n_rows][q_stride]: q_heads heads; NULL: keys and values only */
+    size_t q_stride;
+    int q_heads;
+    const float *k; /* device [n_rows][k_stride]: n_heads heads */
+    size_t k_stride;
+    const float *v; /* device [n_rows][v_stride] */
+    size_t v_stride;
+    const float *q_gamma, *k_gamma; /* device [head_dim]: RMSNorm of every head before the rotation; NULL: none */
+    float eps;                      /* y = x / sqrt(mean(x^2) + eps) * gamma */
+    const qmm_rope *rope;           /* NULL: no rotation */
+    const int32_t *pos;             /* device [n_axes][pos_stride]: positions of the rows; NULL: a row's place in its sequence */
+    size_t pos_stride;              /* >= n_rows */
+    uint16_t *q_out;                /* device fp16 [n_rows][q_out_stride]; with q */
+    size_t q_out_stride;
+} qmm_kv_rows;
+/* Norms and rotates the queries into q_out and the keys into the cache, and
+ * puts the values there. A row whose place is negative or in no valid page
+ * gives its q_out alone. Row pointers and strides are multiples of 16 B
+ * (q_out: of 8 B). |x| < 65520 for an fp16 cache. Two rows written to one
+ * cell (a page held by two sequences): one of them is kept. */
+int qmm_kv_append(qmm_context *ctx, const qmm_kv_batch *batch, const qmm_kv_cache *cache, const qmm_kv_rows *rows);
+
+/* The attention of new rows over their sequences' cache, the new tokens
+ * included (append first). Query head h reads key-value head
+ * h / (q_heads / n_heads). The row at position p sees token j where
+ *   j <= p  and  (window == 0  or  j > p - window  or  j < sinks):
+ * a sliding window whose first `sinks` tokens stay visible. out = sum over the
+ * visible j of softmax(scale * q.k_j) v_j; zeros where nothing is visible. What
+ * lies in a masked cell (any bits) never reaches a row. */
+typedef struct {
+    const uint16_t *q; /* device fp16 [n_rows][q_stride], 16-B aligned rows */
+    size_t q_stride;
+    int q_heads;      /* a multiple of n_heads */
+    float scale;      /* > 0, finite */
+    int window;       /* 0: none */
+    int sinks;        /* with a window */
+    void *out;        /* device [n_rows][out_stride], 8-B aligned rows (F32: 16-B) */
+    uint32_t out_type; /* QMM_TYPE_F16, or QMM_TYPE_F32: the same values as fp32 (the input of the next projection) */
+    size_t out_stride;
+} qmm_attention_args;
+
+/* Device scratch for partial results where a row's tokens are split over
+ * workgroups. Calls that may overlap (two streams, two graphs replayed on two
+ * streams) need one each; calls in stream order can share one. It holds nothing
+ * between calls. A smaller one than qmm_attention_workspace_bytes means fewer
+ * splits, never another result than by the order of the sums. */
+typedef struct qmm_attn_workspace qmm_attn_workspace;
+size_t qmm_attention_workspace_bytes(qmm_context *ctx, const qmm_kv_batch *batch, const qmm_kv_cache *cache,
+                                     const qmm_attention_args *args);
+int qmm_attention_workspace_create(qmm_context *ctx, size_t bytes, qmm_attn_workspace **out);
+int qmm_attention_workspace_destroy(qmm_context *ctx, qmm_attn_workspace *ws); /* (as qmm_rope_destroy) */
+/* ws may be NULL: no split. */
+int qmm_paged_attention(qmm_context *ctx, const qmm_kv_batch *batch, const qmm_kv_cache *cache,
+                        const qmm_attention_args *args, qmm_attn_workspace *ws);
+
 /* -------------------------------------------------------------- dequant */
 /* dequant_contiguous_fast (E:3856-3902): rows x cols packed blocks -> fp16
  * bits [rows][cols] (for validation; not on the matmul path). F16 rows are

@@ -12,13 +12,17 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <mutex>
+#include <new>
 #include <cstdio>
 #include <cstring>
 #include <string>
 #include <vector>
 
 #include "../../include/qmm_hip.h"
+#include "qmm_attn.h"
+#include "qmm_attn_check.h"
 #include "qmm_device.h"
 
 // Device scratch of qmm_gemm_multi_dispatch_noalloc: the quantized input
@@ -55,7 +59,20 @@ struct qmm_context {
     int live_graphs = 0;
     std::vector<void *> retired;
     hipEvent_t ev0 = nullptr, ev1 = nullptr;
+    int cu_count = 0;  // looked up by the first attention call
     std::string err;
+};
+
+// Device tables and scratch that a program keeps (their device is the context's).
+struct qmm_rope {
+    int device = 0, rot_dim = 0, style = 0, n_axes = 0;
+    float scale = 1.0f;
+    qmm::RopePair *pairs = nullptr;
+};
+struct qmm_attn_workspace {
+    int device = 0;
+    void *base = nullptr;
+    size_t bytes = 0;
 };
 
 namespace {
@@ -812,6 +829,211 @@ int qmm_ffn_block_rmsnorm(qmm_context *ctx, const float *x, const float *gamma, 
     if (K > 16384) return fail(ctx, QMM_ESHAPE, "K above 16384");
     if (!aligned(gamma, 16)) return fail(ctx, QMM_EALIGN, "gamma must be 16-B aligned");
     return ffn_block(ctx, x, gamma, nullptr, K, gate, up, down, h_out);
+}
+
+// ------------------------------------------------------ attention and cache
+namespace {
+
+int refuse(qmm_context *ctx, const qmm::Refusal &r) { return fail(ctx, r.code, r.why); }
+
+// The kernels' views of a checked batch and cache, and the host's hints: the
+// most new rows and tokens of a sequence, where not given what the tensors hold.
+void kv_views(const qmm_kv_batch &b, const qmm_kv_cache &c, qmm::KvView &v, int &max_new, int &max_kv) {
+    int shift = 4;
+    while ((1 << shift) < c.page_tokens) ++shift;
+    v = qmm::KvView{b.row_start, b.kv_len, b.pages, b.n_seqs, b.n_rows, b.max_pages, c.n_pages, shift, c.n_heads};
+    const int cap = qmm::kv_capacity(b.max_pages, shift);
+    max_new = b.max_new > 0 ? std::min(b.max_new, b.n_rows) : b.n_rows;
+    max_kv = b.max_kv > 0 ? std::min(b.max_kv, cap) : cap;
+}
+
+int attn_args(qmm_context *ctx, const qmm_kv_batch *b, const qmm_kv_cache *c, const qmm_attention_args *t, qmm::AttnArgs &a) {
+    const qmm::Refusal no = qmm::check_attention(b, c, t);
+    if (no.code) return refuse(ctx, no);
+    kv_views(*b, *c, a.b, a.max_new, a.max_kv);
+    a.q = t->q;
+    a.q_stride = t->q_stride;
+    a.out = t->out;
+    a.out_stride = t->out_stride;
+    a.out_f32 = t->out_type == QMM_TYPE_F32;
+    a.head_dim = c->head_dim;
+    a.group = t->q_heads / c->n_heads;
+    a.scale = t->scale;
+    a.window = t->window;
+    a.sinks = t->window > 0 ? t->sinks : 0;
+    a.kc = c->k;
+    a.vc = c->v;
+    a.ks = c->type == QMM_KV_Q8 ? c->k_scale : nullptr;
+    a.vs = c->type == QMM_KV_Q8 ? c->v_scale : nullptr;
+    return QMM_OK;
+}
+
+// Device memory of a table or workspace the program gives up: kept with the
+// context's retired buffers while a capture is open or graphs are alive.
+int give_up(qmm_context *ctx, void *p) {
+    if (!p) return QMM_OK;
+    if (ctx->capturing || ctx->live_graphs > 0) {
+        ctx->retired.push_back(p);
+        return QMM_OK;
+    }
+    (void)hipStreamSynchronize(ctx->stream);
+    const hipError_t e = hipFree(p);
+    return e == hipSuccess ? QMM_OK : hip_fail(ctx, e, "hipFree");
+}
+
+int cu_count(qmm_context *ctx, int &n) {
+    if (ctx->cu_count <= 0) {
+        int cu = 0;
+        const hipError_t e = hipDeviceGetAttribute(&cu, hipDeviceAttributeMultiprocessorCount, ctx->device);
+        if (e != hipSuccess) return hip_fail(ctx, e, "hipDeviceGetAttribute");
+        ctx->cu_count = cu;
+    }
+    n = ctx->cu_count;
+    return QMM_OK;
+}
+
+}  // namespace
+
+int qmm_rope_create(qmm_context *ctx, const qmm_rope_params *t, qmm_rope **out) {
+    if (!ctx || !out) return QMM_EINVAL;
+    *out = nullptr;
+    const qmm::Refusal no = qmm::check_rope(t);
+    if (no.code) return refuse(ctx, no);
+    const int n = t->rot_dim / 2;
+    qmm::RopePair host[128];
+    for (int j = 0; j < n; ++j) {
+        const double f = t->pair_freq ? t->pair_freq[j] : std::pow(t->base, -2.0 * j / t->rot_dim);
+        host[j].turns = f / 6.283185307179586476925286766559;
+        host[j].axis = t->pair_axis ? t->pair_axis[j] : 0;
+        host[j].pad = 0;
+    }
+    if (ctx->capturing) return fail(ctx, QMM_EINVAL, "no rotation table can be made during graph capture");
+    int rc = use_device(ctx);
+    if (rc) return rc;
+    qmm_rope *r = new (std::nothrow) qmm_rope();
+    if (!r) return fail(ctx, QMM_ENOMEM, "out of host memory");
+    if (hipMalloc(&r->pairs, size_t(n) * sizeof(qmm::RopePair)) != hipSuccess) {
+        (void)hipGetLastError();
+        delete r;
+        return fail(ctx, QMM_ENOMEM, "hipMalloc of a rotation table failed");
+    }
+    hipError_t e = hipMemcpyAsync(r->pairs, host, size_t(n) * sizeof(qmm::RopePair), hipMemcpyHostToDevice, ctx->stream);
+    if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);
+    if (e != hipSuccess) {
+        (void)hipFree(r->pairs);
+        delete r;
+        return hip_fail(ctx, e, "rotation table upload");
+    }
+    r->device = ctx->device;
+    r->rot_dim = t->rot_dim;
+    r->style = t->style;
+    r->n_axes = t->n_axes;
+    r->scale = t->scale == 0.0f ? 1.0f : t->scale;
+    *out = r;
+    return QMM_OK;
+}
+
+int qmm_rope_destroy(qmm_context *ctx, qmm_rope *rope) {
+    if (!ctx || !rope) return fail(ctx, QMM_EINVAL, "bad rope_destroy arguments");
+    if (rope->device != ctx->device) return fail(ctx, QMM_EINVAL, "rotation table of another device");
+    int rc = use_device(ctx);
+    if (rc) return rc;
+    void *p = rope->pairs;
+    delete rope;
+    return give_up(ctx, p);
+}
+
+int qmm_kv_append(qmm_context *ctx, const qmm_kv_batch *batch, const qmm_kv_cache *cache, const qmm_kv_rows *t) {
+    if (!ctx) return QMM_EINVAL;
+    const qmm::Refusal no = qmm::check_append(batch, cache, t, t && t->rope ? t->rope->rot_dim : 0);
+    if (no.code) return refuse(ctx, no);
+    if (t->rope && t->rope->device != ctx->device) return fail(ctx, QMM_EINVAL, "rotation table of another device");
+    if (batch->n_rows == 0 || batch->n_seqs == 0) return QMM_OK;
+    qmm::AppendArgs a{};
+    int max_kv = 0;
+    kv_views(*batch, *cache, a.b, a.max_new, max_kv);
+    a.q = t->q;
+    a.k = t->k;
+    a.v = t->v;
+    a.q_stride = t->q_stride;
+    a.k_stride = t->k_stride;
+    a.v_stride = t->v_stride;
+    a.q_heads = t->q_heads;
+    a.head_dim = cache->head_dim;
+    a.q_gamma = t->q_gamma;
+    a.k_gamma = t->k_gamma;
+    a.eps = t->eps;
+    if (t->rope) {
+        a.pairs = t->rope->pairs;
+        a.rot_dim = t->rope->rot_dim;
+        a.style = t->rope->style;
+        a.rope_scale = t->rope->scale;
+        a.pos = t->pos;
+        a.pos_stride = t->pos_stride;
+    }
+    a.q_out = t->q_out;
+    a.q_out_stride = t->q_out_stride;
+    a.kc = cache->k;
+    a.vc = cache->v;
+    a.ks = cache->type == QMM_KV_Q8 ? cache->k_scale : nullptr;
+    a.vs = cache->type == QMM_KV_Q8 ? cache->v_scale : nullptr;
+    const int rc = use_device(ctx);
+    if (rc) return rc;
+    const hipError_t e = qmm::launch_kv_append(a, ctx->stream);
+    if (e == hipErrorInvalidValue) return fail(ctx, QMM_ESHAPE, "batch too large for one launch");
+    return e == hipSuccess ? QMM_OK : hip_fail(ctx, e, "cache append launch");
+}
+
+size_t qmm_attention_workspace_bytes(qmm_context *ctx, const qmm_kv_batch *batch, const qmm_kv_cache *cache,
+                                     const qmm_attention_args *args) {
+    qmm::AttnArgs a{};
+    int cus = 0;
+    if (!ctx || attn_args(ctx, batch, cache, args, a) || batch->n_rows == 0 || batch->n_seqs == 0) return 0;
+    if (cu_count(ctx, cus)) return 0;
+    return qmm::attn_scratch_bytes(a, cus);
+}
+
+int qmm_attention_workspace_create(qmm_context *ctx, size_t bytes, qmm_attn_workspace **out) {
+    if (!ctx || !out) return QMM_EINVAL;
+    *out = nullptr;
+    if (ctx->capturing) return fail(ctx, QMM_EINVAL, "no workspace can be made during graph capture");
+    int rc = use_device(ctx);
+    if (rc) return rc;
+    qmm_attn_workspace *w = new (std::nothrow) qmm_attn_workspace();
+    if (!w) return fail(ctx, QMM_ENOMEM, "out of host memory");
+    w->device = ctx->device;
+    if (bytes && hipMalloc(&w->base, bytes) != hipSuccess) {
+        (void)hipGetLastError();
+        delete w;
+        return fail(ctx, QMM_ENOMEM, "hipMalloc of an attention workspace failed");
+    }
+    w->bytes = bytes;
+    *out = w;
+    return QMM_OK;
+}
+
+int qmm_attention_workspace_destroy(qmm_context *ctx, qmm_attn_workspace *ws) {
+    if (!ctx || !ws) return fail(ctx, QMM_EINVAL, "bad workspace_destroy arguments");
+    if (ws->device != ctx->device) return fail(ctx, QMM_EINVAL, "workspace of another device");
+    int rc = use_device(ctx);
+    if (rc) return rc;
+    void *p = ws->base;
+    delete ws;
+    return give_up(ctx, p);
+}
+
+int qmm_paged_attention(qmm_context *ctx, const qmm_kv_batch *batch, const qmm_kv_cache *cache,
+                        const qmm_attention_args *args, qmm_attn_workspace *ws) {
+    if (!ctx) return QMM_EINVAL;
+    qmm::AttnArgs a{};
+    int cus = 0;
+    int rc = attn_args(ctx, batch, cache, args, a);
+    if (rc) return rc;
+    if (ws && ws->device != ctx->device) return fail(ctx, QMM_EINVAL, "workspace of another device");
+    if (batch->n_rows == 0 || batch->n_seqs == 0) return QMM_OK;
+    if ((rc = use_device(ctx)) || (rc = cu_count(ctx, cus))) return rc;
+    const hipError_t e = qmm::launch_attention(a, ws ? ws->base : nullptr, ws ? ws->bytes : 0, cus, ctx->stream);
+    return e == hipSuccess ? QMM_OK : hip_fail(ctx, e, "attention launch");
 }
 
 int qmm_dequantize_f16(qmm_context *ctx, const void *w_blocks, uint32_t type, int64_t rows,

@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import weakref
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
@@ -28,6 +29,8 @@ TYPE_F32, TYPE_F16 = 0, 1
 TYPE_Q8_0, TYPE_Q4_K, TYPE_Q5_K, TYPE_Q6_K = 8, 12, 13, 14
 TYPE_NAMES = {TYPE_F32: "F32", TYPE_F16: "F16", TYPE_Q8_0: "Q8_0", TYPE_Q4_K: "Q4_K", TYPE_Q5_K: "Q5_K",
               TYPE_Q6_K: "Q6_K"}
+KV_F16, KV_Q8 = 1, 2  # types of a key-value cache
+ROPE_STYLES = {"half": 0, "pairs": 1}
 BLOCK_BYTES = {TYPE_F32: 4, TYPE_F16: 2, TYPE_Q8_0: 34, TYPE_Q4_K: 144, TYPE_Q5_K: 176, TYPE_Q6_K: 210}
 BLOCK_VALUES = {TYPE_F32: 1, TYPE_F16: 1, TYPE_Q8_0: 32, TYPE_Q4_K: 256, TYPE_Q5_K: 256, TYPE_Q6_K: 256}
 
@@ -58,6 +61,37 @@ class _Task(C.Structure):
         ("res_stride", C.c_size_t), ("rows", C.c_int), ("cols", C.c_int),
         ("start_row", C.c_int),
     ]
+
+
+class KvCache(C.Structure):
+    """qmm_kv_cache: one layer's paged key-value cache."""
+    _fields_ = [("type", C.c_uint32), ("page_tokens", C.c_int), ("n_pages", C.c_int), ("n_heads", C.c_int),
+                ("head_dim", C.c_int), ("k", _p), ("v", _p), ("k_scale", _p), ("v_scale", _p)]
+
+
+class KvBatch(C.Structure):
+    """qmm_kv_batch: the sequences of one call."""
+    _fields_ = [("n_seqs", C.c_int), ("n_rows", C.c_int), ("row_start", _p), ("kv_len", _p), ("pages", _p),
+                ("max_pages", C.c_int), ("max_new", C.c_int), ("max_kv", C.c_int)]
+
+
+class RopeParams(C.Structure):
+    """qmm_rope_params."""
+    _fields_ = [("rot_dim", C.c_int), ("style", C.c_int), ("base", C.c_double), ("pair_freq", C.POINTER(C.c_double)),
+                ("n_axes", C.c_int), ("pair_axis", C.POINTER(C.c_uint8)), ("scale", C.c_float)]
+
+
+class KvRows(C.Structure):
+    """qmm_kv_rows: the projections of one append."""
+    _fields_ = [("q", _p), ("q_stride", C.c_size_t), ("q_heads", C.c_int), ("k", _p), ("k_stride", C.c_size_t),
+                ("v", _p), ("v_stride", C.c_size_t), ("q_gamma", _p), ("k_gamma", _p), ("eps", C.c_float),
+                ("rope", _p), ("pos", _p), ("pos_stride", C.c_size_t), ("q_out", _p), ("q_out_stride", C.c_size_t)]
+
+
+class AttentionArgs(C.Structure):
+    """qmm_attention_args."""
+    _fields_ = [("q", _p), ("q_stride", C.c_size_t), ("q_heads", C.c_int), ("scale", C.c_float), ("window", C.c_int),
+                ("sinks", C.c_int), ("out", _p), ("out_type", C.c_uint32), ("out_stride", C.c_size_t)]
 
 
 # (name, restype, argtypes) of every entry point in include/qmm_hip.h
@@ -113,6 +147,15 @@ _SIGNATURES = [
      [_p, _p, _p, C.c_int, C.c_int, C.POINTER(_Task), C.c_int]),
     ("qmm_gemm_multi_dispatch_noalloc", C.c_int, [_p, _p, C.c_int, C.c_int, C.POINTER(_Task), C.c_int]),
     ("qmm_gemm_multi_dispatch_rmsnorm", C.c_int, [_p, _p, _p, C.c_int, C.c_int, C.POINTER(_Task), C.c_int]),
+    ("qmm_rope_create", C.c_int, [_p, C.POINTER(RopeParams), C.POINTER(_p)]),
+    ("qmm_rope_destroy", C.c_int, [_p, _p]),
+    ("qmm_kv_append", C.c_int, [_p, C.POINTER(KvBatch), C.POINTER(KvCache), C.POINTER(KvRows)]),
+    ("qmm_attention_workspace_bytes", C.c_size_t,
+     [_p, C.POINTER(KvBatch), C.POINTER(KvCache), C.POINTER(AttentionArgs)]),
+    ("qmm_attention_workspace_create", C.c_int, [_p, C.c_size_t, C.POINTER(_p)]),
+    ("qmm_attention_workspace_destroy", C.c_int, [_p, _p]),
+    ("qmm_paged_attention", C.c_int,
+     [_p, C.POINTER(KvBatch), C.POINTER(KvCache), C.POINTER(AttentionArgs), _p]),
     ("qmm_noalloc_scratch_bytes", C.c_size_t, []),
     ("qmm_graph_begin", C.c_int, [_p]),
     ("qmm_graph_end", C.c_int, [_p, C.POINTER(_p)]),
@@ -202,6 +245,25 @@ class DevBuf:
         if self.ptr and self.ctx._h:
             self.ctx._call("qmm_free", self.ctx._h, _p(self.ptr))
         self.ptr = 0
+
+
+class _Handle:
+    """An object the library made for a context: freed with it, or by free()."""
+
+    def __init__(self, ctx: "Context", handle: int, destroy: str):
+        self.ctx, self.handle, self._destroy = ctx, _p(handle), destroy
+        ctx._handles.add(self)
+
+    def free(self):
+        if self.handle and self.ctx._h:
+            self.ctx._call(self._destroy, self.ctx._h, self.handle)
+        self.handle = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
 
 
 @dataclass
@@ -303,6 +365,7 @@ class Context:
                                f"{self.lib.qmm_status_string(rc).decode()}")
         self._h = h
         self._bufs: list[DevBuf] = []
+        self._handles = weakref.WeakSet()
 
     # -- plumbing --------------------------------------------------------
     def _call(self, name, *args):
@@ -324,6 +387,8 @@ class Context:
             for b in self._bufs:
                 b.free()
             self._bufs.clear()
+            for b in list(self._handles):
+                b.free()
             self.lib.qmm_destroy(self._h)
             self._h = None
 
@@ -392,6 +457,33 @@ class Context:
         return b
 
     # -- compute -------------------------------------------------------------
+    def rope(self, rot_dim: int, style: str = "half", base: float = 10000.0, pair_freq=None, n_axes: int = 1,
+             pair_axis=None, scale: float = 1.0) -> _Handle:
+        """qmm_rope_create: the table of one position rotation."""
+        n = rot_dim // 2
+        for x in (pair_freq, pair_axis):
+            if x is not None and len(x) != n:
+                raise ValueError("one frequency and axis for each of the rot_dim / 2 pairs")
+        params = RopeParams(rot_dim, ROPE_STYLES[style], base, (C.c_double * n)(*pair_freq) if pair_freq is not None else None,
+                            n_axes, (C.c_uint8 * n)(*pair_axis) if pair_axis is not None else None, scale)
+        h = _p()
+        self._call("qmm_rope_create", self._h, C.byref(params), C.byref(h))
+        return _Handle(self, h.value, "qmm_rope_destroy")
+
+    def attention_workspace(self, batch: KvBatch, cache: KvCache, args: AttentionArgs) -> _Handle:
+        """A workspace for calls up to this one's size (qmm_attention_workspace_bytes / _create)."""
+        n = self.lib.qmm_attention_workspace_bytes(self._h, C.byref(batch), C.byref(cache), C.byref(args))
+        h = _p()
+        self._call("qmm_attention_workspace_create", self._h, n, C.byref(h))
+        return _Handle(self, h.value, "qmm_attention_workspace_destroy")
+
+    def kv_append(self, batch: KvBatch, cache: KvCache, rows: KvRows):
+        self._call("qmm_kv_append", self._h, C.byref(batch), C.byref(cache), C.byref(rows))
+
+    def paged_attention(self, batch: KvBatch, cache: KvCache, args: AttentionArgs, workspace: Optional[_Handle] = None):
+        self._call("qmm_paged_attention", self._h, C.byref(batch), C.byref(cache), C.byref(args),
+                   workspace.handle if workspace else None)
+
     def quantize_q8k(self, x, M: int, K: int, out):
         self._call("qmm_quantize_q8k", self._h, _p(_addr(x)), M, K, _p(_addr(out)))
 

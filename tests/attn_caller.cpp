@@ -1,0 +1,141 @@
+// The host rules of the cache append and the attention, without a device: which
+// tokens and pages a sequence's rows get, and what the entry points refuse.
+// Prints one line per failure and "ok" at the end.
+#include <cstdio>
+#include <limits>
+#include <vector>
+
+#include "../npu880-mtk-npu-llm-runtime_amd/csrc/qmm_attn.h"
+#include "../npu880-mtk-npu-llm-runtime_amd/csrc/qmm_attn_check.h"
+
+using namespace qmm;
+
+static int bad = 0;
+#define EXPECT(c, ...) do { if (!(c)) { ++bad; std::printf("%s: ", #c); std::printf(__VA_ARGS__); std::printf("\n"); } } while (0)
+
+// every token some row of pmin..pmax sees is in exactly one tile of the span, and each split's tiles together are the span
+static void spans() {
+    for (int pmin = -3; pmin < 300; pmin += 7)
+        for (int rows : {1, 2, 16, 70})
+            for (int window : {0, 1, 16, 63, 64, 65, 130, 400})
+                for (int sinks : {0, 1, 63, 64, 65, 200, 1000}) {
+                    const int pmax = pmin + rows - 1;
+                    const TileSpan t = tile_span(pmin, pmax, window, window ? sinks : 0);
+                    std::vector<int> hit(16, 0);
+                    for (int i = 0; i < t.n; ++i) {
+                        const int k = t.at(i);
+                        if (k < 0 || k >= 16) { EXPECT(false, "tile %d", k); continue; }
+                        ++hit[k];
+                    }
+                    for (int j = 0; j <= pmax; ++j) {
+                        bool seen = false;
+                        for (int p = pmin; p <= pmax; ++p) seen |= j <= p && (!window || j > p - window || j < sinks);
+                        if (seen) EXPECT(hit[j / 64] == 1, "token %d rows %d..%d window %d/%d: %d tiles", j, pmin, pmax, window, sinks, hit[j / 64]);
+                    }
+                    for (int k = 0; k < 16; ++k) EXPECT(hit[k] <= 1, "tile %d twice", k);
+                    for (int nsplit : {1, 2, 3, 7, 100})
+                        for (int chunk : {1, 2, 5, 50}) {
+                            const int per = split_tiles(t.n, nsplit, chunk);
+                            EXPECT(per >= 1 && int64_t(per) * nsplit >= t.n, "per %d of %d", per, t.n);
+                        }
+                }
+}
+
+// what the arrays hold never leads outside the tensors
+static void clamps() {
+    const int big = std::numeric_limits<int>::max(), low = std::numeric_limits<int>::min();
+    const int odd[] = {low, -1, 0, 1, 15, 16, 47, 48, 49, big - 255, big};
+    for (int a : odd)
+        for (int e : odd)
+            for (int len : odd)
+                for (int n_rows : {1, 20, big}) {
+                    const int32_t start[2] = {a, e}, kv[1] = {len}, pages[3] = {7, -1, 9};
+                    const KvView b{start, kv, pages, 1, n_rows, 3, 9, 4, 1};
+                    const SeqView v = seq_view(b, 0);
+                    EXPECT(v.r0 >= 0 && v.n_new >= 0 && int64_t(v.r0) + v.n_new <= n_rows, "%d %d", a, e);
+                    EXPECT(v.len >= 0 && v.len <= 48 && v.pos0 == v.len - v.n_new, "%d", len);
+                    for (int t : odd) {
+                        const int id = page_of(b, 0, t, v.len);
+                        EXPECT(id == -1 || (id == 7 && t >= 0 && t < 16 && t < v.len), "token %d: %d", t, id);
+                    }
+                }
+    EXPECT(kv_capacity(big, 10) == 0x7fffff00 && kv_capacity(3, 4) == 48 && kv_capacity(1, 10) == 1024, "capacity");
+}
+
+static void refusals() {
+    alignas(256) static unsigned char mem[4096];
+    const double freq[4] = {1, 1, 1, std::numeric_limits<double>::infinity()};
+    const uint8_t axis[4] = {0, 1, 2, 3};
+    struct All {
+        qmm_kv_batch b;
+        qmm_kv_cache c;
+        qmm_attention_args t;
+        qmm_kv_rows r;
+        qmm_rope_params p;
+        int rot = 0;
+    } good{};
+
+    int32_t *i32 = reinterpret_cast<int32_t *>(mem);
+    uint16_t *u16 = reinterpret_cast<uint16_t *>(mem);
+    float *f32 = reinterpret_cast<float *>(mem);
+    good.b = qmm_kv_batch{2, 5, i32, i32, i32, 4, 0, 0};
+    good.c = qmm_kv_cache{QMM_KV_Q8, 16, 10, 2, 64, mem, mem, f32, f32};
+    good.t = qmm_attention_args{u16, 256, 4, 0.125f, 0, 0, mem, QMM_TYPE_F16, 256};
+    good.r = qmm_kv_rows{f32, 256, 4, f32, 128, f32, 128, f32, f32, 1e-6f, nullptr, i32, 5, u16, 256};
+    good.p = qmm_rope_params{8, QMM_ROPE_HALF, 1e4, nullptr, 3, nullptr, 0.0f};
+    good.rot = 64;
+    const float nan = std::numeric_limits<float>::quiet_NaN(), inf = std::numeric_limits<float>::infinity();
+    auto all = [&](const All &x, int attn, int app, int rope, const char *what) {
+        EXPECT(check_attention(&x.b, &x.c, &x.t).code == attn, "%s: attention %d", what, check_attention(&x.b, &x.c, &x.t).code);
+        EXPECT(check_append(&x.b, &x.c, &x.r, x.rot).code == app, "%s: append %d", what, check_append(&x.b, &x.c, &x.r, x.rot).code);
+        EXPECT(check_rope(&x.p).code == rope, "%s: rope %d", what, check_rope(&x.p).code);
+    };
+    all(good, 0, 0, 0, "good");
+#define BOTH(change, code) { All x = good; x.change; all(x, code, code, 0, #change); }
+#define ATTN(change, code) { All x = good; x.change; all(x, code, 0, 0, #change); }
+#define APP(change, code) { All x = good; x.change; all(x, 0, code, 0, #change); }
+#define ROPE(change, code) { All x = good; x.change; all(x, 0, 0, code, #change); }
+    BOTH(b.n_seqs = -1, QMM_EINVAL) BOTH(b.n_rows = -1, QMM_EINVAL) BOTH(b.max_pages = 0, QMM_EINVAL)
+    BOTH(b.max_new = -1, QMM_EINVAL) BOTH(b.max_kv = -1, QMM_EINVAL) BOTH(b.row_start = nullptr, QMM_EINVAL)
+    BOTH(b.kv_len = nullptr, QMM_EINVAL) BOTH(b.pages = nullptr, QMM_EINVAL)
+    BOTH(b.pages = reinterpret_cast<int32_t *>(mem + 2), QMM_EALIGN)
+    BOTH(b.n_seqs = 1 << 23, QMM_ESHAPE)
+    BOTH(c.type = 0, QMM_ETYPE) BOTH(c.type = 8, QMM_ETYPE) BOTH(c.page_tokens = 8, QMM_ESHAPE)
+    BOTH(c.page_tokens = 24, QMM_ESHAPE) BOTH(c.page_tokens = 2048, QMM_ESHAPE) BOTH(c.page_tokens = -16, QMM_ESHAPE)
+    BOTH(c.n_pages = 0, QMM_EINVAL) BOTH(c.head_dim = 96, QMM_ESHAPE) BOTH(c.head_dim = 0, QMM_ESHAPE)
+    BOTH(c.n_heads = 0, QMM_EINVAL) BOTH(c.k = nullptr, QMM_EINVAL) BOTH(c.v = nullptr, QMM_EINVAL)
+    BOTH(c.k = mem + 8, QMM_EALIGN) BOTH(c.v = mem + 2, QMM_EALIGN)
+    BOTH(c.k_scale = nullptr, QMM_EINVAL) BOTH(c.v_scale = reinterpret_cast<float *>(mem + 4), QMM_EALIGN)
+    ATTN(t.q_heads = 3, QMM_ESHAPE) ATTN(t.q_heads = 0, QMM_ESHAPE) ATTN(t.scale = 0.0f, QMM_EINVAL)
+    ATTN(t.scale = -1.0f, QMM_EINVAL) ATTN(t.scale = nan, QMM_EINVAL) ATTN(t.scale = inf, QMM_EINVAL)
+    ATTN(t.window = -1, QMM_EINVAL) ATTN(t.sinks = -1, QMM_EINVAL) ATTN(t.q = nullptr, QMM_EINVAL)
+    ATTN(t.out = nullptr, QMM_EINVAL) ATTN(t.q_stride = 255, QMM_EINVAL) ATTN(t.out_stride = 252, QMM_EINVAL)
+    ATTN(t.q_stride = 260, QMM_EALIGN) ATTN(t.out_stride = 258, QMM_EALIGN) ATTN(t.out_type = 8, QMM_ETYPE)
+    ATTN(t.q = u16 + 4, QMM_EALIGN) ATTN(t.out = mem + 4, QMM_EALIGN)
+    { All x = good; x.t.out_type = QMM_TYPE_F32; x.t.out = mem + 8; all(x, QMM_EALIGN, 0, 0, "fp32 out at 8 B"); }
+    APP(r.k = nullptr, QMM_EINVAL) APP(r.v = nullptr, QMM_EINVAL) APP(r.q_out = nullptr, QMM_EINVAL)
+    APP(r.q_heads = 0, QMM_EINVAL) APP(r.k_stride = 124, QMM_EINVAL) APP(r.v_stride = 0, QMM_EINVAL)
+    APP(r.q_stride = 252, QMM_EINVAL) APP(r.q_out_stride = 100, QMM_EINVAL) APP(r.q_stride = 257, QMM_EALIGN)
+    APP(r.k_stride = 130, QMM_EALIGN) APP(r.q_out_stride = 258, QMM_EALIGN) APP(r.k = f32 + 1, QMM_EALIGN)
+    APP(r.v = f32 + 2, QMM_EALIGN) APP(r.q = f32 + 3, QMM_EALIGN) APP(r.q_out = u16 + 2, QMM_EALIGN)
+    APP(r.q_gamma = f32 + 1, QMM_EALIGN) APP(r.k_gamma = f32 + 1, QMM_EALIGN) APP(r.eps = -1.0f, QMM_EINVAL)
+    APP(r.eps = nan, QMM_EINVAL) APP(r.eps = inf, QMM_EINVAL) APP(r.pos_stride = 4, QMM_EINVAL)
+    APP(r.pos = reinterpret_cast<int32_t *>(mem + 1), QMM_EALIGN) APP(rot = 72, QMM_ESHAPE)
+    ROPE(p.rot_dim = 4, QMM_ESHAPE) ROPE(p.rot_dim = 12, QMM_ESHAPE) ROPE(p.rot_dim = 264, QMM_ESHAPE) ROPE(p.style = 2, QMM_EINVAL)
+    ROPE(p.n_axes = 0, QMM_EINVAL) ROPE(p.n_axes = 4, QMM_EINVAL) ROPE(p.base = 0.0, QMM_EINVAL)
+    ROPE(p.base = std::numeric_limits<double>::infinity(), QMM_EINVAL) ROPE(p.scale = nan, QMM_EINVAL)
+    ROPE(p.pair_freq = freq, QMM_EINVAL) ROPE(p.pair_axis = axis, QMM_EINVAL)
+    // nothing to do: the arrays may be absent
+    { All x = good; x.b.n_rows = 0; x.b.row_start = x.b.kv_len = x.b.pages = nullptr; x.t.q = nullptr; x.t.out = nullptr; x.r.k = x.r.v = nullptr; all(x, 0, 0, 0, "no rows"); }
+    EXPECT(check_attention(nullptr, &good.c, &good.t).code == QMM_EINVAL && check_attention(&good.b, nullptr, &good.t).code == QMM_EINVAL &&
+               check_attention(&good.b, &good.c, nullptr).code == QMM_EINVAL && check_append(&good.b, &good.c, nullptr, 0).code == QMM_EINVAL &&
+               check_rope(nullptr).code == QMM_EINVAL, "nulls");
+}
+
+int main() {
+    spans();
+    clamps();
+    refusals();
+    std::printf(bad ? "%d failures\n" : "ok\n", bad);
+    return bad != 0;
+}
