@@ -858,6 +858,7 @@ int attn_args(qmm_context *ctx, const qmm_kv_batch *b, const qmm_kv_cache *c, co
     a.out_f32 = t->out_type == QMM_TYPE_F32;
     a.head_dim = c->head_dim;
     a.group = t->q_heads / c->n_heads;
+    a.group_inv = unsigned((0xffffffffull + a.group) / unsigned(a.group));
     a.scale = t->scale;
     a.window = t->window;
     a.sinks = t->window > 0 ? t->sinks : 0;

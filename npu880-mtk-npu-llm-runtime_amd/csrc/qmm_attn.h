@@ -116,7 +116,8 @@ struct AttnArgs {
     void *out;
     size_t out_stride;
     int out_f32;
-    int head_dim, group;  // query heads per key-value head
+    int head_dim, group;  // query heads per key-value head; n_rows * group < 2^30
+    unsigned group_inv;   // ceil(2^32 / group)
     float scale;
     int window, sinks;
     const void *kc, *vc;

@@ -48,6 +48,8 @@ inline Refusal check_attention(const qmm_kv_batch *b, const qmm_kv_cache *c, con
     if (!t) return {QMM_EINVAL, "null attention arguments"};
     if (t->q_heads <= 0 || t->q_heads > (1 << 20) || t->q_heads % c->n_heads)
         return {QMM_ESHAPE, "q_heads must be a multiple of the cache's heads"};
+    if (int64_t(b->n_rows) * (t->q_heads / c->n_heads) >= (int64_t(1) << 30))
+        return {QMM_ESHAPE, "n_rows * q_heads / n_heads must stay below 2^30"};
     if (!(t->scale > 0.0f) || !std::isfinite(t->scale)) return {QMM_EINVAL, "scale must be positive and finite"};
     if (t->window < 0 || t->sinks < 0) return {QMM_EINVAL, "negative window or sinks"};
     if (t->out_type != QMM_TYPE_F16 && t->out_type != QMM_TYPE_F32) return {QMM_ETYPE, "out_type must be F16 or F32"};

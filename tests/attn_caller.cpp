@@ -106,6 +106,7 @@ static void refusals() {
     BOTH(c.n_heads = 0, QMM_EINVAL) BOTH(c.k = nullptr, QMM_EINVAL) BOTH(c.v = nullptr, QMM_EINVAL)
     BOTH(c.k = mem + 8, QMM_EALIGN) BOTH(c.v = mem + 2, QMM_EALIGN)
     BOTH(c.k_scale = nullptr, QMM_EINVAL) BOTH(c.v_scale = reinterpret_cast<float *>(mem + 4), QMM_EALIGN)
+    { All x = good; x.b.n_rows = 1 << 29; x.r.pos_stride = size_t(1) << 29; all(x, QMM_ESHAPE, 0, 0, "rows"); }
     ATTN(t.q_heads = 3, QMM_ESHAPE) ATTN(t.q_heads = 0, QMM_ESHAPE) ATTN(t.scale = 0.0f, QMM_EINVAL)
     ATTN(t.scale = -1.0f, QMM_EINVAL) ATTN(t.scale = nan, QMM_EINVAL) ATTN(t.scale = inf, QMM_EINVAL)
     ATTN(t.window = -1, QMM_EINVAL) ATTN(t.sinks = -1, QMM_EINVAL) ATTN(t.q = nullptr, QMM_EINVAL)
