@@ -63,11 +63,11 @@ struct qmm_context {
     std::string err;
 };
 
-// Device tables and scratch that a program keeps (their device is the context's).
+// What a program keeps: a rotation (host only, passed to kernels by value), and
+// device scratch.
 struct qmm_rope {
-    int device = 0, rot_dim = 0, style = 0, n_axes = 0;
-    float scale = 1.0f;
-    qmm::RopePair *pairs = nullptr;
+    int n_axes = 0;
+    qmm::RopeTable table{};
 };
 struct qmm_attn_workspace {
     int device = 0;
@@ -900,55 +900,31 @@ int qmm_rope_create(qmm_context *ctx, const qmm_rope_params *t, qmm_rope **out) 
     *out = nullptr;
     const qmm::Refusal no = qmm::check_rope(t);
     if (no.code) return refuse(ctx, no);
-    const int n = t->rot_dim / 2;
-    qmm::RopePair host[128];
-    for (int j = 0; j < n; ++j) {
-        const double f = t->pair_freq ? t->pair_freq[j] : std::pow(t->base, -2.0 * j / t->rot_dim);
-        host[j].turns = f / 6.283185307179586476925286766559;
-        host[j].axis = t->pair_axis ? t->pair_axis[j] : 0;
-        host[j].pad = 0;
-    }
-    if (ctx->capturing) return fail(ctx, QMM_EINVAL, "no rotation table can be made during graph capture");
-    int rc = use_device(ctx);
-    if (rc) return rc;
     qmm_rope *r = new (std::nothrow) qmm_rope();
     if (!r) return fail(ctx, QMM_ENOMEM, "out of host memory");
-    if (hipMalloc(&r->pairs, size_t(n) * sizeof(qmm::RopePair)) != hipSuccess) {
-        (void)hipGetLastError();
-        delete r;
-        return fail(ctx, QMM_ENOMEM, "hipMalloc of a rotation table failed");
-    }
-    hipError_t e = hipMemcpyAsync(r->pairs, host, size_t(n) * sizeof(qmm::RopePair), hipMemcpyHostToDevice, ctx->stream);
-    if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);
-    if (e != hipSuccess) {
-        (void)hipFree(r->pairs);
-        delete r;
-        return hip_fail(ctx, e, "rotation table upload");
-    }
-    r->device = ctx->device;
-    r->rot_dim = t->rot_dim;
-    r->style = t->style;
     r->n_axes = t->n_axes;
-    r->scale = t->scale == 0.0f ? 1.0f : t->scale;
+    r->table.rot_dim = t->rot_dim;
+    r->table.style = t->style;
+    r->table.scale = t->scale == 0.0f ? 1.0f : t->scale;
+    for (int j = 0; j < t->rot_dim / 2; ++j) {
+        const double f = t->pair_freq ? t->pair_freq[j] : std::pow(t->base, -2.0 * j / t->rot_dim);
+        r->table.turns[j] = f / 6.283185307179586476925286766559;
+        r->table.axis[j] = t->pair_axis ? t->pair_axis[j] : 0;
+    }
     *out = r;
     return QMM_OK;
 }
 
 int qmm_rope_destroy(qmm_context *ctx, qmm_rope *rope) {
     if (!ctx || !rope) return fail(ctx, QMM_EINVAL, "bad rope_destroy arguments");
-    if (rope->device != ctx->device) return fail(ctx, QMM_EINVAL, "rotation table of another device");
-    int rc = use_device(ctx);
-    if (rc) return rc;
-    void *p = rope->pairs;
     delete rope;
-    return give_up(ctx, p);
+    return QMM_OK;
 }
 
 int qmm_kv_append(qmm_context *ctx, const qmm_kv_batch *batch, const qmm_kv_cache *cache, const qmm_kv_rows *t) {
     if (!ctx) return QMM_EINVAL;
-    const qmm::Refusal no = qmm::check_append(batch, cache, t, t && t->rope ? t->rope->rot_dim : 0);
+    const qmm::Refusal no = qmm::check_append(batch, cache, t, t && t->rope ? t->rope->table.rot_dim : 0);
     if (no.code) return refuse(ctx, no);
-    if (t->rope && t->rope->device != ctx->device) return fail(ctx, QMM_EINVAL, "rotation table of another device");
     if (batch->n_rows == 0 || batch->n_seqs == 0) return QMM_OK;
     qmm::AppendArgs a{};
     int max_kv = 0;
@@ -965,10 +941,7 @@ int qmm_kv_append(qmm_context *ctx, const qmm_kv_batch *batch, const qmm_kv_cach
     a.k_gamma = t->k_gamma;
     a.eps = t->eps;
     if (t->rope) {
-        a.pairs = t->rope->pairs;
-        a.rot_dim = t->rope->rot_dim;
-        a.style = t->rope->style;
-        a.rope_scale = t->rope->scale;
+        a.rope = t->rope->table;
         a.pos = t->pos;
         a.pos_stride = t->pos_stride;
     }

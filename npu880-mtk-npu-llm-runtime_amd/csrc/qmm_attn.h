@@ -83,10 +83,13 @@ QMM_HD inline int page_of(const KvView &b, int s, int token, int len) {
 #ifdef __HIPCC__
 namespace qmm {
 
-// one pair's turns (not radians) per position, and its position axis
-struct RopePair {
-    double turns;
-    int axis, pad;
+// A rotation, passed by value: each pair's turns (not radians) per position, and
+// its position axis.
+struct RopeTable {
+    int rot_dim, style;  // rot_dim 0: none
+    float scale;
+    double turns[128];
+    uint8_t axis[128];
 };
 
 struct AppendArgs {
@@ -96,9 +99,7 @@ struct AppendArgs {
     int q_heads, head_dim;
     const float *q_gamma, *k_gamma;
     float eps;
-    const RopePair *pairs;  // nullptr: no rotation
-    int rot_dim, style;
-    float rope_scale;
+    RopeTable rope;
     const int32_t *pos;
     size_t pos_stride;
     uint16_t *q_out;

@@ -706,13 +706,31 @@ __device__ inline float halves_sum(float v) {
 // an LDS row are exchanged by an XOR with the row, so that 16 rows' equal pieces
 // lie in 64 different banks.
 template <int D> struct TileShared {
-    __attribute__((aligned(16))) uint8_t kbuf[2][128 * D];  // 64 keys
+    __attribute__((aligned(16))) uint8_t kbuf[2][128 * D];  // 64 keys, as fp16
     __attribute__((aligned(16))) uint8_t vbuf[2][128 * D];
-    float scales[2][2][64];                                 // 8-bit cache: of keys, of values
+    float ksc[4][64], vsc[2][64];                           // 8-bit cache: their scales
     int wild;                                               // a tile had values that are no numbers, hidden from some row
 };
 
-// One row tile over tiles begin .. end - 1 of its span
+// the largest of three (a NaN counts for nothing)
+__device__ inline float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+// lane l's 16 B at src land at LDS byte address lds + 16 l (counted by vmcnt)
+__device__ inline void dma16g(const void *src, uint32_t lds) {
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "s"(lds) : "memory", "m0");
+#pragma clang diagnostic pop
+}
+
+// One row tile over tiles begin .. end - 1 of its span. A step takes tile i's
+// weights and second product beside tile i + 1's scores, so the matrix cores work
+// while the weights' exponentials are computed; the keys of tile i + 2 and the
+// values of tile i + 1 are on their way to LDS meanwhile (fp16 straight from
+// memory, the XOR of an LDS row's pieces in the lanes' addresses).
 template <int D, bool Q8>
 __device__ inline __attribute__((always_inline)) void tile_piece(const SplitArgs &p, TileShared<D> &sh, const SeqView &v,
                                                                  const RowTile &tile, int s, int h, int split, int begin, int end,
@@ -734,213 +752,286 @@ __device__ inline __attribute__((always_inline)) void tile_piece(const SplitArgs
     const int wr = 32 * wid, wrows = min(nrows - wr, 32);  // this wave's rows of the tile (none: <= 0)
     const int row = row0 + (wrows > 0 ? wr + (col < wrows ? col : 0) : 0);
     const int qi = token_of(a, row), qg = row - qi * G, pos = v.pos0 + qi;
-    const int pmin = v.pos0 + token_of(a, row0 + wr), pmax = v.pos0 + token_of(a, row0 + wr + max(wrows, 1) - 1);
+    const int pmin = v.pos0 + token_of(a, row0 + min(wr, nrows - 1)), pmax = v.pos0 + token_of(a, row0 + min(wr + 31, nrows - 1));
+    const int low = a.window > 0 ? max(pos - a.window, -1) : -1;  // the last token the row's window hides
     h8 q[KS];
     {
         const uint16_t *src = a.q + size_t(v.r0 + qi) * a.q_stride + size_t(h * G + qg) * D + 8 * hh;
 #pragma unroll
         for (int k = 0; k < KS; ++k) q[k] = *reinterpret_cast<const h8 *>(src + 16 * k);
     }
-    float m, l, vref;
+    float m = -__builtin_inff(), l = 0.0f, vref = 1e-30f;
     f16v acc[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[d][r] = 0.0f;
 
-    // staging: wave w loads the tile's keys 16w .. 16w + 15 (one page) and D / 4 of its values' rows
-    u4 kr[NL], vr[NL];
-    float sreg = 0.0f;
-    const int vgroup = Q8 ? lane & 3 : (lane & 7) >> 1;  // the 16 tokens this lane loads values of
-    int idk = -1, idv = -1;
-    auto look_up = [&](int i, int &ik, int &iv) {
-        const int t = span.at(i) * kTileKeys;
-        ik = page_of(a.b, s, t + 16 * wid, v.len);
-        iv = page_of(a.b, s, t + 16 * vgroup, v.len);
+    // Staging: wave w brings the tile's keys 16w .. 16w + 15 (of one page) and D / 4 of
+    // its values' rows. Lane l looks up the page of the tile's tokens 16 (l % 4) ..
+    auto look_up = [&](int i) { return i < end ? page_of(a.b, s, span.at(i) * kTileKeys + 16 * (lane & 3), v.len) : -1; };
+    auto k_cell = [&](int i, int g) {  // this wave's first key
+        const int id = max(__builtin_amdgcn_readlane(g, wid), 0);
+        return ((size_t(id) * H + h) << shift) + size_t((span.at(i) * kTileKeys + 16 * wid) & (P - 1));
     };
-    auto load = [&](int i, int ik, int iv) {
-        const int t = span.at(i) * kTileKeys;
-        const size_t kcell = ((size_t(max(ik, 0)) * H + h) << shift) + size_t((t + 16 * wid) & (P - 1));
-        const uint8_t *ksrc = static_cast<const uint8_t *>(a.kc) + kcell * (Q8 ? D : 2 * D) + 16 * lane;
-#pragma unroll
-        for (int j = 0; j < NL; ++j) kr[j] = *reinterpret_cast<const u4 *>(ksrc + 1024 * j);
-        const size_t hv = size_t(max(iv, 0)) * H + h;
-        const int slot = (t + 16 * vgroup) & (P - 1);
-        const int d0 = wid * (D / 4) + (Q8 ? lane >> 2 : lane >> 3);
-        const uint8_t *vsrc = static_cast<const uint8_t *>(a.vc) + ((hv * D + d0) * size_t(P) + slot) * (Q8 ? 1 : 2) +
-                              (Q8 ? 0 : 16 * (lane & 1));
-#pragma unroll
-        for (int j = 0; j < NL; ++j) vr[j] = *reinterpret_cast<const u4 *>(vsrc + size_t(j) * (Q8 ? 16 : 8 * 2) * P);
+    u4 kr[Q8 ? NL : 1], vr[Q8 ? NL : 1];
+    float sreg = 0.0f;
+    auto bring_k = [&](int i, int g, int b) {
+        const uint8_t *src = static_cast<const uint8_t *>(a.kc) + k_cell(i, g) * (Q8 ? D : 2 * D);
         if constexpr (Q8) {
-            if (lane < 32) sreg = (lane < 16 ? a.ks : a.vs)[kcell + (lane & 15)];
+#pragma unroll
+            for (int j = 0; j < NL; ++j) kr[j] = *reinterpret_cast<const u4 *>(src + 1024 * j + 16 * lane);
+        } else {
+#pragma unroll
+            for (int j = 0; j < NL; ++j) {
+                const int r = (64 * j + lane) / (D / 8), ch = (64 * j + lane) % (D / 8);
+                dma16g(src + k_at(r, ch), lds_addr(&sh.kbuf[b][16 * wid * RK + 1024 * j]));
+            }
         }
     };
-    const int low = a.window > 0 ? max(pos - a.window, -1) : -1;  // the last token the row's window hides
-    // a tile of which some row of the workgroup does not see some cell
+    auto bring_v = [&](int i, int g, int b) {
+        const int t = span.at(i) * kTileKeys;
+        if constexpr (Q8) {
+            const int slot = (t + 16 * (lane & 3)) & (P - 1), d0 = wid * (D / 4) + (lane >> 2);
+            const uint8_t *src = static_cast<const uint8_t *>(a.vc) + ((size_t(max(g, 0)) * H + h) * D + d0) * size_t(P) + slot;
+#pragma unroll
+            for (int j = 0; j < NL; ++j) vr[j] = *reinterpret_cast<const u4 *>(src + size_t(16 * j) * P);
+        } else {
+            // rows d = w D / 4 + 8 j + l / 8; the piece that lands at place l % 8 is that XOR (d / 2) % 8
+            const int ch = (lane & 7) ^ (lane >> 4);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {  // (even and odd j: pieces ch and ch ^ 4)
+                const int c = ch ^ (4 * e), id = max(__shfl(g, c >> 1), 0), slot = (t + 16 * (c >> 1)) & (P - 1);
+                const int d0 = wid * (D / 4) + 8 * e + (lane >> 3);
+                const uint8_t *src = static_cast<const uint8_t *>(a.vc) +
+                                     (((size_t(id) * H + h) * D + d0) * size_t(P) + slot) * 2 + 16 * (c & 1);
+#pragma unroll
+                for (int j = e; j < NL; j += 2)
+                    dma16g(src + size_t(8 * (j - e) * 2) * P, lds_addr(&sh.vbuf[b][wid * (D / 4) * 128 + 1024 * j]));
+            }
+        }
+    };
+    // 8-bit: the scales of tile ik's keys and tile iv's values; then codes to LDS as fp16
+    auto bring_scales = [&](int ik, int gk, int iv, int gv) {
+        if (lane < 16 && ik < end) sreg = a.ks[k_cell(ik, gk) + lane];
+        else if (lane >= 16 && lane < 32 && iv < end) sreg = a.vs[k_cell(iv, gv) + (lane & 15)];
+    };
+    auto put_k = [&](int b, int slot) {
+#pragma unroll
+        for (int j = 0; j < (Q8 ? NL : 0); ++j) {
+            const int u = 64 * j + lane, r = 16 * wid + u / (D / 16), ch = u % (D / 16) * 2;
+            *reinterpret_cast<h8 *>(&sh.kbuf[b][k_at(r, ch)]) = codes8(kr[j][0], kr[j][1]);
+            *reinterpret_cast<h8 *>(&sh.kbuf[b][k_at(r, ch + 1)]) = codes8(kr[j][2], kr[j][3]);
+        }
+        if (lane < 16) sh.ksc[slot & 3][16 * wid + lane] = sreg;
+    };
+    auto put_v = [&](int b) {
+#pragma unroll
+        for (int j = 0; j < (Q8 ? NL : 0); ++j) {
+            const int d = wid * (D / 4) + 16 * j + (lane >> 2), c = 2 * (lane & 3);
+            *reinterpret_cast<h8 *>(&sh.vbuf[b][v_at(d, c)]) = codes8(vr[j][0], vr[j][1]);
+            *reinterpret_cast<h8 *>(&sh.vbuf[b][v_at(d, c + 1)]) = codes8(vr[j][2], vr[j][3]);
+        }
+        if (lane >= 16 && lane < 32) sh.vsc[b][16 * wid + (lane & 15)] = sreg;
+    };
+    // Values that are no numbers in a tile of which some row of the workgroup does not see
+    // all: out of the product (a weight of 0 does not hide a NaN), and back after the loop.
+    // A wave looks through what it brought itself.
     auto partial = [&](int i, unsigned ok) {
         const int t = span.at(i) * kTileKeys;
         return ok != 15 || t + kTileKeys - 1 > tile.pmin ||
                (a.window > 0 && t <= tile.pmax - a.window && t + kTileKeys > a.sinks);
     };
-    auto store = [&](int i, int b, unsigned ok) {
-        if constexpr (!Q8) {
-            if (partial(i, ok)) {
-                us2 top = {0, 0};
+    auto take_wild = [&](int b) {
+        u4 *mine = reinterpret_cast<u4 *>(&sh.vbuf[b][wid * (D / 4) * 128 + 16 * lane]);
+        us2 top = {0, 0};
 #pragma unroll
-                for (int j = 0; j < NL; ++j) top = magnitudes(top, vr[j]);
-                if (__any(no_number(top))) {  // (as in the split kernel: out of the product, and back below)
-                    sh.wild = 1;
-#pragma unroll
-                    for (int j = 0; j < NL; ++j) (void)take_nonfinite(vr[j]);
-                }
+        for (int j = 0; j < NL; ++j) top = magnitudes(top, mine[64 * j]);
+        if (__any(no_number(top))) {
+            sh.wild = 1;
+#pragma unroll 1
+            for (int j = 0; j < NL; ++j) {
+                u4 w = mine[64 * j];
+                (void)take_nonfinite(w);
+                mine[64 * j] = w;
             }
         }
-#pragma unroll
-        for (int j = 0; j < NL; ++j) {
-            const int u = 64 * j + lane;
-            if constexpr (Q8) {
-                const int r = 16 * wid + u / (D / 16), ch = u % (D / 16) * 2;
-                *reinterpret_cast<h8 *>(&sh.kbuf[b][k_at(r, ch)]) = codes8(kr[j][0], kr[j][1]);
-                *reinterpret_cast<h8 *>(&sh.kbuf[b][k_at(r, ch + 1)]) = codes8(kr[j][2], kr[j][3]);
-                const int d = wid * (D / 4) + 16 * j + (lane >> 2), c = 2 * (lane & 3);
-                *reinterpret_cast<h8 *>(&sh.vbuf[b][v_at(d, c)]) = codes8(vr[j][0], vr[j][1]);
-                *reinterpret_cast<h8 *>(&sh.vbuf[b][v_at(d, c + 1)]) = codes8(vr[j][2], vr[j][3]);
-            } else {
-                *reinterpret_cast<u4 *>(&sh.kbuf[b][k_at(16 * wid + u / (D / 8), u % (D / 8))]) = kr[j];
-                *reinterpret_cast<u4 *>(&sh.vbuf[b][v_at(wid * (D / 4) + 8 * j + (lane >> 3), lane & 7)]) = vr[j];
-            }
-        }
-        if constexpr (Q8) {
-            if (lane < 32) sh.scales[b][lane >> 4][16 * wid + (lane & 15)] = sreg;
-        }
     };
-    // which of the tile's four groups of 16 tokens have a page
-    auto groups = [&](int iv) {
-        const uint64_t bal = __ballot(iv >= 0);
-        return Q8 ? unsigned(bal & 15) : unsigned((bal & 1) | (bal >> 1 & 2) | (bal >> 2 & 4) | (bal >> 3 & 8));
+    auto groups = [&](int g) { return unsigned(__ballot(g >= 0) & 15); };  // which 16 tokens have a page
+    // Operand pieces in LDS, from one offset each (that of buffer b, with the XOR of the
+    // row in it): the step's own bits are exchanged by another XOR. The offsets are made
+    // anew for each tile: as constants of the loop they would fill the registers.
+    auto key_base = [&](int b) {
+        uint32_t at = uint32_t(b * 64 * RK + k_at(krow, hh));
+        asm volatile("" : "+v"(at));
+        return at;
     };
-    unsigned ok = 0, ok_next = 0;
-    int nk = -1, nv = -1;
-    m = -__builtin_inff();
-    l = 0.0f;
-    vref = 1e-30f;
+    auto value_base = [&](int b) {
+        uint32_t at = uint32_t(b * 128 * D + v_at(col, hh));
+        asm volatile("" : "+v"(at));
+        return at;
+    };
+    auto key = [&](uint32_t base, int n, int k) {
+        return *reinterpret_cast<const h8 *>(&sh.kbuf[0][0] + (base ^ uint32_t(k << 5)) + 32 * n * RK);
+    };
+    auto value = [&](uint32_t base, int d, int u) {
+        return *reinterpret_cast<const u4 *>(&sh.vbuf[0][0] + (base ^ uint32_t(u << 5)) + 32 * d * 128);
+    };
+
+    // a lane's scores of a tile: token t0 + 16 u + 8 hh + j is sc[u / 2][8 (u % 2) + j]
+    f16v sc[2];
 #pragma unroll
-    for (int d = 0; d < DB; ++d)
+    for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) acc[d][r] = 0.0f;
+        for (int r = 0; r < 16; ++r) sc[n][r] = 0.0f;
+    unsigned ok = 0;
+    int g1 = -1, g2 = -1;  // pages of the next two tiles
     if (threadIdx.x == 0) sh.wild = 0;
-    __syncthreads();
     if (begin < end) {
-        look_up(begin, idk, idv);
-        ok = groups(idv);
-        load(begin, idk, idv);
-        if (begin + 1 < end) look_up(begin + 1, nk, nv);
-        store(begin, 0, ok);
+        const int g0 = look_up(begin);
+        g1 = look_up(begin + 1);
+        g2 = look_up(begin + 2);
+        ok = groups(g0);
+        bring_k(begin, g0, 0);
+        bring_v(begin, g0, 0);
+        if constexpr (Q8) {
+            bring_scales(begin, g0, begin, g0);
+            put_k(0, 0);
+            put_v(0);
+        }
+        if (begin + 1 < end) {
+            bring_k(begin + 1, g1, 1);
+            if constexpr (Q8) {
+                bring_scales(begin + 1, g1, end, g1);
+                put_k(1, 1);
+            }
+        }
+        wait_vmcnt<0>();
+        __syncthreads();
+        const uint32_t kb0 = key_base(0);
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int n = 0; n < 2; ++n) sc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(key(kb0, n, k), q[k], sc[n], 0, 0, 0);
     }
     for (int i = begin; i < end; ++i) {
         const int b = (i - begin) & 1;
-        __syncthreads();
-        if (i + 1 < end) {
-            ok_next = groups(nv);
-            load(i + 1, nk, nv);
-            if (i + 2 < end) look_up(i + 2, nk, nv);
+        wait_vmcnt<0>();
+        if constexpr (!Q8) {
+            if (partial(i, ok)) take_wild(b);
         }
+        __syncthreads();  // tile i's values and tile i + 1's keys are in LDS, the buffers filled below are read no more
+        const int g3 = look_up(i + 3);
+        if (i + 2 < end) bring_k(i + 2, g2, b);
+        if (i + 1 < end) bring_v(i + 1, g1, 1 - b);
+        if constexpr (Q8) bring_scales(i + 2, g2, i + 1, g1);
         __builtin_amdgcn_sched_barrier(0);
+
         const int t0 = span.at(i) * kTileKeys;
-        // (a tile that none of this wave's rows sees)
-        const bool none = wrows <= 0 || t0 > pmax ||
-                          (a.window > 0 && t0 + kTileKeys - 1 <= pmin - a.window && t0 >= a.sinks);
-        if (!none) {
-            f16v sc[2];
+        const uint32_t vb = value_base(b), kb = key_base(1 - b);
+        // (8-bit: the scales of the lane's tokens 4x .. 4x + 3 of 32)
+        auto scales4 = [&](const float *of, int x) { return *reinterpret_cast<const f4 *>(of + 16 * (x / 2) + 8 * hh + 4 * (x % 2)); };
+        if constexpr (Q8) {
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
+            for (int x = 0; x < 8; ++x) {
+                const f4 kx = scales4(sh.ksc[(i - begin) & 3], x);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) sc[n][r] = 0.0f;
-#pragma unroll
-                for (int k = 0; k < KS; ++k) {
-                    const h8 kk = *reinterpret_cast<const h8 *>(&sh.kbuf[b][k_at(32 * n + krow, 2 * k + hh)]);
-                    sc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kk, q[k], sc[n], 0, 0, 0);
-                }
+                for (int r = 0; r < 4; ++r) sc[x / 4][4 * (x % 4) + r] *= kx[r];
             }
-            __builtin_amdgcn_sched_barrier(0);
-            // the lane's scores: token t0 + 16 u + 8 hh + j is sc[u / 2][8 (u % 2) + j]
-            float vsc[Q8 ? 32 : 1];
-            if constexpr (Q8) {
-#pragma unroll
-                for (int x = 0; x < 8; ++x) {
-                    const int at = 16 * (x / 2) + 8 * hh + 4 * (x % 2);
-                    const f4 kx = *reinterpret_cast<const f4 *>(&sh.scales[b][0][at]);
-                    const f4 vx = *reinterpret_cast<const f4 *>(&sh.scales[b][1][at]);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        sc[x / 4][4 * (x % 4) + r] *= kx[r];
-                        vsc[4 * x + r] = vx[r];
-                    }
-                }
-            }
-            const bool full = ok == 15 && t0 + kTileKeys - 1 <= pmin &&
-                              (a.window <= 0 || t0 > pmax - a.window || t0 + kTileKeys <= a.sinks);
-            uint32_t seen = 0xffffffffu;
-            if (!full) {
-                seen = 0;
-#pragma unroll
-                for (int u = 0; u < 4; ++u)
-                    seen |= ((ok >> u & 1u) ? seen_bits<8>(t0 + 16 * u + 8 * hh, pos, low, a.sinks) : 0u) << (8 * u);
-#pragma unroll
-                for (int j = 0; j < 32; ++j) sc[j / 16][j % 16] = (seen >> j & 1u) ? sc[j / 16][j % 16] : -__builtin_inff();
-            }
-            float top = sc[0][0];
-#pragma unroll
-            for (int j = 1; j < 32; ++j) top = fmaxf(top, sc[j / 16][j % 16]);
-            const float mn = fmaxf(m, halves_max(top) * p.sl2);
-            const float ms = mn == -__builtin_inff() ? 0.0f : mn;
-            const float lscale = __builtin_amdgcn_exp2f(m - ms);
-            float alpha = lscale, vinv = 1.0f;
-            if constexpr (Q8) {
-                float big = vref;
-#pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    const float x = fabsf(vsc[j]);
-                    big = fmaxf(big, (seen >> j & 1u) && x < __builtin_inff() ? x : 0.0f);
-                }
-                big = halves_max(big);
-                alpha *= vref / big;
-                vref = big;
-                vinv = 1.0f / big;
-            }
-            m = mn;
-            float sum = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j / 16][j % 16], p.sl2, -ms));
-                sum += e;
-                sc[j / 16][j % 16] = e;
-            }
-            l = l * lscale + sum;
-            if (!__all(alpha == 1.0f)) {
-#pragma unroll
-                for (int d = 0; d < DB; ++d) acc[d] *= alpha;
-            }
-            if constexpr (Q8) {
-#pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    const float w = sc[j / 16][j % 16] * (vsc[j] * vinv);
-                    sc[j / 16][j % 16] = (seen >> j & 1u) ? w : 0.0f;
-                }
-            }
-            h8 pb[4];
-#pragma unroll
-            for (int j = 0; j < 32; ++j) pb[j / 8][j % 8] = _Float16(sc[j / 16][j % 16]);
-            __builtin_amdgcn_sched_barrier(0);
+        }
+        const bool full = ok == 15 && t0 + kTileKeys - 1 <= pmin &&
+                          (a.window <= 0 || t0 > pmax - a.window || t0 + kTileKeys <= a.sinks);
+        uint32_t seen = 0xffffffffu;
+        if (!full) {
+            seen = 0;
 #pragma unroll
             for (int u = 0; u < 4; ++u)
+                seen |= ((ok >> u & 1u) ? seen_bits<8>(t0 + 16 * u + 8 * hh, pos, low, a.sinks) : 0u) << (8 * u);
 #pragma unroll
-                for (int d = 0; d < DB; ++d) {
-                    const h8 vv = *reinterpret_cast<const h8 *>(&sh.vbuf[b][v_at(32 * d + col, 2 * u + hh)]);
-                    acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vv, pb[u], acc[d], 0, 0, 0);
+            for (int j = 0; j < 32; ++j) sc[j / 16][j % 16] = (seen >> j & 1u) ? sc[j / 16][j % 16] : -__builtin_inff();
+        }
+        float top = max3(sc[0][0], sc[0][1], sc[0][2]);
+#pragma unroll
+        for (int j = 3; j < 31; j += 2) top = max3(top, sc[j / 16][j % 16], sc[(j + 1) / 16][(j + 1) % 16]);
+        top = fmaxf(top, sc[1][15]);
+        const float mn = fmaxf(m, halves_max(top) * p.sl2);
+        const float ms = mn == -__builtin_inff() ? 0.0f : mn;
+        const float lscale = __builtin_amdgcn_exp2f(m - ms);
+        float alpha = lscale, vinv = 1.0f;
+        if constexpr (Q8) {
+            float big = vref;
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+                const f4 vx = scales4(sh.vsc[b], x);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float y = fabsf(vx[r]);
+                    big = fmaxf(big, ((seen >> (4 * x + r) & 1u) != 0) & (y < __builtin_inff()) ? y : 0.0f);
                 }
+            }
+            big = halves_max(big);
+            alpha *= vref / big;
+            vref = big;
+            vinv = 1.0f / big;
         }
-        __builtin_amdgcn_sched_barrier(0);
-        if (i + 1 < end) {
-            store(i + 1, 1 - b, ok_next);
-            ok = ok_next;
+        m = mn;
+        l *= lscale;
+        if (!__all(alpha == 1.0f)) {
+#pragma unroll
+            for (int d = 0; d < DB; ++d) acc[d] *= alpha;
         }
+
+        f16v sn[2];  // (past the last tile: of what the buffer holds, not used)
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sn[n][r] = 0.0f;
+        h8 pb[4];
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        auto product = [&](int u) {
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+                acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, value(vb, d, u)), pb[u], acc[d], 0, 0, 0);
+        };
+        // in quarters, each between fences: exponentials of 16 tokens, a quarter of the next
+        // scores, and from the third on the product of the quarter two before
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            f4 vx[2];
+            if constexpr (Q8) {
+                vx[0] = scales4(sh.vsc[b], 2 * u) * vinv;
+                vx[1] = scales4(sh.vsc[b], 2 * u + 1) * vinv;
+            }
+#pragma unroll
+            for (int k = u * KS / 4; k < (u + 1) * KS / 4; ++k)
+#pragma unroll
+                for (int n = 0; n < 2; ++n) sn[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(key(kb, n, k), q[k], sn[n], 0, 0, 0);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u / 2][8 * (u % 2) + j], p.sl2, -ms));
+                sum[u] += e;
+                if constexpr (Q8) {
+                    e *= vx[j / 4][j % 4];
+                    e = (seen >> (8 * u + j) & 1u) ? e : 0.0f;
+                }
+                pb[u][j] = _Float16(e);
+            }
+            if (u >= 2) product(u - 2);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        product(2);
+        product(3);
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) sc[n] = sn[n];
+        if constexpr (Q8) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (i + 2 < end) put_k(b, i + 2 - begin);
+            if (i + 1 < end) put_v(1 - b);
+        }
+        ok = groups(g1);
+        g1 = g2;
+        g2 = g3;
     }
 
     if constexpr (!Q8) {
@@ -948,8 +1039,7 @@ __device__ inline __attribute__((always_inline)) void tile_piece(const SplitArgs
         if (sh.wild) {  // of what each row sees of those values, counts, and what they make of its sum
             for (int i = begin; i < end; ++i) {
                 const int t0 = span.at(i) * kTileKeys;
-                look_up(i, idk, idv);
-                if (!partial(i, groups(idv))) continue;
+                if (!partial(i, groups(look_up(i)))) continue;
 #pragma unroll
                 for (int d = 0; d < DB; ++d) {
                     f16v cnt;
@@ -957,10 +1047,10 @@ __device__ inline __attribute__((always_inline)) void tile_piece(const SplitArgs
                     for (int r = 0; r < 16; ++r) cnt[r] = 0.0f;
 #pragma unroll 1
                     for (int u = 0; u < 4; ++u) {
-                        const int key = t0 + 16 * u + 8 * hh, id = page_of(a.b, s, t0 + 16 * u, v.len);
+                        const int at = t0 + 16 * u + 8 * hh, id = page_of(a.b, s, t0 + 16 * u, v.len);
                         u4 w = *reinterpret_cast<const u4 *>(static_cast<const uint8_t *>(a.vc) +
-                            (((size_t(max(id, 0)) * H + h) * D + 32 * d + col) * size_t(P) + size_t(key & (P - 1))) * 2);
-                        const uint32_t bits = id >= 0 ? seen_bits<8>(key, pos, low, a.sinks) : 0u;
+                            (((size_t(max(id, 0)) * H + h) * D + 32 * d + col) * size_t(P) + size_t(at & (P - 1))) * 2);
+                        const uint32_t bits = id >= 0 ? seen_bits<8>(at, pos, low, a.sinks) : 0u;
                         h8 sb;
 #pragma unroll
                         for (int j = 0; j < 8; ++j) sb[j] = _Float16(float(bits >> j & 1u));

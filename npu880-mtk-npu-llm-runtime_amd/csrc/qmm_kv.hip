@@ -58,14 +58,14 @@ __device__ inline void append_qk(const AppendArgs &a, int m, int job, int njobs,
     if (s < 0) return;
     const SeqView v = seq_view(a.b, s);
     const int place = v.pos0 + (m - v.r0);
-    if (a.pairs) {
-        for (int j = t; j < a.rot_dim / 2; j += 256) {
-            const RopePair p = a.pairs[j];
-            const int pos = a.pos ? a.pos[size_t(p.axis) * a.pos_stride + size_t(m)] : place;
-            const double turns = double(pos) * p.turns;
+    const int rot = a.rope.rot_dim, half = rot / 2;
+    if (rot) {
+        if (t < half) {
+            const int pos = a.pos ? a.pos[size_t(a.rope.axis[t]) * a.pos_stride + size_t(m)] : place;
+            const double turns = double(pos) * a.rope.turns[t];
             float sn, co;
             sincospif(2.0f * float(turns - rint(turns)), &sn, &co);
-            cs[j] = make_float2(co * a.rope_scale, sn * a.rope_scale);
+            cs[t] = make_float2(co * a.rope.scale, sn * a.rope.scale);
         }
         __syncthreads();
     }
@@ -73,8 +73,7 @@ __device__ inline void append_qk(const AppendArgs &a, int m, int job, int njobs,
     const int slot = place & ((1 << a.b.page_shift) - 1);
     const int H = a.b.n_heads, HQ = a.q ? a.q_heads : 0, heads = HQ + H;
     const int e = 4 * (lane % LPH);  // this lane's first value of its head
-    const bool turned = a.pairs && e < a.rot_dim, half_style = a.style == 0;
-    const int half = a.rot_dim / 2;
+    const bool turned = e < rot, half_style = a.rope.style == 0;
     const bool first = e < half;
     const int other = (lane & ~(LPH - 1)) + (half_style && turned ? (first ? e + half : e - half) / 4 : lane % LPH);
     for (int g = job * 4 + wid; g * HPW < heads; g += njobs * 4) {
@@ -91,7 +90,7 @@ __device__ inline void append_qk(const AppendArgs &a, int m, int job, int njobs,
             const float4 w = *reinterpret_cast<const float4 *>(gamma + e);
             x = make_float4(x.x * r * w.x, x.y * r * w.y, x.z * r * w.z, x.w * r * w.w);
         }
-        if (a.pairs) {
+        if (rot) {
             if (half_style) {
                 const float4 y = make_float4(__shfl(x.x, other), __shfl(x.y, other), __shfl(x.z, other), __shfl(x.w, other));
                 if (turned) {
