@@ -88,6 +88,18 @@ template <int N> __device__ inline uint32_t seen_bits(int key0, int p, int low, 
     return below(p + 1) & (~below(low + 1) | below(sinks));
 }
 
+// x where bit j of `bits` is set, else -infinity
+__device__ inline float seen_or_none(uint32_t bits, int j, float x) {
+    return int32_t(bits << (31 - j)) < 0 ? x : -__builtin_inff();
+}
+// 8 halves of ones where the token's bit is set, else of zeros
+__device__ inline u4 halves_of(uint32_t bits) {
+    u4 r;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r[j] = ((bits >> 2 * j & 1u) ? 0xffffu : 0u) | ((bits >> (2 * j + 1) & 1u) ? 0xffff0000u : 0u);
+    return r;
+}
+
 // A value that is no number, made a count: +inf 1, -inf 128, NaN 16384 (64
 // tokens' counts stay apart in a sum); finite values 0.
 __device__ inline uint32_t nonfinite_code(uint32_t h) {
@@ -402,7 +414,7 @@ __device__ inline __attribute__((always_inline)) void split_piece(const SplitArg
                 seen[n] = page_ok ? seen_bits<TL>(key0, pos[n], low[n], a.sinks) : 0u;
 #pragma unroll
                 for (int j = 0; j < TL; ++j)
-                    sc[n][j / 4][j % 4] = (seen[n] >> j & 1u) ? sc[n][j / 4][j % 4] : -__builtin_inff();
+                    sc[n][j / 4][j % 4] = seen_or_none(seen[n], j, sc[n][j / 4][j % 4]);
             }
             float top = sc[n][0][0];
 #pragma unroll
@@ -416,7 +428,8 @@ __device__ inline __attribute__((always_inline)) void split_piece(const SplitArg
 #pragma unroll
                 for (int j = 0; j < TL; ++j) {
                     const float x = fabsf(vsc[j / 4][j % 4]);
-                    big = fmaxf(big, ((seen[n] >> j) & 1u) && x < __builtin_inff() ? x : 0.0f);
+                    const bool in = ((seen[n] >> j & 1u) != 0) & (x < __builtin_inff());
+                    big = fmaxf(big, in ? x : 0.0f);
                 }
                 big = groups_max(big);
                 alpha *= vref[n] / big;
@@ -708,7 +721,7 @@ __device__ inline float halves_sum(float v) {
 template <int D> struct TileShared {
     __attribute__((aligned(16))) uint8_t kbuf[2][128 * D];  // 64 keys, as fp16
     __attribute__((aligned(16))) uint8_t vbuf[2][128 * D];
-    float ksc[4][64], vsc[2][64];                           // 8-bit cache: their scales
+    float ksc[4][64], vsc[2][64], vmax[2][4];               // 8-bit cache: their scales; the largest of each 16 values'
     int wild;                                               // a tile had values that are no numbers, hidden from some row
 };
 
@@ -832,6 +845,10 @@ __device__ inline __attribute__((always_inline)) void tile_piece(const SplitArgs
             *reinterpret_cast<h8 *>(&sh.vbuf[b][v_at(d, c)]) = codes8(vr[j][0], vr[j][1]);
             *reinterpret_cast<h8 *>(&sh.vbuf[b][v_at(d, c + 1)]) = codes8(vr[j][2], vr[j][3]);
         }
+        float big = fabsf(sreg) < __builtin_inff() ? fabsf(sreg) : 0.0f;
+#pragma unroll
+        for (int o = 1; o < 16; o *= 2) big = fmaxf(big, __shfl_xor(big, o));
+        if (lane == 16) sh.vmax[b][wid] = big;
         if (lane >= 16 && lane < 32) sh.vsc[b][16 * wid + (lane & 15)] = sreg;
     };
     // Values that are no numbers in a tile of which some row of the workgroup does not see
@@ -948,7 +965,7 @@ __device__ inline __attribute__((always_inline)) void tile_piece(const SplitArgs
             for (int u = 0; u < 4; ++u)
                 seen |= ((ok >> u & 1u) ? seen_bits<8>(t0 + 16 * u + 8 * hh, pos, low, a.sinks) : 0u) << (8 * u);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) sc[j / 16][j % 16] = (seen >> j & 1u) ? sc[j / 16][j % 16] : -__builtin_inff();
+            for (int j = 0; j < 32; ++j) sc[j / 16][j % 16] = seen_or_none(seen, j, sc[j / 16][j % 16]);
         }
         float top = max3(sc[0][0], sc[0][1], sc[0][2]);
 #pragma unroll
@@ -959,17 +976,23 @@ __device__ inline __attribute__((always_inline)) void tile_piece(const SplitArgs
         const float lscale = __builtin_amdgcn_exp2f(m - ms);
         float alpha = lscale, vinv = 1.0f;
         if constexpr (Q8) {
-            float big = vref;
+            const f4 most = *reinterpret_cast<const f4 *>(sh.vmax[b]);
+            float big = fmaxf(max3(most[0], most[1], most[2]), most[3]);
+            if (!full) {  // of those that the row sees
+                big = 0.0f;
 #pragma unroll
-            for (int x = 0; x < 8; ++x) {
-                const f4 vx = scales4(sh.vsc[b], x);
+                for (int x = 0; x < 8; ++x) {
+                    const f4 vx = scales4(sh.vsc[b], x);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float y = fabsf(vx[r]);
-                    big = fmaxf(big, ((seen >> (4 * x + r) & 1u) != 0) & (y < __builtin_inff()) ? y : 0.0f);
+                    for (int r = 0; r < 4; ++r) {
+                        const float y = fabsf(vx[r]);
+                        const bool in = ((seen >> (4 * x + r) & 1u) != 0) & (y < __builtin_inff());
+                        big = fmaxf(big, in ? y : 0.0f);
+                    }
                 }
+                big = halves_max(big);
             }
-            big = halves_max(big);
+            big = fmaxf(big, vref);
             alpha *= vref / big;
             vref = big;
             vinv = 1.0f / big;
@@ -1010,11 +1033,11 @@ __device__ inline __attribute__((always_inline)) void tile_piece(const SplitArgs
             for (int j = 0; j < 8; ++j) {
                 float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u / 2][8 * (u % 2) + j], p.sl2, -ms));
                 sum[u] += e;
-                if constexpr (Q8) {
-                    e *= vx[j / 4][j % 4];
-                    e = (seen >> (8 * u + j) & 1u) ? e : 0.0f;
-                }
+                if constexpr (Q8) e *= vx[j / 4][j % 4];
                 pb[u][j] = _Float16(e);
+            }
+            if constexpr (Q8) {  // (a hidden token's scale may be no number)
+                if (!full) pb[u] = __builtin_bit_cast(h8, u4(__builtin_bit_cast(u4, pb[u]) & halves_of(seen >> 8 * u)));
             }
             if (u >= 2) product(u - 2);
             __builtin_amdgcn_sched_barrier(0);
