@@ -32,13 +32,6 @@ constexpr TileSpan tile_span(int pmin, int pmax, int window, int sinks) {
     const int sink = s < lo ? s : lo;
     return TileSpan{sink, lo, sink + hi - lo};
 }
-// Tiles per split, where the launch has nsplit splits of `chunk` tiles: more
-// than `chunk` where the sequence is longer than the host said.
-constexpr int split_tiles(int n, int nsplit, int chunk) {
-    const int need = (n + nsplit - 1) / nsplit;
-    return need > chunk ? need : chunk;
-}
-
 #ifdef __HIPCC__
 #define QMM_HD __host__ __device__
 #else

@@ -1,7 +1,7 @@
 // qmm_attn.hip — attention of new tokens over a paged key-value cache.
 //
 // A key-value head's query heads times a sequence's new tokens are the rows;
-// 16 NC of them are the columns of the products
+// 16 of them a wave are the columns of the products
 //   S^T [tokens x rows] = K Q^T,   O^T [values x rows] = V^T P^T
 // on 16x16x32 fp16 MFMA, 64 tokens a tile, with the running maximum m and sum l
 // of the softmax in base 2 (exp2(s scale log2 e - m)), fp32. Which token a row
@@ -43,16 +43,20 @@ struct SplitArgs {
     AttnArgs a;
     float sl2;             // scale log2(e)
     int new_min, new_max;  // only sequences of this many new tokens
-    float *part_o;         // partial results, and (m, l) of the same rows:
+    float *part_o;         // partial results, and (m, l) of the same rows
     float2 *part_ml;
-    // tile kernel: [seq][head][split][128 row_tiles][D]
-    int nsplit, chunk, row_tiles;
-    // split kernel: [worker][2][16 NC][D]: a piece that goes on from the worker before, one that the next goes on with
+    // [worker][2][row tile][D]: a piece that goes on from the worker before, one that the next goes on with
     int workers;  // 0: a workgroup takes a head of a sequence whole, nothing is partial
-    SharedSegment *shared;  // [workers]
+    SharedSegment *shared;  // [workers + 1], the last one's pieces: the workers there were
 };
 constexpr int kMaxShared = 512;  // sequences of a call whose tiles workers share
 
+// the largest of three (a NaN counts for nothing)
+__device__ inline float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
 // maximum / sum over the four lane groups (lanes l, l ^ 16, l ^ 32, l ^ 48)
 __device__ inline float groups_max(float v) {
     auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -141,17 +145,20 @@ __device__ inline void put_row(const AttnArgs &a, size_t at, f4 o) {
     else *reinterpret_cast<h4 *>(static_cast<uint16_t *>(a.out) + at) = y;
 }
 
-// One row from n partial results (slot(k): the k-th's place), in this order whatever
-// ran when: wave w takes pieces w, w + 4, .., a lane D / 64 values.
+constexpr int kJoinWaves = 8;  // of a workgroup that joins partial results
+
+// A wave's share of a row's partial results, k = first, first + step, .. below n
+// (slot(k): the k-th's place), a lane D / 64 values.
 template <int D, class Slot>
-__device__ inline void join_row(const SplitArgs &p, int n, Slot slot, float (*part)[D], float2 *ml, size_t dst) {
+__device__ inline void join_pieces(const SplitArgs &p, int first, int step, int n, Slot slot, float (&o)[D / 64], float &m, float &l) {
     constexpr int N = D / 64;
-    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
-    float o[N], m = -__builtin_inff(), l = 0.0f;
+    const int lane = threadIdx.x & 63;
+    m = -__builtin_inff();
+    l = 0.0f;
 #pragma unroll
     for (int j = 0; j < N; ++j) o[j] = 0.0f;
-#pragma unroll 4
-    for (int k = wid; k < n; k += 4) {
+#pragma unroll 8
+    for (int k = first; k < n; k += step) {
         const int64_t s = slot(k);
         const float2 x = p.part_ml[s];
         float y[N];
@@ -164,16 +171,26 @@ __device__ inline void join_row(const SplitArgs &p, int n, Slot slot, float (*pa
 #pragma unroll
         for (int j = 0; j < N; ++j) o[j] = o[j] * wa + y[j] * wb;
     }
+}
+// One row from n partial results, by a workgroup: its waves' shares in turn, in this
+// order whatever ran when.
+template <int D, class Slot>
+__device__ inline void join_row(const SplitArgs &p, int n, Slot slot, float (*part)[D], float2 *ml, size_t dst) {
+    constexpr int W = kJoinWaves;
+    constexpr int N = D / 64;
+    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+    float o[N], m, l;
+    join_pieces<D>(p, wid, W, n, slot, o, m, l);
     if (lane == 0) ml[wid] = make_float2(m, l);
 #pragma unroll
     for (int j = 0; j < N; ++j) part[wid][64 * j + lane] = o[j];
     __syncthreads();
     if (threadIdx.x < D) {
         float top = ml[0].x;
-        for (int w = 1; w < 4; ++w) top = fmaxf(top, ml[w].x);
+        for (int w = 1; w < W; ++w) top = fmaxf(top, ml[w].x);
         const float base = top == -__builtin_inff() ? 0.0f : top;
         float total = 0.0f, sum = 0.0f;
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < W; ++w) {
             const float e = __builtin_amdgcn_exp2f(ml[w].x - base);
             total += ml[w].y * e;
             sum += part[w][threadIdx.x] * e;
@@ -241,30 +258,29 @@ template <int R> __device__ inline RowTile row_tile(const AttnArgs &a, const Seq
     return t;
 }
 
-template <int D, int NC, int NW> struct SplitShared {
-    static constexpr bool kQueries = D * NC > 128;  // queries in LDS: 256 registers do not hold them
-    f4 joined[NW][D < 128 ? D / 16 : 8][64];        // value tiles joined at a time
-    float2 ml[NW][16 * NC];
-    h8 qlds[kQueries ? NC * D / 32 : 1][64];
+template <int D, int NW> struct SplitShared {
+    f4 joined[NW][D < 128 ? D / 16 : 8][64];  // value tiles joined at a time
+    float2 ml[NW][16];
+    h8 queries[D > 128 ? NW : 1][D > 128 ? D / 32 : 1][64];  // where 256 registers do not hold them too
 };
 
-// One piece of a segment: rows of `tile` of head h of sequence s over tiles begin ..
-// end - 1 of its span, by all waves; the rows themselves (direct), or their partial
-// results at slot0.
-template <int D, int NC, int NW, bool Q8>
-__device__ inline __attribute__((always_inline)) void split_piece(const SplitArgs &p, SplitShared<D, NC, NW> &sh, const SeqView &v,
+// One piece of a segment: the up to 16 rows of `tile` of head h of sequence s over
+// tiles begin .. end - 1 of its span, the waves' steps in turn; the rows themselves
+// (direct), or their partial results at slot0.
+template <int D, int NW, bool Q8>
+__device__ inline __attribute__((always_inline)) void split_piece(const SplitArgs &p, SplitShared<D, NW> &sh, const SeqView &v,
                                                                   const RowTile &tile, int s, int h, int begin, int end,
                                                                   bool direct, int slot0) {
     constexpr int KS = D / 32;           // MFMA steps of a score
     constexpr int DT = D / 16;           // value tiles
     constexpr int KR = Q8 ? D / 64 : KS;  // 16-B registers of a key operand
-    constexpr int KT = D * NC <= 128 ? 64 : 32;  // tokens of a wave's step
+    constexpr int KT = D <= 128 ? 64 : 32;  // tokens of a wave's step
     constexpr int NT = KT / 16;          // score MFMAs of a step
     constexpr int TL = KT / 4;           // tokens of a lane: TL c .. TL c + TL - 1
     constexpr int NU = TL / 8;           // MFMA steps of the second product
     constexpr int SUB = kTileKeys / KT;
     // what 256 registers hold: the next step's keys beside this one's values, and the queries
-    constexpr bool AHEAD = D * NC < 256, QLDS = D * NC > 128;
+    constexpr bool AHEAD = D <= 128, QLDS = D > 128;
     constexpr int DG = DT < 8 ? DT : 8;  // value tiles joined at a time
     const AttnArgs &a = p.a;
     const int H = a.b.n_heads, G = a.group;
@@ -273,36 +289,29 @@ __device__ inline __attribute__((always_inline)) void split_piece(const SplitArg
     const TileSpan span = tile.span;
     const int row0 = tile.row0, nrows = tile.nrows, pmin = tile.pmin, pmax = tile.pmax;
 
-    // this lane's rows: queries, positions, the last token a row's window hides
-    h8 q[QLDS ? 1 : NC][QLDS ? 1 : KS];
-    int pos[NC], low[NC];
-#pragma unroll
-    for (int n = 0; n < NC; ++n) {
-        const int r = 16 * n + col, row = row0 + (r < nrows ? r : 0);
-        const int i = token_of(a, row), g = row - i * G;
-        pos[n] = v.pos0 + i;
-        low[n] = a.window > 0 ? max(pos[n] - a.window, -1) : -1;
-        const uint16_t *src = a.q + size_t(v.r0 + i) * a.q_stride + size_t(h * G + g) * D;
+    // this lane's row: its queries, position, the last token its window hides
+    h8 q[QLDS ? 1 : KS];
+    const int row = row0 + (col < nrows ? col : 0);
+    const int qi = token_of(a, row), qg = row - qi * G, pos = v.pos0 + qi;
+    const int low = a.window > 0 ? max(pos - a.window, -1) : -1;
+    {
+        const uint16_t *src = a.q + size_t(v.r0 + qi) * a.q_stride + size_t(h * G + qg) * D;
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
             const h8 x = *reinterpret_cast<const h8 *>(src + (Q8 ? 64 * (k / 2) + 16 * c + 8 * (k % 2) : 32 * k + 8 * c));
-            if constexpr (QLDS) {
-                if ((n * KS + k) % NW == wid) sh.qlds[n * KS + k][lane] = x;
-            } else {
-                q[n][k] = x;
-            }
+            if constexpr (QLDS) sh.queries[wid][k][lane] = x;
+            else q[k] = x;
         }
     }
-    if constexpr (QLDS) __syncthreads();
-    float m[NC], l[NC], vref[NC];
-    f4 acc[NC][DT];
+    float m = -__builtin_inff(), l = 0.0f, vref = 1e-30f;
+    f4 acc[DT];
 
     u4 kr[NT][KR], vr[DT][Q8 ? (NU + 1) / 2 : NU];
     f4 ksc[NT], vsc[NT];
     int id_v = -1;
     bool wild_steps = false;
     const int ck = col >> 2;  // the lane group whose tokens this lane loads keys of
-    // the wave's steps are begin + wid, begin + wid + NW, .. of SUB (end - begin)
+    // the wave's steps are wid, wid + NW, .. of SUB (end - begin)
     const int steps = (end - begin) * SUB;
     auto step_at = [&](int i) { return span.at(begin + i / SUB) * kTileKeys + i % SUB * KT; };
     auto is_full = [&](int t0, bool page_ok) {  // every row sees every token
@@ -325,13 +334,7 @@ __device__ inline __attribute__((always_inline)) void split_piece(const SplitArg
                 kr[t][k] = *reinterpret_cast<const u4 *>(src + t * 4 * (Q8 ? D : 2 * D) + k * 64);
     };
 #pragma unroll
-    for (int n = 0; n < NC; ++n) {
-        m[n] = -__builtin_inff();
-        l[n] = 0.0f;
-        vref[n] = 1e-30f;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) acc[n][d] = f4{0.f, 0.f, 0.f, 0.f};
-    }
+    for (int d = 0; d < DT; ++d) acc[d] = f4{0.f, 0.f, 0.f, 0.f};
     // pages are looked up a step ahead of their loads: loads return in order
     int nk = -1, nv = -1;
     if (wid < steps) {
@@ -373,24 +376,18 @@ __device__ inline __attribute__((always_inline)) void split_piece(const SplitArg
         const bool page_ok = id_v >= 0;
         __builtin_amdgcn_sched_barrier(0);
 
-        f4 sc[NC][NT];
+        f4 sc[NT];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-#pragma unroll
-            for (int n = 0; n < NC; ++n) sc[n][t] = f4{0.f, 0.f, 0.f, 0.f};
+            sc[t] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
-                h8 kk;
+                h8 kk, qq;
                 if constexpr (Q8) kk = codes8(kr[t][k / 2][2 * (k % 2)], kr[t][k / 2][2 * (k % 2) + 1]);
                 else kk = __builtin_bit_cast(h8, kr[t][k]);
-#pragma unroll
-                for (int n = 0; n < NC; ++n)
-                    {
-                    h8 qq;
-                    if constexpr (QLDS) qq = sh.qlds[n * KS + k][lane];
-                    else qq = q[n][k];
-                    sc[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, qq, sc[n][t], 0, 0, 0);
-                }
+                if constexpr (QLDS) qq = sh.queries[wid][k][lane];
+                else qq = q[k];
+                sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, qq, sc[t], 0, 0, 0);
             }
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -402,60 +399,49 @@ __device__ inline __attribute__((always_inline)) void split_piece(const SplitArg
         __builtin_amdgcn_sched_barrier(0);
 
         const bool full = is_full(t0, page_ok);
-        uint32_t seen[NC];  // bit j: token key0 + j is visible to the row
+        uint32_t seen = (1u << TL) - 1u;  // bit j: token key0 + j is visible to the row
+        if constexpr (Q8) {
 #pragma unroll
-        for (int n = 0; n < NC; ++n) {
-            if constexpr (Q8) {
+            for (int t = 0; t < NT; ++t) sc[t] *= ksc[t];
+        }
+        if (!full) {
+            seen = page_ok ? seen_bits<TL>(key0, pos, low, a.sinks) : 0u;
 #pragma unroll
-                for (int t = 0; t < NT; ++t) sc[n][t] *= ksc[t];
-            }
-            seen[n] = (1u << TL) - 1u;
-            if (!full) {
-                seen[n] = page_ok ? seen_bits<TL>(key0, pos[n], low[n], a.sinks) : 0u;
+            for (int j = 0; j < TL; ++j) sc[j / 4][j % 4] = seen_or_none(seen, j, sc[j / 4][j % 4]);
+        }
+        float top = max3(sc[0][0], sc[0][1], sc[0][2]);
 #pragma unroll
-                for (int j = 0; j < TL; ++j)
-                    sc[n][j / 4][j % 4] = seen_or_none(seen[n], j, sc[n][j / 4][j % 4]);
-            }
-            float top = sc[n][0][0];
-#pragma unroll
-            for (int j = 1; j < TL; ++j) top = fmaxf(top, sc[n][j / 4][j % 4]);
-            const float mn = fmaxf(m[n], groups_max(top) * p.sl2);
-            const float ms = mn == -__builtin_inff() ? 0.0f : mn;
-            const float lscale = __builtin_amdgcn_exp2f(m[n] - ms);
-            float alpha = lscale, vinv = 1.0f;
-            if constexpr (Q8) {  // the largest value scale the row has seen: its weights below are relative to it
-                float big = vref[n];
-#pragma unroll
-                for (int j = 0; j < TL; ++j) {
-                    const float x = fabsf(vsc[j / 4][j % 4]);
-                    const bool in = ((seen[n] >> j & 1u) != 0) & (x < __builtin_inff());
-                    big = fmaxf(big, in ? x : 0.0f);
-                }
-                big = groups_max(big);
-                alpha *= vref[n] / big;
-                vref[n] = big;
-                vinv = 1.0f / big;
-            }
-            m[n] = mn;
-            float sum = 0.0f;
+        for (int j = 3; j + 1 < TL; j += 2) top = max3(top, sc[j / 4][j % 4], sc[(j + 1) / 4][(j + 1) % 4]);
+        top = fmaxf(top, sc[NT - 1][3]);
+        const float mn = fmaxf(m, groups_max(top) * p.sl2);
+        const float ms = mn == -__builtin_inff() ? 0.0f : mn;
+        const float lscale = __builtin_amdgcn_exp2f(m - ms);
+        float alpha = lscale, vinv = 1.0f;
+        if constexpr (Q8) {  // the largest value scale the row has seen: its weights below are relative to it
+            float big = vref;
 #pragma unroll
             for (int j = 0; j < TL; ++j) {
-                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][j / 4][j % 4], p.sl2, -ms));
-                sc[n][j / 4][j % 4] = e;
-                sum += e;
+                const float x = fabsf(vsc[j / 4][j % 4]);
+                const bool in = ((seen >> j & 1u) != 0) & (x < __builtin_inff());
+                big = fmaxf(big, in ? x : 0.0f);
             }
-            l[n] = l[n] * lscale + sum;
-            if (!__all(alpha == 1.0f)) {
+            big = groups_max(big);
+            alpha *= vref / big;
+            vref = big;
+            vinv = 1.0f / big;
+        }
+        m = mn;
+        float sum = 0.0f;
 #pragma unroll
-                for (int d = 0; d < DT; ++d) acc[n][d] *= alpha;
-            }
-            if constexpr (Q8) {  // the weights of the codes: p * scale
+        for (int j = 0; j < TL; ++j) {
+            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j / 4][j % 4], p.sl2, -ms));
+            sc[j / 4][j % 4] = e;
+            sum += e;
+        }
+        l = l * lscale + sum;
+        if (!__all(alpha == 1.0f)) {
 #pragma unroll
-                for (int j = 0; j < TL; ++j) {
-                    const float w = sc[n][j / 4][j % 4] * (vsc[j / 4][j % 4] * vinv);
-                    sc[n][j / 4][j % 4] = (seen[n] >> j) & 1u ? w : 0.0f;
-                }
-            }
+            for (int d = 0; d < DT; ++d) acc[d] *= alpha;
         }
         if constexpr (!Q8) {
             if (!full) {
@@ -475,11 +461,19 @@ __device__ inline __attribute__((always_inline)) void split_piece(const SplitArg
                 }
             }
         }
-        h8 pb[NC][NU];
+        h8 pb[NU];
 #pragma unroll
-        for (int n = 0; n < NC; ++n)
+        for (int j = 0; j < TL; ++j) {
+            float w = sc[j / 4][j % 4];
+            if constexpr (Q8) w *= vsc[j / 4][j % 4] * vinv;  // the weights of the codes: p * scale
+            pb[j / 8][j % 8] = _Float16(w);
+        }
+        if constexpr (Q8) {  // (a hidden token's scale may be no number)
+            if (!full) {
 #pragma unroll
-            for (int j = 0; j < TL; ++j) pb[n][j / 8][j % 8] = _Float16(sc[n][j / 4][j % 4]);
+                for (int u = 0; u < NU; ++u) pb[u] = __builtin_bit_cast(h8, u4(__builtin_bit_cast(u4, pb[u]) & halves_of(seen >> 8 * u)));
+            }
+        }
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -487,9 +481,7 @@ __device__ inline __attribute__((always_inline)) void split_piece(const SplitArg
                 h8 vv;
                 if constexpr (Q8) vv = codes8(vr[d][0][2 * u], vr[d][0][2 * u + 1]);
                 else vv = __builtin_bit_cast(h8, vr[d][u]);
-#pragma unroll
-                for (int n = 0; n < NC; ++n)
-                    acc[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, pb[n][u], acc[n][d], 0, 0, 0);
+                acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, pb[u], acc[d], 0, 0, 0);
             }
         if constexpr (!AHEAD) {
             if (i + NW < steps) load_k(i + NW, nk);
@@ -507,30 +499,21 @@ __device__ inline __attribute__((always_inline)) void split_piece(const SplitArg
                 if (is_full(t0, id_v >= 0)) continue;
                 const uint8_t *src = static_cast<const uint8_t *>(a.vc) +
                                      (((size_t(max(id_v, 0)) * H + h) * D + col) * size_t(P) + size_t(key0 & (P - 1))) * 2;
-                h8 sb[NC][NU];
+                const uint32_t bits = id_v >= 0 ? seen_bits<TL>(key0, pos, low, a.sinks) : 0u;
+                h8 sb[NU];
 #pragma unroll
-                for (int n = 0; n < NC; ++n) {
-                    const uint32_t bits = id_v >= 0 ? seen_bits<TL>(key0, pos[n], low[n], a.sinks) : 0u;
-#pragma unroll
-                    for (int j = 0; j < TL; ++j) sb[n][j / 8][j % 8] = _Float16(float(bits >> j & 1u));
-                }
+                for (int j = 0; j < TL; ++j) sb[j / 8][j % 8] = _Float16(float(bits >> j & 1u));
 #pragma unroll
                 for (int d = 0; d < DT; ++d, src += size_t(32) << shift) {
                     asm volatile("" : "+v"(src));  // (one address, not all of them)
-                    h8 code[NU];
+                    f4 cnt = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int u = 0; u < NU; ++u) {
                         u4 w = reinterpret_cast<const u4 *>(src)[u];
-                        code[u] = __builtin_bit_cast(h8, take_nonfinite(w));
+                        cnt = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, take_nonfinite(w)), sb[u], cnt, 0, 0, 0);
                     }
 #pragma unroll
-                    for (int n = 0; n < NC; ++n) {
-                        f4 cnt = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                        for (int u = 0; u < NU; ++u) cnt = __builtin_amdgcn_mfma_f32_16x16x32_f16(code[u], sb[n][u], cnt, 0, 0, 0);
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) acc[n][d][r] += nonfinite_sum(cnt[r]);
-                    }
+                    for (int r = 0; r < 4; ++r) acc[d][r] += nonfinite_sum(cnt[r]);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
@@ -538,167 +521,43 @@ __device__ inline __attribute__((always_inline)) void split_piece(const SplitArg
     }
 
     // the waves' results, joined in LDS
-#pragma unroll
-    for (int n = 0; n < NC; ++n) {
-        const float sum = groups_sum(l[n]);
-        if (c == 0) sh.ml[wid][16 * n + col] = make_float2(m[n], sum);
-    }
+    l = groups_sum(l);
+    if (c == 0) sh.ml[wid][col] = make_float2(m, l);
     __syncthreads();
+    float top = -__builtin_inff(), total = 0.0f;
 #pragma unroll
-    for (int n = 0; n < NC; ++n) {
-        float top = sh.ml[0][16 * n + col].x;
+    for (int w = 0; w < NW; ++w) top = fmaxf(top, sh.ml[w][col].x);
+    const float base = top == -__builtin_inff() ? 0.0f : top;
 #pragma unroll
-        for (int w = 1; w < NW; ++w) top = fmaxf(top, sh.ml[w][16 * n + col].x);
-        const float base = top == -__builtin_inff() ? 0.0f : top;
-        float total = 0.0f;
+    for (int w = 0; w < NW; ++w) {
+        const float2 x = sh.ml[w][col];
+        total += x.y * __builtin_amdgcn_exp2f(x.x - base);
+    }
+    const float mine = __builtin_amdgcn_exp2f(m - base) * (Q8 ? vref : 1.0f);
+    const float inv = direct ? (total > 0.0f || total != total ? 1.0f / total : 0.0f) : 1.0f;
+    const bool in = col < nrows;
+    const int slot = slot0 + col;
+    if (!direct && in && threadIdx.x < 16) p.part_ml[slot] = make_float2(top, total);
+    const size_t dst = size_t(v.r0 + qi) * a.out_stride + size_t(h * G + qg) * D;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) total += sh.ml[w][16 * n + col].y * __builtin_amdgcn_exp2f(sh.ml[w][16 * n + col].x - base);
-        const float mine = __builtin_amdgcn_exp2f(m[n] - base) * (Q8 ? vref[n] : 1.0f);
-        const float inv = direct ? (total > 0.0f || total != total ? 1.0f / total : 0.0f) : 1.0f;
-        const int r = 16 * n + col;
-        const bool in = r < nrows;
-        if (!direct && in && threadIdx.x < 16) p.part_ml[slot0 + r] = make_float2(top, total);
+    for (int d0 = 0; d0 < DT; d0 += DG) {
+        if (d0) __syncthreads();
 #pragma unroll
-        for (int d0 = 0; d0 < DT; d0 += DG) {
-            if (n || d0) __syncthreads();
+        for (int d = 0; d < DG; ++d) sh.joined[wid][d][lane] = acc[d0 + d] * mine;
+        __syncthreads();
 #pragma unroll
-            for (int d = 0; d < DG; ++d) sh.joined[wid][d][lane] = acc[n][d0 + d] * mine;
-            __syncthreads();
+        for (int d = wid; d < DG; d += NW) {
+            f4 o = sh.joined[0][d][lane];
 #pragma unroll
-            for (int d = wid; d < DG; d += NW) {
-                f4 o = sh.joined[0][d][lane];
-#pragma unroll
-                for (int w = 1; w < NW; ++w) o += sh.joined[w][d][lane];
-                if (!in) continue;
-                const int first = 16 * (d0 + d) + 4 * c;
-                if (!direct) {
-                    *reinterpret_cast<f4 *>(p.part_o + (slot0 + r) * D + first) = o;
-                    continue;
-                }
-                o *= inv;
-                const int i = token_of(a, row0 + r), g = row0 + r - i * G;
-                put_row(a, size_t(v.r0 + i) * a.out_stride + size_t(h * G + g) * D + size_t(first), o);
-            }
+            for (int w = 1; w < NW; ++w) o += sh.joined[w][d][lane];
+            if (!in) continue;
+            const int at = 16 * (d0 + d) + 4 * c;
+            if (direct) put_row(a, dst + size_t(at), o * inv);
+            else *reinterpret_cast<f4 *>(p.part_o + size_t(slot) * D + at) = o;
         }
     }
     __syncthreads();
 }
-template <int D, int NC, int NW, bool Q8>
-__global__ __launch_bounds__(64 * NW, NC == 4 && D == 128 ? 1 : 2) void attn_split_kernel(SplitArgs p) {
-    constexpr int R = 16 * NC;  // rows of a row tile
-    __shared__ SplitShared<D, NC, NW> sh;
-    __shared__ int upto[kMaxShared + 1], sums[NW];
-    const AttnArgs &a = p.a;
-    const int H = a.b.n_heads, G = a.group;
-    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int worker = int(blockIdx.x);
-
-    Work work{upto, a.b.n_seqs, H, 0, 0, 0, 0};
-    int at = 0, stop = 1;
-    if (p.workers) {  // the units of every sequence, summed
-        constexpr int N = kMaxShared / (64 * NW);  // sequences of a thread
-        int mine[N], sum = 0;
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const int q = int(threadIdx.x) * N + j;
-            mine[j] = 0;
-            if (q < a.b.n_seqs) {
-                const SeqView v = seq_view(a.b, q);
-                if (v.n_new >= p.new_min && v.n_new <= p.new_max)
-                    for (int rt = 0; rt * R < v.n_new * G; ++rt) mine[j] += row_tile<R>(a, v, rt).units;
-            }
-            sum += mine[j];
-        }
-        int before = sum;
-#pragma unroll
-        for (int o = 1; o < 64; o *= 2) {
-            const int x = __shfl_up(before, o);
-            before += lane >= o ? x : 0;
-        }
-        if (lane == 63) sums[wid] = before;
-        before -= sum;
-        __syncthreads();
-        int total = 0;
-        for (int w = 0; w < NW; ++w) {
-            if (w < wid) before += sums[w];
-            total += sums[w];
-        }
-        if (threadIdx.x == 0) upto[0] = 0;
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            before += mine[j];
-            upto[threadIdx.x * N + j + 1] = before;
-        }
-        __syncthreads();
-        total = __builtin_amdgcn_readfirstlane(total) * H;
-        work.set(total, min(p.workers, (total + NW - 1) / NW));  // a tile for each wave
-        at = stop = 0;
-        if (worker < work.workers) {
-            at = work.bound(worker);
-            stop = work.bound(worker + 1);
-        }
-        if (threadIdx.x == 0) p.shared[worker].pieces = 0;
-    }
-
-    int next_tile = 0;  // (nothing shared: the head's row tiles in turn)
-    while (at < stop) {
-        // the segment that holds unit `at`, and this worker's piece of it
-        int s, h, rt = 0, off = 0;
-        if (p.workers) {
-            s = __builtin_amdgcn_readfirstlane(work.seq_of(at));
-            const int n = upto[s + 1] - upto[s], u = at - upto[s] * H;
-            h = __builtin_amdgcn_readfirstlane(u / n);
-            off = __builtin_amdgcn_readfirstlane(u - h * n);
-        } else {
-            s = worker / H;
-            h = worker - s * H;
-            rt = next_tile++;
-        }
-        const SeqView v = seq_view(a.b, s);
-        if (!p.workers && (v.n_new < p.new_min || v.n_new > p.new_max || rt * R >= v.n_new * G)) return;
-        RowTile tile = row_tile<R>(a, v, rt);
-        while (off >= tile.units) {
-            off -= tile.units;
-            tile = row_tile<R>(a, v, ++rt);
-        }
-        const int begin = off;
-        int end = tile.units;
-        if (p.workers) {
-            end = min(end, begin + (stop - at));
-            at += end - begin;
-        }
-        const bool direct = end - begin == tile.units;
-        const int slot0 = (worker * 2 + (begin == 0)) * R;
-        if (!direct && begin == 0 && threadIdx.x == 0) {
-            // the worker of the segment's last unit
-            const int last = at - end + tile.units - 1;
-            int w = worker + 1;
-            while (work.bound(w + 1) <= last) ++w;
-            p.shared[worker] = SharedSegment{w - worker + 1, s, h, tile.row0, tile.nrows};
-        }
-        end = min(end, tile.span.n);  // (a span of no tiles)
-        split_piece<D, NC, NW, Q8>(p, sh, v, tile, s, h, begin, end, direct, slot0);
-    }
-}
-
-// Joins a segment's pieces: a workgroup for each row of each worker that has a
-// segment's first tile, its waves' shares of the pieces in turn.
-template <int D>
-__global__ __launch_bounds__(256) void attn_pieces_kernel(SplitArgs p, int R) {
-    __shared__ float part[4][D];
-    __shared__ float2 ml[4];
-    const int w = int(blockIdx.x);
-    const SharedSegment seg = p.shared[w];
-    if (seg.pieces < 2) return;
-    const AttnArgs &a = p.a;
-    const SeqView v = seq_view(a.b, seg.seq);
-    for (int r = int(blockIdx.y); r < seg.rows; r += int(gridDim.y)) {
-        const int row = seg.row0 + r, i = token_of(a, row), g = row - i * a.group;
-        join_row<D>(p, seg.pieces, [&](int k) { return int64_t((w + k) * 2 + (k == 0)) * R + r; }, part, ml,
-                    size_t(v.r0 + i) * a.out_stride + size_t(seg.head * a.group + g) * D);
-    }
-}
-
 // maximum / sum over the two lane halves (lanes l, l ^ 32)
 __device__ inline float halves_max(float v) {
     auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -718,19 +577,13 @@ __device__ inline float halves_sum(float v) {
 // so the weights are the second product's operand as they stand. 16-B pieces of
 // an LDS row are exchanged by an XOR with the row, so that 16 rows' equal pieces
 // lie in 64 different banks.
-template <int D> struct TileShared {
+template <int D> struct TileShared {  // (the buffers first: sh_at below is its LDS address)
     __attribute__((aligned(16))) uint8_t kbuf[2][128 * D];  // 64 keys, as fp16
     __attribute__((aligned(16))) uint8_t vbuf[2][128 * D];
     float ksc[4][64], vsc[2][64], vmax[2][4];               // 8-bit cache: their scales; the largest of each 16 values'
     int wild;                                               // a tile had values that are no numbers, hidden from some row
 };
 
-// the largest of three (a NaN counts for nothing)
-__device__ inline float max3(float a, float b, float c) {
-    float r;
-    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-    return r;
-}
 // lane l's 16 B at src land at LDS byte address lds + 16 l (counted by vmcnt)
 __device__ inline void dma16g(const void *src, uint32_t lds) {
 #pragma clang diagnostic push
@@ -745,9 +598,9 @@ __device__ inline void dma16g(const void *src, uint32_t lds) {
 // values of tile i + 1 are on their way to LDS meanwhile (fp16 straight from
 // memory, the XOR of an LDS row's pieces in the lanes' addresses).
 template <int D, bool Q8>
-__device__ inline __attribute__((always_inline)) void tile_piece(const SplitArgs &p, TileShared<D> &sh, const SeqView &v,
-                                                                 const RowTile &tile, int s, int h, int split, int begin, int end,
-                                                                 bool direct) {
+__device__ inline __attribute__((always_inline)) void tile_piece(const SplitArgs &p, TileShared<D> &sh, uint32_t sh_at, const SeqView &v,
+                                                                 const RowTile &tile, int s, int h, int begin, int end,
+                                                                 bool direct, int slot0) {
     constexpr int KS = D / 16, DB = D / 32;
     constexpr int RK = D * 2;                 // bytes of a key's row in LDS
     constexpr int NL = Q8 ? D / 64 : D / 32;  // 16-B loads of a thread for its keys, and for its values
@@ -798,7 +651,7 @@ __device__ inline __attribute__((always_inline)) void tile_piece(const SplitArgs
 #pragma unroll
             for (int j = 0; j < NL; ++j) {
                 const int r = (64 * j + lane) / (D / 8), ch = (64 * j + lane) % (D / 8);
-                dma16g(src + k_at(r, ch), lds_addr(&sh.kbuf[b][16 * wid * RK + 1024 * j]));
+                dma16g(src + k_at(r, ch), sh_at + uint32_t(b * 128 * D + 16 * wid * RK + 1024 * j));
             }
         }
     };
@@ -820,7 +673,7 @@ __device__ inline __attribute__((always_inline)) void tile_piece(const SplitArgs
                                      (((size_t(id) * H + h) * D + d0) * size_t(P) + slot) * 2 + 16 * (c & 1);
 #pragma unroll
                 for (int j = e; j < NL; j += 2)
-                    dma16g(src + size_t(8 * (j - e) * 2) * P, lds_addr(&sh.vbuf[b][wid * (D / 4) * 128 + 1024 * j]));
+                    dma16g(src + size_t(8 * (j - e) * 2) * P, sh_at + uint32_t((2 + b) * 128 * D + wid * (D / 4) * 128 + 1024 * j));
             }
         }
     };
@@ -925,11 +778,11 @@ __device__ inline __attribute__((always_inline)) void tile_piece(const SplitArgs
         }
         wait_vmcnt<0>();
         __syncthreads();
-        const uint32_t kb0 = key_base(0);
+        const uint32_t kb = key_base(0);
 #pragma unroll
         for (int k = 0; k < KS; ++k)
 #pragma unroll
-            for (int n = 0; n < 2; ++n) sc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(key(kb0, n, k), q[k], sc[n], 0, 0, 0);
+            for (int n = 0; n < 2; ++n) sc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(key(kb, n, k), q[k], sc[n], 0, 0, 0);
     }
     for (int i = begin; i < end; ++i) {
         const int b = (i - begin) & 1;
@@ -947,11 +800,12 @@ __device__ inline __attribute__((always_inline)) void tile_piece(const SplitArgs
         const int t0 = span.at(i) * kTileKeys;
         const uint32_t vb = value_base(b), kb = key_base(1 - b);
         // (8-bit: the scales of the lane's tokens 4x .. 4x + 3 of 32)
-        auto scales4 = [&](const float *of, int x) { return *reinterpret_cast<const f4 *>(of + 16 * (x / 2) + 8 * hh + 4 * (x % 2)); };
+        auto key_scales = [&](int x) { return *reinterpret_cast<const f4 *>(&sh.ksc[(i - begin) & 3][16 * (x / 2) + 8 * hh + 4 * (x % 2)]); };
+        auto value_scales = [&](int x) { return *reinterpret_cast<const f4 *>(&sh.vsc[b][16 * (x / 2) + 8 * hh + 4 * (x % 2)]); };
         if constexpr (Q8) {
 #pragma unroll
             for (int x = 0; x < 8; ++x) {
-                const f4 kx = scales4(sh.ksc[(i - begin) & 3], x);
+                const f4 kx = key_scales(x);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) sc[x / 4][4 * (x % 4) + r] *= kx[r];
             }
@@ -982,7 +836,7 @@ __device__ inline __attribute__((always_inline)) void tile_piece(const SplitArgs
                 big = 0.0f;
 #pragma unroll
                 for (int x = 0; x < 8; ++x) {
-                    const f4 vx = scales4(sh.vsc[b], x);
+                    const f4 vx = value_scales(x);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const float y = fabsf(vx[r]);
@@ -1022,8 +876,8 @@ __device__ inline __attribute__((always_inline)) void tile_piece(const SplitArgs
         for (int u = 0; u < 4; ++u) {
             f4 vx[2];
             if constexpr (Q8) {
-                vx[0] = scales4(sh.vsc[b], 2 * u) * vinv;
-                vx[1] = scales4(sh.vsc[b], 2 * u + 1) * vinv;
+                vx[0] = value_scales(2 * u) * vinv;
+                vx[1] = value_scales(2 * u + 1) * vinv;
             }
 #pragma unroll
             for (int k = u * KS / 4; k < (u + 1) * KS / 4; ++k)
@@ -1090,7 +944,7 @@ __device__ inline __attribute__((always_inline)) void tile_piece(const SplitArgs
     if (col < wrows) {
         const float unit = Q8 ? vref : 1.0f;
         if (!direct) {
-            const size_t slot = (((size_t(s) * H + h) * size_t(p.nsplit) + size_t(split)) * size_t(p.row_tiles)) * 128 + size_t(row);
+            const size_t slot = size_t(slot0 + wr + col);
             if (hh == 0) p.part_ml[slot] = make_float2(m, total);
 #pragma unroll
             for (int d = 0; d < DB; ++d)
@@ -1118,63 +972,180 @@ __device__ inline __attribute__((always_inline)) void tile_piece(const SplitArgs
     }
     __syncthreads();  // (the next row tile's first store)
 }
+// The shared work (or, with no workers, a workgroup for each head of a sequence).
+// R 16: few rows, a wave's tokens its own; R 128: the waves' rows, the tokens in LDS.
+template <int D, int R, int NW, bool Q8>
+__global__ __launch_bounds__(64 * NW, R == 128 && D > 128 ? 1 : 2) void attn_split_kernel(SplitArgs p) {
+    constexpr int kLeast = R == 16 ? NW : 4;  // units of a worker, where all are fewer than the workers could take
+    __shared__ std::conditional_t<R == 16, SplitShared<D, NW>, TileShared<D>> sh;
+    __shared__ int upto[kMaxShared + 1], sums[NW];
+    const AttnArgs &a = p.a;
+    const int H = a.b.n_heads, G = a.group;
+    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int worker = int(blockIdx.x);
+
+    Work work{upto, a.b.n_seqs, H, 0, 0, 0, 0};
+    int at = 0, stop = 1;
+    if (p.workers) {  // the units of every sequence, summed
+        constexpr int N = kMaxShared / (64 * NW);  // sequences of a thread
+        int mine[N], sum = 0;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int q = int(threadIdx.x) * N + j;
+            mine[j] = 0;
+            if (q < a.b.n_seqs) {
+                const SeqView v = seq_view(a.b, q);
+                if (v.n_new >= p.new_min && v.n_new <= p.new_max)
+                    for (int rt = 0; rt * R < v.n_new * G; ++rt) mine[j] += row_tile<R>(a, v, rt).units;
+            }
+            sum += mine[j];
+        }
+        int before = sum;
+#pragma unroll
+        for (int o = 1; o < 64; o *= 2) {
+            const int x = __shfl_up(before, o);
+            before += lane >= o ? x : 0;
+        }
+        if (lane == 63) sums[wid] = before;
+        before -= sum;
+        __syncthreads();
+        int total = 0;
+        for (int w = 0; w < NW; ++w) {
+            if (w < wid) before += sums[w];
+            total += sums[w];
+        }
+        if (threadIdx.x == 0) upto[0] = 0;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            before += mine[j];
+            upto[threadIdx.x * N + j + 1] = before;
+        }
+        __syncthreads();
+        total = __builtin_amdgcn_readfirstlane(total) * H;
+        work.set(total, min(p.workers, (total + kLeast - 1) / kLeast));
+        // workgroups b, b + 8, .. run on one XCD: they are neighbours in the work, and the
+        // row tiles of one head, at the same tokens at one time, meet in that XCD's L2
+        const int per = (work.workers + 7) / 8;
+        worker = int(blockIdx.x % 8) * per + int(blockIdx.x / 8);
+        if (threadIdx.x == 0 && blockIdx.x == 0) p.shared[p.workers].pieces = work.workers;  // (for the join)
+        if (int(blockIdx.x / 8) >= per || worker >= work.workers) return;
+        const int edge = work.bound(worker + (lane & 1));  // (both ends at once)
+        at = __builtin_amdgcn_readlane(edge, 0);
+        stop = __builtin_amdgcn_readlane(edge, 1);
+        if (threadIdx.x == 0) p.shared[worker].pieces = 0;
+    }
+
+    int next_tile = 0;  // (nothing shared: the head's row tiles in turn)
+    while (at < stop) {
+        // the segment that holds unit `at`, and this worker's piece of it
+        int s, h, rt = 0, off = 0;
+        if (p.workers) {
+            s = __builtin_amdgcn_readfirstlane(work.seq_of(at));
+            const int n = upto[s + 1] - upto[s], u = at - upto[s] * H;
+            h = __builtin_amdgcn_readfirstlane(u / n);
+            off = __builtin_amdgcn_readfirstlane(u - h * n);
+        } else {
+            s = worker / H;
+            h = worker - s * H;
+            rt = next_tile++;
+        }
+        const SeqView v = seq_view(a.b, s);
+        if (!p.workers && (v.n_new < p.new_min || v.n_new > p.new_max || rt * R >= v.n_new * G)) return;
+        RowTile tile = row_tile<R>(a, v, rt);
+        while (off >= tile.units) {
+            off -= tile.units;
+            tile = row_tile<R>(a, v, ++rt);
+        }
+        const int begin = off;
+        int end = tile.units;
+        if (p.workers) {
+            end = min(end, begin + (stop - at));
+            at += end - begin;
+        }
+        const bool direct = end - begin == tile.units;
+        const int slot0 = (worker * 2 + (begin == 0)) * R;
+        if (!direct && begin == 0 && wid == 0) {
+            // the workers up to the one of the segment's last unit, 64 borders at a time
+            const int last = at - end + tile.units - 1;
+            int n = 2;
+            for (;; n += 64) {
+                const uint64_t past = __ballot(work.bound(worker + n + lane) > last);
+                if (past) {
+                    n += __builtin_ctzll(past);
+                    break;
+                }
+            }
+            if (lane == 0) p.shared[worker] = SharedSegment{n, s, h, tile.row0, tile.nrows};
+        }
+        end = min(end, tile.span.n);  // (a span of no tiles)
+        if constexpr (R == 16) split_piece<D, NW, Q8>(p, sh, v, tile, s, h, begin, end, direct, slot0);
+        else tile_piece<D, Q8>(p, sh, lds_addr(&sh), v, tile, s, h, begin, end, direct, slot0);
+    }
+}
+
+// A workgroup for each row tile, nothing shared: a call of many rows.
 template <int D, bool Q8>
-__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile_kernel(SplitArgs p) {
-    constexpr int R = 128;
+__global__ __launch_bounds__(256, D > 128 ? 1 : 2) void attn_tile_kernel(SplitArgs p) {
     __shared__ TileShared<D> sh;
     const AttnArgs &a = p.a;
-    const int H = a.b.n_heads;
-    const int h = int(blockIdx.x) % H, s = int(blockIdx.x) / H, split = int(blockIdx.y);
+    const int h = int(blockIdx.x) % a.b.n_heads, s = int(blockIdx.x) / a.b.n_heads;
     const SeqView v = seq_view(a.b, s);
     if (v.n_new < p.new_min || v.n_new > p.new_max) return;
     // the last row tiles see most: they go first
-    for (int rt = int(gridDim.z) - 1 - int(blockIdx.z); rt * R < v.n_new * a.group; rt += int(gridDim.z)) {
-        const RowTile tile = row_tile<R>(a, v, rt);
-        // (a row tile past what the host said has no place for partial results: one split takes it whole)
-        const int n = tile.span.n, per = rt < p.row_tiles ? split_tiles(n, p.nsplit, p.chunk) : n;
-        const int begin = split * per, end = min(begin + per, n);
-        if (begin >= end && split > 0) continue;
-        tile_piece<D, Q8>(p, sh, v, tile, s, h, split, begin, end, per >= n);
+    for (int rt = int(gridDim.y) - 1 - int(blockIdx.y); rt * 128 < v.n_new * a.group; rt += int(gridDim.y)) {
+        const RowTile tile = row_tile<128>(a, v, rt);
+        tile_piece<D, Q8>(p, sh, lds_addr(&sh), v, tile, s, h, 0, tile.span.n, true, 0);
     }
 }
 
-// Joins the tile kernel's splits: a workgroup for each row of a head.
-template <int D>
-__global__ __launch_bounds__(256) void attn_join_kernel(SplitArgs p) {
-    constexpr int R = 128;
-    __shared__ float part[4][D];
-    __shared__ float2 ml[4];
+// Joins a segment's pieces, for each worker that has a segment's first tile: a
+// workgroup a row (R 16: few rows, perhaps of many pieces), or a wave a row.
+template <int D, int R>
+__global__ __launch_bounds__(64 * kJoinWaves) void attn_pieces_kernel(SplitArgs p) {
+    __shared__ float part[R == 16 ? kJoinWaves : 1][D];
+    __shared__ float2 ml[kJoinWaves];
+    const int w = int(blockIdx.y);  // (rows across the XCDs: owners may be 8 workers apart)
+    if (w >= p.shared[p.workers].pieces) return;
+    const SharedSegment seg = p.shared[w];
+    if (seg.pieces < 2) return;
     const AttnArgs &a = p.a;
-    const int H = a.b.n_heads, G = a.group;
-    const int h = int(blockIdx.x) % H, s = int(blockIdx.x) / H;
-    const SeqView v = seq_view(a.b, s);
-    if (v.n_new < p.new_min || v.n_new > p.new_max) return;
-    const int cap = p.row_tiles * R, rows = min(v.n_new * G, cap);
-    for (int row = int(blockIdx.y); row < rows; row += int(gridDim.y)) {
-        const TileSpan span = row_tile<128>(a, v, row / 128).span;
-        const int per = split_tiles(span.n, p.nsplit, p.chunk);
-        if (per >= span.n) continue;  // (the tile kernel wrote the row itself)
-        const int64_t slot0 = (int64_t(s) * H + h) * p.nsplit * cap + row;
-        const int i = token_of(a, row);
-        join_row<D>(p, (span.n + per - 1) / per, [&](int k) { return slot0 + int64_t(k) * cap; }, part, ml,
-                    size_t(v.r0 + i) * a.out_stride + size_t(h * G + row - i * G) * D);
+    const SeqView v = seq_view(a.b, seg.seq);
+    auto slot = [&](int k, int r) { return int64_t((w + k) * 2 + (k == 0)) * R + r; };
+    auto place = [&](int r) {
+        const int row = seg.row0 + r, i = token_of(a, row), g = row - i * a.group;
+        return size_t(v.r0 + i) * a.out_stride + size_t(seg.head * a.group + g) * D;
+    };
+    if constexpr (R == 16) {
+        for (int r = int(blockIdx.x); r < seg.rows; r += int(gridDim.x))
+            join_row<D>(p, seg.pieces, [&](int k) { return slot(k, r); }, part, ml, place(r));
+    } else {
+        constexpr int N = D / 64;
+        const int lane = threadIdx.x & 63;
+        for (int r = kJoinWaves * int(blockIdx.x) + int(threadIdx.x >> 6); r < seg.rows; r += kJoinWaves * int(gridDim.x)) {
+            float o[N], m, l;
+            join_pieces<D>(p, 0, 1, seg.pieces, [&](int k) { return slot(k, r); }, o, m, l);
+            const size_t dst = place(r);
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const _Float16 y = _Float16(l > 0.0f || l != l ? o[j] / l : 0.0f);
+                if (a.out_f32) static_cast<float *>(a.out)[dst + 64 * j + lane] = float(y);
+                else static_cast<_Float16 *>(a.out)[dst + 64 * j + lane] = y;
+            }
+        }
     }
 }
 
-// How a call's sequences are launched: those of up to `few` new tokens (64 rows)
-// by the split kernel, longer ones by the tile kernel.
+// How sequences of a call are launched.
 struct SplitPlan {
-    bool tiles;              // the tile kernel
-    int nc, nw, workers;     // split kernel: columns / 16, waves, workers (0: none share)
-    int row_tiles, nsplit, chunk;
+    int rows;      // of a row tile: 16 or 128
+    int workers;   // that share all tiles (0: a workgroup for each head, or with 128 rows each row tile)
+    int nw;        // waves, with 16 rows
+    int row_tiles;
     int new_min, new_max;
-    size_t slots, bytes;     // partial rows; all of the scratch
+    size_t slots, bytes;  // partial rows; all of the scratch
 };
 
-int few_tokens(const AttnArgs &a) {
-    const int most = a.head_dim > 128 ? 16 : 64;
-    return a.group > most ? 1 : most / a.group;
-}
+int few_tokens(const AttnArgs &a) { return a.group > 16 ? 1 : 16 / a.group; }
 
 // tiles of a row tile of R rows, as the host knows it
 int64_t hinted_tiles(const AttnArgs &a, int R) {
@@ -1190,97 +1161,64 @@ constexpr int kShortTiles = 32;  // up to so many a head of a sequence is one wo
 SplitPlan plan_split(const AttnArgs &a, int max_new, int cu_count, size_t scratch) {
     SplitPlan p{};
     const int64_t rows = int64_t(max_new) * a.group;
-    p.nc = rows <= 16 || a.head_dim > 128 ? 1 : rows <= 32 ? 2 : 4;
-    p.nw = 4;
-    const int R = 16 * p.nc;
-    const int64_t tiles = hinted_tiles(a, R), units = int64_t(a.b.n_seqs) * a.b.n_heads;
+    const int R = p.rows = max_new <= few_tokens(a) ? 16 : 128;
+    const int64_t tiles = hinted_tiles(a, R), units = int64_t(a.b.n_seqs) * a.b.n_heads, row_tiles = (rows + R - 1) / R;
+    const int per_cu = R == 128 && a.head_dim > 128 ? 1 : 2;  // workgroups a CU holds
     const size_t each = 2 * size_t(R) * (size_t(a.head_dim) * 4 + 8) + sizeof(SharedSegment);
-    int64_t workers = std::min(cu_count, 512) * int64_t(p.nc == 1 && a.head_dim <= 128 ? 2 : 1);
-    if (size_t(workers) > scratch / each) workers = int64_t(scratch / each);
+    int64_t workers = std::min(cu_count, 512) * int64_t(per_cu);
+    if (size_t(workers) * each + sizeof(SharedSegment) > scratch) workers = int64_t(scratch / each) - 1;
     // (units of the shared work: all that the tensors can hold)
     const int64_t bound = (int64_t(a.b.n_rows) * a.group / R + a.b.n_seqs) * a.b.n_heads *
                           (kv_capacity(a.b.max_pages, a.b.page_shift) / kTileKeys + 1);
-    if (tiles <= kShortTiles || a.b.n_seqs > kMaxShared || workers <= units / 4 || bound >= (int64_t(1) << 31)) {
-        p.nw = p.nc == 1 && a.head_dim <= 128 && units <= 2 * cu_count && tiles > 4 ? 8 : 4;
-    } else {
+    const bool few_tiles = R == 16 ? tiles <= kShortTiles : units * row_tiles >= 2 * per_cu * cu_count || tiles <= 8;
+    p.new_max = 0x7fffffff;
+    if (!few_tiles && a.b.n_seqs <= kMaxShared && workers > units / 4 && bound < (int64_t(1) << 31)) {
         p.workers = int(workers);
         p.slots = size_t(workers) * 2 * R;
-        p.bytes = size_t(workers) * each;
+        p.bytes = size_t(workers) * each + sizeof(SharedSegment);
     }
-    p.new_max = 0x7fffffff;
-    return p;
-}
-
-SplitPlan plan_tiles(const AttnArgs &a, int cu_count, size_t scratch) {
-    SplitPlan p{};
-    constexpr int R = 128;
-    p.tiles = true;
-    const int64_t rows = int64_t(a.max_new) * a.group, rt = (rows + R - 1) / R;
-    p.row_tiles = int(rt < 65535 ? rt : 65535);
-    const int64_t tiles = hinted_tiles(a, R), units = int64_t(a.b.n_seqs) * a.b.n_heads * p.row_tiles;
-    int64_t n = (int64_t(cu_count) * 2 + units - 1) / units;
-    if (n > (tiles + 8 - 1) / 8) n = (tiles + 8 - 1) / 8;
-    const size_t slot = size_t(a.b.n_seqs) * a.b.n_heads * p.row_tiles * R, slot_bytes = slot * (size_t(a.head_dim) * 4 + 8);
-    if (n > 1 && size_t(n) > scratch / slot_bytes) n = int64_t(scratch / slot_bytes);
-    if (n < 1) n = 1;
-    p.chunk = int((tiles + n - 1) / n);
-    p.nsplit = int((tiles + p.chunk - 1) / p.chunk);
-    p.slots = slot * size_t(p.nsplit);
-    p.bytes = p.nsplit > 1 ? slot_bytes * size_t(p.nsplit) : 0;
-    p.new_max = 0x7fffffff;
+    p.nw = R == 16 && !p.workers && a.head_dim <= 128 && units <= 2 * cu_count && tiles > 4 ? 8 : 4;
+    p.row_tiles = int(std::min<int64_t>(row_tiles, 65535));
     return p;
 }
 
 // one or two plans; the number of them
 int plan_call(const AttnArgs &a, int cu_count, size_t scratch, SplitPlan out[2]) {
     const int few = few_tokens(a);
-    if (a.max_new <= few) {
-        out[0] = plan_split(a, a.max_new, cu_count, scratch);
-        return 1;
-    }
-    out[0] = plan_tiles(a, cu_count, scratch);
-    // one sequence, or all of the same many rows: nothing is left for the split kernel
-    if (a.b.n_seqs == 1 || int64_t(a.b.n_seqs) * a.max_new <= a.b.n_rows) return 1;
+    out[0] = plan_split(a, a.max_new, cu_count, scratch);
+    // one row tile at most; one sequence, or all of the same many rows: nothing is left for another kernel
+    if (int64_t(a.max_new) * a.group <= 128 || a.b.n_seqs == 1 || int64_t(a.b.n_seqs) * a.max_new <= a.b.n_rows) return 1;
     out[0].new_min = few + 1;
     out[1] = plan_split(a, few, cu_count, scratch - out[0].bytes);
     out[1].new_max = few;
     return 2;
 }
 
-template <int D, int NC, int NW> void launch_split(const SplitArgs &p, unsigned grid, hipStream_t s) {
-    if (p.a.ks) hipLaunchKernelGGL((attn_split_kernel<D, NC, NW, true>), dim3(grid), dim3(64 * NW), 0, s, p);
-    else hipLaunchKernelGGL((attn_split_kernel<D, NC, NW, false>), dim3(grid), dim3(64 * NW), 0, s, p);
+template <int D, int R, int NW> void launch_split(const SplitArgs &p, dim3 grid, hipStream_t s) {
+    if (p.a.ks) hipLaunchKernelGGL((attn_split_kernel<D, R, NW, true>), grid, dim3(64 * NW), 0, s, p);
+    else hipLaunchKernelGGL((attn_split_kernel<D, R, NW, false>), grid, dim3(64 * NW), 0, s, p);
 }
 
 template <int D> hipError_t launch_plan(SplitArgs &p, const SplitPlan &pl, hipStream_t s) {
     const AttnArgs &a = p.a;
     const unsigned units = unsigned(a.b.n_seqs) * unsigned(a.b.n_heads);
-    if (pl.tiles) {
-        const dim3 grid(units, unsigned(pl.nsplit), unsigned(pl.row_tiles));
-        if (a.ks) hipLaunchKernelGGL((attn_tile_kernel<D, true>), grid, dim3(256), 0, s, p);
-        else hipLaunchKernelGGL((attn_tile_kernel<D, false>), grid, dim3(256), 0, s, p);
-        const hipError_t e = hipGetLastError();
-        if (e != hipSuccess || pl.nsplit == 1) return e;
-        const int64_t rows = int64_t(a.max_new) * a.group;
-        hipLaunchKernelGGL(attn_join_kernel<D>, dim3(units, unsigned(rows < 65535 ? rows : 65535)), dim3(256), 0, s, p);
-        return hipGetLastError();
-    }
-    const unsigned grid = pl.workers ? unsigned(pl.workers) : units;
-    if (pl.nc == 1) {
-        if constexpr (D <= 128) {
-            if (pl.nw == 8) launch_split<D, 1, 8>(p, grid, s);
-            else launch_split<D, 1, 4>(p, grid, s);
-        } else {
-            launch_split<D, 1, 4>(p, grid, s);
-        }
+    const dim3 grid(pl.workers ? unsigned(pl.workers) : units);
+    if (pl.rows == 128) {
+        const dim3 tiles(units, unsigned(pl.row_tiles));
+        if (pl.workers) launch_split<D, 128, 4>(p, grid, s);
+        else if (a.ks) hipLaunchKernelGGL((attn_tile_kernel<D, true>), tiles, dim3(256), 0, s, p);
+        else hipLaunchKernelGGL((attn_tile_kernel<D, false>), tiles, dim3(256), 0, s, p);
     } else if constexpr (D <= 128) {
-        if (pl.nc == 2) launch_split<D, 2, 4>(p, grid, s);
-        else launch_split<D, 4, 4>(p, grid, s);
+        if (pl.nw == 8) launch_split<D, 16, 8>(p, grid, s);
+        else launch_split<D, 16, 4>(p, grid, s);
+    } else {
+        launch_split<D, 16, 4>(p, grid, s);
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || !pl.workers) return e;
-    const int64_t rows = int64_t(a.max_new) * a.group, R = 16 * pl.nc;
-    hipLaunchKernelGGL(attn_pieces_kernel<D>, dim3(grid, unsigned(rows < R ? rows : R)), dim3(256), 0, s, p, int(R));
+    const int64_t rows = std::min<int64_t>(int64_t(a.max_new) * a.group, pl.rows);
+    if (pl.rows == 16) hipLaunchKernelGGL((attn_pieces_kernel<D, 16>), dim3(unsigned(rows), grid.x), dim3(64 * kJoinWaves), 0, s, p);
+    else hipLaunchKernelGGL((attn_pieces_kernel<D, 128>), dim3(unsigned((rows + kJoinWaves - 1) / kJoinWaves), grid.x), dim3(64 * kJoinWaves), 0, s, p);
     return hipGetLastError();
 }
 
@@ -1304,9 +1242,6 @@ hipError_t launch_attention(const AttnArgs &a, void *scratch, size_t scratch_byt
         p.sl2 = a.scale * 1.44269504088896341f;
         p.new_min = pl.new_min;
         p.new_max = pl.new_max;
-        p.nsplit = pl.nsplit;
-        p.chunk = pl.chunk;
-        p.row_tiles = pl.row_tiles;
         p.workers = pl.workers;
         if (pl.bytes) {
             p.part_o = reinterpret_cast<float *>(base);

@@ -13,7 +13,7 @@ using namespace qmm;
 static int bad = 0;
 #define EXPECT(c, ...) do { if (!(c)) { ++bad; std::printf("%s: ", #c); std::printf(__VA_ARGS__); std::printf("\n"); } } while (0)
 
-// every token some row of pmin..pmax sees is in exactly one tile of the span, and each split's tiles together are the span
+// every token some row of pmin..pmax sees is in exactly one tile of the span
 static void spans() {
     for (int pmin = -3; pmin < 300; pmin += 7)
         for (int rows : {1, 2, 16, 70})
@@ -33,11 +33,6 @@ static void spans() {
                         if (seen) EXPECT(hit[j / 64] == 1, "token %d rows %d..%d window %d/%d: %d tiles", j, pmin, pmax, window, sinks, hit[j / 64]);
                     }
                     for (int k = 0; k < 16; ++k) EXPECT(hit[k] <= 1, "tile %d twice", k);
-                    for (int nsplit : {1, 2, 3, 7, 100})
-                        for (int chunk : {1, 2, 5, 50}) {
-                            const int per = split_tiles(t.n, nsplit, chunk);
-                            EXPECT(per >= 1 && int64_t(per) * nsplit >= t.n, "per %d of %d", per, t.n);
-                        }
                 }
 }
 
