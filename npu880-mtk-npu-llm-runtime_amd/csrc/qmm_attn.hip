@@ -1023,12 +1023,15 @@ __global__ __launch_bounds__(64 * NW, R == 128 && D > 128 ? 1 : 2) void attn_spl
         __syncthreads();
         total = __builtin_amdgcn_readfirstlane(total) * H;
         work.set(total, min(p.workers, (total + kLeast - 1) / kLeast));
-        // workgroups b, b + 8, .. run on one XCD: they are neighbours in the work, and the
-        // row tiles of one head, at the same tokens at one time, meet in that XCD's L2
-        const int per = (work.workers + 7) / 8;
-        worker = int(blockIdx.x % 8) * per + int(blockIdx.x / 8);
         if (threadIdx.x == 0 && blockIdx.x == 0) p.shared[p.workers].pieces = work.workers;  // (for the join)
-        if (int(blockIdx.x / 8) >= per || worker >= work.workers) return;
+        if constexpr (R == 128) {
+            // workgroups b, b + 8, .. run on one XCD: they are neighbours in the work, and the
+            // row tiles of one head, at the same tokens at one time, meet in that XCD's L2
+            const int per = (work.workers + 7) / 8;
+            if (int(blockIdx.x / 8) >= per) return;
+            worker = int(blockIdx.x % 8) * per + int(blockIdx.x / 8);
+        }
+        if (worker >= work.workers) return;
         const int edge = work.bound(worker + (lane & 1));  // (both ends at once)
         at = __builtin_amdgcn_readlane(edge, 0);
         stop = __builtin_amdgcn_readlane(edge, 1);
