@@ -353,10 +353,12 @@ typedef struct {
     float scale;              /* 0 means 1 */
 } qmm_rope_params;
 typedef struct qmm_rope qmm_rope;
-/* One rotation, kept by the program: host memory, passed to the kernels by
- * value, so it may serve any context and be destroyed after the calls (and
- * captures) that use it return. */
+/* The device table of one rotation; kept by the program, used by any stream and
+ * graph of the context's device. Not during a capture. */
 int qmm_rope_create(qmm_context *ctx, const qmm_rope_params *params, qmm_rope **out);
+/* Calls on the context's stream are waited for; memory that a living graph may
+ * hold is kept until the last graph is destroyed. Calls that run on another
+ * stream must have ended. */
 int qmm_rope_destroy(qmm_context *ctx, qmm_rope *rope);
 
 /* The rows of one append: fp32 projections, each with its own row stride (in
@@ -412,9 +414,7 @@ typedef struct qmm_attn_workspace qmm_attn_workspace;
 size_t qmm_attention_workspace_bytes(qmm_context *ctx, const qmm_kv_batch *batch, const qmm_kv_cache *cache,
                                      const qmm_attention_args *args);
 int qmm_attention_workspace_create(qmm_context *ctx, size_t bytes, qmm_attn_workspace **out);
-/* Calls on the context's stream are waited for; memory that a living graph may
- * hold is kept until the last graph is destroyed. Calls that run on another
- * stream must have ended. */
+/* (as qmm_rope_destroy) */
 int qmm_attention_workspace_destroy(qmm_context *ctx, qmm_attn_workspace *ws);
 /* ws may be NULL: no split. */
 int qmm_paged_attention(qmm_context *ctx, const qmm_kv_batch *batch, const qmm_kv_cache *cache,

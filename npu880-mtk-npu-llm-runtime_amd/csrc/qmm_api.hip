@@ -63,11 +63,11 @@ struct qmm_context {
     std::string err;
 };
 
-// What a program keeps: a rotation (host only, passed to kernels by value), and
-// device scratch.
+// What a program keeps: rotations and attention scratch, on the context's device.
 struct qmm_rope {
-    int n_axes = 0;
-    qmm::RopeTable table{};
+    int device = 0, rot_dim = 0, style = 0, n_axes = 0;
+    float scale = 1.0f;
+    qmm::RopeTable *table = nullptr;
 };
 struct qmm_attn_workspace {
     int device = 0;
@@ -900,16 +900,35 @@ int qmm_rope_create(qmm_context *ctx, const qmm_rope_params *t, qmm_rope **out) 
     *out = nullptr;
     const qmm::Refusal no = qmm::check_rope(t);
     if (no.code) return refuse(ctx, no);
-    qmm_rope *r = new (std::nothrow) qmm_rope();
-    if (!r) return fail(ctx, QMM_ENOMEM, "out of host memory");
-    r->n_axes = t->n_axes;
-    r->table.rot_dim = t->rot_dim;
-    r->table.style = t->style;
-    r->table.scale = t->scale == 0.0f ? 1.0f : t->scale;
+    if (ctx->capturing) return fail(ctx, QMM_EINVAL, "no rotation can be made during graph capture");
+    qmm::RopeTable table{};
     for (int j = 0; j < t->rot_dim / 2; ++j) {
         const double f = t->pair_freq ? t->pair_freq[j] : std::pow(t->base, -2.0 * j / t->rot_dim);
-        r->table.turns[j] = f / 6.283185307179586476925286766559;
-        r->table.axis[j] = t->pair_axis ? t->pair_axis[j] : 0;
+        table.turns[j] = f / 6.283185307179586476925286766559;
+        table.axis[j] = t->pair_axis ? t->pair_axis[j] : 0;
+    }
+    int rc = use_device(ctx);
+    if (rc) return rc;
+    qmm_rope *r = new (std::nothrow) qmm_rope();
+    if (!r) return fail(ctx, QMM_ENOMEM, "out of host memory");
+    void *p = nullptr;
+    if (hipMalloc(&p, sizeof table) != hipSuccess) {
+        (void)hipGetLastError();
+        delete r;
+        return fail(ctx, QMM_ENOMEM, "hipMalloc of a rotation failed");
+    }
+    r->device = ctx->device;
+    r->rot_dim = t->rot_dim;
+    r->style = t->style;
+    r->n_axes = t->n_axes;
+    r->scale = t->scale == 0.0f ? 1.0f : t->scale;
+    r->table = static_cast<qmm::RopeTable *>(p);
+    hipError_t e = qmm::launch_rope_table(table, r->table, ctx->stream);
+    if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);  // (any stream may use it)
+    if (e != hipSuccess) {
+        (void)hipFree(p);
+        delete r;
+        return hip_fail(ctx, e, "rotation upload");
     }
     *out = r;
     return QMM_OK;
@@ -917,14 +936,19 @@ int qmm_rope_create(qmm_context *ctx, const qmm_rope_params *t, qmm_rope **out) 
 
 int qmm_rope_destroy(qmm_context *ctx, qmm_rope *rope) {
     if (!ctx || !rope) return fail(ctx, QMM_EINVAL, "bad rope_destroy arguments");
+    if (rope->device != ctx->device) return fail(ctx, QMM_EINVAL, "rotation of another device");
+    int rc = use_device(ctx);
+    if (rc) return rc;
+    void *p = rope->table;
     delete rope;
-    return QMM_OK;
+    return give_up(ctx, p);
 }
 
 int qmm_kv_append(qmm_context *ctx, const qmm_kv_batch *batch, const qmm_kv_cache *cache, const qmm_kv_rows *t) {
     if (!ctx) return QMM_EINVAL;
-    const qmm::Refusal no = qmm::check_append(batch, cache, t, t && t->rope ? t->rope->table.rot_dim : 0);
+    const qmm::Refusal no = qmm::check_append(batch, cache, t, t && t->rope ? t->rope->rot_dim : 0);
     if (no.code) return refuse(ctx, no);
+    if (t->rope && t->rope->device != ctx->device) return fail(ctx, QMM_EINVAL, "rotation of another device");
     if (batch->n_rows == 0 || batch->n_seqs == 0) return QMM_OK;
     qmm::AppendArgs a{};
     int max_kv = 0;
@@ -942,6 +966,9 @@ int qmm_kv_append(qmm_context *ctx, const qmm_kv_batch *batch, const qmm_kv_cach
     a.eps = t->eps;
     if (t->rope) {
         a.rope = t->rope->table;
+        a.rot_dim = t->rope->rot_dim;
+        a.style = t->rope->style;
+        a.rope_scale = t->rope->scale;
         a.pos = t->pos;
         a.pos_stride = t->pos_stride;
     }

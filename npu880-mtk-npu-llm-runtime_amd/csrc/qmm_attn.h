@@ -76,14 +76,13 @@ QMM_HD inline int page_of(const KvView &b, int s, int token, int len) {
 #ifdef __HIPCC__
 namespace qmm {
 
-// A rotation, passed by value: each pair's turns (not radians) per position, and
-// its position axis.
+// A rotation: each pair's turns (not radians) per position, and its position axis.
 struct RopeTable {
-    int rot_dim, style;  // rot_dim 0: none
-    float scale;
     double turns[128];
-    uint8_t axis[128];
+    int32_t axis[128];
 };
+// writes it to device memory (by a kernel: nothing is copied from the host's stack later)
+hipError_t launch_rope_table(const RopeTable &t, RopeTable *dst, hipStream_t s);
 
 struct AppendArgs {
     KvView b;
@@ -92,7 +91,9 @@ struct AppendArgs {
     int q_heads, head_dim;
     const float *q_gamma, *k_gamma;
     float eps;
-    RopeTable rope;
+    const RopeTable *rope;  // device; nullptr: no rotation
+    int rot_dim, style;
+    float rope_scale;
     const int32_t *pos;
     size_t pos_stride;
     uint16_t *q_out;

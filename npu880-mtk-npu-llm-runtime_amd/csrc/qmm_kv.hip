@@ -43,85 +43,107 @@ __device__ inline float abs_max4(float4 x) {
 }
 __device__ inline int code8(float x, float inv) { return int(fminf(fmaxf(rintf(x * inv), -127.0f), 127.0f)); }
 
-// one row's queries and keys; job j of nj takes its share of the head groups
+// One row's queries and keys: workgroup `job` of `njobs` takes its share of the head
+// groups, a wave HPW heads at a time. A wave's loads are all under way before it
+// looks for the row's sequence, its page and its angles.
 template <int D>
-__device__ inline void append_qk(const AppendArgs &a, int m, int job, int njobs, float2 *cs, int *found) {
-    constexpr int LPH = D / 4, HPW = 64 / LPH;  // lanes per head, heads per wave
+__device__ inline void append_qk(const AppendArgs &a, int m, int job, int njobs, float2 *cs) {
+    constexpr int LPH = D / 4, HPW = 64 / LPH, NI = 5;  // lanes per head, heads per wave, groups at a time
     const int t = threadIdx.x, lane = t & 63, wid = t >> 6;
+    const int H = a.b.n_heads, HQ = a.q ? a.q_heads : 0, heads = HQ + H;
+    const int e = 4 * (lane % LPH), step = njobs * 4;  // this lane's first value of its head
+    float4 x[NI];
+    auto load = [&](int g0) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const int head = (g0 + i * step) * HPW + lane / LPH;
+            x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (head < heads)
+                x[i] = head < HQ ? *reinterpret_cast<const float4 *>(a.q + size_t(m) * a.q_stride + size_t(head) * D + e)
+                                 : *reinterpret_cast<const float4 *>(a.k + size_t(m) * a.k_stride + size_t(head - HQ) * D + e);
+        }
+    };
+    const int g_first = job * 4 + wid;
+    load(g_first);
     // the sequence that holds row m (the last one where the starts are not ascending)
-    if (t == 0) *found = -1;
-    __syncthreads();
-    for (int s = t; s < a.b.n_seqs; s += 256)
-        if (a.b.row_start[s] <= m && m < a.b.row_start[s + 1]) atomicMax(found, s);
-    __syncthreads();
-    const int s = *found;
-    if (s < 0) return;
+    int s = -1;
+    for (int s0 = 0; s0 < a.b.n_seqs; s0 += 64) {
+        const int q = s0 + lane;
+        const bool in = q < a.b.n_seqs && a.b.row_start[q] <= m && m < a.b.row_start[q + 1];
+        const uint64_t found = __ballot(in);
+        if (found) s = s0 + 63 - __builtin_clzll(found);
+    }
+    if (s < 0) return;  // (all waves alike)
     const SeqView v = seq_view(a.b, s);
     const int place = v.pos0 + (m - v.r0);
-    const int rot = a.rope.rot_dim, half = rot / 2;
+    const int rot = a.rope ? a.rot_dim : 0, half = rot / 2;
     if (rot) {
         if (t < half) {
-            const int pos = a.pos ? a.pos[size_t(a.rope.axis[t]) * a.pos_stride + size_t(m)] : place;
-            const double turns = double(pos) * a.rope.turns[t];
+            const int pos = a.pos ? a.pos[size_t(a.rope->axis[t]) * a.pos_stride + size_t(m)] : place;
+            const double turns = double(pos) * a.rope->turns[t];
             float sn, co;
             sincospif(2.0f * float(turns - rint(turns)), &sn, &co);
-            cs[t] = make_float2(co * a.rope.scale, sn * a.rope.scale);
+            cs[t] = make_float2(co * a.rope_scale, sn * a.rope_scale);
         }
         __syncthreads();
     }
     const int page = page_of(a.b, s, place, v.len);
     const int slot = place & ((1 << a.b.page_shift) - 1);
-    const int H = a.b.n_heads, HQ = a.q ? a.q_heads : 0, heads = HQ + H;
-    const int e = 4 * (lane % LPH);  // this lane's first value of its head
-    const bool turned = e < rot, half_style = a.rope.style == 0;
-    const bool first = e < half;
+    const bool turned = e < rot, half_style = a.style == 0, first = e < half;
     const int other = (lane & ~(LPH - 1)) + (half_style && turned ? (first ? e + half : e - half) / 4 : lane % LPH);
-    for (int g = job * 4 + wid; g * HPW < heads; g += njobs * 4) {
-        const int head = g * HPW + lane / LPH;
-        const bool on = head < heads, is_q = head < HQ;
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (on)
-            x = is_q ? *reinterpret_cast<const float4 *>(a.q + size_t(m) * a.q_stride + size_t(head) * D + e)
-                     : *reinterpret_cast<const float4 *>(a.k + size_t(m) * a.k_stride + size_t(head - HQ) * D + e);
-        const float *gamma = is_q ? a.q_gamma : a.k_gamma;
-        const float ss = head_sum<LPH>(x.x * x.x + x.y * x.y + (x.z * x.z + x.w * x.w));
-        if (gamma) {
-            const float r = 1.0f / sqrtf(ss / float(D) + a.eps);
-            const float4 w = *reinterpret_cast<const float4 *>(gamma + e);
-            x = make_float4(x.x * r * w.x, x.y * r * w.y, x.z * r * w.z, x.w * r * w.w);
-        }
-        if (rot) {
-            if (half_style) {
-                const float4 y = make_float4(__shfl(x.x, other), __shfl(x.y, other), __shfl(x.z, other), __shfl(x.w, other));
-                if (turned) {
-                    const float2 *c = cs + (first ? e : e - half);
-                    const float sg = first ? -1.0f : 1.0f;
-                    x = make_float4(x.x * c[0].x + sg * (y.x * c[0].y), x.y * c[1].x + sg * (y.y * c[1].y),
-                                    x.z * c[2].x + sg * (y.z * c[2].y), x.w * c[3].x + sg * (y.w * c[3].y));
+    float2 c[4];  // this lane's cosines and sines (two of them in PAIRS style)
+    if (turned) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c[j] = half_style ? cs[(first ? e : e - half) + j] : cs[e / 2 + (j & 1)];
+    }
+    const float sg = first ? -1.0f : 1.0f;
+    for (int g0 = g_first;;) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const int g = g0 + i * step;
+            if (g * HPW >= heads) break;  // (the same for the wave)
+            const int head = g * HPW + lane / LPH;
+            const bool is_q = head < HQ;
+            float4 y = x[i];
+            const float *gamma = is_q ? a.q_gamma : a.k_gamma;
+            const float ss = head_sum<LPH>(y.x * y.x + y.y * y.y + (y.z * y.z + y.w * y.w));
+            if (gamma) {
+                const float r = 1.0f / sqrtf(ss / float(D) + a.eps);
+                const float4 w = *reinterpret_cast<const float4 *>(gamma + e);
+                y = make_float4(y.x * r * w.x, y.y * r * w.y, y.z * r * w.z, y.w * r * w.w);
+            }
+            if (rot) {
+                if (half_style) {
+                    const float4 z = make_float4(__shfl(y.x, other), __shfl(y.y, other), __shfl(y.z, other), __shfl(y.w, other));
+                    if (turned)
+                        y = make_float4(y.x * c[0].x + sg * (z.x * c[0].y), y.y * c[1].x + sg * (z.y * c[1].y),
+                                        y.z * c[2].x + sg * (z.z * c[2].y), y.w * c[3].x + sg * (z.w * c[3].y));
+                } else if (turned) {
+                    y = make_float4(y.x * c[0].x - y.y * c[0].y, y.y * c[0].x + y.x * c[0].y, y.z * c[1].x - y.w * c[1].y,
+                                    y.w * c[1].x + y.z * c[1].y);
                 }
-            } else if (turned) {
-                const float2 c0 = cs[e / 2], c1 = cs[e / 2 + 1];
-                x = make_float4(x.x * c0.x - x.y * c0.y, x.y * c0.x + x.x * c0.y, x.z * c1.x - x.w * c1.y,
-                                x.w * c1.x + x.z * c1.y);
+            }
+            const float am = a.ks ? head_max<LPH>(abs_max4(y)) : 0.0f;
+            if (head >= heads) continue;
+            const h4 r = {_Float16(y.x), _Float16(y.y), _Float16(y.z), _Float16(y.w)};
+            if (is_q) {
+                *reinterpret_cast<h4 *>(a.q_out + size_t(m) * a.q_out_stride + size_t(head) * D + e) = r;
+            } else if (page >= 0) {
+                const size_t cell = ((size_t(page) * H + size_t(head - HQ)) << a.b.page_shift) + size_t(slot);
+                if (!a.ks) {
+                    *reinterpret_cast<h4 *>(static_cast<uint16_t *>(a.kc) + cell * D + e) = r;
+                } else {
+                    const float inv = am < kZeroAmax ? 0.0f : 127.0f / am;
+                    const uint32_t w = (code8(y.x, inv) & 255) | (code8(y.y, inv) & 255) << 8 | (code8(y.z, inv) & 255) << 16 |
+                                       uint32_t(code8(y.w, inv)) << 24;
+                    *reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(a.kc) + cell * D + e) = w;
+                    if (e == 0) a.ks[cell] = am < kZeroAmax ? 0.0f : am / 127.0f;
+                }
             }
         }
-        const float am = a.ks ? head_max<LPH>(abs_max4(x)) : 0.0f;
-        if (!on) continue;
-        const h4 y = {_Float16(x.x), _Float16(x.y), _Float16(x.z), _Float16(x.w)};
-        if (is_q) {
-            *reinterpret_cast<h4 *>(a.q_out + size_t(m) * a.q_out_stride + size_t(head) * D + e) = y;
-        } else if (page >= 0) {
-            const size_t cell = ((size_t(page) * H + size_t(head - HQ)) << a.b.page_shift) + size_t(slot);
-            if (!a.ks) {
-                *reinterpret_cast<h4 *>(static_cast<uint16_t *>(a.kc) + cell * D + e) = y;
-            } else {
-                const float inv = am < kZeroAmax ? 0.0f : 127.0f / am;
-                const uint32_t w = (code8(x.x, inv) & 255) | (code8(x.y, inv) & 255) << 8 | (code8(x.z, inv) & 255) << 16 |
-                                   uint32_t(code8(x.w, inv)) << 24;
-                *reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(a.kc) + cell * D + e) = w;
-                if (e == 0) a.ks[cell] = am < kZeroAmax ? 0.0f : am / 127.0f;
-            }
-        }
+        g0 += NI * step;
+        if (g0 * HPW >= heads) break;
+        load(g0);
     }
 }
 
@@ -202,24 +224,32 @@ __device__ inline void append_v(const AppendArgs &a, int s, int group0, int ngro
     }
 }
 
-// Workgroups 0 .. n_rows * njobs - 1: queries and keys of a row; then
-// (sequence, group of 16 slots, 1024 values) of the values.
+// First the values: (sequence, group of 16 slots, 1024 values) a workgroup; then the
+// queries and keys, njobs workgroups a row.
 template <int D>
 __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a, int njobs, int ngroups, int nchunks) {
     __shared__ float2 cs[128];
-    __shared__ int found;
-    const unsigned nqk = unsigned(a.b.n_rows) * unsigned(njobs);
-    if (blockIdx.x < nqk) {
-        append_qk<D>(a, int(blockIdx.x / unsigned(njobs)), int(blockIdx.x % unsigned(njobs)), njobs, cs, &found);
+    const unsigned nv = unsigned(a.b.n_seqs) * unsigned(ngroups) * unsigned(nchunks);
+    if (blockIdx.x >= nv) {
+        const unsigned u = blockIdx.x - nv;
+        append_qk<D>(a, int(u / unsigned(njobs)), int(u % unsigned(njobs)), njobs, cs);
         return;
     }
-    const unsigned u = blockIdx.x - nqk;
-    const int chunk = int(u % unsigned(nchunks));
-    const unsigned sg = u / unsigned(nchunks);
-    append_v<D>(a, int(sg / unsigned(ngroups)), int(sg % unsigned(ngroups)), ngroups, chunk);
+    const unsigned sg = blockIdx.x / unsigned(nchunks);
+    append_v<D>(a, int(sg / unsigned(ngroups)), int(sg % unsigned(ngroups)), ngroups, int(blockIdx.x % unsigned(nchunks)));
+}
+
+__global__ __launch_bounds__(128) void rope_table_kernel(RopeTable t, RopeTable *dst) {
+    dst->turns[threadIdx.x] = t.turns[threadIdx.x];
+    dst->axis[threadIdx.x] = t.axis[threadIdx.x];
 }
 
 }  // namespace
+
+hipError_t launch_rope_table(const RopeTable &t, RopeTable *dst, hipStream_t s) {
+    hipLaunchKernelGGL(rope_table_kernel, dim3(1), dim3(128), 0, s, t, dst);
+    return hipGetLastError();
+}
 
 hipError_t launch_kv_append(const AppendArgs &a, hipStream_t s) {
     const int D = a.head_dim, hpw = 256 / D;
