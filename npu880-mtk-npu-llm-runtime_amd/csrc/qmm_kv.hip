@@ -64,23 +64,41 @@ __device__ inline void append_qk(const AppendArgs &a, int m, int job, int njobs,
         }
     };
     const int g_first = job * 4 + wid;
+    const int rot = a.rope ? a.rot_dim : 0, half = rot / 2;
+    int from = 0, to = 0, axis = 0;
+    double turn = 0.0;
+    if (lane < a.b.n_seqs) {
+        from = a.b.row_start[lane];
+        to = a.b.row_start[lane + 1];
+    }
+    if (t < half) {
+        axis = a.rope->axis[t];
+        turn = a.rope->turns[t];
+    }
+    __builtin_amdgcn_sched_barrier(0);
     load(g_first);
+    __builtin_amdgcn_sched_barrier(0);
     // the sequence that holds row m (the last one where the starts are not ascending)
     int s = -1;
-    for (int s0 = 0; s0 < a.b.n_seqs; s0 += 64) {
-        const int q = s0 + lane;
-        const bool in = q < a.b.n_seqs && a.b.row_start[q] <= m && m < a.b.row_start[q + 1];
-        const uint64_t found = __ballot(in);
+    for (int s0 = 0;;) {
+        const uint64_t found = __ballot(from <= m && m < to);
         if (found) s = s0 + 63 - __builtin_clzll(found);
+        s0 += 64;
+        if (s0 >= a.b.n_seqs) break;
+        from = to = 0;
+        if (s0 + lane < a.b.n_seqs) {
+            from = a.b.row_start[s0 + lane];
+            to = a.b.row_start[s0 + lane + 1];
+        }
     }
     if (s < 0) return;  // (all waves alike)
+    s = __builtin_amdgcn_readfirstlane(s);
     const SeqView v = seq_view(a.b, s);
     const int place = v.pos0 + (m - v.r0);
-    const int rot = a.rope ? a.rot_dim : 0, half = rot / 2;
     if (rot) {
         if (t < half) {
-            const int pos = a.pos ? a.pos[size_t(a.rope->axis[t]) * a.pos_stride + size_t(m)] : place;
-            const double turns = double(pos) * a.rope->turns[t];
+            const int pos = a.pos ? a.pos[size_t(axis) * a.pos_stride + size_t(m)] : place;
+            const double turns = double(pos) * turn;
             float sn, co;
             sincospif(2.0f * float(turns - rint(turns)), &sn, &co);
             cs[t] = make_float2(co * a.rope_scale, sn * a.rope_scale);
@@ -105,8 +123,8 @@ __device__ inline void append_qk(const AppendArgs &a, int m, int job, int njobs,
             const int head = g * HPW + lane / LPH;
             const bool is_q = head < HQ;
             float4 y = x[i];
-            const float *gamma = is_q ? a.q_gamma : a.k_gamma;
             const float ss = head_sum<LPH>(y.x * y.x + y.y * y.y + (y.z * y.z + y.w * y.w));
+            const float *gamma = is_q ? a.q_gamma : a.k_gamma;
             if (gamma) {
                 const float r = 1.0f / sqrtf(ss / float(D) + a.eps);
                 const float4 w = *reinterpret_cast<const float4 *>(gamma + e);
