@@ -27,16 +27,36 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 
 constexpr float kZeroAmax = 7.8886090522101181e-31f;  // 2^-100: smaller rows are zeros (127 / max|x| stays finite)
 
-// sum / maximum over the LPH lanes that hold one head
-template <int LPH> __device__ inline float head_sum(float v) {
-#pragma unroll
-    for (int o = 1; o < LPH; o *= 2) v += __shfl_xor(v, o);
+// sum / maximum over the LPH lanes (16, 32 or 64) that hold one head: neighbours, pairs, mirrored
+// halves and rows of 16 in the vector registers' own lane network, then across the rows
+template <int CTRL> __device__ inline float moved(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 15, 15, true));
+}
+template <int LPH, typename F> __device__ inline float over_head(float v, F f) {
+    v = f(v, moved<0xB1>(v));
+    v = f(v, moved<0x4E>(v));
+    v = f(v, moved<0x141>(v));
+    v = f(v, moved<0x140>(v));
+    if constexpr (LPH >= 32) {
+        auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    }
+    if constexpr (LPH == 64) {
+        auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    }
     return v;
 }
+template <int LPH> __device__ inline float head_sum(float v) {
+    return over_head<LPH>(v, [](float a, float b) { return a + b; });
+}
 template <int LPH> __device__ inline float head_max(float v) {
-#pragma unroll
-    for (int o = 1; o < LPH; o *= 2) v = fmaxf(v, __shfl_xor(v, o));
-    return v;
+    return over_head<LPH>(v, [](float a, float b) { return fmaxf(a, b); });
+}
+// 1 / sqrt(x) to one step of fp32; the instruction takes no number below 2^-126
+__device__ inline float inv_sqrt(float x) {
+    const bool tiny = x < 0x1p-100f;
+    return __builtin_amdgcn_rsqf(tiny ? x * 0x1p100f : x) * (tiny ? 0x1p50f : 1.0f);
 }
 __device__ inline float abs_max4(float4 x) {
     return fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
@@ -49,7 +69,7 @@ __device__ inline int code8(float x, float inv) { return int(fminf(fmaxf(rintf(x
 template <int D>
 __device__ inline void append_qk(const AppendArgs &a, int m, int job, int njobs, float2 *cs) {
     constexpr int LPH = D / 4, HPW = 64 / LPH, NI = 5;  // lanes per head, heads per wave, groups at a time
-    const int t = threadIdx.x, lane = t & 63, wid = t >> 6;
+    const int t = threadIdx.x, lane = t & 63, wid = __builtin_amdgcn_readfirstlane(t >> 6);
     const int H = a.b.n_heads, HQ = a.q ? a.q_heads : 0, heads = HQ + H;
     const int e = 4 * (lane % LPH), step = njobs * 4;  // this lane's first value of its head
     float4 x[NI];
@@ -116,6 +136,7 @@ __device__ inline void append_qk(const AppendArgs &a, int m, int job, int njobs,
     }
     const float sg = first ? -1.0f : 1.0f;
     for (int g0 = g_first;;) {
+        asm volatile("" : "+s"(g0));  // (addresses from g0 each time: five hoisted sets of them cost a third of the waves)
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
             const int g = g0 + i * step;
@@ -126,7 +147,7 @@ __device__ inline void append_qk(const AppendArgs &a, int m, int job, int njobs,
             const float ss = head_sum<LPH>(y.x * y.x + y.y * y.y + (y.z * y.z + y.w * y.w));
             const float *gamma = is_q ? a.q_gamma : a.k_gamma;
             if (gamma) {
-                const float r = 1.0f / sqrtf(ss / float(D) + a.eps);
+                const float r = inv_sqrt(ss * (1.0f / D) + a.eps);
                 const float4 w = *reinterpret_cast<const float4 *>(gamma + e);
                 y = make_float4(y.x * r * w.x, y.y * r * w.y, y.z * r * w.z, y.w * r * w.w);
             }
@@ -166,7 +187,8 @@ __device__ inline void append_qk(const AppendArgs &a, int m, int job, int njobs,
 }
 
 // the values of sequence s's new tokens in aligned groups of 16 slots, 1024
-// values of a token (4 a thread) from `chunk` on
+// values of a token (4 a thread) from `chunk` on; a group in two halves of 8
+// slots, so that a thread holds 32 values at most
 template <int D>
 __device__ inline void append_v(const AppendArgs &a, int s, int group0, int ngroups, int chunk) {
     constexpr int LPH = D / 4;
@@ -176,68 +198,69 @@ __device__ inline void append_v(const AppendArgs &a, int s, int group0, int ngro
     const bool on = i < H * D;
     const int head = i / D, d = i % D;
     const int P = 1 << a.b.page_shift;
-    const int first = max(v.pos0, 0) >> 4;  // (rows at negative places have no cell)
-    for (int g = first + group0; g * 16 < v.len; g += ngroups) {
-        const int lo = max(max(v.pos0, 0), g * 16), hi = min(v.len, g * 16 + 16);
-        if (lo >= hi) break;
-        const int page = page_of(a.b, s, lo, v.len);
+    const int start = max(v.pos0, 0);  // (rows at negative places have no cell)
+    for (int g = (start >> 4) + group0; g * 16 < v.len; g += ngroups) {
+        const int page = page_of(a.b, s, max(start, g * 16), v.len);
         if (page < 0) continue;
-        const int slot = (g * 16) & (P - 1);
-        float4 x[16];
-        const float *src = a.v + size_t(v.r0 - v.pos0 + lo) * a.v_stride + i;  // (row of place p: r0 + p - pos0)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            const int p = g * 16 + j;
-            x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (on && p >= lo && p < hi) x[j] = *reinterpret_cast<const float4 *>(src + size_t(p - lo) * a.v_stride);
-        }
         const size_t row = (size_t(page) * H + size_t(head)) * D + size_t(d);  // the first value's row of P slots
-        const bool whole = hi - lo == 16;
-        if (!a.vs) {
-            if (!on) continue;
-            uint16_t *dst = static_cast<uint16_t *>(a.vc) + row * size_t(P) + slot;
-            if (whole) {
+#pragma unroll 1
+        for (int p0 = g * 16; p0 < g * 16 + 16; p0 += 8) {
+            const int lo = max(start, p0), hi = min(v.len, p0 + 8);
+            if (lo >= hi) continue;
+            const int slot = p0 & (P - 1);
+            const bool whole = hi - lo == 8;
+            float4 x[8];
+            const float *src = a.v + size_t(v.r0 - v.pos0 + lo) * a.v_stride + i;  // (row of place p: r0 + p - pos0)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int p = p0 + j;
+                x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (on && p >= lo && p < hi) x[j] = *reinterpret_cast<const float4 *>(src + size_t(p - lo) * a.v_stride);
+            }
+            if (!a.vs) {
+                if (!on) continue;
+                uint16_t *dst = static_cast<uint16_t *>(a.vc) + row * size_t(P) + slot;
+                if (whole) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        h8 y;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) y[j] = _Float16(reinterpret_cast<const float *>(&x[j])[c]);
+                        *reinterpret_cast<h8 *>(dst + size_t(c) * P) = y;
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const int p = p0 + j;
+                        if (p < lo || p >= hi) continue;
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+                            reinterpret_cast<_Float16 *>(dst)[size_t(c) * P + j] = _Float16(reinterpret_cast<const float *>(&x[j])[c]);
+                    }
+                }
+                continue;
+            }
+            uint32_t w[4][2] = {};  // codes: value c's 8 tokens
+            uint8_t *dst = static_cast<uint8_t *>(a.vc) + row * size_t(P) + slot;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int p = p0 + j;
+                if (p < lo || p >= hi) continue;
+                const float am = head_max<LPH>(abs_max4(x[j]));
+                const float inv = am < kZeroAmax ? 0.0f : 127.0f / am;
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    h8 y[2];
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) y[j / 8][j % 8] = _Float16(reinterpret_cast<const float *>(&x[j])[c]);
-                    *reinterpret_cast<h8 *>(dst + size_t(c) * P) = y[0];
-                    *reinterpret_cast<h8 *>(dst + size_t(c) * P + 8) = y[1];
+                    const uint32_t code = uint32_t(code8(reinterpret_cast<const float *>(&x[j])[c], inv)) & 255u;
+                    w[c][j / 4] |= code << (8 * (j % 4));
+                    if (!whole && on) dst[size_t(c) * P + j] = uint8_t(code);
                 }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const int p = g * 16 + j;
-                    if (p < lo || p >= hi) continue;
-#pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                        reinterpret_cast<_Float16 *>(dst)[size_t(c) * P + j] = _Float16(reinterpret_cast<const float *>(&x[j])[c]);
-                }
+                if (on && d == 0)
+                    a.vs[((size_t(page) * H + size_t(head)) << a.b.page_shift) + size_t(slot + j)] = am < kZeroAmax ? 0.0f : am / 127.0f;
             }
-            continue;
-        }
-        uint32_t w[4][4] = {};  // codes: value c's 16 tokens
-        uint8_t *dst = static_cast<uint8_t *>(a.vc) + row * size_t(P) + slot;
+            if (whole && on) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            const int p = g * 16 + j;
-            if (p < lo || p >= hi) continue;
-            const float am = head_max<LPH>(abs_max4(x[j]));
-            const float inv = am < kZeroAmax ? 0.0f : 127.0f / am;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const uint32_t code = uint32_t(code8(reinterpret_cast<const float *>(&x[j])[c], inv)) & 255u;
-                w[c][j / 4] |= code << (8 * (j % 4));
-                if (!whole && on) dst[size_t(c) * P + j] = uint8_t(code);
+                for (int c = 0; c < 4; ++c) *reinterpret_cast<uint2 *>(dst + size_t(c) * P) = make_uint2(w[c][0], w[c][1]);
             }
-            if (on && d == 0)
-                a.vs[((size_t(page) * H + size_t(head)) << a.b.page_shift) + size_t(slot + j)] = am < kZeroAmax ? 0.0f : am / 127.0f;
-        }
-        if (whole && on) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-                *reinterpret_cast<uint4 *>(dst + size_t(c) * P) = make_uint4(w[c][0], w[c][1], w[c][2], w[c][3]);
         }
     }
 }
