@@ -92,9 +92,24 @@ template <int N> __device__ inline uint32_t seen_bits(int key0, int p, int low, 
     return below(p + 1) & (~below(low + 1) | below(sinks));
 }
 
+// all ones where bit j of `bits` is set, else 0
+__device__ inline uint32_t whole(uint32_t bits, int j) { return uint32_t(int32_t(bits << (31 - j)) >> 31); }
 // x where bit j of `bits` is set, else -infinity
 __device__ inline float seen_or_none(uint32_t bits, int j, float x) {
-    return int32_t(bits << (31 - j)) < 0 ? x : -__builtin_inff();
+    const uint32_t w = whole(bits, j);
+    return __uint_as_float((__float_as_uint(x) & w) | (0xff800000u & ~w));
+}
+// |x|, 0 where it is no number
+__device__ inline float magnitude_or_0(float x) { return fabsf(x) < __builtin_inff() ? fabsf(x) : 0.0f; }
+
+// An 8-bit cache's weights are p 2^-k times the value's scale, in fp16: k (kept as a float)
+// puts the largest scale the row has seen between 2^14 and 2^15, and 2^-k is part of the
+// running maximum, so it costs no operation and the row's sum has it too. From -16 (scales
+// below 1/2 lose the room they do not need: outputs are fp16) to 106 (no finite scale
+// overflows), so that a change of k never takes a sum below fp32's range.
+constexpr float kLeastShift = -16.0f;
+__device__ inline float scale_shift(float largest) {
+    return fminf(fmaxf(float(__builtin_amdgcn_frexp_expf(largest) - 15), kLeastShift), 106.0f);
 }
 // 8 halves of ones where the token's bit is set, else of zeros
 __device__ inline u4 halves_of(uint32_t bits) {
@@ -303,7 +318,7 @@ __device__ inline __attribute__((always_inline)) void split_piece(const SplitArg
             else q[k] = x;
         }
     }
-    float m = -__builtin_inff(), l = 0.0f, vref = 1e-30f;
+    float m = -__builtin_inff(), base = m, l = 0.0f, shift_v = kLeastShift;  // (base: m, plus the shift of an 8-bit cache)
     f4 acc[DT];
 
     u4 kr[NT][KR], vr[DT][Q8 ? (NU + 1) / 2 : NU];
@@ -413,24 +428,20 @@ __device__ inline __attribute__((always_inline)) void split_piece(const SplitArg
 #pragma unroll
         for (int j = 3; j + 1 < TL; j += 2) top = max3(top, sc[j / 4][j % 4], sc[(j + 1) / 4][(j + 1) % 4]);
         top = fmaxf(top, sc[NT - 1][3]);
-        const float mn = fmaxf(m, groups_max(top) * p.sl2);
-        const float ms = mn == -__builtin_inff() ? 0.0f : mn;
-        const float lscale = __builtin_amdgcn_exp2f(m - ms);
-        float alpha = lscale, vinv = 1.0f;
-        if constexpr (Q8) {  // the largest value scale the row has seen: its weights below are relative to it
-            float big = vref;
+        m = fmaxf(m, groups_max(top) * p.sl2);
+        if constexpr (Q8) {  // of the value scales that the row sees, the largest
+            float big = 0.0f;
 #pragma unroll
             for (int j = 0; j < TL; ++j) {
-                const float x = fabsf(vsc[j / 4][j % 4]);
-                const bool in = ((seen >> j & 1u) != 0) & (x < __builtin_inff());
-                big = fmaxf(big, in ? x : 0.0f);
+                float x = vsc[j / 4][j % 4];
+                if (!full) x = __uint_as_float(__float_as_uint(x) & whole(seen, j));
+                big = fmaxf(big, magnitude_or_0(x));
             }
-            big = groups_max(big);
-            alpha *= vref / big;
-            vref = big;
-            vinv = 1.0f / big;
+            shift_v = fmaxf(shift_v, scale_shift(groups_max(big)));
         }
-        m = mn;
+        const float nb = Q8 ? m + shift_v : m, ms = nb == -__builtin_inff() ? 0.0f : nb;
+        const float alpha = __builtin_amdgcn_exp2f(base - ms);
+        base = nb;
         float sum = 0.0f;
 #pragma unroll
         for (int j = 0; j < TL; ++j) {
@@ -438,7 +449,7 @@ __device__ inline __attribute__((always_inline)) void split_piece(const SplitArg
             sc[j / 4][j % 4] = e;
             sum += e;
         }
-        l = l * lscale + sum;
+        l = l * alpha + sum;
         if (!__all(alpha == 1.0f)) {
 #pragma unroll
             for (int d = 0; d < DT; ++d) acc[d] *= alpha;
@@ -465,7 +476,7 @@ __device__ inline __attribute__((always_inline)) void split_piece(const SplitArg
 #pragma unroll
         for (int j = 0; j < TL; ++j) {
             float w = sc[j / 4][j % 4];
-            if constexpr (Q8) w *= vsc[j / 4][j % 4] * vinv;  // the weights of the codes: p * scale
+            if constexpr (Q8) w *= vsc[j / 4][j % 4];  // the weights of the codes
             pb[j / 8][j % 8] = _Float16(w);
         }
         if constexpr (Q8) {  // (a hidden token's scale may be no number)
@@ -522,18 +533,18 @@ __device__ inline __attribute__((always_inline)) void split_piece(const SplitArg
 
     // the waves' results, joined in LDS
     l = groups_sum(l);
-    if (c == 0) sh.ml[wid][col] = make_float2(m, l);
+    if (c == 0) sh.ml[wid][col] = make_float2(base, l);
     __syncthreads();
     float top = -__builtin_inff(), total = 0.0f;
 #pragma unroll
     for (int w = 0; w < NW; ++w) top = fmaxf(top, sh.ml[w][col].x);
-    const float base = top == -__builtin_inff() ? 0.0f : top;
+    const float ref = top == -__builtin_inff() ? 0.0f : top;
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
         const float2 x = sh.ml[w][col];
-        total += x.y * __builtin_amdgcn_exp2f(x.x - base);
+        total += x.y * __builtin_amdgcn_exp2f(x.x - ref);
     }
-    const float mine = __builtin_amdgcn_exp2f(m - base) * (Q8 ? vref : 1.0f);
+    const float mine = __builtin_amdgcn_exp2f(base - ref);
     const float inv = direct ? (total > 0.0f || total != total ? 1.0f / total : 0.0f) : 1.0f;
     const bool in = col < nrows;
     const int slot = slot0 + col;
@@ -626,7 +637,7 @@ __device__ inline __attribute__((always_inline)) void tile_piece(const SplitArgs
 #pragma unroll
         for (int k = 0; k < KS; ++k) q[k] = *reinterpret_cast<const h8 *>(src + 16 * k);
     }
-    float m = -__builtin_inff(), l = 0.0f, vref = 1e-30f;
+    float m = -__builtin_inff(), base = m, l = 0.0f, shift_v = kLeastShift;  // (base: m, plus the shift of an 8-bit cache)
     f16v acc[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d)
@@ -683,26 +694,30 @@ __device__ inline __attribute__((always_inline)) void tile_piece(const SplitArgs
         else if (lane >= 16 && lane < 32 && iv < end) sreg = a.vs[k_cell(iv, gv) + (lane & 15)];
     };
     auto put_k = [&](int b, int slot) {
+        int ln = lane;  // (addresses made anew each time: kept, they would spill)
+        asm volatile("" : "+v"(ln));
 #pragma unroll
         for (int j = 0; j < (Q8 ? NL : 0); ++j) {
-            const int u = 64 * j + lane, r = 16 * wid + u / (D / 16), ch = u % (D / 16) * 2;
+            const int u = 64 * j + ln, r = 16 * wid + u / (D / 16), ch = u % (D / 16) * 2;
             *reinterpret_cast<h8 *>(&sh.kbuf[b][k_at(r, ch)]) = codes8(kr[j][0], kr[j][1]);
             *reinterpret_cast<h8 *>(&sh.kbuf[b][k_at(r, ch + 1)]) = codes8(kr[j][2], kr[j][3]);
         }
-        if (lane < 16) sh.ksc[slot & 3][16 * wid + lane] = sreg;
+        if (ln < 16) sh.ksc[slot & 3][16 * wid + ln] = sreg;
     };
     auto put_v = [&](int b) {
+        int ln = lane;
+        asm volatile("" : "+v"(ln));
 #pragma unroll
         for (int j = 0; j < (Q8 ? NL : 0); ++j) {
-            const int d = wid * (D / 4) + 16 * j + (lane >> 2), c = 2 * (lane & 3);
+            const int d = wid * (D / 4) + 16 * j + (ln >> 2), c = 2 * (ln & 3);
             *reinterpret_cast<h8 *>(&sh.vbuf[b][v_at(d, c)]) = codes8(vr[j][0], vr[j][1]);
             *reinterpret_cast<h8 *>(&sh.vbuf[b][v_at(d, c + 1)]) = codes8(vr[j][2], vr[j][3]);
         }
-        float big = fabsf(sreg) < __builtin_inff() ? fabsf(sreg) : 0.0f;
+        float big = magnitude_or_0(sreg);
 #pragma unroll
         for (int o = 1; o < 16; o *= 2) big = fmaxf(big, __shfl_xor(big, o));
-        if (lane == 16) sh.vmax[b][wid] = big;
-        if (lane >= 16 && lane < 32) sh.vsc[b][16 * wid + (lane & 15)] = sreg;
+        if (ln == 16) sh.vmax[b][wid] = big;
+        if (ln >= 16 && ln < 32) sh.vsc[b][16 * wid + (ln & 15)] = sreg;
     };
     // Values that are no numbers in a tile of which some row of the workgroup does not see
     // all: out of the product (a weight of 0 does not hide a NaN), and back after the loop.
@@ -825,10 +840,7 @@ __device__ inline __attribute__((always_inline)) void tile_piece(const SplitArgs
 #pragma unroll
         for (int j = 3; j < 31; j += 2) top = max3(top, sc[j / 16][j % 16], sc[(j + 1) / 16][(j + 1) % 16]);
         top = fmaxf(top, sc[1][15]);
-        const float mn = fmaxf(m, halves_max(top) * p.sl2);
-        const float ms = mn == -__builtin_inff() ? 0.0f : mn;
-        const float lscale = __builtin_amdgcn_exp2f(m - ms);
-        float alpha = lscale, vinv = 1.0f;
+        m = fmaxf(m, halves_max(top) * p.sl2);
         if constexpr (Q8) {
             const f4 most = *reinterpret_cast<const f4 *>(sh.vmax[b]);
             float big = fmaxf(max3(most[0], most[1], most[2]), most[3]);
@@ -846,13 +858,12 @@ __device__ inline __attribute__((always_inline)) void tile_piece(const SplitArgs
                 }
                 big = halves_max(big);
             }
-            big = fmaxf(big, vref);
-            alpha *= vref / big;
-            vref = big;
-            vinv = 1.0f / big;
+            shift_v = fmaxf(shift_v, scale_shift(big));
         }
-        m = mn;
-        l *= lscale;
+        const float nb = Q8 ? m + shift_v : m, ms = nb == -__builtin_inff() ? 0.0f : nb;
+        const float alpha = __builtin_amdgcn_exp2f(base - ms);
+        base = nb;
+        l *= alpha;
         if (!__all(alpha == 1.0f)) {
 #pragma unroll
             for (int d = 0; d < DB; ++d) acc[d] *= alpha;
@@ -876,8 +887,8 @@ __device__ inline __attribute__((always_inline)) void tile_piece(const SplitArgs
         for (int u = 0; u < 4; ++u) {
             f4 vx[2];
             if constexpr (Q8) {
-                vx[0] = value_scales(2 * u) * vinv;
-                vx[1] = value_scales(2 * u + 1) * vinv;
+                vx[0] = value_scales(2 * u);
+                vx[1] = value_scales(2 * u + 1);
             }
 #pragma unroll
             for (int k = u * KS / 4; k < (u + 1) * KS / 4; ++k)
@@ -942,18 +953,17 @@ __device__ inline __attribute__((always_inline)) void tile_piece(const SplitArgs
     }
     const float total = halves_sum(l);
     if (col < wrows) {
-        const float unit = Q8 ? vref : 1.0f;
         if (!direct) {
             const size_t slot = size_t(slot0 + wr + col);
-            if (hh == 0) p.part_ml[slot] = make_float2(m, total);
+            if (hh == 0) p.part_ml[slot] = make_float2(base, total);
 #pragma unroll
             for (int d = 0; d < DB; ++d)
 #pragma unroll
                 for (int x = 0; x < 4; ++x)
                     *reinterpret_cast<f4 *>(p.part_o + slot * D + 32 * d + 8 * x + 4 * hh) =
-                        f4{acc[d][4 * x], acc[d][4 * x + 1], acc[d][4 * x + 2], acc[d][4 * x + 3]} * unit;
+                        f4{acc[d][4 * x], acc[d][4 * x + 1], acc[d][4 * x + 2], acc[d][4 * x + 3]};
         } else {
-            const float inv = (total > 0.0f || total != total ? 1.0f / total : 0.0f) * unit;
+            const float inv = (total > 0.0f || total != total ? 1.0f / total : 0.0f);
             const size_t dst = size_t(v.r0 + qi) * a.out_stride + size_t(h * G + qg) * D + size_t(4 * hh);
 #pragma unroll
             for (int d = 0; d < DB; ++d)
