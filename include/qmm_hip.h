@@ -295,7 +295,11 @@ int qmm_lm_head_scan_rmsnorm(qmm_context *ctx, const float *x, const float *gamm
  * is clamped to [0, n_rows], kv_len to [0, max_pages * page_tokens], and the
  * cells of a page id outside [0, n_pages) are neither read nor written and are
  * visible to no row. Rows that no sequence holds (past row_start[n_seqs]) keep
- * their outputs as they were. */
+ * their outputs as they were. Largest calls: n_seqs * n_heads below 2^24 and
+ * n_rows * q_heads / n_heads below 2^30; a sequence holds at most 2^31 - 256
+ * tokens. Everything else that a call needs is in its arguments: it keeps
+ * nothing for the next one, and calls on several streams, contexts and graphs
+ * may overlap (with a workspace each). */
 
 /* One layer's cache: n_pages pages of page_tokens tokens (a power of two,
  * 16..1024), n_heads key-value heads of head_dim (64, 128 or 256) values.
@@ -383,7 +387,7 @@ typedef struct {
  * puts the values there. A row whose place is negative or in no valid page
  * gives its q_out alone. Row pointers and strides are multiples of 16 B
  * (q_out: of 8 B). |x| < 65520 for an fp16 cache. Two rows written to one
- * cell (a page held by two sequences): one of them is kept. */
+ * cell (a page that two sequences add to): the cell holds parts of both. */
 int qmm_kv_append(qmm_context *ctx, const qmm_kv_batch *batch, const qmm_kv_cache *cache, const qmm_kv_rows *rows);
 
 /* The attention of new rows over their sequences' cache, the new tokens

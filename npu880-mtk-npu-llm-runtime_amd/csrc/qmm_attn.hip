@@ -308,7 +308,7 @@ __device__ inline __attribute__((always_inline)) void split_piece(const SplitArg
     h8 q[QLDS ? 1 : KS];
     const int row = row0 + (col < nrows ? col : 0);
     const int qi = token_of(a, row), qg = row - qi * G, pos = v.pos0 + qi;
-    const int low = a.window > 0 ? max(pos - a.window, -1) : -1;
+    const int low = a.window > 0 ? max(max(pos, 0) - a.window, -1) : -1;
     {
         const uint16_t *src = a.q + size_t(v.r0 + qi) * a.q_stride + size_t(h * G + qg) * D;
 #pragma unroll
@@ -630,7 +630,7 @@ __device__ inline __attribute__((always_inline)) void tile_piece(const SplitArgs
     const int row = row0 + (wrows > 0 ? wr + (col < wrows ? col : 0) : 0);
     const int qi = token_of(a, row), qg = row - qi * G, pos = v.pos0 + qi;
     const int pmin = v.pos0 + token_of(a, row0 + min(wr, nrows - 1)), pmax = v.pos0 + token_of(a, row0 + min(wr + 31, nrows - 1));
-    const int low = a.window > 0 ? max(pos - a.window, -1) : -1;  // the last token the row's window hides
+    const int low = a.window > 0 ? max(max(pos, 0) - a.window, -1) : -1;  // the last token the row's window hides
     h8 q[KS];
     {
         const uint16_t *src = a.q + size_t(v.r0 + qi) * a.q_stride + size_t(h * G + qg) * D + 8 * hh;
