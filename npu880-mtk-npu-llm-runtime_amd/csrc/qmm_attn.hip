@@ -273,6 +273,20 @@ template <int R> __device__ inline RowTile row_tile(const AttnArgs &a, const Seq
     return t;
 }
 
+// 16 B that no other workgroup reads
+__device__ inline u4 once(const void *p) { return __builtin_nontemporal_load(static_cast<const u4 *>(p)); }
+// Loads that cover whole 128-B lines, made operands: lane l has loaded row l % 8 (a) and row
+// 8 + l % 8 (b), of each the piece 2 (l / 16) + (l / 8) % 2; afterwards row l % 16, pieces
+// 2 (l / 16) and 2 (l / 16) + 1. (Lanes 8 apart exchange halves in the lane network.)
+__device__ inline void rows_of_lines(u4 &a, u4 &b) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int x = int(a[j]), y = int(b[j]);
+        a[j] = uint32_t(__builtin_amdgcn_update_dpp(x, y, 0x128, 15, 12, false));
+        b[j] = uint32_t(__builtin_amdgcn_update_dpp(y, x, 0x128, 15, 3, false));
+    }
+}
+
 template <int D, int NW> struct SplitShared {
     f4 joined[NW][D < 128 ? D / 16 : 8][64];  // value tiles joined at a time
     float2 ml[NW][16];
@@ -296,6 +310,9 @@ __device__ inline __attribute__((always_inline)) void split_piece(const SplitArg
     constexpr int SUB = kTileKeys / KT;
     // what 256 registers hold: the next step's keys beside this one's values, and the queries
     constexpr bool AHEAD = D <= 128, QLDS = D > 128;
+    // A load of 16 rows of 64 B, as an operand has them, takes half a cache line of each; two of
+    // 8 rows take whole lines, which non-temporal loads need: 6.9 TB/s of 6.0
+    constexpr bool KLINES = KR >= 2, VLINES = !Q8 && NU == 2;
     constexpr int DG = DT < 8 ? DT : 8;  // value tiles joined at a time
     const AttnArgs &a = p.a;
     const int H = a.b.n_heads, G = a.group;
@@ -313,7 +330,7 @@ __device__ inline __attribute__((always_inline)) void split_piece(const SplitArg
         const uint16_t *src = a.q + size_t(v.r0 + qi) * a.q_stride + size_t(h * G + qg) * D;
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-            const h8 x = *reinterpret_cast<const h8 *>(src + (Q8 ? 64 * (k / 2) + 16 * c + 8 * (k % 2) : 32 * k + 8 * c));
+            const h8 x = *reinterpret_cast<const h8 *>(src + (!KLINES ? 16 * c + 8 * k : Q8 ? 128 * (k / 4) + 32 * c + 8 * (k % 4) : 64 * (k / 2) + 16 * c + 8 * (k % 2)));
             if constexpr (QLDS) sh.queries[wid][k][lane] = x;
             else q[k] = x;
         }
@@ -325,7 +342,8 @@ __device__ inline __attribute__((always_inline)) void split_piece(const SplitArg
     f4 ksc[NT], vsc[NT];
     int id_v = -1;
     bool wild_steps = false;
-    const int ck = col >> 2;  // the lane group whose tokens this lane loads keys of
+    // the lane groups whose tokens this lane loads keys of, and its piece of a line
+    const int ck = KLINES ? (lane & 7) >> 2 : col >> 2, piece = 2 * c + (lane >> 3 & 1);
     // the wave's steps are wid, wid + NW, .. of SUB (end - begin)
     const int steps = (end - begin) * SUB;
     auto step_at = [&](int i) { return span.at(begin + i / SUB) * kTileKeys + i % SUB * KT; };
@@ -333,46 +351,64 @@ __device__ inline __attribute__((always_inline)) void split_piece(const SplitArg
         return __all(page_ok) && t0 + KT - 1 <= pmin &&
                (a.window <= 0 || t0 > pmax - a.window || t0 + KT <= a.sinks);
     };
-    auto look_up = [&](int i, int &ik, int &iv) {
+    auto look_up = [&](int i, int2 &ik, int &iv) {
         const int t = step_at(i);
-        ik = page_of(a.b, s, t + TL * ck, v.len);
+        ik.x = page_of(a.b, s, t + TL * ck, v.len);
+        if constexpr (KLINES) ik.y = page_of(a.b, s, t + TL * (ck + 2), v.len);
         iv = page_of(a.b, s, t + TL * c, v.len);
     };
-    auto load_k = [&](int i, int id) {
-        const int slot = (step_at(i) + TL * ck) & (P - 1);
-        const size_t cell = ((size_t(max(id, 0)) * H + h) << shift) + size_t(slot + (lane & 3));
-        const uint8_t *src = static_cast<const uint8_t *>(a.kc) + cell * (Q8 ? D : 2 * D) + 16 * c;
+    auto load_k = [&](int i, int2 id) {
+        constexpr int RB = Q8 ? D : 2 * D;  // bytes of a key
+        auto row = [&](int id, int group) {
+            const int slot = (step_at(i) + TL * group) & (P - 1);
+            const size_t cell = ((size_t(max(id, 0)) * H + h) << shift) + size_t(slot + (lane & 3));
+            return static_cast<const uint8_t *>(a.kc) + cell * RB;
+        };
+        const uint8_t *src = row(id.x, ck) + 16 * (KLINES ? piece : c);
+        if constexpr (KLINES) {
+            const uint8_t *next = row(id.y, ck + 2) + 16 * piece;
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+            for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int k = 0; k < KR; ++k)
-                kr[t][k] = *reinterpret_cast<const u4 *>(src + t * 4 * (Q8 ? D : 2 * D) + k * 64);
+                for (int k = 0; k < KR; k += 2) {
+                    kr[t][k] = once(src + t * 4 * RB + k * 64);
+                    kr[t][k + 1] = once(next + t * 4 * RB + k * 64);
+                }
+        } else {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) kr[t][0] = *reinterpret_cast<const u4 *>(src + t * 4 * RB);
+        }
     };
 #pragma unroll
     for (int d = 0; d < DT; ++d) acc[d] = f4{0.f, 0.f, 0.f, 0.f};
     // pages are looked up a step ahead of their loads: loads return in order
-    int nk = -1, nv = -1;
+    int2 nk = make_int2(-1, -1);
+    int nv = -1;
     if (wid < steps) {
         look_up(wid, nk, id_v);
         load_k(wid, nk);
     }
     if (wid + NW < steps) look_up(wid + NW, nk, nv);
     for (int i = wid; i < steps; i += NW) {
-        int nnk = -1, nnv = -1;
+        int2 nnk = make_int2(-1, -1);
+        int nnv = -1;
         if (i + 2 * NW < steps) look_up(i + 2 * NW, nnk, nnv);
         const int t0 = step_at(i), key0 = t0 + TL * c;
         auto load_v = [&] {  // this step's values (and scales)
             const size_t hv = size_t(max(id_v, 0)) * H + h;
             const int slot = key0 & (P - 1);
-            const uint8_t *src = static_cast<const uint8_t *>(a.vc) + ((hv * D + col) * size_t(P) + slot) * (Q8 ? 1 : 2);
+            const int row = VLINES ? lane & 7 : col, at = VLINES ? slot + (lane & 8) : slot;
+            const uint8_t *src = static_cast<const uint8_t *>(a.vc) + ((hv * D + row) * size_t(P) + at) * (Q8 ? 1 : 2);
             const size_t next = size_t(16 * (Q8 ? 1 : 2)) << shift;
 #pragma unroll
             for (int d = 0; d < DT; ++d, src += next) {
-                if constexpr (!Q8) {
-#pragma unroll
-                    for (int u = 0; u < NU; ++u) vr[d][u] = reinterpret_cast<const u4 *>(src)[u];
-                } else if constexpr (NU == 2) {
+                if constexpr (VLINES) {
+                    vr[d][0] = once(src);
+                    vr[d][1] = once(src + next / 2);
+                } else if constexpr (!Q8) {
                     vr[d][0] = *reinterpret_cast<const u4 *>(src);
+                } else if constexpr (NU == 2) {
+                    vr[d][0] = once(src);
                 } else {
                     const uint2 w = *reinterpret_cast<const uint2 *>(src);
                     vr[d][0] = u4{w.x, w.y, 0, 0};
@@ -395,6 +431,8 @@ __device__ inline __attribute__((always_inline)) void split_piece(const SplitArg
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             sc[t] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < (KLINES ? KR : 0); k += 2) rows_of_lines(kr[t][k], kr[t][k + 1]);
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
                 h8 kk, qq;
@@ -486,7 +524,8 @@ __device__ inline __attribute__((always_inline)) void split_piece(const SplitArg
             }
         }
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
+        for (int d = 0; d < DT; ++d) {
+            if constexpr (VLINES) rows_of_lines(vr[d][0], vr[d][1]);
 #pragma unroll
             for (int u = 0; u < NU; ++u) {
                 h8 vv;
@@ -494,6 +533,7 @@ __device__ inline __attribute__((always_inline)) void split_piece(const SplitArg
                 else vv = __builtin_bit_cast(h8, vr[d][u]);
                 acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, pb[u], acc[d], 0, 0, 0);
             }
+        }
         if constexpr (!AHEAD) {
             if (i + NW < steps) load_k(i + NW, nk);
         }
