@@ -296,7 +296,7 @@ template <int D, int NW> struct SplitShared {
 // One piece of a segment: the up to 16 rows of `tile` of head h of sequence s over
 // tiles begin .. end - 1 of its span, the waves' steps in turn; the rows themselves
 // (direct), or their partial results at slot0.
-template <int D, int NW, bool Q8>
+template <int D, int NW, bool Q8, bool LINES>
 __device__ inline __attribute__((always_inline)) void split_piece(const SplitArgs &p, SplitShared<D, NW> &sh, const SeqView &v,
                                                                   const RowTile &tile, int s, int h, int begin, int end,
                                                                   bool direct, int slot0) {
@@ -312,7 +312,7 @@ __device__ inline __attribute__((always_inline)) void split_piece(const SplitArg
     constexpr bool AHEAD = D <= 128, QLDS = D > 128;
     // A load of 16 rows of 64 B, as an operand has them, takes half a cache line of each; two of
     // 8 rows take whole lines, which non-temporal loads need: 6.9 TB/s of 6.0
-    constexpr bool KLINES = KR >= 2, VLINES = !Q8 && NU == 2;
+    constexpr bool KLINES = LINES && KR >= 2, VLINES = LINES && !Q8 && NU == 2;
     constexpr int DG = DT < 8 ? DT : 8;  // value tiles joined at a time
     const AttnArgs &a = p.a;
     const int H = a.b.n_heads, G = a.group;
@@ -330,7 +330,8 @@ __device__ inline __attribute__((always_inline)) void split_piece(const SplitArg
         const uint16_t *src = a.q + size_t(v.r0 + qi) * a.q_stride + size_t(h * G + qg) * D;
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-            const h8 x = *reinterpret_cast<const h8 *>(src + (!KLINES ? 16 * c + 8 * k : Q8 ? 128 * (k / 4) + 32 * c + 8 * (k % 4) : 64 * (k / 2) + 16 * c + 8 * (k % 2)));
+            const h8 x = *reinterpret_cast<const h8 *>(src + (KLINES ? (Q8 ? 128 * (k / 4) + 32 * c + 8 * (k % 4) : 64 * (k / 2) + 16 * c + 8 * (k % 2))
+                                                                 : (Q8 ? 64 * (k / 2) + 16 * c + 8 * (k % 2) : 32 * k + 8 * c)));
             if constexpr (QLDS) sh.queries[wid][k][lane] = x;
             else q[k] = x;
         }
@@ -376,7 +377,9 @@ __device__ inline __attribute__((always_inline)) void split_piece(const SplitArg
                 }
         } else {
 #pragma unroll
-            for (int t = 0; t < NT; ++t) kr[t][0] = *reinterpret_cast<const u4 *>(src + t * 4 * RB);
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int k = 0; k < KR; ++k) kr[t][k] = *reinterpret_cast<const u4 *>(src + t * 4 * RB + k * 64);
         }
     };
 #pragma unroll
@@ -406,9 +409,10 @@ __device__ inline __attribute__((always_inline)) void split_piece(const SplitArg
                     vr[d][0] = once(src);
                     vr[d][1] = once(src + next / 2);
                 } else if constexpr (!Q8) {
-                    vr[d][0] = *reinterpret_cast<const u4 *>(src);
+#pragma unroll
+                    for (int u = 0; u < NU; ++u) vr[d][u] = reinterpret_cast<const u4 *>(src)[u];
                 } else if constexpr (NU == 2) {
-                    vr[d][0] = once(src);
+                    vr[d][0] = LINES ? once(src) : *reinterpret_cast<const u4 *>(src);
                 } else {
                     const uint2 w = *reinterpret_cast<const uint2 *>(src);
                     vr[d][0] = u4{w.x, w.y, 0, 0};
@@ -1024,7 +1028,7 @@ __device__ inline __attribute__((always_inline)) void tile_piece(const SplitArgs
 }
 // The shared work (or, with no workers, a workgroup for each head of a sequence).
 // R 16: few rows, a wave's tokens its own; R 128: the waves' rows, the tokens in LDS.
-template <int D, int R, int NW, bool Q8>
+template <int D, int R, int NW, bool Q8, bool LINES>
 __global__ __launch_bounds__(64 * NW, R == 128 && D > 128 ? 1 : 2) void attn_split_kernel(SplitArgs p) {
     constexpr int kLeast = R == 16 ? NW : 4;  // units of a worker, where all are fewer than the workers could take
     __shared__ std::conditional_t<R == 16, SplitShared<D, NW>, TileShared<D>> sh;
@@ -1131,7 +1135,7 @@ __global__ __launch_bounds__(64 * NW, R == 128 && D > 128 ? 1 : 2) void attn_spl
             if (lane == 0) p.shared[worker] = SharedSegment{n, s, h, tile.row0, tile.nrows};
         }
         end = min(end, tile.span.n);  // (a span of no tiles)
-        if constexpr (R == 16) split_piece<D, NW, Q8>(p, sh, v, tile, s, h, begin, end, direct, slot0);
+        if constexpr (R == 16) split_piece<D, NW, Q8, LINES>(p, sh, v, tile, s, h, begin, end, direct, slot0);
         else tile_piece<D, Q8>(p, sh, lds_addr(&sh), v, tile, s, h, begin, end, direct, slot0);
     }
 }
@@ -1193,6 +1197,7 @@ struct SplitPlan {
     int rows;      // of a row tile: 16 or 128
     int workers;   // that share all tiles (0: a workgroup for each head, or with 128 rows each row tile)
     int nw;        // waves, with 16 rows
+    bool lines;    // loads of whole cache lines, with 16 rows
     int row_tiles;
     int new_min, new_max;
     size_t slots, bytes;  // partial rows; all of the scratch
@@ -1208,7 +1213,17 @@ int64_t hinted_tiles(const AttnArgs &a, int R) {
     return most < tiles ? most : tiles;
 }
 
-constexpr int kShortTiles = 32;  // up to so many a head of a sequence is one workgroup's
+// Tiles up to which a head of a sequence is one workgroup's. A workgroup takes 5 us and 0.62 us
+// a tile; shared work 11.5 us and 4.5 us for 1000 tiles of all heads, its join included. us,
+// whole / shared (8 heads of 128): 8 heads of 11 tiles 11.1 / 13.9, of 16 14.2 / 11.1; 32 of 16
+// 15.9 / 13.0; 64 of 16 16.1 / 16.0, of 28 23.4 / 18.4; 128 of 16 17.0 / 22.0; 256 of 32 44 / 53.
+int64_t short_tiles(int64_t heads) { return std::min<int64_t>(32, 10 + heads / 6); }
+
+// Bytes of cache from which loads take whole lines and leave them in no cache: what is less
+// may be there from one call to the next (the last one holds 256 MB). us, as operands have
+// them / whole lines: 57 MB 21.7 / 23.0, 86 MB 25.8 / 28.6, 115 MB 33.3 / 31.9, 230 MB
+// 56.0 / 49.8; 0.4 MB 8.0 / 8.5 (more code to fetch).
+constexpr int64_t kLargeBytes = int64_t(96) << 20;
 
 // max_new: the most new tokens of the sequences it is for
 SplitPlan plan_split(const AttnArgs &a, int max_new, int cu_count, size_t scratch) {
@@ -1223,7 +1238,7 @@ SplitPlan plan_split(const AttnArgs &a, int max_new, int cu_count, size_t scratc
     // (units of the shared work: all that the tensors can hold)
     const int64_t bound = (int64_t(a.b.n_rows) * a.group / R + a.b.n_seqs) * a.b.n_heads *
                           (kv_capacity(a.b.max_pages, a.b.page_shift) / kTileKeys + 1);
-    const bool few_tiles = R == 16 ? tiles <= kShortTiles : units * row_tiles >= 2 * per_cu * cu_count || tiles <= 8;
+    const bool few_tiles = R == 16 ? tiles <= short_tiles(units) : units * row_tiles >= 2 * per_cu * cu_count || tiles <= 8;
     p.new_max = 0x7fffffff;
     if (!few_tiles && a.b.n_seqs <= kMaxShared && workers > units / 4 && bound < (int64_t(1) << 31)) {
         p.workers = int(workers);
@@ -1231,6 +1246,7 @@ SplitPlan plan_split(const AttnArgs &a, int max_new, int cu_count, size_t scratc
         p.bytes = size_t(workers) * each + sizeof(SharedSegment);
     }
     p.nw = R == 16 && !p.workers && a.head_dim <= 128 && units <= 2 * cu_count && tiles > 4 ? 8 : 4;
+    p.lines = R == 16 && tiles * units * kTileKeys * a.head_dim * (a.ks ? 2 : 4) >= kLargeBytes;
     p.row_tiles = int(std::min<int64_t>(row_tiles, 65535));
     return p;
 }
@@ -1247,9 +1263,9 @@ int plan_call(const AttnArgs &a, int cu_count, size_t scratch, SplitPlan out[2])
     return 2;
 }
 
-template <int D, int R, int NW> void launch_split(const SplitArgs &p, dim3 grid, hipStream_t s) {
-    if (p.a.ks) hipLaunchKernelGGL((attn_split_kernel<D, R, NW, true>), grid, dim3(64 * NW), 0, s, p);
-    else hipLaunchKernelGGL((attn_split_kernel<D, R, NW, false>), grid, dim3(64 * NW), 0, s, p);
+template <int D, int R, int NW, bool LINES> void launch_split(const SplitArgs &p, dim3 grid, hipStream_t s) {
+    if (p.a.ks) hipLaunchKernelGGL((attn_split_kernel<D, R, NW, true, LINES>), grid, dim3(64 * NW), 0, s, p);
+    else hipLaunchKernelGGL((attn_split_kernel<D, R, NW, false, LINES>), grid, dim3(64 * NW), 0, s, p);
 }
 
 template <int D> hipError_t launch_plan(SplitArgs &p, const SplitPlan &pl, hipStream_t s) {
@@ -1258,14 +1274,17 @@ template <int D> hipError_t launch_plan(SplitArgs &p, const SplitPlan &pl, hipSt
     const dim3 grid(pl.workers ? unsigned(pl.workers) : units);
     if (pl.rows == 128) {
         const dim3 tiles(units, unsigned(pl.row_tiles));
-        if (pl.workers) launch_split<D, 128, 4>(p, grid, s);
+        if (pl.workers) launch_split<D, 128, 4, false>(p, grid, s);
         else if (a.ks) hipLaunchKernelGGL((attn_tile_kernel<D, true>), tiles, dim3(256), 0, s, p);
         else hipLaunchKernelGGL((attn_tile_kernel<D, false>), tiles, dim3(256), 0, s, p);
     } else if constexpr (D <= 128) {
-        if (pl.nw == 8) launch_split<D, 16, 8>(p, grid, s);
-        else launch_split<D, 16, 4>(p, grid, s);
+        if (pl.nw == 8 && pl.lines) launch_split<D, 16, 8, true>(p, grid, s);
+        else if (pl.nw == 8) launch_split<D, 16, 8, false>(p, grid, s);
+        else if (pl.lines) launch_split<D, 16, 4, true>(p, grid, s);
+        else launch_split<D, 16, 4, false>(p, grid, s);
     } else {
-        launch_split<D, 16, 4>(p, grid, s);
+        if (pl.lines) launch_split<D, 16, 4, true>(p, grid, s);
+        else launch_split<D, 16, 4, false>(p, grid, s);
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || !pl.workers) return e;
