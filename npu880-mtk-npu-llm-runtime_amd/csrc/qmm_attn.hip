@@ -856,106 +856,108 @@ __device__ inline __attribute__((always_inline)) void tile_piece(const SplitArgs
         if constexpr (Q8) bring_scales(i + 2, g2, i + 1, g1);
         __builtin_amdgcn_sched_barrier(0);
 
-        const int t0 = span.at(i) * kTileKeys;
-        const uint32_t vb = value_base(b), kb = key_base(1 - b);
-        // (8-bit: the scales of the lane's tokens 4x .. 4x + 3 of 32)
-        auto key_scales = [&](int x) { return *reinterpret_cast<const f4 *>(&sh.ksc[(i - begin) & 3][16 * (x / 2) + 8 * hh + 4 * (x % 2)]); };
-        auto value_scales = [&](int x) { return *reinterpret_cast<const f4 *>(&sh.vsc[b][16 * (x / 2) + 8 * hh + 4 * (x % 2)]); };
-        if constexpr (Q8) {
-#pragma unroll
-            for (int x = 0; x < 8; ++x) {
-                const f4 kx = key_scales(x);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) sc[x / 4][4 * (x % 4) + r] *= kx[r];
-            }
-        }
-        const bool full = ok == 15 && t0 + kTileKeys - 1 <= pmin &&
-                          (a.window <= 0 || t0 > pmax - a.window || t0 + kTileKeys <= a.sinks);
-        uint32_t seen = 0xffffffffu;
-        if (!full) {
-            seen = 0;
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-                seen |= ((ok >> u & 1u) ? seen_bits<8>(t0 + 16 * u + 8 * hh, pos, low, a.sinks) : 0u) << (8 * u);
-#pragma unroll
-            for (int j = 0; j < 32; ++j) sc[j / 16][j % 16] = seen_or_none(seen, j, sc[j / 16][j % 16]);
-        }
-        float top = max3(sc[0][0], sc[0][1], sc[0][2]);
-#pragma unroll
-        for (int j = 3; j < 31; j += 2) top = max3(top, sc[j / 16][j % 16], sc[(j + 1) / 16][(j + 1) % 16]);
-        top = fmaxf(top, sc[1][15]);
-        m = fmaxf(m, halves_max(top) * p.sl2);
-        if constexpr (Q8) {
-            const f4 most = *reinterpret_cast<const f4 *>(sh.vmax[b]);
-            float big = fmaxf(max3(most[0], most[1], most[2]), most[3]);
-            if (!full) {  // of those that the row sees
-                big = 0.0f;
+        if (Q8 || wrows > 0) {  // (a wave without rows only brings its part; 8-bit: not worth the registers)
+            const int t0 = span.at(i) * kTileKeys;
+            const uint32_t vb = value_base(b), kb = key_base(1 - b);
+            // (8-bit: the scales of the lane's tokens 4x .. 4x + 3 of 32)
+            auto key_scales = [&](int x) { return *reinterpret_cast<const f4 *>(&sh.ksc[(i - begin) & 3][16 * (x / 2) + 8 * hh + 4 * (x % 2)]); };
+            auto value_scales = [&](int x) { return *reinterpret_cast<const f4 *>(&sh.vsc[b][16 * (x / 2) + 8 * hh + 4 * (x % 2)]); };
+            if constexpr (Q8) {
 #pragma unroll
                 for (int x = 0; x < 8; ++x) {
-                    const f4 vx = value_scales(x);
+                    const f4 kx = key_scales(x);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float y = fabsf(vx[r]);
-                        const bool in = ((seen >> (4 * x + r) & 1u) != 0) & (y < __builtin_inff());
-                        big = fmaxf(big, in ? y : 0.0f);
-                    }
+                    for (int r = 0; r < 4; ++r) sc[x / 4][4 * (x % 4) + r] *= kx[r];
                 }
-                big = halves_max(big);
             }
-            shift_v = fmaxf(shift_v, scale_shift(big));
-        }
-        const float nb = Q8 ? m + shift_v : m, ms = nb == -__builtin_inff() ? 0.0f : nb;
-        const float alpha = __builtin_amdgcn_exp2f(base - ms);
-        base = nb;
-        l *= alpha;
-        if (!__all(alpha == 1.0f)) {
+            const bool full = ok == 15 && t0 + kTileKeys - 1 <= pmin &&
+                              (a.window <= 0 || t0 > pmax - a.window || t0 + kTileKeys <= a.sinks);
+            uint32_t seen = 0xffffffffu;
+            if (!full) {
+                seen = 0;
 #pragma unroll
-            for (int d = 0; d < DB; ++d) acc[d] *= alpha;
-        }
-
-        f16v sn[2];  // (past the last tile: of what the buffer holds, not used)
+                for (int u = 0; u < 4; ++u)
+                    seen |= ((ok >> u & 1u) ? seen_bits<8>(t0 + 16 * u + 8 * hh, pos, low, a.sinks) : 0u) << (8 * u);
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+                for (int j = 0; j < 32; ++j) sc[j / 16][j % 16] = seen_or_none(seen, j, sc[j / 16][j % 16]);
+            }
+            float top = max3(sc[0][0], sc[0][1], sc[0][2]);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) sn[n][r] = 0.0f;
-        h8 pb[4];
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-        auto product = [&](int u) {
-#pragma unroll
-            for (int d = 0; d < DB; ++d)
-                acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, value(vb, d, u)), pb[u], acc[d], 0, 0, 0);
-        };
-        // in quarters, each between fences: exponentials of 16 tokens, a quarter of the next
-        // scores, and from the third on the product of the quarter two before
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            f4 vx[2];
+            for (int j = 3; j < 31; j += 2) top = max3(top, sc[j / 16][j % 16], sc[(j + 1) / 16][(j + 1) % 16]);
+            top = fmaxf(top, sc[1][15]);
+            m = fmaxf(m, halves_max(top) * p.sl2);
             if constexpr (Q8) {
-                vx[0] = value_scales(2 * u);
-                vx[1] = value_scales(2 * u + 1);
-            }
+                const f4 most = *reinterpret_cast<const f4 *>(sh.vmax[b]);
+                float big = fmaxf(max3(most[0], most[1], most[2]), most[3]);
+                if (!full) {  // of those that the row sees
+                    big = 0.0f;
 #pragma unroll
-            for (int k = u * KS / 4; k < (u + 1) * KS / 4; ++k)
+                    for (int x = 0; x < 8; ++x) {
+                        const f4 vx = value_scales(x);
 #pragma unroll
-                for (int n = 0; n < 2; ++n) sn[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(key(kb, n, k), q[k], sn[n], 0, 0, 0);
+                        for (int r = 0; r < 4; ++r) {
+                            const float y = fabsf(vx[r]);
+                            const bool in = ((seen >> (4 * x + r) & 1u) != 0) & (y < __builtin_inff());
+                            big = fmaxf(big, in ? y : 0.0f);
+                        }
+                    }
+                    big = halves_max(big);
+                }
+                shift_v = fmaxf(shift_v, scale_shift(big));
+            }
+            const float nb = Q8 ? m + shift_v : m, ms = nb == -__builtin_inff() ? 0.0f : nb;
+            const float alpha = __builtin_amdgcn_exp2f(base - ms);
+            base = nb;
+            l *= alpha;
+            if (!__all(alpha == 1.0f)) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u / 2][8 * (u % 2) + j], p.sl2, -ms));
-                sum[u] += e;
-                if constexpr (Q8) e *= vx[j / 4][j % 4];
-                pb[u][j] = _Float16(e);
+                for (int d = 0; d < DB; ++d) acc[d] *= alpha;
             }
-            if constexpr (Q8) {  // (a hidden token's scale may be no number)
-                if (!full) pb[u] = __builtin_bit_cast(h8, u4(__builtin_bit_cast(u4, pb[u]) & halves_of(seen >> 8 * u)));
+
+            f16v sn[2];  // (past the last tile: of what the buffer holds, not used)
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sn[n][r] = 0.0f;
+            h8 pb[4];
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            auto product = [&](int u) {
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+                    acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, value(vb, d, u)), pb[u], acc[d], 0, 0, 0);
+            };
+            // in quarters, each between fences: exponentials of 16 tokens, a quarter of the next
+            // scores, and from the third on the product of the quarter two before
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                f4 vx[2];
+                if constexpr (Q8) {
+                    vx[0] = value_scales(2 * u);
+                    vx[1] = value_scales(2 * u + 1);
+                }
+#pragma unroll
+                for (int k = u * KS / 4; k < (u + 1) * KS / 4; ++k)
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) sn[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(key(kb, n, k), q[k], sn[n], 0, 0, 0);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u / 2][8 * (u % 2) + j], p.sl2, -ms));
+                    sum[u] += e;
+                    if constexpr (Q8) e *= vx[j / 4][j % 4];
+                    pb[u][j] = _Float16(e);
+                }
+                if constexpr (Q8) {  // (a hidden token's scale may be no number)
+                    if (!full) pb[u] = __builtin_bit_cast(h8, u4(__builtin_bit_cast(u4, pb[u]) & halves_of(seen >> 8 * u)));
+                }
+                if (u >= 2) product(u - 2);
+                __builtin_amdgcn_sched_barrier(0);
             }
-            if (u >= 2) product(u - 2);
-            __builtin_amdgcn_sched_barrier(0);
+            product(2);
+            product(3);
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+            for (int n = 0; n < 2; ++n) sc[n] = sn[n];
         }
-        product(2);
-        product(3);
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-#pragma unroll
-        for (int n = 0; n < 2; ++n) sc[n] = sn[n];
         if constexpr (Q8) {
             __builtin_amdgcn_sched_barrier(0);
             if (i + 2 < end) put_k(b, i + 2 - begin);
