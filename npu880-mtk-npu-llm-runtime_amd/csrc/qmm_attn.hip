@@ -1,19 +1,31 @@
 // qmm_attn.hip — attention of new tokens over a paged key-value cache.
 //
-// A key-value head's query heads times a sequence's new tokens are the rows;
-// 16 of them a wave are the columns of the products
+// A key-value head's query heads times a sequence's new tokens are the rows of
 //   S^T [tokens x rows] = K Q^T,   O^T [values x rows] = V^T P^T
-// on 16x16x32 fp16 MFMA, 64 tokens a tile, with the running maximum m and sum l
-// of the softmax in base 2 (exp2(s scale log2 e - m)), fp32. Which token a row
-// of an MFMA operand stands for is free, so each lane is given 16 consecutive
-// tokens of the tile's 64 (lane group c = lane / 16: tokens 16c .. 16c + 15):
-//   S:  operand row i of MFMA t is token 16 (i / 4) + 4 t + i % 4, and the lane
-//       finds its scores of tokens 16c + 4t + r in register r of result t;
-//   PV: operand k index 8c + j of step u is token 16c + 8u + j: P stays in the
-//       lane that computed it, and V (stored with a value's tokens side by
-//       side) is read 32 B a lane. A page holds 16 tokens or more, so a lane
-//       looks up one page for its keys and one for its values.
-// Keys and values go from memory straight to the operands.
+// on fp16 MFMA, 64 tokens a tile, with the running maximum m and sum l of the
+// softmax in base 2 (exp2(s scale log2 e - m)), fp32. The weights P are rounded
+// to fp16 for the second product (half a step, 2^-11, of each; their sum l is of
+// the unrounded ones), outputs once more. Which token a row of an MFMA operand
+// stands for is free, so it is chosen that P stays in the lane that computed it.
+//
+// Two kernels, by the rows of a sequence's head:
+//  - up to 16 rows (single tokens; a few drafts): memory-bound, every cache byte
+//    is used once, so keys and values go from memory straight to the operands of
+//    a wave that has all the rows and 64 tokens of its own (split_piece). 5.5 TB/s
+//    for 64 sequences of 500 to 4000 tokens (537 MB in 97 us), 6.0 for one of
+//    131072, with 8 heads of 128; a plain read reaches 6.0, and 6.9 when it
+//    keeps nothing in the caches.
+//  - more rows (prompts, drafts): 128 of them a workgroup that shares the tile
+//    through LDS (tile_piece). Bound by the matrix cores and the exponentials
+//    beside them: 835 TFLOP/s for a causal prompt of 8192 (32 heads of 128 on 8;
+//    the library's own fp16 product of 16384 reaches 1330).
+// 8-bit caches: codes become fp16 exactly, a key's scale multiplies its scores,
+// a value's scale its weights.
+//
+// Who takes which tiles: even shares of all tiles for the workers (2 a CU), and
+// partial results joined by a second kernel; or, where that costs more than it
+// evens out, a workgroup for each head of a sequence or row tile (plan_split).
+// The order of all sums is fixed by the lengths: the same call, the same bits.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -296,6 +308,14 @@ template <int D, int NW> struct SplitShared {
 // One piece of a segment: the up to 16 rows of `tile` of head h of sequence s over
 // tiles begin .. end - 1 of its span, the waves' steps in turn; the rows themselves
 // (direct), or their partial results at slot0.
+// 16x16x32 MFMA; lane group c = lane / 16 has tokens TL c .. TL c + TL - 1 of a step:
+//   S:  operand row i of MFMA t is token TL (i / 4) + 4 t + i % 4, and the lane
+//       finds its scores of tokens TL c + 4t + r in register r of result t;
+//   PV: operand k index 8c + j of step u is token TL c + 8u + j.
+// A page holds 16 tokens or more, so a lane's tokens are in one page. A step's
+// values are under way during its scores, the next step's keys during its softmax
+// and second product; 8 waves of 16 to 32 KB a CU keep memory busy, and the
+// products and exponentials (a tenth of the time) lie under it.
 template <int D, int NW, bool Q8, bool LINES>
 __device__ inline __attribute__((always_inline)) void split_piece(const SplitArgs &p, SplitShared<D, NW> &sh, const SeqView &v,
                                                                   const RowTile &tile, int s, int h, int begin, int end,
@@ -330,8 +350,10 @@ __device__ inline __attribute__((always_inline)) void split_piece(const SplitArg
         const uint16_t *src = a.q + size_t(v.r0 + qi) * a.q_stride + size_t(h * G + qg) * D;
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-            const h8 x = *reinterpret_cast<const h8 *>(src + (KLINES ? (Q8 ? 128 * (k / 4) + 32 * c + 8 * (k % 4) : 64 * (k / 2) + 16 * c + 8 * (k % 2))
-                                                                 : (Q8 ? 64 * (k / 2) + 16 * c + 8 * (k % 2) : 32 * k + 8 * c)));
+            // (the values that the key operand of step k holds)
+            const int at = KLINES ? (Q8 ? 128 * (k / 4) + 32 * c + 8 * (k % 4) : 64 * (k / 2) + 16 * c + 8 * (k % 2))
+                                  : (Q8 ? 64 * (k / 2) + 16 * c + 8 * (k % 2) : 32 * k + 8 * c);
+            const h8 x = *reinterpret_cast<const h8 *>(src + at);
             if constexpr (QLDS) sh.queries[wid][k][lane] = x;
             else q[k] = x;
         }
@@ -623,7 +645,8 @@ __device__ inline float halves_sum(float v) {
     return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
 
-// Many rows: 128 of them a workgroup, 32 a wave, the columns of 32x32x16 MFMA.
+// Many rows: 128 of them a workgroup, 32 a wave, the columns of 32x32x16 MFMA. (64 rows
+// a workgroup read each tile twice as often; 64 a wave need more than 256 registers.)
 // The tile's keys and values are staged through LDS (8-bit ones as fp16) and
 // shared by the four waves; the next tile's loads are in flight meanwhile. A
 // lane (half hh = lane / 32) holds scores of tokens 16u + 8 hh + 0..7, u < 4:
@@ -651,7 +674,9 @@ __device__ inline void dma16g(const void *src, uint32_t lds) {
 // weights and second product beside tile i + 1's scores, so the matrix cores work
 // while the weights' exponentials are computed; the keys of tile i + 2 and the
 // values of tile i + 1 are on their way to LDS meanwhile (fp16 straight from
-// memory, the XOR of an LDS row's pieces in the lanes' addresses).
+// memory, the XOR of an LDS row's pieces in the lanes' addresses). Against scores
+// and product in turn: a prompt of 8192 727 -> 648 us. Nothing may spill here: a
+// spilled value's load waits for all of the loads above (8-bit: 10 to 25 %).
 template <int D, bool Q8>
 __device__ inline __attribute__((always_inline)) void tile_piece(const SplitArgs &p, TileShared<D> &sh, uint32_t sh_at, const SeqView &v,
                                                                  const RowTile &tile, int s, int h, int begin, int end,
@@ -1157,38 +1182,46 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void attn_tile_kernel(SplitAr
     }
 }
 
-// Joins a segment's pieces, for each worker that has a segment's first tile: a
-// workgroup a row (R 16: few rows, perhaps of many pieces), or a wave a row.
-template <int D, int R>
+// Joins the segments' pieces, for each worker that has a segment's first tile. A wave
+// a row; or (ROWS: few segments of many pieces, so the owners are some workers apart) a
+// workgroup a row, which looks at kOwners workers: a quarter of the workgroups.
+constexpr int kOwners = 4;
+template <int D, int R, bool ROWS>
 __global__ __launch_bounds__(64 * kJoinWaves) void attn_pieces_kernel(SplitArgs p) {
-    __shared__ float part[R == 16 ? kJoinWaves : 1][D];
+    __shared__ float part[ROWS ? kJoinWaves : 1][D];
     __shared__ float2 ml[kJoinWaves];
-    const int w = int(blockIdx.y);  // (rows across the XCDs: owners may be 8 workers apart)
-    if (w >= p.shared[p.workers].pieces) return;
-    const SharedSegment seg = p.shared[w];
-    if (seg.pieces < 2) return;
-    const AttnArgs &a = p.a;
-    const SeqView v = seq_view(a.b, seg.seq);
-    auto slot = [&](int k, int r) { return int64_t((w + k) * 2 + (k == 0)) * R + r; };
-    auto place = [&](int r) {
-        const int row = seg.row0 + r, i = token_of(a, row), g = row - i * a.group;
-        return size_t(v.r0 + i) * a.out_stride + size_t(seg.head * a.group + g) * D;
-    };
-    if constexpr (R == 16) {
-        for (int r = int(blockIdx.x); r < seg.rows; r += int(gridDim.x))
-            join_row<D>(p, seg.pieces, [&](int k) { return slot(k, r); }, part, ml, place(r));
-    } else {
-        constexpr int N = D / 64;
-        const int lane = threadIdx.x & 63;
-        for (int r = kJoinWaves * int(blockIdx.x) + int(threadIdx.x >> 6); r < seg.rows; r += kJoinWaves * int(gridDim.x)) {
-            float o[N], m, l;
-            join_pieces<D>(p, 0, 1, seg.pieces, [&](int k) { return slot(k, r); }, o, m, l);
-            const size_t dst = place(r);
+    constexpr int N = D / 64, OWN = ROWS ? kOwners : 1;
+    const int first = int(blockIdx.y) * OWN, workers = p.shared[p.workers].pieces;  // (rows across the XCDs: owners may be 8 workers apart)
+    int pieces[OWN];
 #pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const _Float16 y = _Float16(l > 0.0f || l != l ? o[j] / l : 0.0f);
-                if (a.out_f32) static_cast<float *>(a.out)[dst + 64 * j + lane] = float(y);
-                else static_cast<_Float16 *>(a.out)[dst + 64 * j + lane] = y;
+    for (int i = 0; i < OWN; ++i) pieces[i] = first + i < workers ? p.shared[first + i].pieces : 0;
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) {
+        if (pieces[i] < 2) continue;
+        const int w = first + i;
+        const SharedSegment seg = p.shared[w];
+        const AttnArgs &a = p.a;
+        const SeqView v = seq_view(a.b, seg.seq);
+        auto slot = [&](int k, int r) { return int64_t((w + k) * 2 + (k == 0)) * R + r; };
+        auto place = [&](int r) {
+            const int row = seg.row0 + r, i = token_of(a, row), g = row - i * a.group;
+            return size_t(v.r0 + i) * a.out_stride + size_t(seg.head * a.group + g) * D;
+        };
+        if constexpr (ROWS) {
+            for (int r = int(blockIdx.x); r < seg.rows; r += int(gridDim.x))
+                join_row<D>(p, seg.pieces, [&](int k) { return slot(k, r); }, part, ml, place(r));
+        } else {
+            const int lane = threadIdx.x & 63;
+            for (int r = kJoinWaves * int(blockIdx.x) + int(threadIdx.x >> 6); r < seg.rows; r += kJoinWaves * int(gridDim.x)) {
+                float o[N], m, l;
+                join_pieces<D>(p, 0, 1, seg.pieces, [&](int k) { return slot(k, r); }, o, m, l);
+                const size_t dst = place(r);
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    const _Float16 y = _Float16(l > 0.0f || l != l ? o[j] / l : 0.0f);
+                    if (a.out_f32) static_cast<float *>(a.out)[dst + 64 * j + lane] = float(y);
+                    else static_cast<_Float16 *>(a.out)[dst + 64 * j + lane] = y;
+                }
             }
         }
     }
@@ -1291,8 +1324,11 @@ template <int D> hipError_t launch_plan(SplitArgs &p, const SplitPlan &pl, hipSt
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || !pl.workers) return e;
     const int64_t rows = std::min<int64_t>(int64_t(a.max_new) * a.group, pl.rows);
-    if (pl.rows == 16) hipLaunchKernelGGL((attn_pieces_kernel<D, 16>), dim3(unsigned(rows), grid.x), dim3(64 * kJoinWaves), 0, s, p);
-    else hipLaunchKernelGGL((attn_pieces_kernel<D, 128>), dim3(unsigned((rows + kJoinWaves - 1) / kJoinWaves), grid.x), dim3(64 * kJoinWaves), 0, s, p);
+    const unsigned rows8 = unsigned((rows + kJoinWaves - 1) / kJoinWaves), owners4 = (grid.x + kOwners - 1) / kOwners;
+    const dim3 block(64 * kJoinWaves);
+    if (pl.rows == 128) hipLaunchKernelGGL((attn_pieces_kernel<D, 128, false>), dim3(rows8, grid.x), block, 0, s, p);
+    else if (grid.x > kOwners * units) hipLaunchKernelGGL((attn_pieces_kernel<D, 16, true>), dim3(unsigned(rows), owners4), block, 0, s, p);
+    else hipLaunchKernelGGL((attn_pieces_kernel<D, 16, false>), dim3(rows8, grid.x), block, 0, s, p);
     return hipGetLastError();
 }
 
