@@ -12,8 +12,8 @@
 //  - up to 16 rows (single tokens; a few drafts): memory-bound, every cache byte
 //    is used once, so keys and values go from memory straight to the operands of
 //    a wave that has all the rows and 64 tokens of its own (split_piece). 5.5 TB/s
-//    for 64 sequences of 500 to 4000 tokens (537 MB in 97 us), 6.0 for one of
-//    131072, with 8 heads of 128; a plain read reaches 6.0, and 6.9 when it
+//    for 32 sequences of 210 to 8000 tokens (537 MB in 97 us), 6.0 for one of
+//    131071, with 8 heads of 128; a plain read reaches 6.0, and 6.9 when it
 //    keeps nothing in the caches.
 //  - more rows (prompts, drafts): 128 of them a workgroup that shares the tile
 //    through LDS (tile_piece). Bound by the matrix cores and the exponentials
