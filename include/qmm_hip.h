@@ -360,9 +360,10 @@ typedef struct qmm_rope qmm_rope;
 /* The device table of one rotation; kept by the program, used by any stream and
  * graph of the context's device. Not during a capture. */
 int qmm_rope_create(qmm_context *ctx, const qmm_rope_params *params, qmm_rope **out);
-/* Calls on the context's stream are waited for; memory that a living graph may
- * hold is kept until the last graph is destroyed. Calls that run on another
- * stream must have ended. */
+/* Calls on the context's stream are waited for; memory that a living graph of
+ * this context may hold is kept until its last graph is destroyed. Calls on
+ * other streams must have ended, and graphs of other contexts that use it be
+ * destroyed. */
 int qmm_rope_destroy(qmm_context *ctx, qmm_rope *rope);
 
 /* The rows of one append: fp32 projections, each with its own row stride (in
@@ -386,7 +387,7 @@ typedef struct {
 /* Norms and rotates the queries into q_out and the keys into the cache, and
  * puts the values there. A row whose place is negative or in no valid page
  * gives its q_out alone. Row pointers and strides are multiples of 16 B
- * (q_out: of 8 B). |x| < 65520 for an fp16 cache. Two rows written to one
+ * (q_out: of 8 B); outputs overlap no input. |x| < 65520 for an fp16 cache. Two rows written to one
  * cell (a page that two sequences add to): the cell holds parts of both. */
 int qmm_kv_append(qmm_context *ctx, const qmm_kv_batch *batch, const qmm_kv_cache *cache, const qmm_kv_rows *rows);
 
@@ -396,7 +397,7 @@ int qmm_kv_append(qmm_context *ctx, const qmm_kv_batch *batch, const qmm_kv_cach
  *   j <= p  and  (window == 0  or  j > p - window  or  j < sinks):
  * a sliding window whose first `sinks` tokens stay visible. out = sum over the
  * visible j of softmax(scale * q.k_j) v_j; zeros where nothing is visible. What
- * lies in a masked cell (any bits) never reaches a row. */
+ * lies in a masked cell (any bits) never reaches a row. out does not overlap q. */
 typedef struct {
     const uint16_t *q; /* device fp16 [n_rows][q_stride], 16-B aligned rows */
     size_t q_stride;

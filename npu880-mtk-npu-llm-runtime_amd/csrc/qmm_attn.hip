@@ -1292,7 +1292,7 @@ SplitPlan plan_split(const AttnArgs &a, int max_new, int cu_count, size_t scratc
         p.bytes = size_t(workers) * each + sizeof(SharedSegment);
     }
     p.nw = R == 16 && !p.workers && a.head_dim <= 128 && units <= 2 * cu_count && tiles > 4 ? 8 : 4;
-    p.lines = R == 16 && tiles * units * kTileKeys * a.head_dim * (a.ks ? 2 : 4) >= kLargeBytes;
+    p.lines = R == 16 && tiles * units >= kLargeBytes / (int64_t(kTileKeys) * a.head_dim * (a.ks ? 2 : 4));
     p.row_tiles = int(std::min<int64_t>(row_tiles, 65535));
     return p;
 }
@@ -1317,7 +1317,8 @@ template <int D, int R, int NW, bool LINES> void launch_split(const SplitArgs &p
 template <int D> hipError_t launch_plan(SplitArgs &p, const SplitPlan &pl, hipStream_t s) {
     const AttnArgs &a = p.a;
     const unsigned units = unsigned(a.b.n_seqs) * unsigned(a.b.n_heads);
-    const dim3 grid(pl.workers ? unsigned(pl.workers) : units);
+    // (128 rows: the workers of an XCD are workgroups 8 apart, so all eight need as many)
+    const dim3 grid(!pl.workers ? units : pl.rows == 128 ? unsigned(pl.workers + 7) / 8 * 8 : unsigned(pl.workers));
     if (pl.rows == 128) {
         const dim3 tiles(units, unsigned(pl.row_tiles));
         if (pl.workers) launch_split<D, 128, 4, false>(p, grid, s);

@@ -394,6 +394,28 @@ def test_value_scales_of_all_sizes(ctx, new):
         b.free()
 
 
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("D", [64, 256])
+def test_workspaces_of_any_size(ctx, q8, D):
+    """Draft rows and single tokens over long sequences with room for any number of workers: the same
+    values to rounding, from none that share to all."""
+    for lens, group in (([(2500, 9), (700, 13)], 8), ([(2500, 1), (1900, 1)], 8), ([(1500, 30), (1100, 1), (900, 2)], 8)):
+        b = Batch(lens, 1, D, 16, q8, seed=53)
+        q = queries(b, group)
+        ref, tol = attend(b, q, group, D ** -0.5)
+        b.upload(ctx, max(n for _, n in lens), 2500)
+        rows = 128 if lens[0][1] > 1 else 16
+        each = 2 * rows * (D * 4 + 8) + 32
+        for workers in (1, 2, 3, 5, 7, 8, 9, 13, 15, 17, 26, 31, 100):
+            say(f"workspace for {workers} workers, lens={lens} D={D} q8={q8}")
+            h = C.c_void_p()
+            ctx._call("qmm_attention_workspace_create", ctx._h, (workers + 1) * each, C.byref(h))
+            ws = qmm_hip._Handle(ctx, h.value, "qmm_attention_workspace_destroy")
+            check_rows(run_attention(ctx, b, q, group, D ** -0.5, ws=ws), ref, tol, b.held_rows)
+            ws.free()
+        b.free()
+
+
 def test_refusals(ctx):
     """Bad calls return a status and a reason, and launch nothing."""
     b = Batch([(20, 1)], 2, 64, 16, seed=50).upload(ctx, 1, 20)
