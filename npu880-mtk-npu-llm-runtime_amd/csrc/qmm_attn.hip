@@ -17,7 +17,7 @@
 //    keeps nothing in the caches.
 //  - more rows (prompts, drafts): 128 of them a workgroup that shares the tile
 //    through LDS (tile_piece). Bound by the matrix cores and the exponentials
-//    beside them: 835 TFLOP/s for a causal prompt of 8192 (32 heads of 128 on 8;
+//    beside them: 830 to 870 TFLOP/s for a causal prompt of 8192 (32 heads of 128 on 8;
 //    the library's own fp16 product of 16384 reaches 1330).
 // 8-bit caches: codes become fp16 exactly, a key's scale multiplies its scores,
 // a value's scale its weights.
