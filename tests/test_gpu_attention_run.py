@@ -376,6 +376,30 @@ def test_wide_batches(ctx, lens, heads, group, D):
         b.free()
 
 
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("P", [16, 32, 64, 256])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1100, 3)])
+def test_calls_announced_as_large(ctx, q8, D, P, window, sinks):
+    """Few rows with hints of long sequences: the loads for caches of more than 96 MB, over ragged lengths,
+    pages of every size and cells that hold no numbers; in shares, and (many heads) without."""
+    for lens, heads, longest in (([(n, 1 + n % 4) for n in (4, 15, 16, 65, 127, 300, 511, 1500)], 1, 1 << 17),
+                                 ([(1500 if i % 40 == 9 else 5 + 37 * i % 400, 1) for i in range(130)], 2, 2000)):
+        b = Batch(lens, heads, D, P, q8, seed=D + P, max_pages=longest // P)
+        group = 4 if heads == 1 else 3
+        q = queries(b, group)
+        if not q8:  # a new token's values: the rows before it do not see them
+            p, t = b.cells(3)
+            b.v[p[-1], 0, 5, t[-1]] = np.nan
+            b.v[p[-2], 0, 7, t[-2]] = np.inf
+        say(f"announced as large: {len(lens)} sequences D={D} P={P} q8={q8} window={window}")
+        ref, tol = attend(b, q, group, D ** -0.5, window, sinks)
+        b.upload(ctx, max(n for _, n in lens), longest)
+        one = run_attention(ctx, b, q, group, D ** -0.5, window, sinks)
+        b.free()
+        check_rows(one, ref, tol, b.held_rows)
+
+
 @pytest.mark.parametrize("new", [1, 9, 60])
 def test_value_scales_of_all_sizes(ctx, new):
     """8-bit values from 2^-60 to 2^8 between the tokens, in rising, falling and mixed order; and all zero."""
