@@ -1281,12 +1281,12 @@ SplitPlan plan_split(const AttnArgs &a, int max_new, int cu_count, size_t scratc
     const size_t each = 2 * size_t(R) * (size_t(a.head_dim) * 4 + 8) + sizeof(SharedSegment);
     int64_t workers = std::min(cu_count, 512) * int64_t(per_cu);
     if (size_t(workers) * each + sizeof(SharedSegment) > scratch) workers = int64_t(scratch / each) - 1;
-    // (units of the shared work: all that the tensors can hold)
-    const int64_t bound = (int64_t(a.b.n_rows) * a.group / R + a.b.n_seqs) * a.b.n_heads *
-                          (kv_capacity(a.b.max_pages, a.b.page_shift) / kTileKeys + 1);
+    // (units of the shared work: all that there can be, were every sequence to claim all rows)
+    const int64_t each_seq = (int64_t(a.b.n_rows) * a.group / R + 1) * (kv_capacity(a.b.max_pages, a.b.page_shift) / kTileKeys + 1);
+    const bool countable = each_seq < (int64_t(1) << 31) / units;
     const bool few_tiles = R == 16 ? tiles <= short_tiles(units) : units * row_tiles >= 2 * per_cu * cu_count || tiles <= 8;
     p.new_max = 0x7fffffff;
-    if (!few_tiles && a.b.n_seqs <= kMaxShared && workers > units / 4 && bound < (int64_t(1) << 31)) {
+    if (!few_tiles && a.b.n_seqs <= kMaxShared && workers > units / 4 && countable) {
         p.workers = int(workers);
         p.slots = size_t(workers) * 2 * R;
         p.bytes = size_t(workers) * each + sizeof(SharedSegment);

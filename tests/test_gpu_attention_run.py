@@ -440,6 +440,21 @@ def test_workspaces_of_any_size(ctx, q8, D):
         b.free()
 
 
+@pytest.mark.parametrize("new", [4, 20])
+def test_rows_claimed_twice(ctx, new):
+    """Row starts that fall: two sequences (the same one twice) claim all rows, one between them none."""
+    b = Batch([(3000, new)], 2, 64, 16, seed=59)
+    q = queries(b, 4)
+    ref, tol = attend(b, q, 4, 0.125)
+    b.S, b.pages, b.kv_len = 3, np.repeat(b.pages, 3, 0), np.array([3000, 77, 3000], np.int32)
+    b.row_start = np.array([0, new, 0, new], np.int32)
+    say(f"rows claimed twice, new={new}")
+    b.upload(ctx, new, 3000)
+    got = run_attention(ctx, b, q, 4, 0.125)
+    b.free()
+    check_rows(got, ref, tol, new)
+
+
 def test_refusals(ctx):
     """Bad calls return a status and a reason, and launch nothing."""
     b = Batch([(20, 1)], 2, 64, 16, seed=50).upload(ctx, 1, 20)
