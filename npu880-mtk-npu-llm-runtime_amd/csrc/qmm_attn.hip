@@ -914,7 +914,7 @@ __device__ inline __attribute__((always_inline)) void tile_piece(const SplitArgs
             if constexpr (Q8) {
                 const f4 most = *reinterpret_cast<const f4 *>(sh.vmax[b]);
                 float big = fmaxf(max3(most[0], most[1], most[2]), most[3]);
-                if (!full) {  // of those that the row sees
+                if (!full && __any(scale_shift(big) > shift_v)) {  // of those that the row sees, where that can matter
                     big = 0.0f;
 #pragma unroll
                     for (int x = 0; x < 8; ++x) {
