@@ -309,7 +309,9 @@ int qmm_lm_head_scan_rmsnorm(qmm_context *ctx, const float *x, const float *gamm
  * QMM_KV_F16: fp16. QMM_KV_Q8: int8 codes, and one fp32 scale for each token's
  * head in k_scale / v_scale [n_pages][n_heads][page_tokens]: value = code *
  * scale, scale = max|x| / 127, code = rint(x * (127 / max|x|)); where max|x| is
- * below 2^-100 both are 0. k and v 16-B aligned, scales 16-B aligned. */
+ * below 2^-100 both are 0. A token's head with a value that is no number (NaN, an
+ * infinity) has codes of 0 and a scale of NaN: all of it is NaN to the rows that
+ * see it. k and v 16-B aligned, scales 16-B aligned. */
 #define QMM_KV_F16 1
 #define QMM_KV_Q8 2
 typedef struct {

@@ -3,7 +3,8 @@
 //
 //   norm      y = x / sqrt(mean(x^2) + eps) * gamma   over a head's D values, fp32
 //   rotation  (a, b) -> f (a cos t - b sin t, b cos t + a sin t), t = pos * freq(pair)
-//   store     fp16, or code = rint(x 127 / max|x|) with scale max|x| / 127
+//   store     fp16, or code = rint(x 127 / max|x|) with scale max|x| / 127; a head with a value that is
+//             no number has none: codes of 0 with a scale of NaN
 //
 // Bound: memory. Every projection value is read once as fp32 and written once
 // as fp16 (or 8 bits): 8192 tokens of 32 + 8 + 8 heads of 128 (302 MB) in 70 us,
@@ -32,39 +33,52 @@ constexpr float kZeroAmax = 7.8886090522101181e-31f;  // 2^-100: smaller rows ar
 
 // sum / maximum over the LPH lanes (16, 32 or 64) that hold one head: neighbours, pairs, mirrored
 // halves and rows of 16 in the vector registers' own lane network, then across the rows
-template <int CTRL> __device__ inline float moved(float v) {
-    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 15, 15, true));
+template <int CTRL> __device__ inline uint32_t moved(uint32_t v) {
+    return uint32_t(__builtin_amdgcn_update_dpp(0, int(v), CTRL, 15, 15, true));
 }
-template <int LPH, typename F> __device__ inline float over_head(float v, F f) {
+template <int LPH, typename F> __device__ inline uint32_t over_head(uint32_t v, F f) {
     v = f(v, moved<0xB1>(v));
     v = f(v, moved<0x4E>(v));
     v = f(v, moved<0x141>(v));
     v = f(v, moved<0x140>(v));
     if constexpr (LPH >= 32) {
-        auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-        v = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+        auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        v = f(a[0], a[1]);
     }
     if constexpr (LPH == 64) {
-        auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-        v = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+        auto a = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        v = f(a[0], a[1]);
     }
     return v;
 }
 template <int LPH> __device__ inline float head_sum(float v) {
-    return over_head<LPH>(v, [](float a, float b) { return a + b; });
-}
-template <int LPH> __device__ inline float head_max(float v) {
-    return over_head<LPH>(v, [](float a, float b) { return fmaxf(a, b); });
+    return __uint_as_float(over_head<LPH>(
+        __float_as_uint(v), [](uint32_t a, uint32_t b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); }));
 }
 // 1 / sqrt(x) to one step of fp32; the instruction takes no number below 2^-126
 __device__ inline float inv_sqrt(float x) {
     const bool tiny = x < 0x1p-100f;
     return __builtin_amdgcn_rsqf(tiny ? x * 0x1p100f : x) * (tiny ? 0x1p50f : 1.0f);
 }
-__device__ inline float abs_max4(float4 x) {
-    return fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+// What an 8-bit cache keeps of one head: its scale, what makes codes of its values, and the codes' bits
+// (none where a value is no number: 255 otherwise).
+struct HeadCodes {
+    float scale, inv;
+    uint32_t bits;
+};
+// The largest magnitude over a head's lanes as an integer: there an infinity is above all numbers and
+// a NaN above both, where a maximum of floats would pass over the NaN.
+template <int LPH> __device__ inline HeadCodes head_codes(float4 x) {
+    auto top = [](uint32_t a, uint32_t b) { return max(a, b); };
+    auto size = [](float v) { return __float_as_uint(v) & 0x7fffffffu; };
+    const uint32_t most = over_head<LPH>(max(max(size(x.x), size(x.y)), max(size(x.z), size(x.w))), top);
+    const float am = __uint_as_float(most);
+    if (most >= 0x7f800000u) return HeadCodes{__builtin_nanf(""), 0.0f, 0u};
+    return am < kZeroAmax ? HeadCodes{0.0f, 0.0f, 255u} : HeadCodes{am / 127.0f, 127.0f / am, 255u};
 }
-__device__ inline int code8(float x, float inv) { return int(fminf(fmaxf(rintf(x * inv), -127.0f), 127.0f)); }
+__device__ inline uint32_t code8(float x, const HeadCodes &h) {
+    return uint32_t(int(fminf(fmaxf(rintf(x * h.inv), -127.0f), 127.0f))) & h.bits;
+}
 
 // One row's queries and keys: workgroup `job` of `njobs` takes its share of the head
 // groups, a wave HPW heads at a time. A wave's loads are all under way before it
@@ -165,7 +179,7 @@ __device__ inline void append_qk(const AppendArgs &a, int m, int job, int njobs,
                                     y.w * c[1].x + y.z * c[1].y);
                 }
             }
-            const float am = a.ks ? head_max<LPH>(abs_max4(y)) : 0.0f;
+            const HeadCodes hc = a.ks ? head_codes<LPH>(y) : HeadCodes{};
             if (head >= heads) continue;
             const h4 r = {_Float16(y.x), _Float16(y.y), _Float16(y.z), _Float16(y.w)};
             if (is_q) {
@@ -175,11 +189,9 @@ __device__ inline void append_qk(const AppendArgs &a, int m, int job, int njobs,
                 if (!a.ks) {
                     *reinterpret_cast<h4 *>(static_cast<uint16_t *>(a.kc) + cell * D + e) = r;
                 } else {
-                    const float inv = am < kZeroAmax ? 0.0f : 127.0f / am;
-                    const uint32_t w = (code8(y.x, inv) & 255) | (code8(y.y, inv) & 255) << 8 | (code8(y.z, inv) & 255) << 16 |
-                                       uint32_t(code8(y.w, inv)) << 24;
+                    const uint32_t w = code8(y.x, hc) | code8(y.y, hc) << 8 | code8(y.z, hc) << 16 | code8(y.w, hc) << 24;
                     *reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(a.kc) + cell * D + e) = w;
-                    if (e == 0) a.ks[cell] = am < kZeroAmax ? 0.0f : am / 127.0f;
+                    if (e == 0) a.ks[cell] = hc.scale;
                 }
             }
         }
@@ -249,16 +261,14 @@ __device__ inline void append_v(const AppendArgs &a, int s, int group0, int ngro
             for (int j = 0; j < 8; ++j) {
                 const int p = p0 + j;
                 if (p < lo || p >= hi) continue;
-                const float am = head_max<LPH>(abs_max4(x[j]));
-                const float inv = am < kZeroAmax ? 0.0f : 127.0f / am;
+                const HeadCodes hc = head_codes<LPH>(x[j]);
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    const uint32_t code = uint32_t(code8(reinterpret_cast<const float *>(&x[j])[c], inv)) & 255u;
+                    const uint32_t code = code8(reinterpret_cast<const float *>(&x[j])[c], hc);
                     w[c][j / 4] |= code << (8 * (j % 4));
                     if (!whole && on) dst[size_t(c) * P + j] = uint8_t(code);
                 }
-                if (on && d == 0)
-                    a.vs[((size_t(page) * H + size_t(head)) << a.b.page_shift) + size_t(slot + j)] = am < kZeroAmax ? 0.0f : am / 127.0f;
+                if (on && d == 0) a.vs[((size_t(page) * H + size_t(head)) << a.b.page_shift) + size_t(slot + j)] = hc.scale;
             }
             if (whole && on) {
 #pragma unroll
