@@ -102,3 +102,30 @@ def test_no_numbers_into_an_fp16_cache(ctx):
             page, slot, r = p[n - new + i], t[n - new + i], b.row_start[s] + i
             assert np.array_equal(got["k"][page, :, slot].reshape(-1), want[r, :H * D], equal_nan=True)
             assert np.array_equal(got["v"][page, :, :, slot].reshape(-1), want[r, H * D:], equal_nan=True)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_smallest_scales_of_an_8_bit_cache(ctx, D):
+    """Largest values just below 2^-100: codes and scale of 0. From 2^-100 on: codes up to 127."""
+    H = 2
+    b = Batch(LENS, H, D, 16, True, seed=D).upload(ctx, 19, 40)
+    rng = np.random.default_rng(D)
+    x = rng.uniform(-0.9, 0.9, (b.M, 2 * H, D))
+    edge = np.nextafter(np.float32(2.0 ** -100), np.float32(0))
+    x *= 2.0 ** -100
+    x[:, :, D // 2] = np.where((np.arange(b.M) % 2 == 0)[:, None], edge, np.float32(-2.0 ** -100))
+    say(f"smallest scales D={D}")
+    got = _append(ctx, b, x.reshape(b.M, -1).astype(np.float32))
+    b.free()
+    for s, (n, new) in enumerate(b.lens):
+        p, t = b.cells(s)
+        for i in range(new):
+            page, slot, r = p[n - new + i], t[n - new + i], b.row_start[s] + i
+            for codes, scale, ref in ((got["k"][page, :, slot], got["ks"][page, :, slot], x[r, :H]),
+                                      (got["v"][page, :, :, slot], got["vs"][page, :, slot], x[r, H:])):
+                if r % 2 == 0:
+                    assert (codes == 0).all() and (scale == 0).all()
+                else:
+                    assert (codes[:, D // 2] == -127).all() and (np.abs(scale * 127 / 2.0 ** -100 - 1) < 2.0 ** -22).all()
+                    # half a step of the code, and its quotient's last bits
+                    assert np.abs(codes * scale[:, None].astype(np.float64) - ref).max() <= scale.max() * (0.5 + 127 * 2.0 ** -22)
