@@ -119,9 +119,10 @@ __device__ inline float magnitude_or_0(float x) { return fabsf(x) < __builtin_in
 // running maximum, so it costs no operation and the row's sum has it too. From -16 (scales
 // below 1/2 lose the room they do not need: outputs are fp16) to 106 (no finite scale
 // overflows), so that a change of k never takes a sum below fp32's range.
+// The exponent is taken from the bits: 0, where a row sees no scale, has the least of all.
 constexpr float kLeastShift = -16.0f;
-__device__ inline float scale_shift(float largest) {
-    return fminf(fmaxf(float(__builtin_amdgcn_frexp_expf(largest) - 15), kLeastShift), 106.0f);
+__device__ inline float scale_shift(float largest) {  // (no number below 0)
+    return fminf(fmaxf(float(int(__float_as_uint(largest) >> 23) - (126 + 15)), kLeastShift), 106.0f);
 }
 // 8 halves of ones where the token's bit is set, else of zeros
 __device__ inline u4 halves_of(uint32_t bits) {
