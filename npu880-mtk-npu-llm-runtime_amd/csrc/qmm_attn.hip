@@ -124,6 +124,10 @@ constexpr float kLeastShift = -16.0f;
 __device__ inline float scale_shift(float largest) {  // (no number below 0)
     return fminf(fmaxf(float(int(__float_as_uint(largest) >> 23) - (126 + 15)), kLeastShift), 106.0f);
 }
+// What a row's exponents are taken relative to: its maximum and the shift, or above by up to two units
+// in the maximum's last place, never below. Both were rounded, so a score of 2^24 and more (a float's
+// digits end above the point there) could else make a weight twice what fp16 has room for.
+__device__ inline float raised(float m, float shift) { return m + __builtin_fmaf(fabsf(m), 0x1p-23f, shift); }
 // 8 halves of ones where the token's bit is set, else of zeros
 __device__ inline u4 halves_of(uint32_t bits) {
     u4 r;
@@ -504,9 +508,10 @@ __device__ inline __attribute__((always_inline)) void split_piece(const SplitArg
             }
             shift_v = fmaxf(shift_v, scale_shift(groups_max(big)));
         }
-        const float nb = Q8 ? m + shift_v : m, ms = nb == -__builtin_inff() ? 0.0f : nb;
+        const bool none = m == -__builtin_inff();
+        const float ms = none ? 0.0f : Q8 ? raised(m, shift_v) : m;
         const float alpha = __builtin_amdgcn_exp2f(base - ms);
-        base = nb;
+        base = none ? m : ms;
         float sum = 0.0f;
 #pragma unroll
         for (int j = 0; j < TL; ++j) {
@@ -931,9 +936,10 @@ __device__ inline __attribute__((always_inline)) void tile_piece(const SplitArgs
                 }
                 shift_v = fmaxf(shift_v, scale_shift(big));
             }
-            const float nb = Q8 ? m + shift_v : m, ms = nb == -__builtin_inff() ? 0.0f : nb;
+            const bool none = m == -__builtin_inff();
+            const float ms = none ? 0.0f : Q8 ? raised(m, shift_v) : m;
             const float alpha = __builtin_amdgcn_exp2f(base - ms);
-            base = nb;
+            base = none ? m : ms;
             l *= alpha;
             if (!__all(alpha == 1.0f)) {
 #pragma unroll

@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 import qmm_hip
-from attn_ref import Batch, queries, run_attention
+from attn_ref import F16_HALF, Batch, queries, run_attention
 from gpu_util import say
 
 pytestmark = pytest.mark.gpu
@@ -26,3 +26,36 @@ def test_scales_of_hidden_cells(ctx, D, n, new):
         b.free()
         assert np.isfinite(got[-1]).all() and (got[-1] != 0).any()
         assert np.array_equal(got[0].view(np.uint32), got[-1].view(np.uint32)), f"hidden scales of {hidden} reached a row"
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("n,new", [(300, 1), (9000, 1), (200, 40), (9000, 40)])
+def test_scores_past_the_digits_of_a_float(ctx, n, new, D, sign, q8):
+    """Scores of 2^16 to 2^26 (or their negatives), far apart: a row is the value of its one largest score.
+    Where 24 bits end above the point, no rounding of the maximum makes a weight overflow."""
+    b = Batch([(n, new)], 1, D, 64, q8, seed=n + D)
+    rng = np.random.default_rng(D + new)
+    p, t = b.cells(0)
+    best = rng.integers(0, n - new + 1)  # (every row sees it)
+    size = np.full(n, 0.5 if sign > 0 else 1.0)
+    size[best] = 1.0 if sign > 0 else 0.5
+    if q8:
+        b.k[p, :, t], b.ks[p, :, t] = 64 * sign, size[:, None].astype(np.float32)
+        b.vs[p, :, t] = 0.9995
+    else:
+        b.k[p, :, t] = (64 * sign * size)[:, None, None]
+    v = b.dense(0)[1][0, best]
+    # q . k scale = 64 D q scale, in base 2 times log2 e: spread over 2^16 .. 2^26, with all digits
+    group = 4
+    q = (2.0 ** rng.uniform(0, 10, (new, group))).astype(np.float16)
+    scale = 2.0 ** 16 / (64 * D * 1.4427)
+    say(f"scores of up to 2^26, sign {sign} n={n} new={new} D={D} q8={q8}")
+    b.upload(ctx, new, n)
+    got = run_attention(ctx, b, np.repeat(q, D, 1), group, scale).astype(np.float64)
+    b.free()
+    assert np.isfinite(got).all(), f"{np.count_nonzero(~np.isfinite(got))} values are no numbers"
+    # one weight, of fp16 over the unrounded sum; its product with the scale; the output
+    tol = (2 * F16_HALF + 2.0 ** -20) * np.abs(v) + F16_HALF * 2.0 ** -14
+    assert (np.abs(got.reshape(new, group, D) - v) <= tol).all()
