@@ -4,9 +4,10 @@
 //   S^T [tokens x rows] = K Q^T,   O^T [values x rows] = V^T P^T
 // on fp16 MFMA, 64 tokens a tile, with the running maximum m and sum l of the
 // softmax in base 2 (exp2(s scale log2 e - m)), fp32. The weights P are rounded
-// to fp16 for the second product (half a step, 2^-11, of each; their sum l is of
-// the unrounded ones), outputs once more. Which token a row of an MFMA operand
-// stands for is free, so it is chosen that P stays in the lane that computed it.
+// to fp16 for the second product, 2^15 times as large (half a step, 2^-11, of each
+// down to 2^-29 of the largest, 2^-40 of it below; their sum l is of the unrounded
+// ones), outputs once more. Which token a row of an MFMA operand stands for is
+// free, so it is chosen that P stays in the lane that computed it.
 //
 // Two kernels, by the rows of a sequence's head:
 //  - up to 16 rows (single tokens; a few drafts): memory-bound, every cache byte
@@ -121,6 +122,10 @@ __device__ inline float magnitude_or_0(float x) { return fabsf(x) < __builtin_in
 // overflows), so that a change of k never takes a sum below fp32's range.
 // The exponent is taken from the bits: 0, where a row sees no scale, has the least of all.
 constexpr float kLeastShift = -16.0f;
+// An fp16 cache's weights are p 2^15: all of an fp16's bits down to 2^-29 of the row's largest (the tail
+// of a long context behind one strong key is made of many such weights).
+constexpr float kWeightShift = -15.0f;
+constexpr float kNoScore = -3.402823466e38f;  // the maximum of no score: finite, so that a row of none has weights of 0 without a test
 __device__ inline float scale_shift(float largest) {  // (no number below 0)
     return fminf(fmaxf(float(int(__float_as_uint(largest) >> 23) - (126 + 15)), kLeastShift), 106.0f);
 }
@@ -363,7 +368,7 @@ __device__ inline __attribute__((always_inline)) void split_piece(const SplitArg
             else q[k] = x;
         }
     }
-    float m = -__builtin_inff(), base = m, l = 0.0f, shift_v = kLeastShift;  // (base: m, plus the shift of an 8-bit cache)
+    float m = kNoScore, base = m, l = 0.0f, shift_v = kLeastShift;  // (base: m and the shift, raised)
     f4 acc[DT];
 
     u4 kr[NT][KR], vr[DT][Q8 ? (NU + 1) / 2 : NU];
@@ -508,10 +513,9 @@ __device__ inline __attribute__((always_inline)) void split_piece(const SplitArg
             }
             shift_v = fmaxf(shift_v, scale_shift(groups_max(big)));
         }
-        const bool none = m == -__builtin_inff();
-        const float ms = none ? 0.0f : Q8 ? raised(m, shift_v) : m;
+        const float ms = raised(m, Q8 ? shift_v : kWeightShift);
         const float alpha = __builtin_amdgcn_exp2f(base - ms);
-        base = none ? m : ms;
+        base = ms;
         float sum = 0.0f;
 #pragma unroll
         for (int j = 0; j < TL; ++j) {
@@ -712,7 +716,7 @@ __device__ inline __attribute__((always_inline)) void tile_piece(const SplitArgs
 #pragma unroll
         for (int k = 0; k < KS; ++k) q[k] = *reinterpret_cast<const h8 *>(src + 16 * k);
     }
-    float m = -__builtin_inff(), base = m, l = 0.0f, shift_v = kLeastShift;  // (base: m, plus the shift of an 8-bit cache)
+    float m = kNoScore, base = m, l = 0.0f, shift_v = kLeastShift;  // (base: m and the shift, raised)
     f16v acc[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d)
@@ -936,10 +940,9 @@ __device__ inline __attribute__((always_inline)) void tile_piece(const SplitArgs
                 }
                 shift_v = fmaxf(shift_v, scale_shift(big));
             }
-            const bool none = m == -__builtin_inff();
-            const float ms = none ? 0.0f : Q8 ? raised(m, shift_v) : m;
+            const float ms = raised(m, Q8 ? shift_v : kWeightShift);
             const float alpha = __builtin_amdgcn_exp2f(base - ms);
-            base = none ? m : ms;
+            base = ms;
             l *= alpha;
             if (!__all(alpha == 1.0f)) {
 #pragma unroll

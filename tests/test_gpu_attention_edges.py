@@ -3,10 +3,55 @@ import numpy as np
 import pytest
 
 import qmm_hip
-from attn_ref import F16_HALF, Batch, queries, run_attention
+from attn_ref import F16_HALF, F32_HALF, Batch, queries, run_attention
 from gpu_util import say
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("n,new,group,hint", [
+    (19000, 1, 4, 19000),     # tokens split over workgroups
+    (2000, 1, 4, 2000),
+    (500, 1, 4, 500),         # one workgroup
+    (19000, 1, 4, 1 << 21),   # loads of whole lines
+    (6000, 30, 4, 6000),      # 128 rows, split
+    (400, 40, 4, 400),        # 128 rows, whole
+])
+def test_flat_tail_behind_a_strong_key(ctx, q8, D, n, new, group, hint):
+    """One key takes nearly all of the weight and has no value; what is left is the many others', each
+    1.4 * 2^-24 of it. Weights keep all of an fp16's bits down to 2^-29 of the largest, so the sum is
+    right to its own size, whatever the number of tokens."""
+    b = Batch([(n, new)], 1, D, 64, q8, seed=n + D, max_pages=max(hint, n) // 64 + 1)
+    q = np.ones((b.M, group * D), np.float16)
+    scale = 1.0 / D
+    score = np.log(2.0 ** 24 / 1.4)  # of the first key; 0 of the others
+    p, t = b.cells(0)
+    b.k[p, :, t] = 0
+    b.v[p, :, :, t] = 127 if q8 else 1
+    b.v[p[0], :, :, t[0]] = 0
+    if q8:
+        b.ks[p, :, t], b.vs[p, :, t] = 1.0, 1 / np.float32(127)
+        b.k[p[0], :, t[0]], b.ks[p[0], :, t[0]] = 127, np.float32(score / 127)
+    else:
+        b.k[p[0], :, t[0]] = score
+    say(f"flat tail n={n} new={new} D={D} q8={q8} hint={hint}")
+    b.upload(ctx, new, hint)
+    got = run_attention(ctx, b, q, group, scale, out_type=qmm_hip.TYPE_F32).astype(np.float64)
+    b.free()
+    k, v = b.dense(0)
+    first = np.exp(-(k[0, 0] @ q[0, :D].astype(np.float64)) * scale)
+    for i in range(new):
+        tail = (n - new + i) * first
+        ref = tail / (1 + tail) * v[0, 1, 0]
+        # the first score: D products of equal size summed in fp32, and its product with the scale in base 2; the
+        # exponential; each weight's rounding (2^-25 of 2^15 at the largest, 8-bit of 2^9); the output's
+        e = 2 * (D + 8) * F32_HALF * score + F16_HALF + (n / 8 + 32) * F32_HALF
+        small = n * 2.0 ** -25 * 2.0 ** -(9 if q8 else 15)
+        tol = 1.01 * (F16_HALF * (ref + 2.0 ** -14) + e * ref + small)
+        d = np.abs(got[i] - ref).max()
+        assert d <= tol, f"row {i}: off by {d:.3g} of {ref:.3g}, bound {tol:.3g}"
 
 
 @pytest.mark.parametrize("D", [64, 128, 256])
