@@ -64,11 +64,10 @@ struct SplitArgs {
 };
 constexpr int kMaxShared = 512;  // sequences of a call whose tiles workers share
 
-// the largest of three (a NaN counts for nothing)
+// The largest of three (a NaN counts for nothing), as one instruction. Not as inline assembly: the
+// compiler puts no wait between an MFMA and assembly that reads its result.
 __device__ inline float max3(float a, float b, float c) {
-    float r;
-    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-    return r;
+    return __builtin_elementwise_maximumnum(__builtin_elementwise_maximumnum(a, b), c);
 }
 // maximum / sum over the four lane groups (lanes l, l ^ 16, l ^ 32, l ^ 48)
 __device__ inline float groups_max(float v) {
