@@ -21,8 +21,8 @@
 #include <vector>
 
 #include "../../include/qmm_hip.h"
-#include "qmm_attn.h"
 #include "qmm_attn_check.h"
+#include "qmm_attn_plan.h"
 #include "qmm_device.h"
 
 // Device scratch of qmm_gemm_multi_dispatch_noalloc: the quantized input

@@ -71,6 +71,22 @@ QMM_HD inline int page_of(const KvView &b, int s, int token, int len) {
     return unsigned(id) < unsigned(b.n_pages) ? id : -1;
 }
 
+struct AttnArgs {
+    KvView b;
+    const uint16_t *q;
+    size_t q_stride;
+    void *out;
+    size_t out_stride;
+    int out_f32;
+    int head_dim, group;  // query heads per key-value head; n_rows * group < 2^30
+    unsigned group_inv;   // ceil(2^32 / group)
+    float scale;
+    int window, sinks;
+    const void *kc, *vc;
+    const float *ks, *vs;
+    int max_new, max_kv;  // the host's hints, > 0
+};
+
 }  // namespace qmm
 
 #ifdef __HIPCC__
@@ -104,23 +120,6 @@ struct AppendArgs {
 };
 hipError_t launch_kv_append(const AppendArgs &a, hipStream_t s);
 
-struct AttnArgs {
-    KvView b;
-    const uint16_t *q;
-    size_t q_stride;
-    void *out;
-    size_t out_stride;
-    int out_f32;
-    int head_dim, group;  // query heads per key-value head; n_rows * group < 2^30
-    unsigned group_inv;   // ceil(2^32 / group)
-    float scale;
-    int window, sinks;
-    const void *kc, *vc;
-    const float *ks, *vs;
-    int max_new, max_kv;  // the host's hints, > 0
-};
-// scratch a call makes use of (0: it does not split)
-size_t attn_scratch_bytes(const AttnArgs &a, int cu_count);
 hipError_t launch_attention(const AttnArgs &a, void *scratch, size_t scratch_bytes, int cu_count, hipStream_t s);
 
 }  // namespace qmm

@@ -1,0 +1,99 @@
+// qmm_attn_plan.h — how a call of the attention is launched: row tiles, who
+// shares which work, and the scratch that takes. Plain C++: a host program can
+// check it without a device.
+#pragma once
+
+#include <algorithm>
+
+#include "qmm_attn.h"
+
+namespace qmm {
+
+constexpr int kMaxShared = 512;  // sequences of a call whose tiles workers share
+// A segment (a row tile of a sequence's head) whose tiles several workers of the
+// split kernel share, as the worker that has its first tile leaves it for the join.
+struct SharedSegment {
+    int pieces;  // its own and those of the next workers; below 2: nothing to join
+    int seq, head, row0, rows, pad[3];
+};
+
+// How sequences of a call are launched.
+struct SplitPlan {
+    int rows;      // of a row tile: 16 or 128
+    int workers;   // that share all tiles (0: a workgroup for each head, or with 128 rows each row tile)
+    int nw;        // waves, with 16 rows
+    bool lines;    // loads of whole cache lines, with 16 rows
+    int row_tiles;
+    int new_min, new_max;
+    size_t slots, bytes;  // partial rows; all of the scratch
+};
+
+inline int few_tokens(const AttnArgs &a) { return a.group > 16 ? 1 : 16 / a.group; }
+
+// tiles of a row tile of R rows, as the host knows it
+inline int64_t hinted_tiles(const AttnArgs &a, int R) {
+    const int64_t tiles = (a.max_kv - 1) / kTileKeys + 1;
+    if (a.window <= 0) return tiles;
+    const int64_t most = (int64_t(a.window) + R / a.group + 1) / kTileKeys + (int64_t(a.sinks) + kTileKeys - 1) / kTileKeys + 3;
+    return most < tiles ? most : tiles;
+}
+
+// Tiles up to which a head of a sequence is one workgroup's. A workgroup takes 5 us and 0.62 us
+// a tile; shared work 11.5 us and 4.5 us for 1000 tiles of all heads, its join included. us,
+// whole / shared (8 heads of 128): 8 heads of 11 tiles 11.1 / 13.9, of 16 14.2 / 11.1; 32 of 16
+// 15.9 / 13.0; 64 of 16 16.1 / 16.0, of 28 23.4 / 18.4; 128 of 16 17.0 / 22.0; 256 of 32 44 / 53.
+inline int64_t short_tiles(int64_t heads) { return std::min<int64_t>(32, 10 + heads / 6); }
+
+// Bytes of cache from which loads take whole lines and leave them in no cache: what is less
+// may be there from one call to the next (the last one holds 256 MB). us, as operands have
+// them / whole lines: 57 MB 21.7 / 23.0, 86 MB 25.8 / 28.6, 115 MB 33.3 / 31.9, 230 MB
+// 56.0 / 49.8; 0.4 MB 8.0 / 8.5 (more code to fetch).
+constexpr int64_t kLargeBytes = int64_t(96) << 20;
+
+// max_new: the most new tokens of the sequences it is for
+inline SplitPlan plan_split(const AttnArgs &a, int max_new, int cu_count, size_t scratch) {
+    SplitPlan p{};
+    const int64_t rows = int64_t(max_new) * a.group;
+    const int R = p.rows = max_new <= few_tokens(a) ? 16 : 128;
+    const int64_t tiles = hinted_tiles(a, R), units = int64_t(a.b.n_seqs) * a.b.n_heads, row_tiles = (rows + R - 1) / R;
+    const int per_cu = R == 128 && a.head_dim > 128 ? 1 : 2;  // workgroups a CU holds
+    const size_t each = 2 * size_t(R) * (size_t(a.head_dim) * 4 + 8) + sizeof(SharedSegment);
+    int64_t workers = std::min(cu_count, 512) * int64_t(per_cu);
+    if (size_t(workers) * each + sizeof(SharedSegment) > scratch) workers = int64_t(scratch / each) - 1;
+    // (units of the shared work: all that there can be, were every sequence to claim all rows)
+    const int64_t each_seq = (int64_t(a.b.n_rows) * a.group / R + 1) * (kv_capacity(a.b.max_pages, a.b.page_shift) / kTileKeys + 1);
+    const bool countable = each_seq < (int64_t(1) << 31) / units;
+    const bool few_tiles = R == 16 ? tiles <= short_tiles(units) : units * row_tiles >= 2 * per_cu * cu_count || tiles <= 8;
+    p.new_max = 0x7fffffff;
+    if (!few_tiles && a.b.n_seqs <= kMaxShared && workers > units / 4 && countable) {
+        p.workers = int(workers);
+        p.slots = size_t(workers) * 2 * R;
+        p.bytes = size_t(workers) * each + sizeof(SharedSegment);
+    }
+    p.nw = R == 16 && !p.workers && a.head_dim <= 128 && units <= 2 * cu_count && tiles > 4 ? 8 : 4;
+    p.lines = R == 16 && tiles * units >= kLargeBytes / (int64_t(kTileKeys) * a.head_dim * (a.ks ? 2 : 4));
+    p.row_tiles = int(std::min<int64_t>(row_tiles, 65535));
+    return p;
+}
+
+// one or two plans; the number of them
+inline int plan_call(const AttnArgs &a, int cu_count, size_t scratch, SplitPlan out[2]) {
+    const int few = few_tokens(a);
+    out[0] = plan_split(a, a.max_new, cu_count, scratch);
+    // one row tile at most; one sequence, or all of the same many rows: nothing is left for another kernel
+    if (int64_t(a.max_new) * a.group <= 128 || a.b.n_seqs == 1 || int64_t(a.b.n_seqs) * a.max_new <= a.b.n_rows) return 1;
+    out[0].new_min = few + 1;
+    out[1] = plan_split(a, few, cu_count, scratch - out[0].bytes);
+    out[1].new_max = few;
+    return 2;
+}
+
+// scratch a call makes use of (0: it does not split)
+inline size_t attn_scratch_bytes(const AttnArgs &a, int cu_count) {
+    SplitPlan pl[2];
+    size_t n = 0;
+    for (int i = plan_call(a, cu_count, ~size_t(0), pl); i-- > 0;) n += pl[i].bytes;
+    return n;
+}
+
+}  // namespace qmm
