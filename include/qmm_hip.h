@@ -415,8 +415,12 @@ typedef struct {
 /* Device scratch for partial results where a row's tokens are split over
  * workgroups. Calls that may overlap (two streams, two graphs replayed on two
  * streams) need one each; calls in stream order can share one. It holds nothing
- * between calls. A smaller one than qmm_attention_workspace_bytes means fewer
- * splits, never another result than by the order of the sums. */
+ * between calls. qmm_attention_workspace_bytes is what this call and every other
+ * over as many heads of this size, with as many query heads and no more new
+ * tokens of a sequence (max_new; 0: n_rows), makes use of, whatever the number
+ * of sequences and their lengths: a program asks once, for its longest prompt. A
+ * smaller one means fewer splits or none, never another result than by the order
+ * of the sums. */
 typedef struct qmm_attn_workspace qmm_attn_workspace;
 size_t qmm_attention_workspace_bytes(qmm_context *ctx, const qmm_kv_batch *batch, const qmm_kv_cache *cache,
                                      const qmm_attention_args *args);

@@ -50,25 +50,42 @@ inline int64_t short_tiles(int64_t heads) { return std::min<int64_t>(32, 10 + he
 // 56.0 / 49.8; 0.4 MB 8.0 / 8.5 (more code to fetch).
 constexpr int64_t kLargeBytes = int64_t(96) << 20;
 
+// All workers of shared work with row tiles of R rows, and what one takes of the scratch: partial
+// results of two pieces, and a segment.
+struct Sharing {
+    int64_t workers;
+    size_t each;
+    size_t bytes() const { return size_t(workers) * each + sizeof(SharedSegment); }
+};
+inline int workgroups_of_cu(const AttnArgs &a, int R) { return R == 128 && a.head_dim > 128 ? 1 : 2; }
+inline Sharing sharing(const AttnArgs &a, int R, int cu_count) {
+    return Sharing{std::min(cu_count, 512) * int64_t(workgroups_of_cu(a, R)), 2 * size_t(R) * (size_t(a.head_dim) * 4 + 8) + sizeof(SharedSegment)};
+}
+
 // max_new: the most new tokens of the sequences it is for
 inline SplitPlan plan_split(const AttnArgs &a, int max_new, int cu_count, size_t scratch) {
     SplitPlan p{};
     const int64_t rows = int64_t(max_new) * a.group;
     const int R = p.rows = max_new <= few_tokens(a) ? 16 : 128;
     const int64_t tiles = hinted_tiles(a, R), units = int64_t(a.b.n_seqs) * a.b.n_heads, row_tiles = (rows + R - 1) / R;
-    const int per_cu = R == 128 && a.head_dim > 128 ? 1 : 2;  // workgroups a CU holds
-    const size_t each = 2 * size_t(R) * (size_t(a.head_dim) * 4 + 8) + sizeof(SharedSegment);
-    int64_t workers = std::min(cu_count, 512) * int64_t(per_cu);
-    if (size_t(workers) * each + sizeof(SharedSegment) > scratch) workers = int64_t(scratch / each) - 1;
+    const Sharing all = sharing(a, R, cu_count);
+    // Room for fewer workers than all: only where they are no fewer than the workgroups that run at
+    // once without sharing.
+    int64_t workers = all.workers;
+    bool enough = workers > units / 4;
+    if (all.bytes() > scratch) {
+        workers = int64_t(scratch / all.each) - 1;
+        enough = workers >= std::min(all.workers, R == 16 ? units : units * row_tiles);
+    }
     // (units of the shared work: all that there can be, were every sequence to claim all rows)
     const int64_t each_seq = (int64_t(a.b.n_rows) * a.group / R + 1) * (kv_capacity(a.b.max_pages, a.b.page_shift) / kTileKeys + 1);
     const bool countable = each_seq < (int64_t(1) << 31) / units;
-    const bool few_tiles = R == 16 ? tiles <= short_tiles(units) : units * row_tiles >= 2 * per_cu * cu_count || tiles <= 8;
+    const bool few_tiles = R == 16 ? tiles <= short_tiles(units) : units * row_tiles >= 2 * workgroups_of_cu(a, R) * cu_count || tiles <= 8;
     p.new_max = 0x7fffffff;
-    if (!few_tiles && a.b.n_seqs <= kMaxShared && workers > units / 4 && countable) {
+    if (!few_tiles && a.b.n_seqs <= kMaxShared && enough && countable) {
         p.workers = int(workers);
         p.slots = size_t(workers) * 2 * R;
-        p.bytes = size_t(workers) * each + sizeof(SharedSegment);
+        p.bytes = Sharing{workers, all.each}.bytes();
     }
     p.nw = R == 16 && !p.workers && a.head_dim <= 128 && units <= 2 * cu_count && tiles > 4 ? 8 : 4;
     p.lines = R == 16 && tiles * units >= kLargeBytes / (int64_t(kTileKeys) * a.head_dim * (a.ks ? 2 : 4));
@@ -88,11 +105,11 @@ inline int plan_call(const AttnArgs &a, int cu_count, size_t scratch, SplitPlan 
     return 2;
 }
 
-// scratch a call makes use of (0: it does not split)
+// Scratch with which no call is short of workers: this one, or any other over as many heads of this
+// size with no more new tokens of a sequence. (How many workers share does not depend on the lengths.)
 inline size_t attn_scratch_bytes(const AttnArgs &a, int cu_count) {
-    SplitPlan pl[2];
-    size_t n = 0;
-    for (int i = plan_call(a, cu_count, ~size_t(0), pl); i-- > 0;) n += pl[i].bytes;
+    size_t n = sharing(a, 16, cu_count).bytes();
+    if (a.max_new > few_tokens(a)) n += sharing(a, 128, cu_count).bytes();  // (both, where a call has sequences of both kinds)
     return n;
 }
 

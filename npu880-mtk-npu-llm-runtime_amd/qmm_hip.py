@@ -471,7 +471,8 @@ class Context:
         return _Handle(self, h.value, "qmm_rope_destroy")
 
     def attention_workspace(self, batch: KvBatch, cache: KvCache, args: AttentionArgs) -> _Handle:
-        """A workspace for calls up to this one's size (qmm_attention_workspace_bytes / _create)."""
+        """A workspace for this call and all others over as many heads of this size with no more new tokens of a
+        sequence (qmm_attention_workspace_bytes / _create)."""
         n = self.lib.qmm_attention_workspace_bytes(self._h, C.byref(batch), C.byref(cache), C.byref(args))
         h = _p()
         self._call("qmm_attention_workspace_create", self._h, n, C.byref(h))

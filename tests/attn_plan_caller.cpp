@@ -1,0 +1,85 @@
+// How calls of the attention are launched, without a device: what a workspace
+// made for one call does to others. Prints one line per failure and "ok" at the end.
+#include <cstdio>
+#include <random>
+
+#include "../npu880-mtk-npu-llm-runtime_amd/csrc/qmm_attn_plan.h"
+
+using namespace qmm;
+
+static int bad = 0;
+#define EXPECT(c, ...) do { if (!(c)) { if (++bad < 20) { std::printf("%s: ", #c); std::printf(__VA_ARGS__); std::printf("\n"); } } } while (0)
+
+static AttnArgs call(int seqs, int rows, int max_new, int max_kv, int heads = 8, int group = 4, int dim = 128) {
+    AttnArgs a{};
+    a.b = KvView{nullptr, nullptr, nullptr, seqs, rows, 1 << 14, 1 << 20, 6, heads};
+    a.group = group;
+    a.head_dim = dim;
+    a.max_new = max_new;
+    a.max_kv = max_kv;
+    return a;
+}
+static const size_t kAny = ~size_t(0) / 2;
+static const int kCus = 256;
+
+static bool same(const SplitPlan &x, const SplitPlan &y) {
+    return x.rows == y.rows && x.workers == y.workers && x.nw == y.nw && x.lines == y.lines && x.row_tiles == y.row_tiles &&
+           x.new_min == y.new_min && x.new_max == y.new_max && x.bytes == y.bytes;
+}
+
+// `later` with the workspace of `made` runs as with any
+static void covered(const AttnArgs &made, const AttnArgs &later, const char *what) {
+    SplitPlan with[2], free[2];
+    const int n = plan_call(later, kCus, attn_scratch_bytes(made, kCus), with);
+    EXPECT(plan_call(later, kCus, kAny, free) == n, "%s", what);
+    for (int i = 0; i < n; ++i) EXPECT(same(with[i], free[i]), "%s: %d workers of %d", what, with[i].workers, free[i].workers);
+}
+
+// workgroups of a plan that can run at once
+static int64_t at_once(const AttnArgs &a, const SplitPlan &p, int max_new) {
+    const int64_t units = int64_t(a.b.n_seqs) * a.b.n_heads, most = sharing(a, p.rows, kCus).workers;
+    const int64_t tiles = (int64_t(max_new) * a.group + p.rows - 1) / p.rows;
+    return std::min(most, p.workers ? p.workers : p.rows == 16 ? units : units * tiles);
+}
+static void no_worse_than_none(const AttnArgs &a, size_t scratch, const char *what) {
+    SplitPlan with[2], none[2];
+    const int n = plan_call(a, kCus, scratch, with);
+    EXPECT(plan_call(a, kCus, 0, none) == n, "%s", what);
+    size_t bytes = 0;
+    for (int i = 0; i < n; ++i) {
+        const int rows = i ? few_tokens(a) : a.max_new;
+        bytes += with[i].bytes;
+        EXPECT(at_once(a, with[i], rows) >= at_once(a, none[i], rows), "%s: %d workers, %lld workgroups without", what, with[i].workers,
+               (long long)at_once(a, none[i], rows));
+    }
+    EXPECT(bytes <= scratch, "%s: %zu bytes of %zu", what, bytes, scratch);
+}
+
+int main() {
+    const AttnArgs prompt = call(1, 8192, 8192, 8192), token = call(1, 1, 1, 131071), batch = call(32, 32, 1, 8000);
+    const AttnArgs drafts = call(28, 28 * 8, 8, 4000), many = call(600, 600, 1, 2000), mixed = call(9, 600, 512, 9000);
+    covered(prompt, token, "a prompt's workspace, one token");
+    covered(prompt, batch, "a prompt's workspace, a batch");
+    covered(prompt, drafts, "a prompt's workspace, drafts");
+    covered(prompt, mixed, "a prompt's workspace, prompts and tokens");
+    covered(many, token, "that of many sequences, one token");
+    covered(batch, token, "a batch's, one token");
+    covered(token, batch, "one token's, a batch");
+    for (size_t scratch : {size_t(0), size_t(1) << 16, size_t(1) << 20, attn_scratch_bytes(token, kCus), attn_scratch_bytes(prompt, kCus), kAny})
+        for (const AttnArgs *a : {&prompt, &token, &batch, &drafts, &many, &mixed}) no_worse_than_none(*a, scratch, "scratch of any size");
+
+    std::mt19937 rng(5);
+    auto any = [&](int lo, int hi) { return std::uniform_int_distribution<int>(lo, hi)(rng); };
+    for (int i = 0; i < 20000; ++i) {
+        const int heads = any(1, 16), group = any(1, 20), dim = 64 << any(0, 2);
+        auto one = [&](int most_new) {
+            const int seqs = any(1, 1 << any(0, 10)), max_new = any(1, most_new);
+            return call(seqs, any(max_new, std::max(max_new, seqs * max_new)), max_new, any(max_new, 1 << any(13, 19)), heads, group, dim);
+        };
+        const AttnArgs made = one(1 << any(0, 12)), later = one(made.max_new);
+        covered(made, later, "any call");
+        no_worse_than_none(later, size_t(any(0, 1 << any(4, 30))), "any scratch");
+    }
+    std::printf(bad ? "%d failures\n" : "ok\n", bad);
+    return bad != 0;
+}

@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 import qmm_hip
-from attn_ref import F16_HALF, F32_HALF, Batch, queries, run_attention
+from attn_ref import F16_HALF, F32_HALF, Batch, attend, check_rows, queries, run_attention
 from gpu_util import say
 
 pytestmark = pytest.mark.gpu
@@ -104,3 +104,28 @@ def test_scores_past_the_digits_of_a_float(ctx, n, new, D, sign, q8):
     # one weight, of fp16 over the unrounded sum; its product with the scale; the output
     tol = (2 * F16_HALF + 2.0 ** -20) * np.abs(v) + F16_HALF * 2.0 ** -14
     assert (np.abs(got.reshape(new, group, D) - v) <= tol).all()
+
+
+@pytest.mark.parametrize("q8", [False, True])
+def test_workspace_of_another_call(ctx, q8):
+    """One made for a prompt serves single tokens, drafts and both together: the bits of a workspace of
+    their own, as they run on as many workgroups."""
+    prompt = Batch([(700, 700)], 2, 128, 64, q8, seed=61).upload(ctx, 700, 700)
+    q = queries(prompt, 4)
+    args = qmm_hip.AttentionArgs(1 << 20, q.shape[1], 8, 0.1, 0, 0, 1 << 20, qmm_hip.TYPE_F16, q.shape[1])  # (not run)
+    ws = ctx.attention_workspace(prompt.batch, prompt.cache, args)
+    prompt.free()
+    for lens in ([(9000, 1)], [(5000, 7), (3000, 3)], [(4000, 60), (6000, 1), (2500, 2)]):
+        b = Batch(lens, 2, 128, 64, q8, seed=62).upload(ctx, max(n for _, n in lens), max(n for n, _ in lens))
+        q = queries(b, 4)
+        say(f"a prompt's workspace for {lens} q8={q8}")
+        got = run_attention(ctx, b, q, 4, 0.1, ws=ws)
+        own = run_attention(ctx, b, q, 4, 0.1)
+        none = run_attention(ctx, b, q, 4, 0.1, workspace=False)
+        b.free()
+        ref, tol = attend(b, q, 4, 0.1)
+        for o in (got, none):
+            check_rows(o, ref, tol, b.held_rows)
+        assert np.array_equal(got.view(np.uint16), own.view(np.uint16))
+        assert not np.array_equal(got.view(np.uint16), none.view(np.uint16)), "work was not shared"
+    ws.free()
