@@ -418,7 +418,8 @@ typedef struct {
  * between calls. qmm_attention_workspace_bytes is what this call and every other
  * over as many heads of this size, with as many query heads and no more new
  * tokens of a sequence (max_new; 0: n_rows), makes use of, whatever the number
- * of sequences and their lengths: a program asks once, for its longest prompt. A
+ * of sequences and their lengths: a program asks once, for its longest prompt (0:
+ * arguments that the attention refuses; qmm_last_error has the reason). A
  * smaller one means fewer splits or none, never another result than by the order
  * of the sums. */
 typedef struct qmm_attn_workspace qmm_attn_workspace;

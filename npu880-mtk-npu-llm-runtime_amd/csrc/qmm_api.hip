@@ -989,7 +989,7 @@ size_t qmm_attention_workspace_bytes(qmm_context *ctx, const qmm_kv_batch *batch
                                      const qmm_attention_args *args) {
     qmm::AttnArgs a{};
     int cus = 0;
-    if (!ctx || attn_args(ctx, batch, cache, args, a) || batch->n_rows == 0 || batch->n_seqs == 0) return 0;
+    if (!ctx || attn_args(ctx, batch, cache, args, a)) return 0;
     if (cu_count(ctx, cus)) return 0;
     return qmm::attn_scratch_bytes(a, cus);
 }

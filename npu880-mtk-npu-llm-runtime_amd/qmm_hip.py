@@ -474,6 +474,8 @@ class Context:
         """A workspace for this call and all others over as many heads of this size with no more new tokens of a
         sequence (qmm_attention_workspace_bytes / _create)."""
         n = self.lib.qmm_attention_workspace_bytes(self._h, C.byref(batch), C.byref(cache), C.byref(args))
+        if n == 0:
+            raise QmmError(QMM_EINVAL, f"qmm_attention_workspace_bytes: {self.last_error()}")
         h = _p()
         self._call("qmm_attention_workspace_create", self._h, n, C.byref(h))
         return _Handle(self, h.value, "qmm_attention_workspace_destroy")

@@ -129,3 +129,18 @@ def test_workspace_of_another_call(ctx, q8):
         assert np.array_equal(got.view(np.uint16), own.view(np.uint16))
         assert not np.array_equal(got.view(np.uint16), none.view(np.uint16)), "work was not shared"
     ws.free()
+
+
+def test_workspace_of_refused_arguments(ctx):
+    """No workspace for a call that the attention refuses, with its reason; one for a call of no rows."""
+    b = Batch([(20, 1)], 2, 64, 16, seed=50).upload(ctx, 1, 20)
+    make = lambda **kw: qmm_hip.AttentionArgs(**{**dict(  # noqa: E731
+        q=1 << 20, q_stride=256, q_heads=4, scale=0.1, out=1 << 20, out_type=qmm_hip.TYPE_F16, out_stride=256), **kw})
+    say("workspaces of refused arguments")
+    for kw, why in ((dict(q_heads=3), "q_heads"), (dict(scale=0.0), "scale"), (dict(window=-1), "window"), (dict(q_stride=8), "stride")):
+        with pytest.raises(qmm_hip.QmmError, match=why):
+            ctx.attention_workspace(b.batch, b.cache, make(**kw))
+    ctx.attention_workspace(b.batch, b.cache, make()).free()
+    b.batch.n_rows = 0
+    ctx.attention_workspace(b.batch, b.cache, make(q=None, out=None)).free()
+    b.free()
