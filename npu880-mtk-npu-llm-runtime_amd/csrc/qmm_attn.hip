@@ -1071,7 +1071,8 @@ template <int D, int R, int NW, bool Q8, bool LINES>
 __global__ __launch_bounds__(64 * NW, R == 128 && D > 128 ? 1 : 2) void attn_split_kernel(SplitArgs p) {
     constexpr int kLeast = R == 16 ? NW : 4;  // units of a worker, where all are fewer than the workers could take
     __shared__ std::conditional_t<R == 16, SplitShared<D, NW>, TileShared<D>> sh;
-    __shared__ int upto[kMaxShared + 1], sums[NW];
+    __shared__ int upto[kMaxShared + 1];
+    __shared__ uint32_t sums[NW];
     const AttnArgs &a = p.a;
     const int H = a.b.n_heads, G = a.group;
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1081,41 +1082,41 @@ __global__ __launch_bounds__(64 * NW, R == 128 && D > 128 ? 1 : 2) void attn_spl
     int at = 0, stop = 1;
     if (p.workers) {  // the units of every sequence, summed
         constexpr int N = kMaxShared / (64 * NW);  // sequences of a thread
-        int mine[N], sum = 0;
+        uint32_t mine[N], sum = 0;
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             const int q = int(threadIdx.x) * N + j;
             mine[j] = 0;
             if (q < a.b.n_seqs) {
                 const SeqView v = seq_view(a.b, q);
-                if (v.n_new >= p.new_min && v.n_new <= p.new_max)
-                    for (int rt = 0; rt * R < v.n_new * G; ++rt) mine[j] += row_tile<R>(a, v, rt).units;
+                if (v.n_new >= p.new_min && v.n_new <= p.new_max)  // (one sequence's stay below 2^31)
+                    for (int rt = 0; rt * R < v.n_new * G; ++rt) mine[j] += unsigned(row_tile<R>(a, v, rt).units);
             }
-            sum += mine[j];
+            sum = capped_sum(sum, mine[j]);
         }
-        int before = sum;
+        uint32_t before = sum;
 #pragma unroll
         for (int o = 1; o < 64; o *= 2) {
-            const int x = __shfl_up(before, o);
-            before += lane >= o ? x : 0;
+            const uint32_t x = __shfl_up(before, o);
+            before = capped_sum(before, lane >= o ? x : 0);
         }
         if (lane == 63) sums[wid] = before;
         before -= sum;
         __syncthreads();
-        int total = 0;
+        uint32_t total = 0;
         for (int w = 0; w < NW; ++w) {
             if (w < wid) before += sums[w];
-            total += sums[w];
+            total = capped_sum(total, sums[w]);
         }
         if (threadIdx.x == 0) upto[0] = 0;
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             before += mine[j];
-            upto[threadIdx.x * N + j + 1] = before;
+            upto[threadIdx.x * N + j + 1] = int(before);
         }
         __syncthreads();
-        total = __builtin_amdgcn_readfirstlane(total) * H;
-        work.set(total, min(p.workers, (total + kLeast - 1) / kLeast));
+        const int units = call_units(__builtin_amdgcn_readfirstlane(total), H);  // (none: no worker reads upto)
+        work.set(units, min(p.workers, units / kLeast + (units % kLeast != 0)));
         if (threadIdx.x == 0 && blockIdx.x == 0) p.shared[p.workers].pieces = work.workers;  // (for the join)
         if constexpr (R == 128) {
             // workgroups b, b + 8, .. run on one XCD: they are neighbours in the work, and the

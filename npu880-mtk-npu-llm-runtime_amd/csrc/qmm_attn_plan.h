@@ -17,6 +17,15 @@ struct SharedSegment {
     int seq, head, row0, rows, pad[3];
 };
 
+// Units (tiles of row tiles) of one head, summed over sequences: at the top instead of past it, and
+// those of all heads: 0, nothing to share, from 2^31 on. Row starts that fall let every sequence claim
+// all rows, so the count can pass what the host allowed for.
+constexpr int64_t kMostUnits = int64_t(1) << 31;
+QMM_HD constexpr uint32_t capped_sum(uint32_t x, uint32_t y) { return x + y < x ? ~0u : x + y; }
+QMM_HD constexpr int call_units(uint32_t of_head, int heads) {
+    return uint64_t(of_head) * unsigned(heads) < uint64_t(kMostUnits) ? int(of_head * unsigned(heads)) : 0;
+}
+
 // How sequences of a call are launched.
 struct SplitPlan {
     int rows;      // of a row tile: 16 or 128
@@ -77,9 +86,10 @@ inline SplitPlan plan_split(const AttnArgs &a, int max_new, int cu_count, size_t
         workers = int64_t(scratch / all.each) - 1;
         enough = workers >= std::min(all.workers, R == 16 ? units : units * row_tiles);
     }
-    // (units of the shared work: all that there can be, were every sequence to claim all rows)
-    const int64_t each_seq = (int64_t(a.b.n_rows) * a.group / R + 1) * (kv_capacity(a.b.max_pages, a.b.page_shift) / kTileKeys + 1);
-    const bool countable = each_seq < (int64_t(1) << 31) / units;
+    // Units of the shared work, were every row tile to see all that a sequence can hold (row starts that
+    // ascend; others are counted where they are read)
+    const int64_t most_tiles = int64_t(a.b.n_rows) * a.group / R + a.b.n_seqs, most_span = kv_capacity(a.b.max_pages, a.b.page_shift) / kTileKeys + 1;
+    const bool countable = most_tiles * most_span < kMostUnits / a.b.n_heads;
     const bool few_tiles = R == 16 ? tiles <= short_tiles(units) : units * row_tiles >= 2 * workgroups_of_cu(a, R) * cu_count || tiles <= 8;
     p.new_max = 0x7fffffff;
     if (!few_tiles && a.b.n_seqs <= kMaxShared && enough && countable) {

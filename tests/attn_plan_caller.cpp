@@ -1,5 +1,5 @@
-// How calls of the attention are launched, without a device: what a workspace
-// made for one call does to others. Prints one line per failure and "ok" at the end.
+// How calls of the attention are launched, without a device: when work is
+// shared, and what a workspace made for one call does to others. Prints one line per failure and "ok" at the end.
 #include <cstdio>
 #include <random>
 
@@ -55,7 +55,43 @@ static void no_worse_than_none(const AttnArgs &a, size_t scratch, const char *wh
     EXPECT(bytes <= scratch, "%s: %zu bytes of %zu", what, bytes, scratch);
 }
 
+// Where work is shared, its units stay below 2^31 for every ragged batch of ascending row starts;
+// and page tables of room for long sequences do not keep short ones from sharing.
+static void counts() {
+    SplitPlan p[2];
+    AttnArgs a = call(256, 256, 1, 9000, 4, 8);
+    a.b.max_pages = 1 << 14;  // of 64 tokens
+    plan_call(a, kCus, kAny, p);
+    EXPECT(p[0].workers == 512, "%d workers for 256 sequences with tables of 2^20 tokens", p[0].workers);
+    std::mt19937 rng(6);
+    auto any = [&](int lo, int hi) { return std::uniform_int_distribution<int>(lo, hi)(rng); };
+    int shared = 0;
+    for (int i = 0; i < 20000; ++i) {
+        const int seqs = any(1, 1 << any(0, 9)), rows = any(1, 1 << any(0, 16));
+        AttnArgs a = call(seqs, rows, any(1, rows), any(1, 1 << 20), any(1, 1 << any(0, 8)), any(1, 40));
+        a.b.max_pages = any(1, 1 << any(0, 24));
+        for (int n = plan_call(a, kCus, kAny, p), k = 0; k < n; ++k) {
+            if (!p[k].workers) continue;
+            ++shared;
+            const int64_t span = kv_capacity(a.b.max_pages, a.b.page_shift) / kTileKeys + 1;
+            int64_t units = 0, left = rows;
+            for (int s = 0; s < seqs; ++s) {
+                const int64_t mine = s + 1 < seqs ? any(0, int(left)) : left;
+                units += (mine * a.group + p[k].rows - 1) / p[k].rows * span;
+                left -= mine;
+            }
+            EXPECT(units * a.b.n_heads < kMostUnits, "%lld units", (long long)(units * a.b.n_heads));
+            EXPECT(call_units(uint32_t(units), a.b.n_heads) == units * a.b.n_heads, "units");
+        }
+    }
+    EXPECT(shared > 2000, "%d plans that share", shared);
+    EXPECT(capped_sum(~0u - 3, 3) == ~0u && capped_sum(~0u - 3, 4) == ~0u && capped_sum(~0u, ~0u) == ~0u && capped_sum(7, 8) == 15, "sums");
+    EXPECT(call_units(1u << 30, 2) == 0 && call_units((1u << 30) - 1, 2) == 0x7ffffffe && call_units(~0u, 65535) == 0 && call_units(~0u, 1) == 0 &&
+               call_units(0, 9) == 0 && call_units(0x7fffffffu, 1) == 0x7fffffff, "units of a call");
+}
+
 int main() {
+    counts();
     const AttnArgs prompt = call(1, 8192, 8192, 8192), token = call(1, 1, 1, 131071), batch = call(32, 32, 1, 8000);
     const AttnArgs drafts = call(28, 28 * 8, 8, 4000), many = call(600, 600, 1, 2000), mixed = call(9, 600, 512, 9000);
     covered(prompt, token, "a prompt's workspace, one token");

@@ -5,9 +5,9 @@ import subprocess
 HERE = os.path.dirname(os.path.abspath(__file__))
 
 
-def test_workspaces_of_other_calls(tmp_path):
-    """A workspace serves calls of any length and batch as one of their own would, and a small one never
-    leaves fewer workgroups than none."""
+def test_launches(tmp_path):
+    """A workspace serves calls of any length and batch as one of their own would, a small one never leaves
+    fewer workgroups than none, and shared work can always be counted."""
     exe = str(tmp_path / "attn_plan_caller")
     r = subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-fsanitize=undefined", "-fno-sanitize-recover=all",
                         os.path.join(HERE, "attn_plan_caller.cpp"), "-o", exe], capture_output=True, text=True, timeout=120)

@@ -144,3 +144,30 @@ def test_workspace_of_refused_arguments(ctx):
     b.batch.n_rows = 0
     ctx.attention_workspace(b.batch, b.cache, make(q=None, out=None)).free()
     b.free()
+
+
+def test_rows_claimed_past_any_count(ctx):
+    """Row starts that fall, so that 256 sequences of 2^21 tokens claim all 1024 rows: more work than can be
+    counted is not begun, and the next call is as always."""
+    S, H, P, D, M, group = 512, 3, 1024, 64, 1024, 16
+    b = Batch([(3000, 1)], H, D, P, seed=63).upload(ctx, 1, 3000)
+    q = queries(b, group)
+    want = run_attention(ctx, b, q, group, 0.125)
+    starts = np.zeros(S + 1, np.int32)
+    starts[1::2] = M
+    up = [ctx.upload(a) for a in (starts, np.full(S, 2 ** 31 - 1, np.int32), np.full((S, 2048), -1, np.int32),
+                                  np.zeros((M, H * group * D), np.float16), np.full((M, H * group * D), 7, np.float16))]
+    batch = qmm_hip.KvBatch(S, M, int(up[0]), int(up[1]), int(up[2]), 2048, 1, 2 ** 21)
+    width = H * group * D
+    args = qmm_hip.AttentionArgs(int(up[3]), width, H * group, 0.125, 0, 0, int(up[4]), qmm_hip.TYPE_F16, width)
+    ws = ctx.attention_workspace(batch, b.cache, args)
+    say("rows claimed past any count")
+    ctx.paged_attention(batch, b.cache, args, ws)
+    ctx.sync()
+    assert (ctx.d2h(up[4], np.float16, (M, width)) == 7).all()
+    got = run_attention(ctx, b, q, group, 0.125, ws=ws)
+    assert np.array_equal(got.view(np.uint16), want.view(np.uint16))
+    ws.free()
+    for x in up:
+        ctx.free(x)
+    b.free()
