@@ -1,6 +1,6 @@
-// qmm_attn_plan.h — how a call of the attention is launched: row tiles, who
-// shares which work, and the scratch that takes. Plain C++: a host program can
-// check it without a device.
+// qmm_attn_plan.h — how an append and a call of the attention are launched: the
+// append's workgroups; row tiles, who shares which work, and the scratch that
+// takes. Plain C++: a host program can check it without a device.
 #pragma once
 
 #include <algorithm>
@@ -8,6 +8,27 @@
 #include "qmm_attn.h"
 
 namespace qmm {
+
+// Workgroups of an append: njobs for each row of queries and keys, and for each sequence ngroups (in
+// turn) for its groups of 16 slots of values, times nchunks of 1024 values. workgroups 0: more than one
+// launch has (2^32 threads in 256s).
+struct AppendGrid {
+    int njobs, ngroups, nchunks;
+    unsigned workgroups;
+};
+inline AppendGrid append_grid(int n_rows, int n_seqs, int n_heads, int head_dim, int q_heads, int max_new) {
+    constexpr int64_t kMost = (int64_t(1) << 24) - 1;
+    const int hpw = 256 / head_dim, groups = (q_heads + n_heads + hpw - 1) / hpw;  // head groups of a row, one a wave
+    AppendGrid g{1, 0, int((int64_t(n_heads) * head_dim + 1023) / 1024), 0};
+    const int64_t values = int64_t(n_seqs) * g.nchunks;
+    if (n_rows + values > kMost) return g;
+    // few rows: every head group its own wave; many: one workgroup a row, the angles reduced once
+    while (g.njobs * 4 < groups && int64_t(n_rows) * g.njobs < 1024 && int64_t(n_rows) * (g.njobs + 1) + values <= kMost) ++g.njobs;
+    // aligned groups that max_new tokens can touch, or as many as there is room for
+    g.ngroups = int(std::min<int64_t>((int64_t(max_new) + 14) / 16 + 1, (kMost - int64_t(n_rows) * g.njobs) / values));
+    g.workgroups = unsigned(int64_t(n_rows) * g.njobs + values * g.ngroups);
+    return g;
+}
 
 constexpr int kMaxShared = 512;  // sequences of a call whose tiles workers share
 // A segment (a row tile of a sequence's head) whose tiles several workers of the

@@ -21,7 +21,7 @@
 //    error below 1e-6 rad) into a table in LDS that all heads share.
 #include <hip/hip_runtime.h>
 
-#include "qmm_attn.h"
+#include "qmm_attn_plan.h"
 
 namespace qmm {
 namespace {
@@ -306,16 +306,10 @@ hipError_t launch_rope_table(const RopeTable &t, RopeTable *dst, hipStream_t s) 
 }
 
 hipError_t launch_kv_append(const AppendArgs &a, hipStream_t s) {
-    const int D = a.head_dim, hpw = 256 / D;
-    const int groups = ((a.q ? a.q_heads : 0) + a.b.n_heads + hpw - 1) / hpw;  // head groups of a row, one a wave
-    // few rows: every head group its own wave; many: one workgroup a row, the angles reduced once
-    int njobs = 1;
-    while (njobs * 4 < groups && int64_t(a.b.n_rows) * njobs < 1024) ++njobs;
-    const int ngroups = (a.max_new + 14) / 16 + 1;  // aligned groups that max_new tokens can touch
-    const int nchunks = (a.b.n_heads * D + 1023) / 1024;
-    const uint64_t grid = uint64_t(a.b.n_rows) * uint64_t(njobs) + uint64_t(a.b.n_seqs) * uint64_t(ngroups) * uint64_t(nchunks);
-    if (grid >= (uint64_t(1) << 31)) return hipErrorInvalidValue;
-#define QMM_KV(DD) hipLaunchKernelGGL(kv_append_kernel<DD>, dim3(unsigned(grid)), dim3(256), 0, s, a, njobs, ngroups, nchunks)
+    const AppendGrid g = append_grid(a.b.n_rows, a.b.n_seqs, a.b.n_heads, a.head_dim, a.q ? a.q_heads : 0, a.max_new);
+    if (!g.workgroups) return hipErrorInvalidValue;
+    const int D = a.head_dim;
+#define QMM_KV(DD) hipLaunchKernelGGL(kv_append_kernel<DD>, dim3(g.workgroups), dim3(256), 0, s, a, g.njobs, g.ngroups, g.nchunks)
     if (D == 64) QMM_KV(64);
     else if (D == 128) QMM_KV(128);
     else QMM_KV(256);

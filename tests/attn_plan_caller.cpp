@@ -90,8 +90,36 @@ static void counts() {
                call_units(0, 9) == 0 && call_units(0x7fffffffu, 1) == 0x7fffffff, "units of a call");
 }
 
+// every group of 16 slots and every row of an append has its workgroup, in one launch (below 2^32 threads)
+static void append_grids() {
+    std::mt19937 rng(7);
+    auto any = [&](int lo, int hi) { return std::uniform_int_distribution<int>(lo, hi)(rng); };
+    const int64_t most = (int64_t(1) << 32) / 256;
+    for (int i = 0; i < 200000; ++i) {
+        const int rows = any(1, 1 << any(0, 26)), heads = any(1, 1 << any(0, 16)) % 65536 + 1, dim = 64 << any(0, 2);
+        const int seqs = any(1, std::max(1, std::min(1 << any(0, 24), ((1 << 24) - 1) / heads)));
+        const int max_new = any(1, rows), q_heads = any(0, 8) * heads;
+        const int64_t chunks = (int64_t(heads) * dim + 1023) / 1024;
+        const AppendGrid g = append_grid(rows, seqs, heads, dim, q_heads, max_new);
+        if (rows + seqs * chunks >= most) {
+            EXPECT(g.workgroups == 0, "%d rows %d sequences %d heads", rows, seqs, heads);
+            continue;
+        }
+        EXPECT(g.workgroups > 0 && g.workgroups < most && g.njobs >= 1 && g.ngroups >= 1 && g.nchunks == chunks &&
+                   g.workgroups == int64_t(rows) * g.njobs + int64_t(seqs) * g.ngroups * g.nchunks,
+               "%d rows %d sequences %d heads of %d, %d new: %u workgroups", rows, seqs, heads, dim, max_new, g.workgroups);
+        EXPECT(g.ngroups <= (max_new + 14) / 16 + 1, "%d groups", g.ngroups);
+    }
+    const AppendGrid g = append_grid(65536, 256, 64, 256, 0, 65536);  // one long prompt, or max_new not known
+    EXPECT(g.workgroups && g.ngroups > 4000, "%u workgroups, %d groups a sequence", g.workgroups, g.ngroups);
+    const AppendGrid one = append_grid(1, 1, 8, 128, 32, 1), many = append_grid(8192, 1, 8, 128, 32, 8192);
+    EXPECT(one.njobs == 5 && one.ngroups == 1 && one.workgroups == 6 && many.njobs == 1 && many.workgroups == 8192 + 513, "%d %u %u", one.njobs,
+           one.workgroups, many.workgroups);
+}
+
 int main() {
     counts();
+    append_grids();
     const AttnArgs prompt = call(1, 8192, 8192, 8192), token = call(1, 1, 1, 131071), batch = call(32, 32, 1, 8000);
     const AttnArgs drafts = call(28, 28 * 8, 8, 4000), many = call(600, 600, 1, 2000), mixed = call(9, 600, 512, 9000);
     covered(prompt, token, "a prompt's workspace, one token");

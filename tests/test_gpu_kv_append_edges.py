@@ -129,3 +129,23 @@ def test_smallest_scales_of_an_8_bit_cache(ctx, D):
                     assert (codes[:, D // 2] == -127).all() and (np.abs(scale * 127 / 2.0 ** -100 - 1) < 2.0 ** -22).all()
                     # half a step of the code, and its quotient's last bits
                     assert np.abs(codes * scale[:, None].astype(np.float64) - ref).max() <= scale.max() * (0.5 + 127 * 2.0 ** -22)
+
+
+@pytest.mark.parametrize("q8", [False, True])
+def test_many_sequences_without_hints(ctx, q8):
+    """4096 sequences of 16 rows with max_new not known: each could have all 65536, and 2^24 workgroups of
+    values would be more than a launch has."""
+    S, D, rng = 4096, 64, np.random.default_rng(3)
+    b = Batch([(16 + int(n), 16) for n in rng.integers(0, 3, S)], 1, D, 32, q8, seed=5).upload(ctx)
+    x = rng.standard_normal((b.M, 2 * D)).astype(np.float32)
+    say(f"{S} sequences without hints q8={q8}")
+    got = _append(ctx, b, x)
+    b.free()
+    page = np.repeat(b.pages[:, 0], 16)
+    slot = (b.kv_len[:, None] - 16 + np.arange(16)).reshape(-1)
+    for codes, scale, ref in ((got["k"][page, 0, slot], "ks", x[:, :D]), (got["v"][page, 0, :, slot], "vs", x[:, D:])):
+        if not q8:
+            assert np.array_equal(codes, ref.astype(np.float16))
+        else:
+            s = got[scale][page, 0, slot].astype(np.float64)[:, None]
+            assert (np.abs(codes * s - ref) <= s * (0.5 + 127 * 2.0 ** -22)).all()
