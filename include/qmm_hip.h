@@ -340,7 +340,8 @@ typedef struct {
     int max_pages;
     /* What the host knows of the device arrays, for choosing a launch: the
      * most new rows of a sequence and the largest kv_len (0: not known). A
-     * captured graph may be replayed with others: they change no result. */
+     * captured graph may be replayed with others: they change no result but by
+     * the order of the attention's sums. */
     int max_new;
     int max_kv;
 } qmm_kv_batch;
@@ -401,7 +402,10 @@ int qmm_kv_append(qmm_context *ctx, const qmm_kv_batch *batch, const qmm_kv_cach
  *   j <= p  and  (window == 0  or  j > p - window  or  j < sinks):
  * a sliding window whose first `sinks` tokens stay visible. out = sum over the
  * visible j of softmax(scale * q.k_j) v_j; zeros where nothing is visible. What
- * lies in a masked cell (any bits) never reaches a row. out does not overlap q. */
+ * lies in a masked cell (any bits) never reaches a row; an infinite value makes
+ * its dimension infinite or NaN in the rows that see it. out does not overlap q.
+ * The same call on the same kind of device gives the same bits: the order of the
+ * sums goes by the lengths, the hints and the workspace's size alone. */
 typedef struct {
     const uint16_t *q; /* device fp16 [n_rows][q_stride], 16-B aligned rows */
     size_t q_stride;

@@ -26,7 +26,8 @@
 // Who takes which tiles: even shares of all tiles for the workers (2 a CU), and
 // partial results joined by a second kernel; or, where that costs more than it
 // evens out, a workgroup for each head of a sequence or row tile (plan_split).
-// The order of all sums is fixed by the lengths: the same call, the same bits.
+// The order of all sums is fixed by the lengths, the hints, the workspace's size and the CUs: the same
+// call, the same bits.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -676,8 +677,10 @@ __device__ inline void dma16g(const void *src, uint32_t lds) {
 // while the weights' exponentials are computed; the keys of tile i + 2 and the
 // values of tile i + 1 are on their way to LDS meanwhile (fp16 straight from
 // memory, the XOR of an LDS row's pieces in the lanes' addresses). Against scores
-// and product in turn: a prompt of 8192 727 -> 648 us. Nothing may spill here: a
-// spilled value's load waits for all of the loads above (8-bit: 10 to 25 %).
+// and product in turn: a prompt of 8192 727 -> 648 us. Nothing may spill in this
+// loop: a spilled value's load waits for all of the loads above (8-bit: 10 to
+// 25 %). Three of the forms of 128 values keep up to 8 registers in scratch, read
+// between pieces.
 template <int D, bool Q8>
 __device__ inline __attribute__((always_inline)) void tile_piece(const SplitArgs &p, TileShared<D> &sh, uint32_t sh_at, const SeqView &v,
                                                                  const RowTile &tile, int s, int h, int begin, int end,
