@@ -74,6 +74,24 @@ def test_scales_of_hidden_cells(ctx, D, n, new):
 
 
 @pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("lens", [[(700, 1)] * 3, [(100, 20), (2000, 1)], [(90, 90)]])
+def test_hints_change_the_order_of_sums_only(ctx, lens, q8):
+    """Hints choose the launch: the results agree to the roundings of sums in another order."""
+    outs = []
+    for hints in ((0, 0), (1, 64), (1, 1), (2, 100000), (max(n for _, n in lens), max(n for n, _ in lens))):
+        b = Batch(lens, 2, 64, 16, q8, seed=11)
+        q = queries(b, 4)
+        b.upload(ctx, *hints)
+        say(f"hints {hints} lens={lens} q8={q8}")
+        outs.append(run_attention(ctx, b, q, 4, 0.125).astype(np.float64))
+        b.free()
+    ref, tol = attend(b, q, 4, 0.125)
+    for o in outs:
+        check_rows(o, ref, tol, b.held_rows)
+        assert (np.abs(o - outs[0]) <= 2 * tol).all()
+
+
+@pytest.mark.parametrize("q8", [False, True])
 @pytest.mark.parametrize("sign", [1, -1])
 @pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("n,new", [(300, 1), (9000, 1), (200, 40), (9000, 40)])
