@@ -72,12 +72,22 @@ inline int64_t hinted_tiles(const AttnArgs &a, int R) {
 // a tile; shared work 11.5 us and 4.5 us for 1000 tiles of all heads, its join included. us,
 // whole / shared (8 heads of 128): 8 heads of 11 tiles 11.1 / 13.9, of 16 14.2 / 11.1; 32 of 16
 // 15.9 / 13.0; 64 of 16 16.1 / 16.0, of 28 23.4 / 18.4; 128 of 16 17.0 / 22.0; 256 of 32 44 / 53.
-inline int64_t short_tiles(int64_t heads) { return std::min<int64_t>(32, 10 + heads / 6); }
+// Heads of 64, and 8-bit ones of 128: 8 of 16 11.2 / 10.2, 13.0 / 11.2; 64 of 22 15.4 / 16.5,
+// 18.3 / 19.6; 256 of 30 24.4 / 29.8, 29.0 / 34.5. Heads of 256 have 4 waves, not 8, and 1.6 to
+// 2 us a tile: 8 of 9 17.7 / 19.5, of 12 21.5 / 16.2; 64 of 20 36.9 / 25.6; 128 of 9 20.7 / 27.6,
+// of 18 38.4 / 35.4; 256 of 20 58.9 / 64.6; 8-bit 64 of 12 25.6 / 19.4, 256 of 20 45.5 / 42.5.
+inline int64_t short_tiles(int64_t heads, int head_dim) {
+    return std::min<int64_t>(32, head_dim <= 128 ? 10 + heads / 6 : 10 + heads * heads / 6000);
+}
 
-// Bytes of cache from which loads take whole lines and leave them in no cache: what is less
+// Bytes of cache (as the hints have it: the longest sequence times all) from which loads take whole
+// lines and leave them in no cache: what is less
 // may be there from one call to the next (the last one holds 256 MB). us, as operands have
 // them / whole lines: 57 MB 21.7 / 23.0, 86 MB 25.8 / 28.6, 115 MB 33.3 / 31.9, 230 MB
-// 56.0 / 49.8; 0.4 MB 8.0 / 8.5 (more code to fetch).
+// 56.0 / 49.8; 0.4 MB 8.0 / 8.5 (more code to fetch). 8-bit, and heads of 64: 48 MB 18.9 / 20.7,
+// 16.1 / 17.4, 193 MB 48.7 / 46.0, 44.8 / 40.5; heads of 256 as well either way (102 MB 33.5 / 32.7,
+// 195 MB 61.8 / 62.5). Where the cache has been driven out in between, whole lines are no slower from
+// 5 MB on (13 MB 8.9 / 7.9, 51 MB 17.9 / 16.8): the rule leaves up to 10 % there.
 constexpr int64_t kLargeBytes = int64_t(96) << 20;
 
 // All workers of shared work with row tiles of R rows, and what one takes of the scratch: partial
@@ -111,7 +121,7 @@ inline SplitPlan plan_split(const AttnArgs &a, int max_new, int cu_count, size_t
     // ascend; others are counted where they are read)
     const int64_t most_tiles = int64_t(a.b.n_rows) * a.group / R + a.b.n_seqs, most_span = kv_capacity(a.b.max_pages, a.b.page_shift) / kTileKeys + 1;
     const bool countable = most_tiles * most_span < kMostUnits / a.b.n_heads;
-    const bool few_tiles = R == 16 ? tiles <= short_tiles(units) : units * row_tiles >= 2 * workgroups_of_cu(a, R) * cu_count || tiles <= 8;
+    const bool few_tiles = R == 16 ? tiles <= short_tiles(units, a.head_dim) : units * row_tiles >= 2 * workgroups_of_cu(a, R) * cu_count || tiles <= 8;
     p.new_max = 0x7fffffff;
     if (!few_tiles && a.b.n_seqs <= kMaxShared && enough && countable) {
         p.workers = int(workers);

@@ -90,6 +90,20 @@ static void counts() {
                call_units(0, 9) == 0 && call_units(0x7fffffffu, 1) == 0x7fffffff, "units of a call");
 }
 
+// heads of 256 values take a workgroup three times as long a tile: they share sooner
+static void short_heads() {
+    SplitPlan p[2];
+    auto workers = [&](int heads, int seqs, int dim, int tiles) {
+        const AttnArgs a = call(seqs, seqs, 1, tiles * 64, heads, 4, dim);
+        plan_call(a, kCus, kAny, p);
+        return p[0].workers;
+    };
+    EXPECT(workers(8, 1, 256, 8) == 0 && workers(8, 1, 256, 12) == 512 && workers(8, 8, 256, 18) == 512 && workers(8, 16, 256, 9) == 0 &&
+               workers(8, 16, 256, 18) == 512 && workers(8, 32, 256, 18) == 0 && workers(8, 32, 256, 33) == 512, "heads of 256");
+    EXPECT(workers(8, 1, 128, 11) == 0 && workers(8, 1, 128, 16) == 512 && workers(8, 8, 128, 20) == 0 && workers(8, 8, 128, 28) == 512 &&
+               workers(8, 16, 64, 22) == 0 && workers(8, 32, 128, 32) == 0, "heads of 64 and 128");
+}
+
 // every group of 16 slots and every row of an append has its workgroup, in one launch (below 2^32 threads)
 static void append_grids() {
     std::mt19937 rng(7);
@@ -119,6 +133,7 @@ static void append_grids() {
 
 int main() {
     counts();
+    short_heads();
     append_grids();
     const AttnArgs prompt = call(1, 8192, 8192, 8192), token = call(1, 1, 1, 131071), batch = call(32, 32, 1, 8000);
     const AttnArgs drafts = call(28, 28 * 8, 8, 4000), many = call(600, 600, 1, 2000), mixed = call(9, 600, 512, 9000);
