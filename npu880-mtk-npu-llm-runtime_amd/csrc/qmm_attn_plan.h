@@ -80,6 +80,27 @@ inline int64_t short_tiles(int64_t heads, int head_dim) {
     return std::min<int64_t>(32, head_dim <= 128 ? 10 + heads / 6 : 10 + heads * heads / 6000);
 }
 
+// Whether row tiles of 128 are shared: `whole` of them, `tiles` tiles long, of `rows` rows in use. Whole,
+// they take us_tile for each tile of the longest; shared, what they leave idle of the chip is used (two
+// 8-bit ones on a CU, bound by their conversions, cost each other less), but 8 us and those of the
+// partial results are added. us, whole / shared (8 heads of 128, group 4), new tokens x tiles:
+//   fp16    1 x 512 rows: of 8 18.8 / 36.3, of 24 43.1 / 49.9, of 47 78.7 / 64.4; 1 x 1024 of 16 31.8 / 53.4,
+//           of 79 124 / 136; 1 x 128 of 13 26.2 / 28.0, of 18 33.6 / 28.6; 4 x 256 of 36 61.8 / 86.5
+//   drafts  8 rows: 1 of 12 21.9 / 16.7; 16 of 19 32.3 / 32.0, of 63 94.6 / 66.7; 24 of 24 43.1 / 54.0
+//   8-bit   1 x 512 of 8 25.1 / 39.3, of 24 62.2 / 54.6; 1 x 1024 of 16 44.8 / 58.2, of 79 189 / 161; drafts
+//           24 of 24 61.4 / 54.7, 32 of 125 296 / 223; 1 x 2048 of 32 86.1 / 115
+//   of 64   1 x 512 of 24 32.5 / 39.5, of 47 60.2 / 47.8; drafts 16 of 19 25.7 / 23.2, of 63 75.4 / 45.6
+//   of 256  1 x 512 of 8 34.6 / 55.4, of 24 81.2 / 79.1; drafts 16 of 11 45.8 / 42.5, 32 of 125 392 / 451;
+//           8-bit 1 x 512 of 8 42.4 / 57.9, of 24 106 / 90.1, 1 x 1024 of 79 323 / 369
+inline bool shares_row_tiles(const AttnArgs &a, int64_t tiles, int64_t whole, int64_t rows, int cu_count) {
+    constexpr double kTile[] = {1.2, 1.6, 3.0}, kPartial[] = {7, 12, 24};
+    const bool q8 = a.ks != nullptr;
+    const int kind = a.head_dim == 64 ? 0 : a.head_dim == 128 ? 1 : 2;
+    const double us_tile = kTile[kind] * (q8 ? 1.5 : 1.0), us_partial = kPartial[kind];
+    const double idle = 1.0 - (q8 && kind < 2 ? 0.65 : 1.0) * double(whole) / cu_count;
+    return us_tile * double(tiles) * idle > 8.0 + us_partial * double(rows) / 128;
+}
+
 // Bytes of cache (as the hints have it: the longest sequence times all) from which loads take whole
 // lines and leave them in no cache: what is less
 // may be there from one call to the next (the last one holds 256 MB). us, as operands have
@@ -121,7 +142,8 @@ inline SplitPlan plan_split(const AttnArgs &a, int max_new, int cu_count, size_t
     // ascend; others are counted where they are read)
     const int64_t most_tiles = int64_t(a.b.n_rows) * a.group / R + a.b.n_seqs, most_span = kv_capacity(a.b.max_pages, a.b.page_shift) / kTileKeys + 1;
     const bool countable = most_tiles * most_span < kMostUnits / a.b.n_heads;
-    const bool few_tiles = R == 16 ? tiles <= short_tiles(units, a.head_dim) : units * row_tiles >= 2 * workgroups_of_cu(a, R) * cu_count || tiles <= 8;
+    const int64_t whole = a.b.n_heads * std::min(a.b.n_seqs * row_tiles, int64_t(a.b.n_rows) * a.group / R + a.b.n_seqs);
+    const bool few_tiles = R == 16 ? tiles <= short_tiles(units, a.head_dim) : !shares_row_tiles(a, tiles, whole, std::min<int64_t>(rows, R), cu_count);
     p.new_max = 0x7fffffff;
     if (!few_tiles && a.b.n_seqs <= kMaxShared && enough && countable) {
         p.workers = int(workers);

@@ -104,6 +104,26 @@ static void short_heads() {
                workers(8, 16, 64, 22) == 0 && workers(8, 32, 128, 32) == 0, "heads of 64 and 128");
 }
 
+// row tiles of 128: a prompt of its own is not shared, as its row tiles do not differ enough for what
+// that costs; long pasts and drafts are
+static void row_tiles() {
+    SplitPlan p[2];
+    auto workers = [&](int seqs, int rows, int past, bool q8 = false) {
+        AttnArgs a = call(seqs, seqs * rows, rows, rows + past);
+        static const float scale = 1;
+        a.ks = q8 ? &scale : nullptr;
+        plan_call(a, kCus, kAny, p);
+        return p[0].workers;
+    };
+    EXPECT(workers(1, 512, 0) == 0 && workers(1, 1024, 0) == 0 && workers(1, 2048, 0) == 0 && workers(4, 256, 2000) == 0 &&
+               workers(1, 8192, 0) == 0 && workers(1, 1024, 0, true) == 0 && workers(1, 2048, 0, true) == 0, "prompts whole");
+    EXPECT(workers(1, 512, 4000) == 512 && workers(1, 256, 2000) == 512 && workers(8, 12, 2000) == 512 && workers(1, 8, 760) == 512 &&
+               workers(1, 1024, 4000, true) == 512 && workers(24, 8, 1500, true) == 512, "long pasts shared");
+    AttnArgs a = call(8, 519, 512, 4512);  // one long prompt among single tokens: the rows there are count
+    plan_call(a, kCus, kAny, p);
+    EXPECT(p[0].rows == 128 && p[0].workers == 512, "%d workers for one prompt among single tokens", p[0].workers);
+}
+
 // every group of 16 slots and every row of an append has its workgroup, in one launch (below 2^32 threads)
 static void append_grids() {
     std::mt19937 rng(7);
@@ -134,6 +154,7 @@ static void append_grids() {
 int main() {
     counts();
     short_heads();
+    row_tiles();
     append_grids();
     const AttnArgs prompt = call(1, 8192, 8192, 8192), token = call(1, 1, 1, 131071), batch = call(32, 32, 1, 8000);
     const AttnArgs drafts = call(28, 28 * 8, 8, 4000), many = call(600, 600, 1, 2000), mixed = call(9, 600, 512, 9000);
