@@ -150,7 +150,10 @@ inline SplitPlan plan_split(const AttnArgs &a, int max_new, int cu_count, size_t
         p.slots = size_t(workers) * 2 * R;
         p.bytes = Sharing{workers, all.each}.bytes();
     }
-    p.nw = R == 16 && !p.workers && a.head_dim <= 128 && units <= 2 * cu_count && tiles > 4 ? 8 : 4;
+    // 8 waves: one workgroup a CU (registers), so for no more heads than CUs. us, 4 / 8 waves: 8 heads of 4
+    // tiles 6.9 / 7.2, of 5 8.2 / 7.9, of 10 10.8 / 10.6; 256 of 10 17.2 / 16.4; 512 of 8 24.7 / 28.2; heads of 64,
+    // and 8-bit ones: 256 of 10 11.0 / 10.4, 14.3 / 13.2; 512 of 8 14.0 / 17.2, 17.0 / 20.7
+    p.nw = R == 16 && !p.workers && a.head_dim <= 128 && units <= cu_count && tiles > 4 ? 8 : 4;
     p.lines = R == 16 && tiles * units >= kLargeBytes / (int64_t(kTileKeys) * a.head_dim * (a.ks ? 2 : 4));
     p.row_tiles = int(std::min<int64_t>(row_tiles, 65535));
     return p;

@@ -104,6 +104,18 @@ static void short_heads() {
                workers(8, 16, 64, 22) == 0 && workers(8, 32, 128, 32) == 0, "heads of 64 and 128");
 }
 
+// a workgroup of 8 waves takes a CU: for no more heads than CUs, and more tiles than 4
+static void waves() {
+    SplitPlan p[2];
+    auto waves = [&](int seqs, int tiles, int dim) {
+        const AttnArgs a = call(seqs, seqs, 1, tiles * 64, 8, 4, dim);
+        EXPECT(plan_call(a, kCus, 0, p) == 1 && p[0].workers == 0, "waves");
+        return p[0].nw;
+    };
+    EXPECT(waves(1, 5, 128) == 8 && waves(32, 10, 64) == 8 && waves(1, 4, 128) == 4 && waves(1, 10, 256) == 4, "few heads");
+    EXPECT(waves(33, 8, 128) == 4 && waves(64, 8, 128) == 4 && waves(64, 10, 64) == 4, "more heads than CUs");
+}
+
 // row tiles of 128: a prompt of its own is not shared, as its row tiles do not differ enough for what
 // that costs; long pasts and drafts are
 static void row_tiles() {
@@ -155,6 +167,7 @@ int main() {
     counts();
     short_heads();
     row_tiles();
+    waves();
     append_grids();
     const AttnArgs prompt = call(1, 8192, 8192, 8192), token = call(1, 1, 1, 131071), batch = call(32, 32, 1, 8000);
     const AttnArgs drafts = call(28, 28 * 8, 8, 4000), many = call(600, 600, 1, 2000), mixed = call(9, 600, 512, 9000);
