@@ -189,3 +189,41 @@ def test_rows_claimed_past_any_count(ctx):
     for x in up:
         ctx.free(x)
     b.free()
+
+
+@pytest.mark.parametrize("q8", [False, True])
+def test_captured_prompts_and_single_tokens(q8):
+    """A call of both kernels and their joins, captured and replayed with other lengths, rows and queries,
+    eager calls of the same context and workspace between: the eager bits each time."""
+    group, D, P, H = 4, 64, 64, 2
+    with qmm_hip.Context(0) as c:
+        b = Batch([(5000, 60), (6000, 1), (2500, 2)], H, D, P, q8, seed=65, max_pages=100).upload(c, 60, 6400)
+        b.pages[:, :] = b.pages[:, :1]  # (any length is held: the same page again)
+        c.h2d(b.bufs["pages"], b.pages)
+        width, rng = H * group * D, np.random.default_rng(4)
+        qb = c.upload(queries(b, group))
+        outs = [c.upload(np.zeros((b.M, width), np.float16)) for _ in range(2)]
+        args = [qmm_hip.AttentionArgs(int(qb), width, H * group, 0.125, 0, 0, int(o), qmm_hip.TYPE_F16, width) for o in outs]
+        ws = c.attention_workspace(b.batch, b.cache, args[0])
+        c.sync()
+        c.graph_begin()
+        c.paged_attention(b.batch, b.cache, args[0], ws)
+        g = c.graph_end()
+        for rep in range(5):
+            new = [(60, 1, 2), (1, 61, 1), (20, 20, 23), (0, 0, 63), (63, 0, 0)][rep]
+            c.h2d(b.bufs["row_start"], np.concatenate([[0], np.cumsum(new)]).astype(np.int32))
+            c.h2d(b.bufs["kv_len"], rng.integers(64, 6400, 3).astype(np.int32))
+            c.h2d(qb, (rng.standard_normal((b.M, width)) * 2).astype(np.float16))
+            for o in outs:
+                c.h2d(o, np.full((b.M, width), np.nan, np.float16))
+            say(f"captured prompts and single tokens, replay {rep} new={new} q8={q8}")
+            c.graph_launch(g)
+            c.paged_attention(b.batch, b.cache, args[1], ws)  # (in stream order behind it)
+            c.sync()
+            one, two = (c.d2h(o, np.float16, (b.M, width)) for o in outs)
+            assert np.isfinite(two).all() and np.array_equal(one.view(np.uint16), two.view(np.uint16)), rep
+        c.graph_destroy(g)
+        ws.free()
+        for x in (qb, *outs):
+            c.free(x)
+        b.free()
