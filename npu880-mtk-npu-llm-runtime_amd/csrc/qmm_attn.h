@@ -71,6 +71,16 @@ QMM_HD inline int page_of(const KvView &b, int s, int token, int len) {
     return unsigned(id) < unsigned(b.n_pages) ? id : -1;
 }
 
+// The aligned groups of 16 slots that hold a sequence's new tokens: first .. end - 1. By their own
+// number, not their first slot: groups past the end are looked at too, and 16 times those can be past
+// the largest int.
+struct SlotGroups {
+    int first, end;
+};
+QMM_HD constexpr SlotGroups slot_groups(const SeqView &v) {  // (rows at negative places have no cell)
+    return SlotGroups{(v.pos0 < 0 ? 0 : v.pos0) >> 4, v.n_new > 0 ? (v.len + 15) >> 4 : 0};
+}
+
 struct AttnArgs {
     KvView b;
     const uint16_t *q;

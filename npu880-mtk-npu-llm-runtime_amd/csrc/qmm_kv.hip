@@ -214,7 +214,8 @@ __device__ inline void append_v(const AppendArgs &a, int s, int group0, int ngro
     const int head = i / D, d = i % D;
     const int P = 1 << a.b.page_shift;
     const int start = max(v.pos0, 0);  // (rows at negative places have no cell)
-    for (int g = (start >> 4) + group0; g * 16 < v.len; g += ngroups) {
+    const SlotGroups groups = slot_groups(v);
+    for (int g = groups.first + group0; g < groups.end; g += ngroups) {
         const int page = page_of(a.b, s, max(start, g * 16), v.len);
         if (page < 0) continue;
         const size_t row = (size_t(page) * H + size_t(head)) * D + size_t(d);  // the first value's row of P slots

@@ -163,8 +163,29 @@ static void append_grids() {
            one.workgroups, many.workgroups);
 }
 
+// a sequence's workgroups take each of its groups of slots once and end, up to the largest length
+static void slots() {
+    std::mt19937 rng(8);
+    auto any = [&](int lo, int hi) { return std::uniform_int_distribution<int>(lo, hi)(rng); };
+    const int cap = kv_capacity(1 << 30, 10);
+    for (int i = 0; i < 3000; ++i) {
+        const int len = i % 2 ? cap - any(0, 40) : any(0, 3000), n_new = any(0, 1 << any(0, 11)), ngroups = any(1, 1 << any(0, 23));
+        const SeqView v{0, n_new, len, len - n_new};
+        const SlotGroups g = slot_groups(v);
+        int seen = 0;
+        for (int group0 = 0; group0 < std::min(ngroups, 200); ++group0)
+            for (int k = g.first + group0; k < g.end; k += ngroups) {
+                EXPECT(k >= 0 && k * 16 < len && (k + 1) * 16 > v.pos0, "group %d of %d..%d", k, v.pos0, len);
+                if (++seen > 1000) break;
+            }
+        const int want = n_new && len ? (len - 1) / 16 - std::max(v.pos0, 0) / 16 + 1 : 0;
+        EXPECT(seen == want, "%d groups of %d: %d new of %d, %d at a time", seen, want, n_new, len, ngroups);
+    }
+}
+
 int main() {
     counts();
+    slots();
     short_heads();
     row_tiles();
     waves();

@@ -227,3 +227,45 @@ def test_captured_prompts_and_single_tokens(q8):
         for x in (qb, *outs):
             c.free(x)
         b.free()
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("new", [1, 300])
+def test_largest_sequence(ctx, new, q8):
+    """A sequence of 2^31 - 256 tokens, of whose pages only the last is there: its new rows are appended (by
+    20 workgroups in turn where nothing is known of their number) and attended to, with a window and (one
+    row) over all of its 2^25 tiles."""
+    D, P, group, cap = 64, 1024, 4, 2 ** 31 - 256
+    b = Batch([(P, new)], 1, D, P, q8, seed=71, spare_pages=0)
+    table = np.full((1, 2 ** 21), -1, np.int32)
+    table[0, -1] = 0
+    b.pages, b.max_pages, b.kv_len = table, 2 ** 21, np.array([2 ** 31 - 1], np.int32)  # (the length is clamped)
+    b.upload(ctx)
+    rng = np.random.default_rng(72)
+    x = rng.standard_normal((new, 2 * D)).astype(np.float32)
+    xb = ctx.upload(x)
+    say(f"largest sequence new={new} q8={q8}")
+    ctx.kv_append(b.batch, b.cache, qmm_hip.KvRows(k=int(xb), k_stride=2 * D, v=int(xb) + 4 * D, v_stride=2 * D))
+    ctx.sync()
+    slots = cap % P  # of the last page
+    near = Batch([(slots, new)], 1, D, P, q8, seed=71, spare_pages=0)  # the same page as a short sequence
+    near.pages = np.zeros((1, 1), np.int32)
+    for n in ("k", "v") + (("ks", "vs") if q8 else ()):
+        kept = getattr(b, n)
+        got = ctx.d2h(b.bufs[n], kept.dtype, kept.shape)
+        axis = 3 if n == "v" else 2
+        old = np.delete(kept, np.s_[slots - new:slots], axis)
+        assert np.array_equal(np.delete(got, np.s_[slots - new:slots], axis).view(np.uint8), old.view(np.uint8)), f"other cells of {n}"
+        setattr(near, n, got)
+    k, v = (a[0, -new:] for a in near.dense(0))
+    half = np.abs(x.reshape(new, 2, D)).max(2).T[..., None] * ((0.5 + 2.0 ** -14) / 127 if q8 else F16_HALF)
+    assert (np.abs(k - x[:, :D]) <= half[0]).all() and (np.abs(v - x[:, D:]) <= half[1]).all()
+    q = queries(b, group)
+    for window, sinks in ((100, 0), (500, 0), (0, 0)):
+        if window == 0 and new > 1:
+            continue
+        say(f"largest sequence: window {window}")
+        ref, tol = attend(near, q, group, 0.125, window, sinks)
+        check_rows(run_attention(ctx, b, q, group, 0.125, window, sinks), ref, tol, new)
+    ctx.free(xb)
+    b.free()
