@@ -296,12 +296,12 @@ int qmm_lm_head_scan_rmsnorm(qmm_context *ctx, const float *x, const float *gamm
  * cells of a page id outside [0, n_pages) are neither read nor written and are
  * visible to no row. Rows that no sequence holds (past row_start[n_seqs]) keep
  * their outputs as they were; with row starts that do not ascend, rows that
- * several sequences claim hold any one's results or are as they were. Largest calls: n_seqs * n_heads below 2^24 and
- * n_rows * q_heads / n_heads below 2^30; in an append n_rows + n_seqs *
- * ceil(n_heads * head_dim / 1024) below 2^24; a sequence holds at most 2^31 - 256
- * tokens. Everything else that a call needs is in its arguments: it keeps
- * nothing for the next one, and calls on several streams, contexts and graphs
- * may overlap (with a workspace each). */
+ * several sequences claim hold any one's results or are as they were. Largest
+ * calls: n_seqs * n_heads below 2^24 and n_rows * q_heads / n_heads below 2^30;
+ * in an append n_rows + n_seqs * ceil(n_heads * head_dim / 1024) below 2^24; a
+ * sequence holds at most 2^31 - 256 tokens. Everything else that a call needs is
+ * in its arguments: it keeps nothing for the next one, and calls on several
+ * streams, contexts and graphs may overlap (with a workspace each). */
 
 /* One layer's cache: n_pages pages of page_tokens tokens (a power of two,
  * 16..1024), n_heads key-value heads of head_dim (64, 128 or 256) values.
