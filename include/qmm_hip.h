@@ -438,6 +438,141 @@ int qmm_attention_workspace_destroy(qmm_context *ctx, qmm_attn_workspace *ws);
 int qmm_paged_attention(qmm_context *ctx, const qmm_kv_batch *batch, const qmm_kv_cache *cache,
                         const qmm_attention_args *args, qmm_attn_workspace *ws);
 
+/* ------------------------------------- linear attention, carried states */
+/* The layers that keep a state of fixed size instead of a cache: a short causal
+ * convolution over the fused q / k / v projection, then the gated delta rule (the
+ * engine's GDR worker, E:7483-7785; here in fp32, not its numerics). A call works
+ * on a batch of sequences, each with any number of new rows (0, 1 while it
+ * decodes, a few draft tokens, a prompt or a part of one). The state that a
+ * sequence starts from and the one it leaves are slots of a pool: the same slot,
+ * or two where a program may have to go back (drafts that are not taken: the
+ * accepted ones are run again from the old slot, E:8356) or where beams change
+ * parents (an heir reads its parent's slot).
+ *
+ * Sequence s's new rows are row_start[s] .. row_start[s + 1] of the row tensors.
+ * slot_in[s] outside [0, n_slots), or slot_in NULL: the sequence is new, its state
+ * is zero. slot_out[s] outside, or slot_out NULL: the state is not kept. No slot
+ * is read by one sequence and written by another in the same call, and none is
+ * written by two (both are safe, but leave parts of either). A sequence without
+ * new rows leaves the state it starts from.
+ *
+ * Device arrays are bounds-checked where they are used (row starts as in a cache
+ * batch). Rows that no sequence holds keep their outputs. Sums, norms, decays and
+ * states are fp32 (sums of log decays 64 bits). Inputs are finite with |x| < 65520;
+ * a value that is none spoils its own sequence alone. Rows of fp32 tensors are
+ * 16-B aligned, strides (in values) multiples of 4; outputs overlap no input.
+ * Calls keep nothing for the next one; the same call on the same kind of device
+ * gives the same bits. */
+typedef struct {
+    int n_seqs;               /* n_seqs * v_heads (* channels / 1024) below 2^24 */
+    int n_rows;               /* rows of the row tensors, below 2^30 */
+    const int32_t *row_start; /* device [n_seqs + 1], ascending */
+    const int32_t *slot_in;   /* device [n_seqs], or NULL */
+    const int32_t *slot_out;  /* device [n_seqs], or NULL */
+    int n_slots;
+    int max_new;              /* the most new rows of a sequence, as far as the host knows (0: not known): a choice of
+                                 launch, no result but by the order of sums */
+} qmm_state_batch;
+
+/* out = act(bias + sum over i < width of weight[c][i] * x_{t - width + 1 + i}[c]),
+ * act(y) = y / (1 + exp(-y)) with silu, else y. The inputs before a sequence's
+ * first new row are its state: [n_slots][width - 1][channels], oldest first. */
+typedef struct {
+    const float *x;      /* device [n_rows][x_stride] */
+    size_t x_stride;
+    int channels;        /* a multiple of 4 */
+    int width;           /* 2..4 */
+    const float *weight; /* device [channels][width]; weight[c][width - 1] is the newest row's */
+    const float *bias;   /* device [channels], or NULL */
+    float *state;        /* device; NULL with neither slot array */
+    int silu;
+    float *out;          /* device [n_rows][out_stride] */
+    size_t out_stride;
+} qmm_conv_args;
+int qmm_short_conv(qmm_context *ctx, const qmm_state_batch *batch, const qmm_conv_args *args);
+
+/* The gated delta rule: with q and k scaled to unit length,
+ *   q^ = scale * q / sqrt(sum q^2 + qk_eps),  k^ = k / sqrt(sum k^2 + qk_eps),
+ *   decay = exp(rate[h] * softplus(a + dt_bias[h])),  beta = 1 / (1 + exp(-b)),
+ * every token, in order, does for value head h (with key head h / (v_heads / qk_heads))
+ *   S <- decay * S;   S <- S + k^ (beta * (v - S' k^))';   o = S' q^
+ * on the state S [key_dim][value_dim], and its output is
+ *   o, or with gamma  o / sqrt(mean o^2 + gamma_eps) * gamma,  with z times z / (1 + exp(-z)).
+ * A rate above 0 counts as 0. Few new rows go through the state one after another;
+ * prompts in groups of 32 on the matrix units, their operands as pairs of fp16
+ * values that hold 22 bits, where a workspace allows it. */
+typedef struct {
+    const float *q, *k;   /* device [n_rows][..]: qk_heads heads of key_dim values */
+    size_t q_stride, k_stride;
+    const float *v;       /* device [n_rows][v_stride]: v_heads heads of value_dim values */
+    size_t v_stride;
+    int qk_heads, v_heads; /* v_heads a multiple of qk_heads */
+    int key_dim, value_dim; /* 64 or 128 each */
+    const float *a, *b;   /* device [n_rows][..]: v_heads values; 4-B aligned, any stride */
+    size_t a_stride, b_stride;
+    const float *rate, *dt_bias; /* device [v_heads]; rate = -exp(A_log) */
+    float scale;          /* of the queries; > 0 */
+    float qk_eps;         /* > 0 */
+    float *state;         /* device [n_slots][v_heads][key_dim][value_dim]; NULL with neither slot array */
+    const float *z;       /* device [n_rows][z_stride], or NULL */
+    size_t z_stride;
+    const float *gamma;   /* device [value_dim], or NULL */
+    float gamma_eps;      /* >= 0 */
+    float *out;           /* device [n_rows][out_stride]: v_heads heads of value_dim values */
+    size_t out_stride;
+} qmm_delta_args;
+/* Bytes of a workspace (qmm_attention_workspace_create; its rules, and one made
+ * for the attention serves here too) for calls of these heads with no more
+ * sequences and rows; 0: arguments that the call refuses (qmm_last_error). A
+ * smaller one, or NULL, makes prompts slower, and no result other than by the
+ * order of sums. */
+size_t qmm_gated_delta_workspace_bytes(qmm_context *ctx, const qmm_state_batch *batch, const qmm_delta_args *args);
+int qmm_gated_delta(qmm_context *ctx, const qmm_state_batch *batch, const qmm_delta_args *args, qmm_attn_workspace *ws);
+
+/* ----------------------------------------------------------- beam search */
+/* One step's selection: of every item, the n_keep best continuations of its
+ * n_beams beams. Beam b continued by token j has
+ *   total = score[b] + logits[b][j] - log(sum over i of exp(logits[b][i]));
+ * an ended beam has one continuation, end_token, at its own score, and its
+ * logits are not read. Order: the larger total (64 bits); among equal ones the
+ * lower beam, then the larger logit, then the lower token. A logit or score that
+ * is NaN or +infinite counts as -infinite (a token that is ruled out); all
+ * continuations of a beam without a finite one have a total of -infinite, and
+ * come last, by beam and token. What the LM head wrote as logits_out is read in
+ * place. */
+typedef struct {
+    const float *logits;  /* device [n_items * n_beams][stride] */
+    size_t stride;        /* >= vocab; any */
+    int vocab;            /* below 2^30 */
+    int n_items;
+    int n_beams;          /* 1..64; n_items * n_beams below 2^20 */
+    const float *score;   /* device [n_items * n_beams], or NULL: zeros */
+    const int32_t *ended; /* device [n_items * n_beams], nonzero where ended; or NULL */
+    int end_token;        /* with ended: 0..vocab - 1 */
+    int n_keep;           /* 1..64, at most n_beams * vocab */
+    int32_t *token;       /* device [n_items][n_keep], best first */
+    int32_t *parent;      /* device [n_items][n_keep]: the beam's number in its item */
+    float *score_out;     /* device [n_items][n_keep]: the totals */
+} qmm_beam_args;
+/* Bytes of the workspace (qmm_attention_workspace_create) that the call needs;
+ * 0: refused arguments. A smaller one is refused with QMM_ENOMEM. */
+size_t qmm_beam_workspace_bytes(qmm_context *ctx, const qmm_beam_args *args);
+int qmm_beam_select(qmm_context *ctx, const qmm_beam_args *args, qmm_attn_workspace *ws);
+
+/* Beams that change parents: slot src[i] of every pool is copied to slot dst[i],
+ * for all i and pools in one launch (pools past 64: one more). A slot is whatever
+ * the program keeps in one: a layer's recurrent state, its carried inputs, a page
+ * of a cache's keys, values or scales (a full page is shared through the page
+ * table; the last one, which heirs go on filling, is copied). No slot is both
+ * source and destination, or destination twice (both are safe, but leave parts of
+ * either); a pair with a slot outside the pool, or twice the same, copies nothing. */
+typedef struct {
+    void *base;        /* device, 16-B aligned */
+    size_t slot_bytes; /* a multiple of 16 */
+    int n_slots;
+} qmm_slot_pool;
+int qmm_copy_slots(qmm_context *ctx, const qmm_slot_pool *pools, int n_pools, const int32_t *src, const int32_t *dst, int n);
+
 /* -------------------------------------------------------------- dequant */
 /* dequant_contiguous_fast (E:3856-3902): rows x cols packed blocks -> fp16
  * bits [rows][cols] (for validation; not on the matmul path). F16 rows are

@@ -22,6 +22,8 @@
 
 #include "../../include/qmm_hip.h"
 #include "qmm_attn_check.h"
+#include "qmm_state.h"
+#include "qmm_state_check.h"
 #include "qmm_attn_plan.h"
 #include "qmm_device.h"
 
@@ -1035,6 +1037,158 @@ int qmm_paged_attention(qmm_context *ctx, const qmm_kv_batch *batch, const qmm_k
     if ((rc = use_device(ctx)) || (rc = cu_count(ctx, cus))) return rc;
     const hipError_t e = qmm::launch_attention(a, ws ? ws->base : nullptr, ws ? ws->bytes : 0, cus, ctx->stream);
     return e == hipSuccess ? QMM_OK : hip_fail(ctx, e, "attention launch");
+}
+
+namespace {
+
+void state_view(const qmm_state_batch &b, const float *state, qmm::StateView &v) {
+    v = {b.row_start, b.slot_in, b.slot_out, b.n_seqs, b.n_rows, state ? b.n_slots : 0};
+}
+
+// checks the arguments and fills in what the kernels take
+int delta_args(qmm_context *ctx, const qmm_state_batch *batch, const qmm_delta_args *t, qmm::DeltaArgs &a) {
+    const qmm::Refusal no = qmm::check_delta(batch, t);
+    if (no.code) return refuse(ctx, no);
+    state_view(*batch, t->state, a.b);
+    a.q = t->q;
+    a.k = t->k;
+    a.v = t->v;
+    a.a = t->a;
+    a.beta = t->b;
+    a.rate = t->rate;
+    a.dt_bias = t->dt_bias;
+    a.z = t->z;
+    a.gamma = t->gamma;
+    a.q_stride = t->q_stride;
+    a.k_stride = t->k_stride;
+    a.v_stride = t->v_stride;
+    a.a_stride = t->a_stride;
+    a.b_stride = t->b_stride;
+    a.z_stride = t->z_stride;
+    a.out_stride = t->out_stride;
+    a.qk_heads = t->qk_heads;
+    a.v_heads = t->v_heads;
+    a.key_dim = t->key_dim;
+    a.value_dim = t->value_dim;
+    a.max_new = batch->max_new > 0 && batch->max_new < batch->n_rows ? batch->max_new : batch->n_rows;
+    a.scale = t->scale;
+    a.qk_eps = t->qk_eps;
+    a.gamma_eps = t->gamma_eps;
+    a.state = t->state;
+    a.out = t->out;
+    return QMM_OK;
+}
+
+}  // namespace
+
+int qmm_short_conv(qmm_context *ctx, const qmm_state_batch *batch, const qmm_conv_args *t) {
+    if (!ctx) return QMM_EINVAL;
+    const qmm::Refusal no = qmm::check_conv(batch, t);
+    if (no.code) return refuse(ctx, no);
+    if (batch->n_seqs == 0) return QMM_OK;
+    qmm::ConvArgs a{};
+    state_view(*batch, t->state, a.b);
+    a.x = t->x;
+    a.weight = t->weight;
+    a.bias = t->bias;
+    a.x_stride = t->x_stride;
+    a.out_stride = t->out_stride;
+    a.channels = t->channels;
+    a.width = t->width;
+    a.silu = t->silu != 0;
+    a.max_new = batch->max_new;
+    a.state = t->state;
+    a.out = t->out;
+    const int rc = use_device(ctx);
+    if (rc) return rc;
+    const hipError_t e = qmm::launch_conv(a, ctx->stream);
+    return e == hipSuccess ? QMM_OK : hip_fail(ctx, e, "convolution launch");
+}
+
+size_t qmm_gated_delta_workspace_bytes(qmm_context *ctx, const qmm_state_batch *batch, const qmm_delta_args *args) {
+    qmm::DeltaArgs a{};
+    if (!ctx || delta_args(ctx, batch, args, a)) return 0;
+    return qmm::delta_scratch_bytes(a);
+}
+
+int qmm_gated_delta(qmm_context *ctx, const qmm_state_batch *batch, const qmm_delta_args *args, qmm_attn_workspace *ws) {
+    if (!ctx) return QMM_EINVAL;
+    qmm::DeltaArgs a{};
+    int cus = 0;
+    int rc = delta_args(ctx, batch, args, a);
+    if (rc) return rc;
+    if (ws && ws->device != ctx->device) return fail(ctx, QMM_EINVAL, "workspace of another device");
+    if (batch->n_seqs == 0) return QMM_OK;
+    if ((rc = use_device(ctx)) || (rc = cu_count(ctx, cus))) return rc;
+    const hipError_t e = qmm::launch_delta(a, ws ? ws->base : nullptr, ws ? ws->bytes : 0, cus, ctx->stream);
+    return e == hipSuccess ? QMM_OK : hip_fail(ctx, e, "delta rule launch");
+}
+
+size_t qmm_beam_workspace_bytes(qmm_context *ctx, const qmm_beam_args *args) {
+    if (!ctx) return 0;
+    const qmm::Refusal no = qmm::check_beam(args);
+    if (no.code) {
+        refuse(ctx, no);
+        return 0;
+    }
+    return qmm::beam_scratch_bytes(int64_t(args->n_items) * args->n_beams, args->vocab, args->n_keep);
+}
+
+int qmm_beam_select(qmm_context *ctx, const qmm_beam_args *t, qmm_attn_workspace *ws) {
+    if (!ctx) return QMM_EINVAL;
+    const qmm::Refusal no = qmm::check_beam(t);
+    if (no.code) return refuse(ctx, no);
+    if (ws && ws->device != ctx->device) return fail(ctx, QMM_EINVAL, "workspace of another device");
+    if (t->n_items == 0) return QMM_OK;
+    const int64_t rows = int64_t(t->n_items) * t->n_beams;
+    if (!ws || ws->bytes < qmm::beam_scratch_bytes(rows, t->vocab, t->n_keep))
+        return fail(ctx, QMM_ENOMEM, "no workspace, or one below qmm_beam_workspace_bytes");
+    if (rows * qmm::beam_slices(t->vocab) >= (int64_t(1) << 26)) return fail(ctx, QMM_ESHAPE, "too many logits for one launch");
+    qmm::BeamArgs a{};
+    a.logits = t->logits;
+    a.score = t->score;
+    a.ended = t->ended;
+    a.stride = t->stride;
+    a.vocab = t->vocab;
+    a.n_items = t->n_items;
+    a.n_beams = t->n_beams;
+    a.n_keep = t->n_keep;
+    a.end_token = t->end_token;
+    a.token = t->token;
+    a.parent = t->parent;
+    a.score_out = t->score_out;
+    a.list = static_cast<uint64_t *>(ws->base);
+    a.stat = reinterpret_cast<float *>(static_cast<char *>(ws->base) + qmm::beam_list_bytes(rows, t->vocab, t->n_keep));
+    const int rc = use_device(ctx);
+    if (rc) return rc;
+    const hipError_t e = qmm::launch_beam(a, ctx->stream);
+    return e == hipSuccess ? QMM_OK : hip_fail(ctx, e, "beam selection launch");
+}
+
+int qmm_copy_slots(qmm_context *ctx, const qmm_slot_pool *pools, int n_pools, const int32_t *src, const int32_t *dst, int n) {
+    if (!ctx) return QMM_EINVAL;
+    const qmm::Refusal no = qmm::check_copy(pools, n_pools, src, dst, n);
+    if (no.code) return refuse(ctx, no);
+    if (n == 0) return QMM_OK;
+    const int rc = use_device(ctx);
+    if (rc) return rc;
+    for (int first = 0; first < n_pools; first += 64) {
+        qmm::CopyArgs a{};
+        const int count = n_pools - first < 64 ? n_pools - first : 64;
+        size_t most = 0;
+        for (int i = 0; i < count; ++i) {
+            const qmm_slot_pool &p = pools[first + i];
+            a.pool[i] = {static_cast<char *>(p.base), p.slot_bytes, p.n_slots};
+            if (p.n_slots > 1 && p.slot_bytes > most) most = p.slot_bytes;
+        }
+        a.src = src;
+        a.dst = dst;
+        a.n = n;
+        if (!most) continue;
+        const hipError_t e = qmm::launch_copy(a, count, most, ctx->stream);
+        if (e != hipSuccess) return hip_fail(ctx, e, "slot copy launch");
+    }
+    return QMM_OK;
 }
 
 int qmm_dequantize_f16(qmm_context *ctx, const void *w_blocks, uint32_t type, int64_t rows,

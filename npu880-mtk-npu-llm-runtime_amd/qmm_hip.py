@@ -94,6 +94,39 @@ class AttentionArgs(C.Structure):
                 ("sinks", C.c_int), ("out", _p), ("out_type", C.c_uint32), ("out_stride", C.c_size_t)]
 
 
+class StateBatch(C.Structure):
+    """qmm_state_batch: the sequences of one call to a layer with carried states."""
+    _fields_ = [("n_seqs", C.c_int), ("n_rows", C.c_int), ("row_start", _p), ("slot_in", _p), ("slot_out", _p),
+                ("n_slots", C.c_int), ("max_new", C.c_int)]
+
+
+class ConvArgs(C.Structure):
+    """qmm_conv_args: the short causal convolution."""
+    _fields_ = [("x", _p), ("x_stride", C.c_size_t), ("channels", C.c_int), ("width", C.c_int), ("weight", _p), ("bias", _p),
+                ("state", _p), ("silu", C.c_int), ("out", _p), ("out_stride", C.c_size_t)]
+
+
+class DeltaArgs(C.Structure):
+    """qmm_delta_args: the gated delta rule."""
+    _fields_ = [("q", _p), ("k", _p), ("q_stride", C.c_size_t), ("k_stride", C.c_size_t), ("v", _p), ("v_stride", C.c_size_t),
+                ("qk_heads", C.c_int), ("v_heads", C.c_int), ("key_dim", C.c_int), ("value_dim", C.c_int), ("a", _p), ("b", _p),
+                ("a_stride", C.c_size_t), ("b_stride", C.c_size_t), ("rate", _p), ("dt_bias", _p), ("scale", C.c_float),
+                ("qk_eps", C.c_float), ("state", _p), ("z", _p), ("z_stride", C.c_size_t), ("gamma", _p), ("gamma_eps", C.c_float),
+                ("out", _p), ("out_stride", C.c_size_t)]
+
+
+class BeamArgs(C.Structure):
+    """qmm_beam_args: one step's selection of a beam search."""
+    _fields_ = [("logits", _p), ("stride", C.c_size_t), ("vocab", C.c_int), ("n_items", C.c_int), ("n_beams", C.c_int),
+                ("score", _p), ("ended", _p), ("end_token", C.c_int), ("n_keep", C.c_int), ("token", _p), ("parent", _p),
+                ("score_out", _p)]
+
+
+class SlotPool(C.Structure):
+    """qmm_slot_pool: slots of one size, side by side."""
+    _fields_ = [("base", _p), ("slot_bytes", C.c_size_t), ("n_slots", C.c_int)]
+
+
 # (name, restype, argtypes) of every entry point in include/qmm_hip.h
 _SIGNATURES = [
     ("qmm_init", C.c_int, [C.c_int, C.POINTER(_p)]),
@@ -156,6 +189,12 @@ _SIGNATURES = [
     ("qmm_attention_workspace_destroy", C.c_int, [_p, _p]),
     ("qmm_paged_attention", C.c_int,
      [_p, C.POINTER(KvBatch), C.POINTER(KvCache), C.POINTER(AttentionArgs), _p]),
+    ("qmm_short_conv", C.c_int, [_p, C.POINTER(StateBatch), C.POINTER(ConvArgs)]),
+    ("qmm_gated_delta_workspace_bytes", C.c_size_t, [_p, C.POINTER(StateBatch), C.POINTER(DeltaArgs)]),
+    ("qmm_gated_delta", C.c_int, [_p, C.POINTER(StateBatch), C.POINTER(DeltaArgs), _p]),
+    ("qmm_beam_workspace_bytes", C.c_size_t, [_p, C.POINTER(BeamArgs)]),
+    ("qmm_beam_select", C.c_int, [_p, C.POINTER(BeamArgs), _p]),
+    ("qmm_copy_slots", C.c_int, [_p, C.POINTER(SlotPool), C.c_int, _p, _p, C.c_int]),
     ("qmm_noalloc_scratch_bytes", C.c_size_t, []),
     ("qmm_graph_begin", C.c_int, [_p]),
     ("qmm_graph_end", C.c_int, [_p, C.POINTER(_p)]),
@@ -473,12 +512,36 @@ class Context:
     def attention_workspace(self, batch: KvBatch, cache: KvCache, args: AttentionArgs) -> _Handle:
         """A workspace for this call and all others over as many heads of this size with no more new tokens of a
         sequence (qmm_attention_workspace_bytes / _create)."""
-        n = self.lib.qmm_attention_workspace_bytes(self._h, C.byref(batch), C.byref(cache), C.byref(args))
+        return self._workspace("qmm_attention_workspace_bytes", C.byref(batch), C.byref(cache), C.byref(args))
+
+    def _workspace(self, sizes: str, *args) -> _Handle:
+        n = getattr(self.lib, sizes)(self._h, *args)
         if n == 0:
-            raise QmmError(QMM_EINVAL, f"qmm_attention_workspace_bytes: {self.last_error()}")
+            raise QmmError(QMM_EINVAL, f"{sizes}: {self.last_error()}")
         h = _p()
         self._call("qmm_attention_workspace_create", self._h, n, C.byref(h))
         return _Handle(self, h.value, "qmm_attention_workspace_destroy")
+
+    def gated_delta_workspace(self, batch: StateBatch, args: DeltaArgs) -> _Handle:
+        """A workspace for this call and all others over these heads with no more sequences and rows."""
+        return self._workspace("qmm_gated_delta_workspace_bytes", C.byref(batch), C.byref(args))
+
+    def beam_workspace(self, args: BeamArgs) -> _Handle:
+        """The workspace that this selection needs, and every one of no more beams, logits and kept ones."""
+        return self._workspace("qmm_beam_workspace_bytes", C.byref(args))
+
+    def short_conv(self, batch: StateBatch, args: ConvArgs):
+        self._call("qmm_short_conv", self._h, C.byref(batch), C.byref(args))
+
+    def gated_delta(self, batch: StateBatch, args: DeltaArgs, workspace: Optional[_Handle] = None):
+        self._call("qmm_gated_delta", self._h, C.byref(batch), C.byref(args), workspace.handle if workspace else None)
+
+    def beam_select(self, args: BeamArgs, workspace: _Handle):
+        self._call("qmm_beam_select", self._h, C.byref(args), workspace.handle)
+
+    def copy_slots(self, pools: Sequence[SlotPool], src, dst, n: int):
+        """qmm_copy_slots: slot src[i] of every pool to its slot dst[i] (device int32 arrays)."""
+        self._call("qmm_copy_slots", self._h, (SlotPool * len(pools))(*pools), len(pools), _p(_addr(src)), _p(_addr(dst)), n)
 
     def kv_append(self, batch: KvBatch, cache: KvCache, rows: KvRows):
         self._call("qmm_kv_append", self._h, C.byref(batch), C.byref(cache), C.byref(rows))
