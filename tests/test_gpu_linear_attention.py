@@ -161,3 +161,12 @@ def test_delta_same_bits(ctx):
     for news in ([1, 1, 5], [300, 70]):
         a, b = delta_case(ctx, news, HK=2, seed=5), delta_case(ctx, news, HK=2, seed=5)
         assert all(np.array_equal(x.view(np.uint32), y.view(np.uint32)) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("DK,DV", [(64, 64), (64, 128), (128, 64), (128, 128)])
+def test_delta_many_heads(ctx, DK, DV):
+    """More heads than compute units: a workgroup has all columns of one."""
+    rng = np.random.default_rng(DK + DV)
+    news = [int(n) for n in rng.integers(0, 70, 33)] + [100]
+    delta_case(ctx, news, 3, 3, DK, DV, gap=4, extra=2, seed=DV)
+    delta_case(ctx, news, 3, 3, DK, DV, gamma=False, gate=False, slots=[(i, i) for i in range(34)], seed=DK)
