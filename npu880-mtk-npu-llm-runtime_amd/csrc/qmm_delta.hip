@@ -176,21 +176,32 @@ typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 
-// An operand of 16 rows and 32 columns k in LDS: lane (row r, group g of lanes) reads 16 B at 272 g + 16 r: columns
-// 4 g .. + 3 and 16 + 4 g .. + 3. That is the order in which a group of lanes holds the rows of two tiles of
-// a product, so a product's result is the next product's right operand as it stands. (272, not 256: pieces of
-// 8 B of four columns then lie on all banks when they are written.)
-constexpr int kBlock = 4 * 272;
+// An operand of 16 rows and 32 columns k in LDS, 1 KB: lane (row r, group g of lanes) reads the 16 B of place 16 g + (r ^ g),
+// columns 4 g .. + 3 and 16 + 4 g .. + 3. That is the order in which a group of lanes holds the rows of two tiles
+// of a product, so a product's result is the next product's right operand as it stands. (r ^ g, not r: pieces of
+// 8 B of four columns, written by the lanes of four rows and all g at once, then lie on all banks.)
+constexpr int kBlock = 1024;
 __device__ inline int operand_at(int row, int col) {  // of the aligned 4 columns from `col` (of 32)
-    return (col % 16 / 4) * 272 + (row % 16) * 16 + col / 16 * 8;
+    const int g = col % 16 / 4;
+    return g * 256 + (row % 16 ^ g) * 16 + col / 16 * 8;
 }
 __device__ inline f4 mfma(h8 a, h8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
-// x = hi + lo + at most 2^-22 |x| (and 2^-25)
+// x f = hi + lo + at most 2^-22 |x f| (and 2^-25). `f` is no constant the compiler sees, so that the low part is one
+// operation on the fp16 high part.
+__device__ inline void split4(f4 x, float f, h4 &hi, h4 &lo) {
+    hi = __builtin_convertvector(x * f, h4);
+    f4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = __builtin_fmaf(x[i], f, -float(hi[i]));
+    lo = __builtin_convertvector(r, h4);
+}
 __device__ inline void split4(f4 x, h4 &hi, h4 &lo) {
+    float one = 1.0f;
+    asm("" : "+s"(one));
     hi = __builtin_convertvector(x, h4);
     f4 r;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = __builtin_fmaf(float(hi[i]), -1.0f, x[i]);
+    for (int i = 0; i < 4; ++i) r[i] = __builtin_fmaf(x[i], one, -float(hi[i]));
     lo = __builtin_convertvector(r, h4);
 }
 struct Pair {
@@ -207,6 +218,31 @@ __device__ inline Pair operand(const char *p) {  // p: this lane's place in the 
 }
 __device__ inline f4 product(const Pair &a, const Pair &b, f4 c) { return mfma(a.lo, b.hi, mfma(a.hi, b.lo, mfma(a.hi, b.hi, c))); }
 
+// K S and Q S of both token tiles, the three products of each pair apart, as each adds to the one before
+template <int NT> __device__ inline void products(const Pair (&op)[4], const Pair (&b)[NT], f4 (&ks)[2][NT], f4 (&qs)[2][NT]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            f4 &c = i < 2 ? ks[i][j] : qs[i - 2][j];
+            c = mfma(op[i].hi, b[j].hi, c);
+        }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            f4 &c = i < 2 ? ks[i][j] : qs[i - 2][j];
+            c = mfma(op[i].hi, b[j].lo, c);
+        }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            f4 &c = i < 2 ? ks[i][j] : qs[i - 2][j];
+            c = mfma(op[i].lo, b[j].hi, c);
+        }
+}
+
 struct DeltaScratch {
     char *matrices;  // [groups][v_heads]: T diag(beta), then P: two tiles of 16 rows, each 1 KB hi and 1 KB lo
     float *decays;   // [groups][v_heads][64]: e^G_i, e^(G_last - G_i)
@@ -214,55 +250,48 @@ struct DeltaScratch {
 };
 __device__ inline int64_t first_group(const StateSeq &v, int s) { return v.r0 / kChunk + s; }
 
+// Up to 32 rows from `p` on, of which `left` are the sequence's, as a buffer: loads past them give 0 and stores nothing, without a
+// branch. p: row 0 of one head, `before` values into its row; stride below 2^24 values, so that all offsets fit.
+__device__ inline __amdgpu_buffer_rsrc_t group_rows(const float *p, size_t stride, int before, int left) {
+    const uint32_t bytes = left > 0 ? (uint32_t(min(left, kChunk)) * uint32_t(stride) - uint32_t(before)) * 4u : 0u;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(p), short(0), int(bytes), 0x00020000);
+}
+
 // 4 tokens x 4 values of q or k for item `i` of a group's 2 * 8 * DK / 4: eight lanes side by side take 128 B
 template <int DK> struct Item {
     int is_q, token, at;
     __device__ explicit Item(int i) {
         constexpr int kAll = 8 * DK / 4;
-        is_q = i / kAll;
+        is_q = __builtin_amdgcn_readfirstlane(i / kAll);  // (a wave has one kind)
         const int r = i % kAll;
         token = r / 8 % 8 * 4;
         at = (r / 64 * 8 + r % 8) * 4;
     }
-    __device__ void load(const DeltaArgs &a, int hk, int r0, int left, float4 x[4]) const {
-        const float *src = (is_q ? a.q : a.k) + size_t(hk) * DK + at;
+    // from rows r0 .. of which `left` are the sequence's
+    __device__ void load(const DeltaArgs &a, int hk, int r0, int left, f4 x[4]) const {
         const size_t stride = is_q ? a.q_stride : a.k_stride;
+        const __amdgpu_buffer_rsrc_t rows = group_rows((is_q ? a.q : a.k) + size_t(r0) * stride + size_t(hk) * DK, stride, hk * DK, left);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (token + j < left) x[j] = load4(src + size_t(r0 + token + j) * stride);
-        }
+        for (int j = 0; j < 4; ++j)
+            x[j] = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(rows, (unsigned(token + j) * unsigned(stride) + unsigned(at)) * 4u, 0, 0));
     }
-    // as left operand, rows the tokens: tiles of 16 tokens, each DK / 32 blocks of hi and lo
-    __device__ void store(char *base, const float4 x[4], const float *inv) const {
+    // times 2^4 / length as left operand, rows the tokens (tiles of 16, each DK / 32 blocks of hi and lo) and, where
+    // `turned`, rows the values (tiles of 16, each one block)
+    __device__ void store(char *base, char *turned, const f4 x[4], f4 inv) const {
+        h4 hi[4], lo[4];
+        char *p = base + ((token / 16) * (DK / 32) + at / 32) * 2 * kBlock;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const float f = inv[j] * 16.0f;
-            h4 hi, lo;
-            split4(f4{x[j].x * f, x[j].y * f, x[j].z * f, x[j].w * f}, hi, lo);
-            char *p = base + ((token / 16) * (DK / 32) + at / 32) * 2 * kBlock + operand_at(token + j, at % 32);
-            *reinterpret_cast<h4 *>(p) = hi;
-            *reinterpret_cast<h4 *>(p + kBlock) = lo;
+            split4(x[j], inv[j] * 16.0f, hi[j], lo[j]);
+            *reinterpret_cast<h4 *>(p + operand_at(token + j, at % 32)) = hi[j];
+            *reinterpret_cast<h4 *>(p + operand_at(token + j, at % 32) + kBlock) = lo[j];
         }
-    }
-    // as left operand, rows the values: tiles of 16 values, each one block of hi and lo
-    __device__ void store_turned(char *base, const float4 x[4], const float *inv) const {
-        f4 y[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float f = inv[j] * 16.0f;
-            y[0][j] = x[j].x * f;
-            y[1][j] = x[j].y * f;
-            y[2][j] = x[j].z * f;
-            y[3][j] = x[j].w * f;
-        }
+        if (!turned) return;
+        p = turned + (at / 16) * 2 * kBlock;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-            h4 hi, lo;
-            split4(y[c], hi, lo);
-            char *p = base + (at / 16) * 2 * kBlock + operand_at(at + c, token);
-            *reinterpret_cast<h4 *>(p) = hi;
-            *reinterpret_cast<h4 *>(p + kBlock) = lo;
+            *reinterpret_cast<h4 *>(p + operand_at(at + c, token)) = h4{hi[0][c], hi[1][c], hi[2][c], hi[3][c]};
+            *reinterpret_cast<h4 *>(p + operand_at(at + c, token) + kBlock) = h4{lo[0][c], lo[1][c], lo[2][c], lo[3][c]};
         }
     }
 };
@@ -280,7 +309,7 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, DeltaSc
     constexpr int NU = DK / 32, NI = DK / 64, kRow = 36;
     __shared__ __attribute__((aligned(16))) char rows[2][2 * NU * 2 * kBlock];  // k and q as operands
     __shared__ float sums[2][32][NU];
-    __shared__ float inv[2][32];
+    __shared__ __attribute__((aligned(16))) float inv[2][32];
     __shared__ float kk[32][kRow], qk[32][kRow];
     __shared__ float A[2][32][kRow], T[2][32][kRow];
     __shared__ double G[2][32];
@@ -292,7 +321,7 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, DeltaSc
     for (int tile = st % tiles; int64_t(tile) * kChunk < v.n; tile += tiles) {
         const int r0 = v.r0 + tile * kChunk, left = v.n - tile * kChunk;
         const size_t group = size_t(first_group(v, s) + tile);
-        float4 x[NI][4];
+        f4 x[NI][4];
 #pragma unroll
         for (int i = 0; i < NI; ++i) Item<DK>(t + 256 * i).load(a, hk, r0, left, x[i]);
 #pragma unroll
@@ -300,7 +329,7 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, DeltaSc
             const Item<DK> it(t + 256 * i);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                float ss = dot4(x[i][j], x[i][j]);  // over the eight lanes that share a token
+                float ss = (x[i][j][0] * x[i][j][0] + x[i][j][1] * x[i][j][1]) + (x[i][j][2] * x[i][j][2] + x[i][j][3] * x[i][j][3]);  // over the eight lanes that share a token
                 ss += lane_moved<0xB1>(ss);
                 ss += lane_moved<0x4E>(ss);
                 ss += lane_moved<0x141>(ss);
@@ -320,12 +349,12 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, DeltaSc
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
             const Item<DK> it(t + 256 * i);
-            it.store(rows[it.is_q], x[i], &inv[it.is_q][it.token]);
+            it.store(rows[it.is_q], nullptr, x[i], *reinterpret_cast<const f4 *>(&inv[it.is_q][it.token]));
         }
         __syncthreads();
         for (int task = wid; task < 6; task += 4) {  // k k' and q k', the tiles on and below the diagonal
             const int is_q = task / 3, ti = task % 3 != 0, tj = task % 3 == 2;
-            const int at = (lane / 16) * 272 + (lane % 16) * 16;
+            const int at = (lane / 16) * 256 + (lane % 16 ^ lane / 16) * 16;
             f4 c{};
 #pragma unroll
             for (int u = 0; u < NU; ++u)
@@ -424,7 +453,7 @@ __device__ inline float over_groups(float x) {  // sum over the four lanes of a 
 // rows, as sums of matrix products; nothing of it leaves the wave's registers from group to group. Four
 // more waves bring the next group's K, Q, T diag(beta) and P into LDS as operands meanwhile.
 template <int DK, int NW, int NT>
-__global__ __launch_bounds__(64 * (NW + 4)) void delta_walk_kernel(DeltaArgs a, DeltaScratch w, int splits) {
+__global__ __launch_bounds__(512) void delta_walk_kernel(DeltaArgs a, DeltaScratch w, int splits) {
     constexpr int NU = DK / 32, NI = DK / 64;
     constexpr int kK = 0, kQ = kK + 2 * NU * 2 * kBlock, kTurned = kQ + 2 * NU * 2 * kBlock, kM = kTurned + DK / 16 * 2 * kBlock;
     constexpr int kP = kM + 4 * kBlock, kDecays = kP + 4 * kBlock, kBuffer = kDecays + 256;
@@ -440,71 +469,90 @@ __global__ __launch_bounds__(64 * (NW + 4)) void delta_walk_kernel(DeltaArgs a, 
     const int t = threadIdx.x, lane = t & 63, wid = __builtin_amdgcn_readfirstlane(t >> 6);
 
     if (wid >= NW) {
-        const int i = t - 64 * NW;  // of 256
-        float4 x[NI][4];
-        float inv[NI][4];
-        uint4 m0, m1;
-        float decay = 0.0f;
-        auto load = [&](int n) {
-            const size_t group = group0 + n;
+        // (waves go to the four SIMDs in turns: with two walking ones, the two after the first four would share theirs)
+        if (NW == 2 && (wid & 2) == 0) return;
+        const int i = NW == 2 ? (wid / 4 * 2 + wid % 2) * 64 + lane : t - 64 * NW;  // of 256
+        // what a thread holds of a group while it comes from memory
+        struct Held {
+            f4 x[NI][4];
+            f4 inv[NI];
+            uint4 m0, m1;
+            float decay;
+        };
+        auto load = [&](int n, Held &y) {  // (past the last group: rows of zeros, the last one's matrices)
+            const size_t group = group0 + min(n, n_groups - 1);
 #pragma unroll
             for (int j = 0; j < NI; ++j) {
                 const Item<DK> it(i + 256 * j);
-                it.load(a, hk, v.r0 + n * kChunk, v.n - n * kChunk, x[j]);
-                const float4 r = load4(w.inverse + (group * a.qk_heads + hk) * 64 + it.is_q * 32 + it.token);
-                inv[j][0] = r.x;
-                inv[j][1] = r.y;
-                inv[j][2] = r.z;
-                inv[j][3] = r.w;
+                it.load(a, hk, v.r0 + n * kChunk, v.n - n * kChunk, y.x[j]);
+                y.inv[j] = *reinterpret_cast<const f4 *>(w.inverse + (group * a.qk_heads + hk) * 64 + it.is_q * 32 + it.token);
             }
             const uint4 *src = reinterpret_cast<const uint4 *>(w.matrices + (group * a.v_heads + h) * kDeltaMatrices);
-            m0 = src[i];
-            m1 = src[i + 256];
-            if (i < 64) decay = w.decays[(group * a.v_heads + h) * 64 + i];
+            y.m0 = src[i];
+            y.m1 = src[i + 256];
+            if (i < 64) y.decay = w.decays[(group * a.v_heads + h) * 64 + i];
         };
-        auto store = [&](char *buf) {
+        auto store = [&](int n, const Held &y) {
+            char *buf = lds + n % 2 * kBuffer;
 #pragma unroll
             for (int j = 0; j < NI; ++j) {
                 const Item<DK> it(i + 256 * j);
-                it.store(buf + (it.is_q ? kQ : kK), x[j], inv[j]);
-                if (!it.is_q) it.store_turned(buf + kTurned, x[j], inv[j]);
+                it.store(buf + (it.is_q ? kQ : kK), it.is_q ? nullptr : buf + kTurned, y.x[j], y.inv[j]);
             }
-            char *to = buf + kM + i / 64 * kBlock + i % 64 / 16 * 272 + i % 16 * 16;
-            *reinterpret_cast<uint4 *>(to) = m0;
-            *reinterpret_cast<uint4 *>(to + 4 * kBlock) = m1;
-            if (i < 64) reinterpret_cast<float *>(buf + kDecays)[i] = decay;
+            char *to = buf + kM + i / 64 * kBlock + i % 64 / 16 * 256 + (i % 16 ^ i % 64 / 16) * 16;
+            *reinterpret_cast<uint4 *>(to) = y.m0;
+            *reinterpret_cast<uint4 *>(to + 4 * kBlock) = y.m1;
+            if (i < 64) reinterpret_cast<float *>(buf + kDecays)[i] = y.decay;
         };
-        if (n_groups > 0) {
-            load(0);
-            store(lds);
+        if (n_groups == 0) {
+            __syncthreads();
+            return;
         }
-        if (n_groups > 1) load(1);
+        Held even, odd;  // two groups are under way, so that a walk's step may be shorter than the memory's latency
+        load(0, even);
+        load(1, odd);
+        store(0, even);
+        load(2, even);
         __syncthreads();
-        for (int n = 0; n < n_groups; ++n) {
-            if (n + 1 < n_groups) store(lds + (n + 1) % 2 * kBuffer);
-            if (n + 2 < n_groups) load(n + 2);
+        for (int n = 0; n < n_groups; n += 2) {
+            store(n + 1, odd);
+            load(n + 3, odd);
+            __syncthreads();
+            if (n + 1 >= n_groups) break;
+            store(n + 2, even);
+            load(n + 4, even);
             __syncthreads();
         }
         return;
     }
 
-    const int g = lane / 16, lane_at = g * 272 + (lane % 16) * 16;
+    __builtin_amdgcn_s_setprio(2);  // before the waves that bring operands
+    const int g = lane / 16, lane_at = g * 256 + (lane % 16 ^ g) * 16;
     const int col = (split_no * NW + wid) * 16 * NT + lane % 16;  // of column tile 0
     const int DV = a.value_dim;
     const size_t place = size_t(h) * DK * DV + col, pool = size_t(a.v_heads) * DK * DV;
     f4 S[2 * NU][NT];
-    f4 val[2][NT];
-    float bound[NT], sum[NT];  // of the column's length; of the next values' sizes
+    f4 val[2][NT], ahead[2][NT];  // values of this group and the next
+    float bound[NT], sum[NT];     // of the column's length; of the values' sizes
     int scale[NT];             // S is kept times 2^scale
-    auto load_values = [&](int n) {
+    float out_scale[NT];
+    unsigned v_at[2][4], out_at[2][4];  // bytes from a group's first row to this lane's, of its row tensors
+#pragma unroll
+    for (int ti = 0; ti < 2; ++ti)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            v_at[ti][r] = (unsigned(16 * ti + 4 * g + r) * unsigned(a.v_stride) + unsigned(col)) * 4u;
+            out_at[ti][r] = (unsigned(16 * ti + 4 * g + r) * unsigned(a.out_stride) + unsigned(col)) * 4u;
+        }
+    auto load_values = [&](int n, f4 (&to)[2][NT]) {
+        const __amdgpu_buffer_rsrc_t rows =
+            group_rows(a.v + size_t(v.r0 + n * kChunk) * a.v_stride + size_t(h) * DV, a.v_stride, h * DV, v.n - n * kChunk);
 #pragma unroll
         for (int ti = 0; ti < 2; ++ti)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int m = n * kChunk + 16 * ti + 4 * g + r;
+            for (int r = 0; r < 4; ++r)
 #pragma unroll
-                for (int j = 0; j < NT; ++j) val[ti][j][r] = m < v.n ? a.v[size_t(v.r0 + m) * a.v_stride + size_t(h) * DV + col + 16 * j] : 0.0f;
-            }
+                for (int j = 0; j < NT; ++j) to[ti][j][r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rows, v_at[ti][r] + 64u * j, 0, 0));
     };
     auto sum_values = [&](int j) {
         float x = 0.0f;
@@ -514,7 +562,8 @@ __global__ __launch_bounds__(64 * (NW + 4)) void delta_walk_kernel(DeltaArgs a, 
             for (int r = 0; r < 4; ++r) x += fabsf(val[ti][j][r]);
         return over_groups(x);
     };
-    load_values(0);
+    load_values(0, val);
+    load_values(1, ahead);
 #pragma unroll
     for (int k = 0; k < 2 * NU; ++k)
 #pragma unroll
@@ -550,33 +599,48 @@ __global__ __launch_bounds__(64 * (NW + 4)) void delta_walk_kernel(DeltaArgs a, 
     for (int n = 0; n < n_groups; ++n) {
         const char *buf = lds + n % 2 * kBuffer + lane_at;
         const float *decays = reinterpret_cast<const float *>(lds + n % 2 * kBuffer + kDecays);
+        // Operands are read a step ahead of their products: a wave waits about as long for LDS as eight products take,
+        // and has no other wave beside it to fill the gap.
         f4 ks[2][NT], qs[2][NT];
 #pragma unroll
         for (int ti = 0; ti < 2; ++ti)
 #pragma unroll
             for (int j = 0; j < NT; ++j) ks[ti][j] = qs[ti][j] = f4{0.f, 0.f, 0.f, 0.f};
+        Pair ops[2][4];  // of two steps: K and Q of both token tiles
+        auto read_step = [&](int u, Pair (&to)[4]) {
 #pragma unroll
-        for (int u = 0; u < NU; ++u) {
-            Pair b[NT];
+            for (int i = 0; i < 4; ++i) to[i] = operand(buf + (i < 2 ? kK : kQ) + (i % 2 * NU + u) * 2 * kBlock);
+        };
+        read_step(0, ops[0]);
+        Pair b[2][NT];  // S of two steps as right operands: split a step ahead, beside the products
 #pragma unroll
-            for (int j = 0; j < NT; ++j) b[j] = split(S[2 * u][j], S[2 * u + 1][j]);
-#pragma unroll
-            for (int ti = 0; ti < 2; ++ti) {
-                const Pair k = operand(buf + kK + (ti * NU + u) * 2 * kBlock), q = operand(buf + kQ + (ti * NU + u) * 2 * kBlock);
-#pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    ks[ti][j] = product(k, b[j], ks[ti][j]);
-                    qs[ti][j] = product(q, b[j], qs[ti][j]);
-                }
-            }
-        }
+        for (int j = 0; j < NT; ++j) b[0][j] = split(S[0][j], S[1][j]);
+        Pair m[2], p[2], kt[2][2];
         f4 eg[2], el[2];
 #pragma unroll
-        for (int ti = 0; ti < 2; ++ti) {
-            eg[ti] = *reinterpret_cast<const f4 *>(decays + 16 * ti + 4 * g);
-            el[ti] = *reinterpret_cast<const f4 *>(decays + 32 + 16 * ti + 4 * g);
+        for (int u = 0; u < NU; ++u) {
+            if (u + 1 < NU) {
+                read_step(u + 1, ops[(u + 1) % 2]);
+            } else {
+#pragma unroll
+                for (int ti = 0; ti < 2; ++ti) {
+                    m[ti] = operand(buf + kM + ti * 2 * kBlock);
+                    eg[ti] = *reinterpret_cast<const f4 *>(decays + 16 * ti + 4 * g);
+                    el[ti] = *reinterpret_cast<const f4 *>(decays + 32 + 16 * ti + 4 * g);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            products<NT>(ops[u % 2], b[u % 2], ks, qs);
+            if (u + 1 < NU) {
+#pragma unroll
+                for (int j = 0; j < NT; ++j) b[(u + 1) % 2][j] = split(S[2 * u + 2][j], S[2 * u + 3][j]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
         const float all = decays[31];
+#pragma unroll
+        for (int ti = 0; ti < 2; ++ti) p[ti] = operand(buf + kP + ti * 2 * kBlock);
+        __builtin_amdgcn_sched_barrier(0);
         Pair xb[NT];
 #pragma unroll
         for (int j = 0; j < NT; ++j) {  // V - e^G K S, times 2^(scale - 4)
@@ -587,47 +651,63 @@ __global__ __launch_bounds__(64 * (NW + 4)) void delta_walk_kernel(DeltaArgs a, 
                 for (int r = 0; r < 4; ++r) x[ti][r] = __builtin_fmaf(eg[ti][r] * -0x1p-8f, ks[ti][j][r], val[ti][j][r] * two_to(scale[j] - 4));
             xb[j] = split(x[0], x[1]);
         }
-        load_values(n + 1);
+#pragma unroll
+        for (int ti = 0; ti < 2; ++ti)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) val[ti][j] = ahead[ti][j];
+        load_values(n + 2, ahead);
         f4 d[2][NT];  // D times 2^scale
 #pragma unroll
-        for (int ti = 0; ti < 2; ++ti) {
-            const Pair m = operand(buf + kM + ti * 2 * kBlock);
+        for (int ti = 0; ti < 2; ++ti)
 #pragma unroll
-            for (int j = 0; j < NT; ++j) d[ti][j] = product(m, xb[j], f4{0.f, 0.f, 0.f, 0.f});
-        }
-        f4 o[2][NT];
-#pragma unroll
-        for (int j = 0; j < NT; ++j) xb[j] = split(d[0][j], d[1][j]);
-#pragma unroll
-        for (int ti = 0; ti < 2; ++ti) {
-            const Pair p = operand(buf + kP + ti * 2 * kBlock);
-#pragma unroll
-            for (int j = 0; j < NT; ++j) o[ti][j] = product(p, xb[j], qs[ti][j] * eg[ti]);
-        }
+            for (int j = 0; j < NT; ++j) d[ti][j] = product(m[ti], xb[j], f4{0.f, 0.f, 0.f, 0.f});
+        float turn[NT];
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-            const float f = a.scale * two_to(-(scale[j] + 4));
-#pragma unroll
-            for (int ti = 0; ti < 2; ++ti)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int m = n * kChunk + 16 * ti + 4 * g + r;
-                    if (m < v.n) a.out[size_t(v.r0 + m) * a.out_stride + size_t(h) * DV + col + 16 * j] = o[ti][j][r] * f;
-                }
             bound[j] = __builtin_fmaf(all, bound[j], sum[j]);
             sum[j] = sum_values(j);
             const int next = scale_for(bound[j] + sum[j]);
-            const float turn = two_to(next - scale[j]);
+            turn[j] = two_to(next - scale[j]);
+            out_scale[j] = a.scale * two_to(-(scale[j] + 4));
             scale[j] = next;
 #pragma unroll
-            for (int k = 0; k < 2 * NU; ++k) S[k][j] *= all * turn;
-            xb[j] = split(d[0][j] * (el[0] * (turn * 0x1p-4f)), d[1][j] * (el[1] * (turn * 0x1p-4f)));
+            for (int k = 0; k < 2 * NU; ++k) S[k][j] *= all * turn[j];
         }
+        auto read_turned = [&](int k, Pair (&to)[2]) {
+            to[0] = operand(buf + kTurned + k * 2 * kBlock);
+            to[1] = operand(buf + kTurned + (k + 1) * 2 * kBlock);
+        };
+        read_turned(0, kt[0]);
+        __builtin_amdgcn_sched_barrier(0);
+        f4 o[2][NT];
 #pragma unroll
-        for (int k = 0; k < 2 * NU; ++k) {
-            const Pair kt = operand(buf + kTurned + k * 2 * kBlock);
+        for (int j = 0; j < NT; ++j) {
+            const Pair db = split(d[0][j], d[1][j]);
 #pragma unroll
-            for (int j = 0; j < NT; ++j) S[k][j] = product(kt, xb[j], S[k][j]);
+            for (int ti = 0; ti < 2; ++ti) o[ti][j] = product(p[ti], db, qs[ti][j] * eg[ti]);
+            xb[j] = split(d[0][j] * (el[0] * (turn[j] * 0x1p-4f)), d[1][j] * (el[1] * (turn[j] * 0x1p-4f)));
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int k = 0; k < 2 * NU; k += 2) {
+            if (k + 2 < 2 * NU) read_turned(k + 2, kt[k / 2 % 2 ^ 1]);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) S[k + i][j] = product(kt[k / 2 % 2][i], xb[j], S[k + i][j]);
+            if (k == 0) {
+                const __amdgpu_buffer_rsrc_t rows =
+                    group_rows(a.out + size_t(v.r0 + n * kChunk) * a.out_stride + size_t(h) * DV, a.out_stride, h * DV, v.n - n * kChunk);
+#pragma unroll
+                for (int ti = 0; ti < 2; ++ti)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+#pragma unroll
+                        for (int j = 0; j < NT; ++j)
+                            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(o[ti][j][r] * out_scale[j]), rows, out_at[ti][r] + 64u * j, 0, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
         __syncthreads();
     }
@@ -675,7 +755,7 @@ template <int DK, int NW, int NT> hipError_t launch_walk(const DeltaArgs &a, con
     constexpr int kBuffer = ((2 * 2 * (DK / 32) + DK / 16) * 2 + 8) * kBlock + 256;
     const int splits = a.value_dim / (16 * NW * NT), per = a.v_heads / a.qk_heads * splits;
     const int units = a.b.n_seqs * a.qk_heads;
-    hipLaunchKernelGGL((delta_walk_kernel<DK, NW, NT>), dim3(unsigned((units + 7) / 8) * 8u * unsigned(per)), dim3(64 * (NW + 4)),
+    hipLaunchKernelGGL((delta_walk_kernel<DK, NW, NT>), dim3(unsigned((units + 7) / 8) * 8u * unsigned(per)), dim3(512),
                        2 * kBuffer, s, a, w, splits);
     return hipGetLastError();
 }
@@ -700,8 +780,10 @@ template <int DK> hipError_t launch_groups(const DeltaArgs &a, const DeltaScratc
 }  // namespace
 
 hipError_t launch_delta(const DeltaArgs &a, void *scratch, size_t scratch_bytes, int cu_count, hipStream_t s) {
-    // (a walk of 2^22 heads would be past 2^32 threads)
-    if (a.max_new > kStepRows && scratch && scratch_bytes >= delta_scratch_bytes(a) && int64_t(a.b.n_seqs) * a.v_heads < (1 << 22)) {
+    // (a walk of 2^22 heads would be past 2^32 threads; lanes reach 12 rows in 32 bits of bytes)
+    const size_t widest = max(max(a.q_stride, a.k_stride), max(a.v_stride, a.out_stride));
+    if (a.max_new > kStepRows && scratch && scratch_bytes >= delta_scratch_bytes(a) && int64_t(a.b.n_seqs) * a.v_heads < (1 << 22) &&
+        widest < (1 << 24)) {
         const size_t groups = size_t(delta_groups(a.b.n_rows, a.b.n_seqs));
         DeltaScratch w;
         w.matrices = static_cast<char *>(scratch);
