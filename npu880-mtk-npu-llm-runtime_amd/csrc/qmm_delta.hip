@@ -218,29 +218,20 @@ __device__ inline Pair operand(const char *p) {  // p: this lane's place in the 
 }
 __device__ inline f4 product(const Pair &a, const Pair &b, f4 c) { return mfma(a.lo, b.hi, mfma(a.hi, b.lo, mfma(a.hi, b.hi, c))); }
 
-// K S and Q S of both token tiles, the three products of each pair apart, as each adds to the one before
-template <int NT> __device__ inline void products(const Pair (&op)[4], const Pair (&b)[NT], f4 (&ks)[2][NT], f4 (&qs)[2][NT]) {
+// The products of two tiles of rows, the three of each pair apart, as each adds to the one before
+__device__ inline void products(const Pair (&op)[2], const Pair &b, f4 (&c)[2]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int part = 0; part < 3; ++part)
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            f4 &c = i < 2 ? ks[i][j] : qs[i - 2][j];
-            c = mfma(op[i].hi, b[j].hi, c);
-        }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            f4 &c = i < 2 ? ks[i][j] : qs[i - 2][j];
-            c = mfma(op[i].hi, b[j].lo, c);
-        }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            f4 &c = i < 2 ? ks[i][j] : qs[i - 2][j];
-            c = mfma(op[i].lo, b[j].hi, c);
-        }
+        for (int i = 0; i < 2; ++i) c[i] = mfma(part < 2 ? op[i].hi : op[i].lo, part == 1 ? b.lo : b.hi, c[i]);
+}
+// the order of what stands since the last barrier of the scheduler: N times one matrix product and K vector instructions
+template <int N, int K> __device__ inline void mix() {
+    if constexpr (N > 0) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, K, 0);
+        mix<N - 1, K>();
+    }
 }
 
 struct DeltaScratch {
@@ -253,17 +244,18 @@ __device__ inline int64_t first_group(const StateSeq &v, int s) { return v.r0 / 
 // Up to 32 rows from `p` on, of which `left` are the sequence's, as a buffer: loads past them give 0 and stores nothing, without a
 // branch. p: row 0 of one head, `before` values into its row; stride below 2^24 values, so that all offsets fit.
 __device__ inline __amdgpu_buffer_rsrc_t group_rows(const float *p, size_t stride, int before, int left) {
-    const uint32_t bytes = left > 0 ? (uint32_t(min(left, kChunk)) * uint32_t(stride) - uint32_t(before)) * 4u : 0u;
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(p), short(0), int(bytes), 0x00020000);
+    const uint32_t rows = uint32_t(min(max(left, 0), kChunk));
+    const uint32_t bytes = (rows * uint32_t(stride) - (rows ? uint32_t(before) : 0u)) * 4u;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(p), short(0), __builtin_amdgcn_readfirstlane(int(bytes)), 0x00020000);
 }
 
-// 4 tokens x 4 values of q or k for item `i` of a group's 2 * 8 * DK / 4: eight lanes side by side take 128 B
+// 4 tokens x 4 values of q or k, one of a group's 2 * 8 * DK / 4: eight lanes side by side take 128 B
 template <int DK> struct Item {
     int is_q, token, at;
-    __device__ explicit Item(int i) {
+    __device__ Item(int t, int j) {  // thread t's j-th of DK / 64; a wave has one kind
         constexpr int kAll = 8 * DK / 4;
-        is_q = __builtin_amdgcn_readfirstlane(i / kAll);  // (a wave has one kind)
-        const int r = i % kAll;
+        is_q = DK == 128 ? j : __builtin_amdgcn_readfirstlane(t / kAll);
+        const int r = t % kAll;
         token = r / 8 % 8 * 4;
         at = (r / 64 * 8 + r % 8) * 4;
     }
@@ -277,12 +269,14 @@ template <int DK> struct Item {
     }
     // times 2^4 / length as left operand, rows the tokens (tiles of 16, each DK / 32 blocks of hi and lo) and, where
     // `turned`, rows the values (tiles of 16, each one block)
-    __device__ void store(char *base, char *turned, const f4 x[4], f4 inv) const {
-        h4 hi[4], lo[4];
+    __device__ void convert(const f4 x[4], f4 inv, h4 hi[4], h4 lo[4]) const {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) split4(x[j], inv[j] * 16.0f, hi[j], lo[j]);
+    }
+    __device__ void store(char *base, char *turned, const h4 hi[4], const h4 lo[4]) const {
         char *p = base + ((token / 16) * (DK / 32) + at / 32) * 2 * kBlock;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            split4(x[j], inv[j] * 16.0f, hi[j], lo[j]);
             *reinterpret_cast<h4 *>(p + operand_at(token + j, at % 32)) = hi[j];
             *reinterpret_cast<h4 *>(p + operand_at(token + j, at % 32) + kBlock) = lo[j];
         }
@@ -307,11 +301,13 @@ __device__ inline double shfl_up(double x, int d) {
 template <int DK>
 __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, DeltaScratch w, int tiles) {
     constexpr int NU = DK / 32, NI = DK / 64, kRow = 36;
-    __shared__ __attribute__((aligned(16))) char rows[2][2 * NU * 2 * kBlock];  // k and q as operands
+    constexpr int kRows = 2 * NU * 2 * kBlock, kTriangles = 2 * 2 * 32 * kRow * 4;
+    __shared__ __attribute__((aligned(16))) char shared[2 * kRows > kTriangles ? 2 * kRows : kTriangles];
+    char *const rows = shared;  // k and q as operands; after their products A and T of two heads
+    auto A = reinterpret_cast<float(*)[32][kRow]>(shared), T = reinterpret_cast<float(*)[32][kRow]>(shared + kTriangles / 2);
     __shared__ float sums[2][32][NU];
     __shared__ __attribute__((aligned(16))) float inv[2][32];
     __shared__ float kk[32][kRow], qk[32][kRow];
-    __shared__ float A[2][32][kRow], T[2][32][kRow];
     __shared__ double G[2][32];
     __shared__ float beta[2][32];
     const int t = threadIdx.x, lane = t & 63, wid = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -323,10 +319,10 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, DeltaSc
         const size_t group = size_t(first_group(v, s) + tile);
         f4 x[NI][4];
 #pragma unroll
-        for (int i = 0; i < NI; ++i) Item<DK>(t + 256 * i).load(a, hk, r0, left, x[i]);
+        for (int i = 0; i < NI; ++i) Item<DK>(t, i).load(a, hk, r0, left, x[i]);
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-            const Item<DK> it(t + 256 * i);
+            const Item<DK> it(t, i);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 float ss = (x[i][j][0] * x[i][j][0] + x[i][j][1] * x[i][j][1]) + (x[i][j][2] * x[i][j][2] + x[i][j][3] * x[i][j][3]);  // over the eight lanes that share a token
@@ -348,8 +344,10 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, DeltaSc
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-            const Item<DK> it(t + 256 * i);
-            it.store(rows[it.is_q], nullptr, x[i], *reinterpret_cast<const f4 *>(&inv[it.is_q][it.token]));
+            const Item<DK> it(t, i);
+            h4 hi[4], lo[4];
+            it.convert(x[i], *reinterpret_cast<const f4 *>(&inv[it.is_q][it.token]), hi, lo);
+            it.store(rows + it.is_q * kRows, nullptr, hi, lo);
         }
         __syncthreads();
         for (int task = wid; task < 6; task += 4) {  // k k' and q k', the tiles on and below the diagonal
@@ -358,11 +356,12 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, DeltaSc
             f4 c{};
 #pragma unroll
             for (int u = 0; u < NU; ++u)
-                c = product(operand(rows[is_q] + (ti * NU + u) * 2 * kBlock + at), operand(rows[0] + (tj * NU + u) * 2 * kBlock + at), c);
+                c = product(operand(rows + is_q * kRows + (ti * NU + u) * 2 * kBlock + at), operand(rows + (tj * NU + u) * 2 * kBlock + at), c);
             float(*to)[kRow] = is_q ? qk : kk;
 #pragma unroll
             for (int r = 0; r < 4; ++r) to[16 * ti + 4 * (lane / 16) + r][16 * tj + lane % 16] = c[r] * 0x1p-8f;
         }
+        __syncthreads();
         for (int h0 = 0; h0 < of; h0 += 2) {
             const int nh = min(2, of - h0);
             if (wid == 0) {  // a head in half a wave, a token per lane
@@ -449,10 +448,10 @@ __device__ inline float over_groups(float x) {  // sum over the four lanes of a 
     return __uint_as_float(q[0]) + __uint_as_float(q[1]);
 }
 
-// The walk over a sequence's groups. A workgroup has 16 NT columns of the state in each of its NW first waves, all
-// rows, as sums of matrix products; nothing of it leaves the wave's registers from group to group. Four
-// more waves bring the next group's K, Q, T diag(beta) and P into LDS as operands meanwhile.
-template <int DK, int NW, int NT>
+// The walk over a sequence's groups. A workgroup has 16 columns of the state in each of its NW first waves, all rows, as
+// sums of matrix products; nothing of it leaves the wave's registers from group to group. Four more waves bring the
+// next group's K, Q, T diag(beta) and P into LDS as operands meanwhile.
+template <int DK, int NW>
 __global__ __launch_bounds__(512) void delta_walk_kernel(DeltaArgs a, DeltaScratch w, int splits) {
     constexpr int NU = DK / 32, NI = DK / 64;
     constexpr int kK = 0, kQ = kK + 2 * NU * 2 * kBlock, kTurned = kQ + 2 * NU * 2 * kBlock, kM = kTurned + DK / 16 * 2 * kBlock;
@@ -462,7 +461,7 @@ __global__ __launch_bounds__(512) void delta_walk_kernel(DeltaArgs a, DeltaScrat
     // workgroups that read the same keys on one XCD (they go to the eight in turns)
     const int unit = int(blockIdx.x / 8 / unsigned(per)) * 8 + int(blockIdx.x % 8), part = int(blockIdx.x / 8 % unsigned(per));
     if (unit >= a.b.n_seqs * a.qk_heads) return;
-    const int s = unit / a.qk_heads, hk = unit % a.qk_heads, h = hk * of + part / splits, split_no = part % splits;
+    const int s = unit / a.qk_heads, hk = unit % a.qk_heads, h = hk * of + part / splits;
     const StateSeq v = state_seq(a.b, s);
     const int n_groups = (v.n + kChunk - 1) / kChunk;
     const size_t group0 = size_t(first_group(v, s));
@@ -476,33 +475,43 @@ __global__ __launch_bounds__(512) void delta_walk_kernel(DeltaArgs a, DeltaScrat
         struct Held {
             f4 x[NI][4];
             f4 inv[NI];
-            uint4 m0, m1;
+            f4 m0, m1;
             float decay;
         };
         auto load = [&](int n, Held &y) {  // (past the last group: rows of zeros, the last one's matrices)
             const size_t group = group0 + min(n, n_groups - 1);
 #pragma unroll
             for (int j = 0; j < NI; ++j) {
-                const Item<DK> it(i + 256 * j);
+                const Item<DK> it(i, j);
                 it.load(a, hk, v.r0 + n * kChunk, v.n - n * kChunk, y.x[j]);
                 y.inv[j] = *reinterpret_cast<const f4 *>(w.inverse + (group * a.qk_heads + hk) * 64 + it.is_q * 32 + it.token);
             }
-            const uint4 *src = reinterpret_cast<const uint4 *>(w.matrices + (group * a.v_heads + h) * kDeltaMatrices);
+            const f4 *src = reinterpret_cast<const f4 *>(w.matrices + (group * a.v_heads + h) * kDeltaMatrices);
             y.m0 = src[i];
             y.m1 = src[i + 256];
-            if (i < 64) y.decay = w.decays[(group * a.v_heads + h) * 64 + i];
+            y.decay = w.decays[(group * a.v_heads + h) * 64 + lane];
         };
-        auto store = [&](int n, const Held &y) {
+        // One step: group n from the registers to LDS, and group n + 2 on its way to them. The writes come last: LDS is the
+        // walking waves' while they read the first operands of their step.
+        auto pass = [&](int n, Held &y) {
             char *buf = lds + n % 2 * kBuffer;
+            h4 hi[NI][4], lo[NI][4];
+#pragma unroll
+            for (int j = 0; j < NI; ++j) Item<DK>(i, j).convert(y.x[j], y.inv[j], hi[j], lo[j]);
+            const f4 m0 = y.m0, m1 = y.m1;
+            const float decay = y.decay;
+            __builtin_amdgcn_sched_barrier(0);
+            load(n + 2, y);
+            __builtin_amdgcn_sched_barrier(0);
+            char *to = buf + kM + i / 64 * kBlock + i % 64 / 16 * 256 + (i % 16 ^ i % 64 / 16) * 16;
+            *reinterpret_cast<f4 *>(to) = m0;
+            *reinterpret_cast<f4 *>(to + 4 * kBlock) = m1;
+            reinterpret_cast<float *>(buf + kDecays)[lane] = decay;
 #pragma unroll
             for (int j = 0; j < NI; ++j) {
-                const Item<DK> it(i + 256 * j);
-                it.store(buf + (it.is_q ? kQ : kK), it.is_q ? nullptr : buf + kTurned, y.x[j], y.inv[j]);
+                const Item<DK> it(i, j);
+                it.store(buf + (it.is_q ? kQ : kK), it.is_q ? nullptr : buf + kTurned, hi[j], lo[j]);
             }
-            char *to = buf + kM + i / 64 * kBlock + i % 64 / 16 * 256 + (i % 16 ^ i % 64 / 16) * 16;
-            *reinterpret_cast<uint4 *>(to) = y.m0;
-            *reinterpret_cast<uint4 *>(to + 4 * kBlock) = y.m1;
-            if (i < 64) reinterpret_cast<float *>(buf + kDecays)[i] = y.decay;
         };
         if (n_groups == 0) {
             __syncthreads();
@@ -511,31 +520,25 @@ __global__ __launch_bounds__(512) void delta_walk_kernel(DeltaArgs a, DeltaScrat
         Held even, odd;  // two groups are under way, so that a walk's step may be shorter than the memory's latency
         load(0, even);
         load(1, odd);
-        store(0, even);
-        load(2, even);
+        pass(0, even);
         __syncthreads();
-        for (int n = 0; n < n_groups; n += 2) {
-            store(n + 1, odd);
-            load(n + 3, odd);
+        int n = 0;  // (no way out between the two steps: the waits count the loads of one path)
+        for (; n + 1 < n_groups; n += 2) {
+            pass(n + 1, odd);
             __syncthreads();
-            if (n + 1 >= n_groups) break;
-            store(n + 2, even);
-            load(n + 4, even);
+            pass(n + 2, even);
             __syncthreads();
         }
+        if (n < n_groups) __syncthreads();
         return;
     }
 
     __builtin_amdgcn_s_setprio(2);  // before the waves that bring operands
     const int g = lane / 16, lane_at = g * 256 + (lane % 16 ^ g) * 16;
-    const int col = (split_no * NW + wid) * 16 * NT + lane % 16;  // of column tile 0
-    const int DV = a.value_dim;
+    const int col = (part % splits * NW + wid) * 16 + lane % 16, DV = a.value_dim;
     const size_t place = size_t(h) * DK * DV + col, pool = size_t(a.v_heads) * DK * DV;
-    f4 S[2 * NU][NT];
-    f4 val[2][NT], ahead[2][NT];  // values of this group and the next
-    float bound[NT], sum[NT];     // of the column's length; of the values' sizes
-    int scale[NT];             // S is kept times 2^scale
-    float out_scale[NT];
+    const f4 zero = {0.f, 0.f, 0.f, 0.f};
+    f4 S[2 * NU], val[2], ahead[2];     // values of this group and the next
     unsigned v_at[2][4], out_at[2][4];  // bytes from a group's first row to this lane's, of its row tensors
 #pragma unroll
     for (int ti = 0; ti < 2; ++ti)
@@ -544,168 +547,148 @@ __global__ __launch_bounds__(512) void delta_walk_kernel(DeltaArgs a, DeltaScrat
             v_at[ti][r] = (unsigned(16 * ti + 4 * g + r) * unsigned(a.v_stride) + unsigned(col)) * 4u;
             out_at[ti][r] = (unsigned(16 * ti + 4 * g + r) * unsigned(a.out_stride) + unsigned(col)) * 4u;
         }
-    auto load_values = [&](int n, f4 (&to)[2][NT]) {
+    auto load_values = [&](int n, f4 (&to)[2]) {
         const __amdgpu_buffer_rsrc_t rows =
             group_rows(a.v + size_t(v.r0 + n * kChunk) * a.v_stride + size_t(h) * DV, a.v_stride, h * DV, v.n - n * kChunk);
 #pragma unroll
         for (int ti = 0; ti < 2; ++ti)
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-#pragma unroll
-                for (int j = 0; j < NT; ++j) to[ti][j][r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rows, v_at[ti][r] + 64u * j, 0, 0));
+            for (int r = 0; r < 4; ++r) to[ti][r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rows, v_at[ti][r], 0, 0));
     };
-    auto sum_values = [&](int j) {
-        float x = 0.0f;
+    auto sizes = [](const f4 (&x)[2]) {
+        float y = 0.0f;
 #pragma unroll
         for (int ti = 0; ti < 2; ++ti)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) x += fabsf(val[ti][j][r]);
-        return over_groups(x);
+            for (int r = 0; r < 4; ++r) y += fabsf(x[ti][r]);
+        return over_groups(y);
     };
     load_values(0, val);
     load_values(1, ahead);
 #pragma unroll
     for (int k = 0; k < 2 * NU; ++k)
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                S[k][j][r] = v.in >= 0 ? a.state[size_t(v.in) * pool + place + size_t(16 * k + 4 * g + r) * DV + 16 * j] : 0.0f;
+        for (int r = 0; r < 4; ++r) S[k][r] = v.in >= 0 ? a.state[size_t(v.in) * pool + place + size_t(16 * k + 4 * g + r) * DV] : 0.0f;
     if (n_groups == 0) {
         __syncthreads();
         if (v.out >= 0)
 #pragma unroll
             for (int k = 0; k < 2 * NU; ++k)
 #pragma unroll
-                for (int j = 0; j < NT; ++j)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) a.state[size_t(v.out) * pool + place + size_t(16 * k + 4 * g + r) * DV + 16 * j] = S[k][j][r];
+                for (int r = 0; r < 4; ++r) a.state[size_t(v.out) * pool + place + size_t(16 * k + 4 * g + r) * DV] = S[k][r];
         return;
     }
+    float bound = 0.0f, sum = sizes(val);  // of the column's length; of the values' sizes
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-        float x = 0.0f;
+    for (int k = 0; k < 2 * NU; ++k)
 #pragma unroll
-        for (int k = 0; k < 2 * NU; ++k)
+        for (int r = 0; r < 4; ++r) bound += fabsf(S[k][r]);
+    bound = over_groups(bound);
+    int scale = scale_for(bound + sum);  // S is kept times 2^scale
 #pragma unroll
-            for (int r = 0; r < 4; ++r) x += fabsf(S[k][j][r]);
-        bound[j] = over_groups(x);
-        sum[j] = sum_values(j);
-        scale[j] = scale_for(bound[j] + sum[j]);
-#pragma unroll
-        for (int k = 0; k < 2 * NU; ++k) S[k][j] *= two_to(scale[j]);
-    }
+    for (int k = 0; k < 2 * NU; ++k) S[k] *= two_to(scale);
     __syncthreads();
     for (int n = 0; n < n_groups; ++n) {
         const char *buf = lds + n % 2 * kBuffer + lane_at;
         const float *decays = reinterpret_cast<const float *>(lds + n % 2 * kBuffer + kDecays);
-        // Operands are read a step ahead of their products: a wave waits about as long for LDS as eight products take,
-        // and has no other wave beside it to fill the gap.
-        f4 ks[2][NT], qs[2][NT];
+        // A wave has no other beside it to fill its gaps: operands are read ahead of their products, and Q S, for which
+        // nothing waits, runs beside the steps from K S to D.
+        f4 ks[2] = {zero, zero}, qs[2] = {zero, zero}, eg[2], el[2];
+        Pair ops[2][2], b[NU], m[2], p[2];
+        auto read_rows = [&](int at, int u, Pair (&to)[2]) {  // both token tiles
 #pragma unroll
-        for (int ti = 0; ti < 2; ++ti)
-#pragma unroll
-            for (int j = 0; j < NT; ++j) ks[ti][j] = qs[ti][j] = f4{0.f, 0.f, 0.f, 0.f};
-        Pair ops[2][4];  // of two steps: K and Q of both token tiles
-        auto read_step = [&](int u, Pair (&to)[4]) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) to[i] = operand(buf + (i < 2 ? kK : kQ) + (i % 2 * NU + u) * 2 * kBlock);
+            for (int ti = 0; ti < 2; ++ti) to[ti] = operand(buf + at + (ti * NU + u) * 2 * kBlock);
         };
-        read_step(0, ops[0]);
-        Pair b[2][NT];  // S of two steps as right operands: split a step ahead, beside the products
-#pragma unroll
-        for (int j = 0; j < NT; ++j) b[0][j] = split(S[0][j], S[1][j]);
-        Pair m[2], p[2], kt[2][2];
-        f4 eg[2], el[2];
+        read_rows(kK, 0, ops[0]);
+        read_rows(kK, 1, ops[1]);
+        b[0] = split(S[0], S[1]);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
-            if (u + 1 < NU) {
-                read_step(u + 1, ops[(u + 1) % 2]);
-            } else {
+            products(ops[u % 2], b[u], ks);
+            if (u + 1 < NU) b[u + 1] = split(S[2 * u + 2], S[2 * u + 3]);
+            mix<6, 3>();
+            __builtin_amdgcn_sched_barrier(0);
+            if (u + 2 < NU) {
+                read_rows(kK, u + 2, ops[u % 2]);
+            } else if (u + 2 == NU) {
 #pragma unroll
                 for (int ti = 0; ti < 2; ++ti) {
                     m[ti] = operand(buf + kM + ti * 2 * kBlock);
                     eg[ti] = *reinterpret_cast<const f4 *>(decays + 16 * ti + 4 * g);
-                    el[ti] = *reinterpret_cast<const f4 *>(decays + 32 + 16 * ti + 4 * g);
                 }
-            }
-            __builtin_amdgcn_sched_barrier(0);
-            products<NT>(ops[u % 2], b[u % 2], ks, qs);
-            if (u + 1 < NU) {
-#pragma unroll
-                for (int j = 0; j < NT; ++j) b[(u + 1) % 2][j] = split(S[2 * u + 2][j], S[2 * u + 3][j]);
+                read_rows(kQ, 0, ops[u % 2]);
+            } else {
+                read_rows(kQ, 1, ops[u % 2]);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
         const float all = decays[31];
+        f4 x[2];  // V - e^G K S, times 2^(scale - 4)
 #pragma unroll
-        for (int ti = 0; ti < 2; ++ti) p[ti] = operand(buf + kP + ti * 2 * kBlock);
+        for (int ti = 0; ti < 2; ++ti)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[ti][r] = __builtin_fmaf(eg[ti][r] * -0x1p-8f, ks[ti][r], val[ti][r] * two_to(scale - 4));
+        const Pair xb = split(x[0], x[1]);
+        products(ops[0], b[0], qs);
+        mix<6, 6>();
         __builtin_amdgcn_sched_barrier(0);
-        Pair xb[NT];
+        if (NU > 2) read_rows(kQ, 2, ops[0]);
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {  // V - e^G K S, times 2^(scale - 4)
-            f4 x[2];
-#pragma unroll
-            for (int ti = 0; ti < 2; ++ti)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) x[ti][r] = __builtin_fmaf(eg[ti][r] * -0x1p-8f, ks[ti][j][r], val[ti][j][r] * two_to(scale[j] - 4));
-            xb[j] = split(x[0], x[1]);
+        for (int ti = 0; ti < 2; ++ti) {
+            p[ti] = operand(buf + kP + ti * 2 * kBlock);
+            val[ti] = ahead[ti];
         }
-#pragma unroll
-        for (int ti = 0; ti < 2; ++ti)
-#pragma unroll
-            for (int j = 0; j < NT; ++j) val[ti][j] = ahead[ti][j];
         load_values(n + 2, ahead);
-        f4 d[2][NT];  // D times 2^scale
+        __builtin_amdgcn_sched_barrier(0);
+        f4 d[2] = {zero, zero};  // D times 2^scale
+        products(m, xb, d);
+        products(ops[1], b[1], qs);
+        bound = __builtin_fmaf(all, bound, sum);
+        sum = sizes(val);
+        const int next = scale_for(bound + sum);
+        const float turn = two_to(next - scale), out_scale = a.scale * two_to(-(scale + 4));
+        scale = next;
 #pragma unroll
-        for (int ti = 0; ti < 2; ++ti)
-#pragma unroll
-            for (int j = 0; j < NT; ++j) d[ti][j] = product(m[ti], xb[j], f4{0.f, 0.f, 0.f, 0.f});
-        float turn[NT];
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            bound[j] = __builtin_fmaf(all, bound[j], sum[j]);
-            sum[j] = sum_values(j);
-            const int next = scale_for(bound[j] + sum[j]);
-            turn[j] = two_to(next - scale[j]);
-            out_scale[j] = a.scale * two_to(-(scale[j] + 4));
-            scale[j] = next;
-#pragma unroll
-            for (int k = 0; k < 2 * NU; ++k) S[k][j] *= all * turn[j];
-        }
+        for (int k = 0; k < 2 * NU; ++k) S[k] *= all * turn;
+        mix<12, 5>();
+        __builtin_amdgcn_sched_barrier(0);
+        Pair kt[2][2];
         auto read_turned = [&](int k, Pair (&to)[2]) {
             to[0] = operand(buf + kTurned + k * 2 * kBlock);
             to[1] = operand(buf + kTurned + (k + 1) * 2 * kBlock);
         };
+        if (NU > 2) read_rows(kQ, 3, ops[1]);
+#pragma unroll
+        for (int ti = 0; ti < 2; ++ti) el[ti] = *reinterpret_cast<const f4 *>(decays + 32 + 16 * ti + 4 * g);
         read_turned(0, kt[0]);
         __builtin_amdgcn_sched_barrier(0);
-        f4 o[2][NT];
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            const Pair db = split(d[0][j], d[1][j]);
-#pragma unroll
-            for (int ti = 0; ti < 2; ++ti) o[ti][j] = product(p[ti], db, qs[ti][j] * eg[ti]);
-            xb[j] = split(d[0][j] * (el[0] * (turn[j] * 0x1p-4f)), d[1][j] * (el[1] * (turn[j] * 0x1p-4f)));
-        }
+        if constexpr (NU > 2) products(ops[0], b[2], qs);
+        const Pair db = split(d[0] * (el[0] * (turn * 0x1p-4f)), d[1] * (el[1] * (turn * 0x1p-4f))), dp = split(d[0], d[1]);
+        mix<6, 10>();
         __builtin_amdgcn_sched_barrier(0);
+        f4 o[2];
+        if constexpr (NU > 2) products(ops[1], b[3], qs);
 #pragma unroll
         for (int k = 0; k < 2 * NU; k += 2) {
             if (k + 2 < 2 * NU) read_turned(k + 2, kt[k / 2 % 2 ^ 1]);
             __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < NT; ++j) S[k + i][j] = product(kt[k / 2 % 2][i], xb[j], S[k + i][j]);
+            f4 step[2] = {S[k], S[k + 1]};
+            products(kt[k / 2 % 2], db, step);
+            S[k] = step[0];
+            S[k + 1] = step[1];
             if (k == 0) {
+                o[0] = qs[0] * eg[0];
+                o[1] = qs[1] * eg[1];
+            }
+            if (k == (NU > 2 ? 2 : 0)) products(p, dp, o);
+            if (k == 2 * NU - 2) {
                 const __amdgpu_buffer_rsrc_t rows =
                     group_rows(a.out + size_t(v.r0 + n * kChunk) * a.out_stride + size_t(h) * DV, a.out_stride, h * DV, v.n - n * kChunk);
 #pragma unroll
                 for (int ti = 0; ti < 2; ++ti)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-#pragma unroll
-                        for (int j = 0; j < NT; ++j)
-                            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(o[ti][j][r] * out_scale[j]), rows, out_at[ti][r] + 64u * j, 0, 0);
+                    for (int r = 0; r < 4; ++r) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(o[ti][r] * out_scale), rows, out_at[ti][r], 0, 0);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -715,10 +698,7 @@ __global__ __launch_bounds__(512) void delta_walk_kernel(DeltaArgs a, DeltaScrat
 #pragma unroll
         for (int k = 0; k < 2 * NU; ++k)
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    a.state[size_t(v.out) * pool + place + size_t(16 * k + 4 * g + r) * DV + 16 * j] = S[k][j][r] * two_to(-scale[j]);
+            for (int r = 0; r < 4; ++r) a.state[size_t(v.out) * pool + place + size_t(16 * k + 4 * g + r) * DV] = S[k][r] * two_to(-scale);
     }
 }
 
@@ -751,12 +731,11 @@ __global__ __launch_bounds__(256) void delta_norm_kernel(DeltaArgs a, int tiles)
         }
 }
 
-template <int DK, int NW, int NT> hipError_t launch_walk(const DeltaArgs &a, const DeltaScratch &w, hipStream_t s) {
+template <int DK, int NW> hipError_t launch_walk(const DeltaArgs &a, const DeltaScratch &w, hipStream_t s) {
     constexpr int kBuffer = ((2 * 2 * (DK / 32) + DK / 16) * 2 + 8) * kBlock + 256;
-    const int splits = a.value_dim / (16 * NW * NT), per = a.v_heads / a.qk_heads * splits;
+    const int splits = a.value_dim / (16 * NW), per = a.v_heads / a.qk_heads * splits;
     const int units = a.b.n_seqs * a.qk_heads;
-    hipLaunchKernelGGL((delta_walk_kernel<DK, NW, NT>), dim3(unsigned((units + 7) / 8) * 8u * unsigned(per)), dim3(512),
-                       2 * kBuffer, s, a, w, splits);
+    hipLaunchKernelGGL((delta_walk_kernel<DK, NW>), dim3(unsigned((units + 7) / 8) * 8u * unsigned(per)), dim3(512), 2 * kBuffer, s, a, w, splits);
     return hipGetLastError();
 }
 
@@ -767,9 +746,9 @@ template <int DK> hipError_t launch_groups(const DeltaArgs &a, const DeltaScratc
     hipLaunchKernelGGL(delta_prepare_kernel<DK>, dim3(unsigned(a.b.n_seqs) * unsigned(tiles) * unsigned(a.qk_heads)), dim3(256), 0, s, a, w, tiles);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    if (lists < cu_count) e = launch_walk<DK, 2, 1>(a, w, s);
-    else if (a.value_dim == 64) e = launch_walk<DK, 2, 2>(a, w, s);
-    else e = launch_walk<DK, 4, 2>(a, w, s);
+    // Where workgroups of 32 columns find a CU each they are a little faster (a prompt of 8192 and 32 heads: 411 us, with 64
+    // columns 423), else those of 64 (six prompts of 4887 tokens in all: 106 us, with 32 columns 144).
+    e = lists * (a.value_dim / 32) <= cu_count ? launch_walk<DK, 2>(a, w, s) : launch_walk<DK, 4>(a, w, s);
     if (e != hipSuccess || (!a.gamma && !a.z)) return e;
     const dim3 grid(unsigned(lists) * unsigned(tiles));
     if (a.value_dim == 64) hipLaunchKernelGGL(delta_norm_kernel<64>, grid, dim3(256), 0, s, a, tiles);
