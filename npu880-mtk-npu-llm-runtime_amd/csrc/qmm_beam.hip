@@ -24,7 +24,7 @@ namespace qmm {
 namespace {
 
 constexpr int kPerLane = kBeamSlice / 64;
-constexpr float kInf = __builtin_huge_valf();
+constexpr float kInf = __builtin_huge_valf(), kLog2e = 1.4426950408889634f;
 
 __device__ inline uint32_t ordered(float x) {
     const uint32_t u = __float_as_uint(x + 0.0f);  // (-0 counts as 0)
@@ -39,25 +39,24 @@ __device__ inline void wave_sync() {
     __builtin_amdgcn_wave_barrier();
 }
 
+// The largest T of the bits `from` .. `to` - 1 (the lower ones 0, those above as in T) that at least n of the lanes where
+// `on` have at or above.
+__device__ inline uint32_t nth_bits(uint32_t x, bool on, int n, uint32_t T, int from, int to) {
+#pragma unroll 1
+    for (int bit = to - 1; bit >= from; --bit) {
+        const uint32_t c = T | 1u << bit;
+        if (__popcll(__ballot(on && x >= c)) >= n) T = c;
+    }
+    return T;
+}
 // The largest key T with at least `n` of the lanes' keys (all different, or 0 for none) at or above it; 0
 // where there are fewer.
 __device__ inline uint64_t nth_key(uint64_t key, int n) {
     const uint32_t hi = uint32_t(key >> 32), lo = uint32_t(key);
-    uint32_t T = 0;
-#pragma unroll 1
-    for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t c = T | 1u << bit;
-        if (__popcll(__ballot(hi >= c)) >= n) T = c;
-    }
+    const uint32_t T = nth_bits(hi, true, n, 0, 0, 32);
     const int need = n - __popcll(__ballot(hi > T));
     if (__popcll(__ballot(hi == T)) <= need) return uint64_t(T) << 32;
-    uint32_t L = 0;
-#pragma unroll 1
-    for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t c = L | 1u << bit;
-        if (__popcll(__ballot(hi == T && lo >= c)) >= need) L = c;
-    }
-    return uint64_t(T) << 32 | L;
+    return uint64_t(T) << 32 | nth_bits(lo, hi == T, need, 0, 0, 32);
 }
 
 // The n_keep best of `n` different keys in LDS, in order, to `out` (0 where there are fewer): by counting
@@ -120,41 +119,53 @@ __global__ __launch_bounds__(256) void beam_slice_kernel(BeamArgs a, int slices)
             for (int j = 0; j < 4; ++j) v[i + j] = place(i + j) < n ? x[place(i + j)] : -kInf;
         }
     }
-    float m = -kInf;
-    uint64_t best = 0;
+    // First as if all were numbers or -infinity; where one is not, the sum is no number, or infinite.
+    float top, m, sum;
+    auto look = [&] {
+        top = fmaxf(v[0], v[1]);
 #pragma unroll
-    for (int i = 0; i < kPerLane; ++i) {
-        v[i] = allowed(v[i]);
-        m = fmaxf(m, v[i]);
+        for (int i = 2; i < kPerLane; i += 2) top = fmaxf(fmaxf(top, v[i]), v[i + 1]);
+        m = lanes_max<64>(top);
+        const float base = m == -kInf ? 0.0f : m;
+        float s[4] = {};
+#pragma unroll
+        for (int i = 0; i < kPerLane; ++i) s[i % 4] += __builtin_amdgcn_exp2f((v[i] - base) * kLog2e);  // (a rounded base would shift all)
+        sum = lanes_sum<64>((s[0] + s[1]) + (s[2] + s[3]));
+    };
+    look();
+    if (!(sum < kInf)) {
+#pragma unroll
+        for (int i = 0; i < kPerLane; ++i) v[i] = allowed(v[i]);
+        look();
     }
-    {
-        int at = -1;  // the lane's first value that equals its maximum
-#pragma unroll
-        for (int i = kPerLane - 1; i >= 0; --i)
-            if (v[i] == m && place(i) < n) at = place(i);
-        if (at >= 0) best = uint64_t(ordered(m)) << 32 | uint32_t(~uint32_t(first + at));
-    }
-    m = lanes_max<64>(m);
-    float sum = 0.0f;
-    const float base = m == -kInf ? 0.0f : m;
-#pragma unroll
-    for (int i = 0; i < kPerLane; ++i) sum += __builtin_amdgcn_exp2f((v[i] - base) * 1.4426950408889634f);
-    sum = lanes_sum<64>(sum);
     if (lane == 0) {
         float *st = a.stat + (size_t(row) * slices + slice) * 2;
         st[0] = m;
         st[1] = sum;
     }
-    const uint64_t T = nth_key(best, a.n_keep);
-    const uint32_t T_hi = uint32_t(T >> 32);
+    // The n_keep-th of the lanes' largest values, first by its upper half: seldom do more lanes reach that.
+    uint32_t T = nth_bits(ordered(top), true, a.n_keep, 0, 16, 32), T_place = 0;
+    if (__popcll(__ballot(ordered(top) >= T)) > a.n_keep) {
+        T = nth_bits(ordered(top), true, a.n_keep, T, 0, 16);
+        const bool at_T = ordered(top) == T;
+        const int need = a.n_keep - __popcll(__ballot(ordered(top) > T));
+        if (__popcll(__ballot(at_T)) > need) {  // equal values: those of the lanes whose first one comes first
+            uint32_t first_at = 0;
+#pragma unroll
+            for (int i = kPerLane - 1; i >= 0; --i)
+                if (v[i] == top && place(i) < n) first_at = ~uint32_t(first + place(i));
+            T_place = nth_bits(first_at, at_T, need, 0, 0, 32);
+        }
+    }
+    const uint64_t T_key = uint64_t(T) << 32 | T_place;
+    // (the least float that is at or above T; all of them where T is below -infinity)
+    const float T_value = T < ordered(-kInf) ? -kInf : unordered(T);
     int count = 0;
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i) {
-        const uint32_t hi = ordered(v[i]);
-        bool in = hi >= T_hi && place(i) < n;
-        if (__ballot(in) == 0) continue;
-        const uint64_t key = uint64_t(hi) << 32 | uint32_t(~uint32_t(first + place(i)));
-        in = in && key >= T;
+        if (__ballot(v[i] >= T_value) == 0) continue;
+        const uint64_t key = uint64_t(ordered(v[i])) << 32 | uint32_t(~uint32_t(first + place(i)));
+        const bool in = key >= T_key && place(i) < n;
         const uint64_t who = __ballot(in);
         if (in) list[count + __popcll(who & ((uint64_t(1) << lane) - 1))] = key;
         count += __popcll(who);
@@ -171,9 +182,15 @@ constexpr int kJoinCap = 512;  // candidates of one beam in LDS
 __device__ inline void join_lists(const uint64_t *lists, int slices, int full, int n_keep, uint64_t *cand, int *counter, uint64_t *out) {
     const int lane = threadIdx.x & 63;
     uint64_t T = 0;
+    constexpr int kFirst = 4;  // keys of a list that are read at once
+    uint64_t first[2][kFirst];  // of this lane's first two lists
+#pragma unroll
+    for (int l = 0; l < 2; ++l)
+#pragma unroll
+        for (int i = 0; i < kFirst; ++i) first[l][i] = lane + 64 * l < slices && i < n_keep ? lists[size_t(lane + 64 * l) * n_keep + i] : 0;
     if (full >= n_keep) {
-        uint64_t head = 0;  // the best of this lane's lists
-        for (int s = lane; s < slices; s += 64) {
+        uint64_t head = first[0][0] > first[1][0] ? first[0][0] : first[1][0];  // the best of this lane's lists
+        for (int s = lane + 128; s < slices; s += 64) {
             const uint64_t k = lists[size_t(s) * n_keep];
             head = k > head ? k : head;
         }
@@ -185,13 +202,21 @@ __device__ inline void join_lists(const uint64_t *lists, int slices, int full, i
     }
     if (lane == 0) *counter = 0;
     wave_sync();
-    for (int s = lane; s < slices; s += 64)
-        for (int i = 0; i < n_keep; ++i) {
-            const uint64_t k = lists[size_t(s) * n_keep + i];
-            if (k == 0 || k < T) break;
-            const int at = atomicAdd(counter, 1);
-            if (at < kJoinCap) cand[at] = k;
-        }
+    auto take = [&](uint64_t k) {
+        if (k == 0 || k < T) return false;
+        const int at = atomicAdd(counter, 1);
+        if (at < kJoinCap) cand[at] = k;
+        return true;
+    };
+#pragma unroll
+    for (int l = 0; l < 2; ++l) {
+        bool more = true;
+#pragma unroll
+        for (int i = 0; i < kFirst; ++i) more = more && take(first[l][i]);
+        for (int i = kFirst; more && i < n_keep; ++i) more = take(lists[size_t(lane + 64 * l) * n_keep + i]);
+    }
+    for (int s = lane + 128; s < slices; s += 64)
+        for (int i = 0; i < n_keep && take(lists[size_t(s) * n_keep + i]); ++i) {}
     wave_sync();
     const int n = __builtin_amdgcn_readfirstlane(*counter);
     if (n <= kJoinCap) {
@@ -243,7 +268,7 @@ __global__ __launch_bounds__(1024) void beam_item_kernel(BeamArgs a, int slices)
             none = m == -kInf;
             double sum = 0.0;
             for (int s = lane; s < slices; s += 64)
-                if (st[2 * s] > -kInf) sum += double(st[2 * s + 1]) * double(__builtin_amdgcn_exp2f((st[2 * s] - m) * 1.4426950408889634f));
+                if (st[2 * s] > -kInf) sum += double(st[2 * s + 1]) * double(__builtin_amdgcn_exp2f((st[2 * s] - m) * kLog2e));
             for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
             lse = double(m) + log(sum);
         }
