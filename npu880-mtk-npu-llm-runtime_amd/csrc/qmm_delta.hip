@@ -11,7 +11,7 @@
 namespace qmm {
 namespace {
 
-constexpr int kStepRows = 24;  // new rows up to which a token at a time is faster
+constexpr int kStepRows = 8;  // new rows up to which a token at a time is faster than a group of 32
 constexpr int kGroup = 8;  // tokens whose inputs are in LDS at a time
 
 __device__ inline float softplus(float x) { return x > 0.0f ? x + log1pf(expf(-x)) : log1pf(expf(x)); }
@@ -24,6 +24,29 @@ __device__ inline float step_size(const DeltaArgs &a, int row, int h) {
 
 __device__ inline float4 load4(const float *p) { return *reinterpret_cast<const float4 *>(p); }
 __device__ inline float dot4(float4 x, float4 y) { return x.x * y.x + x.y * y.y + (x.z * y.z + x.w * y.w); }
+
+// Rows r0 .. below r0 + n out, half a wave each, with the norm and the gate; get(m, e): four values of row r0 + m
+template <int DV, typename F> __device__ inline void write_rows(const DeltaArgs &a, int h, int r0, int n, int t, int threads, F get) {
+    const int e = 4 * (t % 32);
+    const bool on = e < DV;
+    for (int m = t / 32; m < n; m += threads / 32) {
+        const size_t row = size_t(r0 + m);
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (on) o = get(m, e);
+        if (a.gamma) {
+            const float r = inv_root(lanes_sum<32>(dot4(o, o)) * (1.0f / DV) + a.gamma_eps);
+            if (on) {
+                const float4 w = load4(a.gamma + e);
+                o = make_float4(o.x * r * w.x, o.y * r * w.y, o.z * r * w.z, o.w * r * w.w);
+            }
+        }
+        if (on && a.z) {
+            const float4 z = load4(a.z + row * a.z_stride + size_t(h) * DV + e);
+            o = make_float4(o.x * silu(z.x), o.y * silu(z.y), o.z * silu(z.z), o.w * silu(z.w));
+        }
+        if (on) *reinterpret_cast<float4 *>(a.out + row * a.out_stride + size_t(h) * DV + e) = o;
+    }
+}
 
 // One token after another through the state, for few new rows: a workgroup per
 // sequence and head, a wave 16 * CL / 4 columns (4 a lane) of all rows, in
@@ -131,25 +154,7 @@ __global__ __launch_bounds__(256, 3) void delta_step_kernel(DeltaArgs a) {
             if (rl == 0) *reinterpret_cast<float4 *>(&vo[m][col]) = make_float4(qs[0], qs[1], qs[2], qs[3]);
         }
         __syncthreads();
-        // rows out: half a wave each, with the norm and the gate
-        for (int m = 2 * wid + lane / HL; m < nt; m += 8) {
-            const bool on = 4 * sub < DV;
-            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (on) o = load4(&vo[m][4 * sub]);
-            const size_t row = size_t(v.r0 + t0 + m);
-            if (a.gamma) {
-                const float r = inv_root(lanes_sum<HL>(dot4(o, o)) * (1.0f / DV) + a.gamma_eps);
-                if (on) {
-                    const float4 w = load4(a.gamma + 4 * sub);
-                    o = make_float4(o.x * r * w.x, o.y * r * w.y, o.z * r * w.z, o.w * r * w.w);
-                }
-            }
-            if (on && a.z) {
-                const float4 z = load4(a.z + row * a.z_stride + size_t(h) * DV + 4 * sub);
-                o = make_float4(o.x * silu(z.x), o.y * silu(z.y), o.z * silu(z.z), o.w * silu(z.w));
-            }
-            if (on) *reinterpret_cast<float4 *>(a.out + row * a.out_stride + size_t(h) * DV + 4 * sub) = o;
-        }
+        write_rows<DV>(a, h, v.r0 + t0, nt, t, 256, [&](int m, int e) { return load4(&vo[m][e]); });
         __syncthreads();
     }
     if (v.out >= 0) {
@@ -295,19 +300,110 @@ __device__ inline double shfl_up(double x, int d) {
     return __longlong_as_double((uint64_t(uint32_t(__shfl_up(int(u >> 32), d, 32))) << 32) | uint32_t(__shfl_up(int(u), d, 32)));
 }
 
-// T diag(beta) and P of one group and key head, for its value heads two at a time. The inverse of the unit
-// lower triangle: two 16 x 16 triangles a head by substitution, a column per lane (both heads in one wave), then
-// T21 = -T22 A21 T11 on the matrix units in fp32.
+constexpr int kRow = 36;  // floats of a row of a 32 x 32 matrix in LDS
+typedef float Square[32][kRow];
+// The pieces of T diag(beta) and P of one group.
+// squares of an item's rows, summed over the eight lanes that share them, to sums[kind][token][of 32 values]
+template <int DK> __device__ inline void row_squares(const Item<DK> &it, const f4 x[4], float (*sums)[32][DK / 32]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        float ss = (x[j][0] * x[j][0] + x[j][1] * x[j][1]) + (x[j][2] * x[j][2] + x[j][3] * x[j][3]);
+        ss += lane_moved<0xB1>(ss);
+        ss += lane_moved<0x4E>(ss);
+        ss += lane_moved<0x141>(ss);
+        if (threadIdx.x % 8 == 0) sums[it.is_q][it.token + j][it.at / 32] = ss;
+    }
+}
+template <int DK> __device__ inline float inverse_length(const float (&sums)[DK / 32], float eps) {
+#pragma unroll
+    for (int u = 0; u < DK / 32; ++u) eps += sums[u];
+    return inv_root(eps);
+}
+// sums of the log decays of a head and its step sizes, a token per lane of half a wave
+__device__ inline void head_steps(const DeltaArgs &a, int row, int h, int m, bool on, double *G, float *beta) {
+    double g = on ? double(log_decay(a, row, h)) : 0.0;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+        const double o = shfl_up(g, d);
+        if (m >= d) g += o;
+    }
+    G[m] = g;
+    beta[m] = on ? step_size(a, row, h) : 0.0f;
+}
+// one of the six tiles of k k' (0..2) and q k' (3..5) on and below the diagonal, by a wave
+template <int DK> __device__ inline void tile_of(int task, int lane, const char *k, const char *q, Square &kk, Square &qk) {
+    constexpr int NU = DK / 32;
+    const int is_q = task / 3, ti = task % 3 != 0, tj = task % 3 == 2;
+    const int at = (lane / 16) * 256 + (lane % 16 ^ lane / 16) * 16;
+    f4 c{};
+#pragma unroll
+    for (int u = 0; u < NU; ++u) c = product(operand((is_q ? q : k) + (ti * NU + u) * 2 * kBlock + at), operand(k + (tj * NU + u) * 2 * kBlock + at), c);
+    Square &to = is_q ? qk : kk;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) to[16 * ti + 4 * (lane / 16) + r][16 * tj + lane % 16] = c[r] * 0x1p-8f;
+}
+// four values of a 32 x 32 matrix as operand: `place` is that of row and column (operand_at) in the row's tile
+__device__ inline void store_operand(char *matrix, int i, int place, f4 x) {
+    h4 hi, lo;
+    split4(x, hi, lo);
+    *reinterpret_cast<h4 *>(matrix + i / 16 * 2 * kBlock + place) = hi;
+    *reinterpret_cast<h4 *>(matrix + i / 16 * 2 * kBlock + place + kBlock) = lo;
+}
+// row i, columns c .. c + 3 of A, and of P times 2^4
+__device__ inline f4 mask_and_decay(const Square &kk, const Square &qk, const double *G, const float *beta, int i, int c, Square &A) {
+    f4 p;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float e = c + j <= i ? expf(float(G[i] - G[c + j])) : 0.0f;
+        A[i][c + j] = c + j < i ? beta[i] * e * kk[i][c + j] : 0.0f;
+        p[j] = c + j <= i ? e * qk[i][c + j] * 16.0f : 0.0f;  // (above the diagonal's tiles nothing was written)
+    }
+    return p;
+}
+// The inverse of I + A: its two 16 x 16 triangles by substitution, a column per lane, then T21 = -T22 A21 T11 on the matrix
+// units in fp32.
+__device__ inline void invert_half(const Square &A, int b, int col, Square &T) {
+    float x[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        float y = r == col ? 1.0f : 0.0f;
+#pragma unroll
+        for (int j = 0; j < r; ++j) y = __builtin_fmaf(-A[b + r][b + j], x[j], y);
+        x[r] = y;
+        T[b + r][b + col] = y;
+    }
+}
+__device__ inline void invert_corner(const Square &A, int lane, Square &T) {  // (a wave)
+    const int g = lane / 16, col = lane % 16;
+    f4 y{}, z{};
+#pragma unroll
+    for (int k = 0; k < 16; k += 4) y = __builtin_amdgcn_mfma_f32_16x16x4f32(A[16 + col][k + g], T[k + g][col], y, 0, 0, 0);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) z = __builtin_amdgcn_mfma_f32_16x16x4f32(T[16 + col][16 + 4 * g + r], y[r], z, 0, 0, 0);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) T[16 + 4 * g + r][col] = -z[r];
+}
+// row i, columns c .. c + 3 of T diag(beta), times 2^4
+__device__ inline f4 weighted(const Square &T, const float *beta, int i, int c) {
+    f4 p;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) p[j] = c / 16 <= i / 16 ? T[i][c + j] * beta[c + j] * 16.0f : 0.0f;
+    return p;
+}
+// of 64 decays: e^G_i, then e^(G_last - G_i)
+__device__ inline float decay_of(const double *G, int i) { return expf(float(i < 32 ? G[i] : G[31] - G[i - 32])); }
+
+// T diag(beta) and P of one group and key head, for its value heads two at a time (both inverses in one wave).
 template <int DK>
 __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, DeltaScratch w, int tiles) {
-    constexpr int NU = DK / 32, NI = DK / 64, kRow = 36;
-    constexpr int kRows = 2 * NU * 2 * kBlock, kTriangles = 2 * 2 * 32 * kRow * 4;
+    constexpr int NU = DK / 32, NI = DK / 64;
+    constexpr int kRows = 2 * NU * 2 * kBlock, kTriangles = 4 * sizeof(Square);
     __shared__ __attribute__((aligned(16))) char shared[2 * kRows > kTriangles ? 2 * kRows : kTriangles];
     char *const rows = shared;  // k and q as operands; after their products A and T of two heads
-    auto A = reinterpret_cast<float(*)[32][kRow]>(shared), T = reinterpret_cast<float(*)[32][kRow]>(shared + kTriangles / 2);
+    Square *const A = reinterpret_cast<Square *>(shared), *const T = A + 2;
     __shared__ float sums[2][32][NU];
     __shared__ __attribute__((aligned(16))) float inv[2][32];
-    __shared__ float kk[32][kRow], qk[32][kRow];
+    __shared__ Square kk, qk;
     __shared__ double G[2][32];
     __shared__ float beta[2][32];
     const int t = threadIdx.x, lane = t & 63, wid = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -321,23 +417,10 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, DeltaSc
 #pragma unroll
         for (int i = 0; i < NI; ++i) Item<DK>(t, i).load(a, hk, r0, left, x[i]);
 #pragma unroll
-        for (int i = 0; i < NI; ++i) {
-            const Item<DK> it(t, i);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float ss = (x[i][j][0] * x[i][j][0] + x[i][j][1] * x[i][j][1]) + (x[i][j][2] * x[i][j][2] + x[i][j][3] * x[i][j][3]);  // over the eight lanes that share a token
-                ss += lane_moved<0xB1>(ss);
-                ss += lane_moved<0x4E>(ss);
-                ss += lane_moved<0x141>(ss);
-                if (lane % 8 == 0) sums[it.is_q][it.token + j][it.at / 32] = ss;
-            }
-        }
+        for (int i = 0; i < NI; ++i) row_squares<DK>(Item<DK>(t, i), x[i], sums);
         __syncthreads();
         if (t < 64) {
-            float ss = a.qk_eps;
-#pragma unroll
-            for (int u = 0; u < NU; ++u) ss += sums[t / 32][t % 32][u];
-            const float r = inv_root(ss);
+            const float r = inverse_length<DK>(sums[t / 32][t % 32], a.qk_eps);
             inv[t / 32][t % 32] = r;
             w.inverse[(group * a.qk_heads + hk) * 64 + t] = r;
         }
@@ -350,87 +433,26 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, DeltaSc
             it.store(rows + it.is_q * kRows, nullptr, hi, lo);
         }
         __syncthreads();
-        for (int task = wid; task < 6; task += 4) {  // k k' and q k', the tiles on and below the diagonal
-            const int is_q = task / 3, ti = task % 3 != 0, tj = task % 3 == 2;
-            const int at = (lane / 16) * 256 + (lane % 16 ^ lane / 16) * 16;
-            f4 c{};
-#pragma unroll
-            for (int u = 0; u < NU; ++u)
-                c = product(operand(rows + is_q * kRows + (ti * NU + u) * 2 * kBlock + at), operand(rows + (tj * NU + u) * 2 * kBlock + at), c);
-            float(*to)[kRow] = is_q ? qk : kk;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) to[16 * ti + 4 * (lane / 16) + r][16 * tj + lane % 16] = c[r] * 0x1p-8f;
-        }
+        for (int task = wid; task < 6; task += 4) tile_of<DK>(task, lane, rows, rows + kRows, kk, qk);
         __syncthreads();
         for (int h0 = 0; h0 < of; h0 += 2) {
             const int nh = min(2, of - h0);
-            if (wid == 0) {  // a head in half a wave, a token per lane
-                const int hh = lane / 32, m = lane % 32, h = hk * of + h0 + hh;
-                const bool on = hh < nh && m < left;
-                double g = on ? double(log_decay(a, r0 + m, h)) : 0.0;
-#pragma unroll
-                for (int d = 1; d < 32; d *= 2) {
-                    const double o = shfl_up(g, d);
-                    if (m >= d) g += o;
-                }
-                G[hh][m] = g;
-                beta[hh][m] = on ? step_size(a, r0 + m, h) : 0.0f;
+            const size_t first = group * a.v_heads + hk * of + h0;
+            if (wid == 0) {
+                const int hh = lane / 32, m = lane % 32;
+                head_steps(a, r0 + m, hk * of + h0 + hh, m, hh < nh && m < left, G[hh], beta[hh]);
             }
             __syncthreads();
-            if (t < 64 * nh) {
-                const int hh = t / 64, m = t % 32;
-                w.decays[(group * a.v_heads + hk * of + h0 + hh) * 64 + t % 64] = expf(float(t % 64 < 32 ? G[hh][m] : G[hh][31] - G[hh][m]));
-            }
-            const int i = t / 8, c = t % 8 * 4;  // row i, columns c .. c + 3
-            for (int hh = 0; hh < nh; ++hh) {
-                f4 p;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float e = c + j <= i ? expf(float(G[hh][i] - G[hh][c + j])) : 0.0f;
-                    A[hh][i][c + j] = c + j < i ? beta[hh][i] * e * kk[i][c + j] : 0.0f;
-                    p[j] = c + j <= i ? e * qk[i][c + j] * 16.0f : 0.0f;  // (above the diagonal's tiles nothing was written)
-                }
-                h4 hi, lo;
-                split4(p, hi, lo);
-                char *to = w.matrices + (group * a.v_heads + hk * of + h0 + hh) * kDeltaMatrices + 4096 + i / 16 * 2048 + (c % 16 / 4) * 256 + i % 16 * 16 + c / 16 * 8;
-                *reinterpret_cast<h4 *>(to) = hi;
-                *reinterpret_cast<h4 *>(to + 1024) = lo;
-            }
+            if (t < 64 * nh) w.decays[(first + t / 64) * 64 + t % 64] = decay_of(G[t / 64], t % 64);
+            const int i = t / 8, c = t % 8 * 4, place = (c % 16 / 4) * 256 + i % 16 * 16 + c / 16 * 8;
+            for (int hh = 0; hh < nh; ++hh)
+                store_operand(w.matrices + (first + hh) * kDeltaMatrices + 4 * kBlock, i, place, mask_and_decay(kk, qk, G[hh], beta[hh], i, c, A[hh]));
             __syncthreads();
-            if (wid == 0 && lane / 32 < nh) {
-                const int hh = lane / 32, b = lane / 16 % 2 * 16, col = lane % 16;
-                float x[16];
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    float y = r == col ? 1.0f : 0.0f;
-#pragma unroll
-                    for (int j = 0; j < r; ++j) y = __builtin_fmaf(-A[hh][b + r][b + j], x[j], y);
-                    x[r] = y;
-                    T[hh][b + r][b + col] = y;
-                }
-            }
+            if (wid == 0 && lane / 32 < nh) invert_half(A[lane / 32], lane / 16 % 2 * 16, lane % 16, T[lane / 32]);
             __syncthreads();
-            if (wid < nh) {
-                const int g = lane / 16, col = lane % 16;
-                f4 y{}, z{};
-#pragma unroll
-                for (int k = 0; k < 16; k += 4) y = __builtin_amdgcn_mfma_f32_16x16x4f32(A[wid][16 + col][k + g], T[wid][k + g][col], y, 0, 0, 0);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) z = __builtin_amdgcn_mfma_f32_16x16x4f32(T[wid][16 + col][16 + 4 * g + r], y[r], z, 0, 0, 0);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) T[wid][16 + 4 * g + r][col] = -z[r];
-            }
+            if (wid < nh) invert_corner(A[wid], lane, T[wid]);
             __syncthreads();
-            for (int hh = 0; hh < nh; ++hh) {
-                f4 p;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) p[j] = c / 16 <= i / 16 ? T[hh][i][c + j] * beta[hh][c + j] * 16.0f : 0.0f;
-                h4 hi, lo;
-                split4(p, hi, lo);
-                char *to = w.matrices + (group * a.v_heads + hk * of + h0 + hh) * kDeltaMatrices + i / 16 * 2048 + (c % 16 / 4) * 256 + i % 16 * 16 + c / 16 * 8;
-                *reinterpret_cast<h4 *>(to) = hi;
-                *reinterpret_cast<h4 *>(to + 1024) = lo;
-            }
+            for (int hh = 0; hh < nh; ++hh) store_operand(w.matrices + (first + hh) * kDeltaMatrices, i, place, weighted(T[hh], beta[hh], i, c));
             __syncthreads();
         }
         __syncthreads();
@@ -702,6 +724,165 @@ __global__ __launch_bounds__(512) void delta_walk_kernel(DeltaArgs a, DeltaScrat
     }
 }
 
+// Few groups, drafts mostly: all of the above in one workgroup per sequence and head, that makes a group's matrices itself and
+// has all columns of the state (16 a wave), so that the norm needs no launch of its own.
+template <int DK, int DV>
+__global__ __launch_bounds__(512, 4) void delta_group_kernel(DeltaArgs a) {
+    constexpr int NU = DK / 32, kRows = 2 * NU * 2 * kBlock;
+    __shared__ __attribute__((aligned(16))) char rows[3 * kRows];  // k, its transpose and q as operands
+    __shared__ __attribute__((aligned(16))) char matrices[8 * kBlock];
+    __shared__ __attribute__((aligned(16))) Square squares[4];  // k k', q k', A, T; then the outputs
+    static_assert(sizeof(squares) >= 32 * (DV + 4) * 4);
+    __shared__ float sums[2][32][NU];
+    __shared__ __attribute__((aligned(16))) float inv[2][32], decays[64];
+    __shared__ double G[32];
+    __shared__ float beta[32];
+    const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int s = int(blockIdx.x / unsigned(a.v_heads)), h = int(blockIdx.x % unsigned(a.v_heads));
+    const int hk = h / (a.v_heads / a.qk_heads);
+    const StateSeq v = state_seq(a.b, s);
+    const int col = wid * 16 + threadIdx.x % 16;
+    const bool walks = wid < DV / 16, has_item = DK == 128 || wid < 4;
+    const size_t place = size_t(h) * DK * DV + size_t(4 * (threadIdx.x % 64 / 16)) * DV + col, pool = size_t(a.v_heads) * DK * DV;
+    const f4 zero = {0.f, 0.f, 0.f, 0.f};
+    f4 x[4], S[2 * NU];
+    auto load_rows = [&](int t, int n) {
+        if (has_item) Item<DK>(t % 256, wid / 4).load(a, hk, v.r0 + n * kChunk, v.n - n * kChunk, x);
+    };
+    load_rows(threadIdx.x, 0);
+#pragma unroll
+    for (int k = 0; k < 2 * NU; ++k)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) S[k][r] = walks && v.in >= 0 ? a.state[size_t(v.in) * pool + place + size_t(16 * k + r) * DV] : 0.0f;
+    float bound = 0.0f;
+    int scale = 0;  // S is kept times 2^scale
+    const int n_groups = (v.n + kChunk - 1) / kChunk;
+    for (int n = 0; n < n_groups; ++n) {
+        const int r0 = v.r0 + n * kChunk, left = v.n - n * kChunk;
+        int t = threadIdx.x;
+        asm("" : "+v"(t));  // there is one group mostly: no places in LDS are worked out ahead of the loop, for which registers lack
+        t &= 511;
+        const int lane = t % 64, g = lane / 16, lane_at = g * 256 + (lane % 16 ^ g) * 16;
+        f4 val[2];
+        const __amdgpu_buffer_rsrc_t v_rows = group_rows(a.v + size_t(r0) * a.v_stride + size_t(h) * DV, a.v_stride, h * DV, left);
+#pragma unroll
+        for (int ti = 0; ti < 2; ++ti)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                val[ti][r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(v_rows, (unsigned(16 * ti + 4 * g + r) * unsigned(a.v_stride) + unsigned(walks ? col : 0)) * 4u, 0, 0));
+        const Item<DK> it(t % 256, wid / 4);
+        if (has_item) row_squares<DK>(it, x, sums);
+        if (wid == 7 && lane < 32) head_steps(a, r0 + lane, h, lane, lane < left, G, beta);
+        __syncthreads();
+        if (wid == 0) inv[lane / 32][lane % 32] = inverse_length<DK>(sums[lane / 32][lane % 32], a.qk_eps);
+        if (wid == 7) decays[lane] = decay_of(G, lane);
+        __syncthreads();
+        if (has_item) {
+            h4 hi[4], lo[4];
+            it.convert(x, *reinterpret_cast<const f4 *>(&inv[it.is_q][it.token]), hi, lo);
+            it.store(rows + it.is_q * 2 * kRows, it.is_q ? nullptr : rows + kRows, hi, lo);
+        }
+        __syncthreads();
+        if (n + 1 < n_groups) load_rows(t, n + 1);
+        if (wid < 6) tile_of<DK>(wid, lane, rows, rows + 2 * kRows, squares[0], squares[1]);
+        __syncthreads();
+        const int i = t / 8, c = t % 8 * 4;
+        if (t < 256) store_operand(matrices + 4 * kBlock, i, operand_at(i, c), mask_and_decay(squares[0], squares[1], G, beta, i, c, squares[2]));
+        __syncthreads();
+        if (wid == 7) {  // (the others have products to make meanwhile)
+            if (lane < 32) invert_half(squares[2], lane / 16 * 16, lane % 16, squares[3]);
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();  // lanes read what others of the wave wrote
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+            invert_corner(squares[2], lane, squares[3]);
+        }
+        f4 ks[2] = {zero, zero}, qs[2] = {zero, zero};
+        float sum = 0.0f;
+        if (walks) {
+#pragma unroll
+            for (int ti = 0; ti < 2; ++ti)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) sum += fabsf(val[ti][r]);
+            sum = over_groups(sum);
+            if (n == 0) {
+#pragma unroll
+                for (int k = 0; k < 2 * NU; ++k)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) bound += fabsf(S[k][r]);
+                bound = over_groups(bound);
+            }
+            const int next = scale_for(bound + sum);
+            const float turn = two_to(next - scale);
+            scale = next;
+#pragma unroll
+            for (int u = 0; u < NU; ++u) {
+                S[2 * u] *= turn;
+                S[2 * u + 1] *= turn;
+                const Pair b = split(S[2 * u], S[2 * u + 1]);
+                Pair k[2], q[2];
+#pragma unroll
+                for (int ti = 0; ti < 2; ++ti) {
+                    k[ti] = operand(rows + (ti * NU + u) * 2 * kBlock + lane_at);
+                    q[ti] = operand(rows + 2 * kRows + (ti * NU + u) * 2 * kBlock + lane_at);
+                }
+                products(k, b, ks);
+                products(q, b, qs);
+                __builtin_amdgcn_sched_barrier(0);  // (registers: not all operands ahead)
+            }
+        }
+        __syncthreads();
+        if (t < 256) store_operand(matrices, i, operand_at(i, c), weighted(squares[3], beta, i, c));
+        __syncthreads();
+        float(*const out)[DV + 4] = reinterpret_cast<float(*)[DV + 4]>(squares);
+        if (walks) {
+            f4 eg[2], el[2], y[2], d[2] = {zero, zero};
+            Pair m[2], p[2];
+#pragma unroll
+            for (int ti = 0; ti < 2; ++ti) {
+                eg[ti] = *reinterpret_cast<const f4 *>(decays + 16 * ti + 4 * g);
+                el[ti] = *reinterpret_cast<const f4 *>(decays + 32 + 16 * ti + 4 * g);
+                m[ti] = operand(matrices + ti * 2 * kBlock + lane_at);
+                p[ti] = operand(matrices + (4 + ti * 2) * kBlock + lane_at);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) y[ti][r] = __builtin_fmaf(eg[ti][r] * -0x1p-8f, ks[ti][r], val[ti][r] * two_to(scale - 4));
+            }
+            products(m, split(y[0], y[1]), d);
+            f4 o[2] = {qs[0] * eg[0], qs[1] * eg[1]};
+            products(p, split(d[0], d[1]), o);
+            const float f = a.scale * two_to(-(scale + 4)), all = decays[31];
+#pragma unroll
+            for (int ti = 0; ti < 2; ++ti)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) out[16 * ti + 4 * g + r][col] = o[ti][r] * f;
+            const Pair db = split(d[0] * (el[0] * 0x1p-4f), d[1] * (el[1] * 0x1p-4f));
+            bound = __builtin_fmaf(all, bound, sum);
+#pragma unroll
+            for (int u = 0; u < NU; ++u) {
+                Pair kt[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) kt[j] = operand(rows + kRows + (2 * u + j) * 2 * kBlock + lane_at);
+                f4 step[2] = {S[2 * u] * all, S[2 * u + 1] * all};
+                products(kt, db, step);
+                S[2 * u] = step[0];
+                S[2 * u + 1] = step[1];
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        __syncthreads();
+        write_rows<DV>(a, h, r0, min(left, kChunk), t, 512, [&](int m, int e) { return *reinterpret_cast<const float4 *>(&out[m][e]); });
+        __syncthreads();
+    }
+    if (walks && v.out >= 0) {
+#pragma unroll
+        for (int k = 0; k < 2 * NU; ++k)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float y = S[k][r];
+                a.state[size_t(v.out) * pool + place + size_t(16 * k + r) * DV] = n_groups ? y * two_to(-scale) : y;
+            }
+    }
+}
+
 // The norm and the gate of rows as the walk leaves them, in place: half a wave per row and head
 template <int DV>
 __global__ __launch_bounds__(256) void delta_norm_kernel(DeltaArgs a, int tiles) {
@@ -759,10 +940,17 @@ template <int DK> hipError_t launch_groups(const DeltaArgs &a, const DeltaScratc
 }  // namespace
 
 hipError_t launch_delta(const DeltaArgs &a, void *scratch, size_t scratch_bytes, int cu_count, hipStream_t s) {
-    // (a walk of 2^22 heads would be past 2^32 threads; lanes reach 12 rows in 32 bits of bytes)
+    // A token at a time (T tokens) or one group of 32, of 1, 8 and 32 sequences of 32 heads: T = 4 7.7, 10.8, 28.6 us;
+    // T = 8 10.7, 14.8, 35.5; T = 12 14.9, 19.6, 44; a group 11.4 to 12, 15.2 to 17, 40 to 47.
     const size_t widest = max(max(a.q_stride, a.k_stride), max(a.v_stride, a.out_stride));
-    if (a.max_new > kStepRows && scratch && scratch_bytes >= delta_scratch_bytes(a) && int64_t(a.b.n_seqs) * a.v_heads < (1 << 22) &&
-        widest < (1 << 24)) {
+    const int64_t lists = int64_t(a.b.n_seqs) * a.v_heads;
+    const bool grouped = a.max_new > kStepRows && widest < (1 << 24) && lists < (1 << 20);  // (32 rows in 32 bits of bytes; threads)
+    // All in one launch takes about 4 us and 8.4 for each group of the longest sequence; three launches 17 us and the longer of
+    // 1.9 for each of its groups and 0.029 for each group of any head (one launch has 0.025 of that). Measured, one launch
+    // and three: 1 sequence of 64 tokens 20.2, 20.9, of 128 36.3, 24.2; 8 of 64 26.1, 36.2, of 192 60.1, 66.4; 32 of 192 175, 249.
+    const double steps = double((int64_t(a.max_new) + kChunk - 1) / kChunk);
+    const double all = min(steps * a.b.n_seqs, double(a.b.n_rows / kChunk + a.b.n_seqs)) * a.v_heads;
+    if (grouped && 8.4 * steps > 13 + max(1.9 * steps, 0.029 * all) && scratch && scratch_bytes >= delta_scratch_bytes(a)) {
         const size_t groups = size_t(delta_groups(a.b.n_rows, a.b.n_seqs));
         DeltaScratch w;
         w.matrices = static_cast<char *>(scratch);
@@ -771,7 +959,11 @@ hipError_t launch_delta(const DeltaArgs &a, void *scratch, size_t scratch_bytes,
         return a.key_dim == 128 ? launch_groups<128>(a, w, cu_count, s) : launch_groups<64>(a, w, cu_count, s);
     }
     const dim3 grid(unsigned(a.b.n_seqs) * unsigned(a.v_heads));
-#define QMM_STEP(K, V) hipLaunchKernelGGL((delta_step_kernel<K, V>), grid, dim3(256), 0, s, a)
+#define QMM_STEP(K, V) \
+    do { \
+        if (grouped) hipLaunchKernelGGL((delta_group_kernel<K, V>), grid, dim3(512), 0, s, a); \
+        else hipLaunchKernelGGL((delta_step_kernel<K, V>), grid, dim3(256), 0, s, a); \
+    } while (0)
     if (a.key_dim == 128) {
         if (a.value_dim == 128) QMM_STEP(128, 128);
         else QMM_STEP(128, 64);

@@ -48,8 +48,10 @@ class States:
         return p
 
     def upload(self, ctx, hints=True):
+        """hints: the longest sequence's new rows; False: none; a number: that."""
         self.bufs = [ctx.upload(a) for a in (self.row_start, self.slot_in, self.slot_out)]
-        self.batch = qmm_hip.StateBatch(self.S, self.M, *(int(b) for b in self.bufs), self.n_slots, max([0] + self.news) if hints else 0)
+        self.batch = qmm_hip.StateBatch(self.S, self.M, *(int(b) for b in self.bufs), self.n_slots,
+                                        max([0] + self.news) if hints is True else int(hints))
         return self
 
     def sequences(self):

@@ -170,3 +170,16 @@ def test_delta_many_heads(ctx, DK, DV):
     news = [int(n) for n in rng.integers(0, 70, 33)] + [100]
     delta_case(ctx, news, 3, 3, DK, DV, gap=4, extra=2, seed=DV)
     delta_case(ctx, news, 3, 3, DK, DV, gamma=False, gate=False, slots=[(i, i) for i in range(34)], seed=DK)
+
+
+@pytest.mark.parametrize("DK,DV,of", [(64, 64, 65), (64, 128, 33), (128, 64, 65), (128, 128, 33)])
+def test_delta_long_many_heads(ctx, DK, DV, of):
+    """Heads that fill the compute units, of sequences long enough for three launches, one of them not a multiple of a group."""
+    delta_case(ctx, [201], 2, of, DK, DV, gap=4, extra=2, seed=DV)
+
+
+@pytest.mark.parametrize("ws", [False, True])
+@pytest.mark.parametrize("hint", [1, 9, 40, 1000])
+def test_delta_wrong_hints(ctx, hint, ws):
+    """Sequences longer than the host knew, and shorter: a choice of launch only."""
+    delta_case(ctx, [70, 0, 1, 33, 260], 2, 2, hints=hint, ws=ws, slots=[(0, 0), (1, 1), (2, 2), (3, 4), (5, 5)])
