@@ -170,13 +170,15 @@ __global__ __launch_bounds__(256, 3) void delta_step_kernel(DeltaArgs a) {
 // Of a group of up to 32 tokens, with G_i the sum of its log decays up to token i, k and q its unit rows and
 // S the state before it:
 //   A_ij = beta_i e^(G_i - G_j) k_i.k_j  (j < i),   T = (I + A)^-1,   P_ij = e^(G_i - G_j) q_i.k_j  (j <= i)
-//   D = (T diag(beta)) (V - diag(e^G) K S),   O = diag(e^G) Q S + P D,   S <- e^(G_last) S + K' diag(e^(G_last - G)) D
-// The first kernel makes T diag(beta) and P of every group at once; the second walks a
+//   D = T diag(beta) (V - diag(e^G) K S),   O = diag(e^G) Q S + P D,   S <- e^(G_last) S + K' diag(e^(G_last - G)) D
+// The first kernel makes T and P of every group at once; the second walks a
 // sequence's groups. All products but the inverse run on the matrix units in fp16, each operand as a
-// pair hi + lo of 22 bits (three products: hi hi, hi lo, lo hi), sums in fp32. K, Q, T diag(beta) and P are at
-// most 1 in size and kept 2^4 times as large, so that their low parts are no subnormals; the scale of S, D
-// and V is a power of two for each column, from a bound of the column that holds for the group
-// (|S column| grows by |v| at most, as a step makes no column longer).
+// pair hi + lo of 22 bits (three products: hi hi, hi lo, lo hi), sums in fp32. A low part is a multiple of 2^-24, so
+// operands are kept large: K, at most 1 in size and of length 1, 2^4 times; Q, T and P, at most 1 in size, 2^14
+// times (their small values meet large ones of D where decays are strong); the scale of a column of S, D
+// and V is a power of two, from a bound of the column that holds for the group (|S column| grows by |v| at most, as a
+// step makes no column longer). What is left of a value is good to 2^-22, or 2^-39 of that bound. beta is no part of T:
+// small ones would lose bits there.
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
@@ -240,8 +242,8 @@ template <int N, int K> __device__ inline void mix() {
 }
 
 struct DeltaScratch {
-    char *matrices;  // [groups][v_heads]: T diag(beta), then P: two tiles of 16 rows, each 1 KB hi and 1 KB lo
-    float *decays;   // [groups][v_heads][64]: e^G_i, e^(G_last - G_i)
+    char *matrices;  // [groups][v_heads]: T, then P: two tiles of 16 rows, each 1 KB hi and 1 KB lo
+    float *factors;  // [groups][v_heads][96]: e^G_i, e^(G_last - G_i), beta_i
     float *inverse;  // [groups][qk_heads][64]: 1 / |k_i|, 1 / |q_i|
 };
 __device__ inline int64_t first_group(const StateSeq &v, int s) { return v.r0 / kChunk + s; }
@@ -272,11 +274,11 @@ template <int DK> struct Item {
         for (int j = 0; j < 4; ++j)
             x[j] = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(rows, (unsigned(token + j) * unsigned(stride) + unsigned(at)) * 4u, 0, 0));
     }
-    // times 2^4 / length as left operand, rows the tokens (tiles of 16, each DK / 32 blocks of hi and lo) and, where
+    // times 2^4 (k) or 2^14 (q) / length as left operand, rows the tokens (tiles of 16, each DK / 32 blocks of hi and lo) and, where
     // `turned`, rows the values (tiles of 16, each one block)
     __device__ void convert(const f4 x[4], f4 inv, h4 hi[4], h4 lo[4]) const {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) split4(x[j], inv[j] * 16.0f, hi[j], lo[j]);
+        for (int j = 0; j < 4; ++j) split4(x[j], inv[j] * (is_q ? 0x1p14f : 0x1p4f), hi[j], lo[j]);
     }
     __device__ void store(char *base, char *turned, const h4 hi[4], const h4 lo[4]) const {
         char *p = base + ((token / 16) * (DK / 32) + at / 32) * 2 * kBlock;
@@ -302,7 +304,7 @@ __device__ inline double shfl_up(double x, int d) {
 
 constexpr int kRow = 36;  // floats of a row of a 32 x 32 matrix in LDS
 typedef float Square[32][kRow];
-// The pieces of T diag(beta) and P of one group.
+// The pieces of T and P of one group.
 // squares of an item's rows, summed over the eight lanes that share them, to sums[kind][token][of 32 values]
 template <int DK> __device__ inline void row_squares(const Item<DK> &it, const f4 x[4], float (*sums)[32][DK / 32]) {
 #pragma unroll
@@ -340,7 +342,7 @@ template <int DK> __device__ inline void tile_of(int task, int lane, const char 
     for (int u = 0; u < NU; ++u) c = product(operand((is_q ? q : k) + (ti * NU + u) * 2 * kBlock + at), operand(k + (tj * NU + u) * 2 * kBlock + at), c);
     Square &to = is_q ? qk : kk;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) to[16 * ti + 4 * (lane / 16) + r][16 * tj + lane % 16] = c[r] * 0x1p-8f;
+    for (int r = 0; r < 4; ++r) to[16 * ti + 4 * (lane / 16) + r][16 * tj + lane % 16] = c[r] * (is_q ? 0x1p-18f : 0x1p-8f);
 }
 // four values of a 32 x 32 matrix as operand: `place` is that of row and column (operand_at) in the row's tile
 __device__ inline void store_operand(char *matrix, int i, int place, f4 x) {
@@ -349,14 +351,14 @@ __device__ inline void store_operand(char *matrix, int i, int place, f4 x) {
     *reinterpret_cast<h4 *>(matrix + i / 16 * 2 * kBlock + place) = hi;
     *reinterpret_cast<h4 *>(matrix + i / 16 * 2 * kBlock + place + kBlock) = lo;
 }
-// row i, columns c .. c + 3 of A, and of P times 2^4
+// row i, columns c .. c + 3 of A, and of P times 2^14
 __device__ inline f4 mask_and_decay(const Square &kk, const Square &qk, const double *G, const float *beta, int i, int c, Square &A) {
     f4 p;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const float e = c + j <= i ? expf(float(G[i] - G[c + j])) : 0.0f;
         A[i][c + j] = c + j < i ? beta[i] * e * kk[i][c + j] : 0.0f;
-        p[j] = c + j <= i ? e * qk[i][c + j] * 16.0f : 0.0f;  // (above the diagonal's tiles nothing was written)
+        p[j] = c + j <= i ? e * qk[i][c + j] * 0x1p14f : 0.0f;  // (above the diagonal's tiles nothing was written)
     }
     return p;
 }
@@ -383,17 +385,19 @@ __device__ inline void invert_corner(const Square &A, int lane, Square &T) {  //
 #pragma unroll
     for (int r = 0; r < 4; ++r) T[16 + 4 * g + r][col] = -z[r];
 }
-// row i, columns c .. c + 3 of T diag(beta), times 2^4
-__device__ inline f4 weighted(const Square &T, const float *beta, int i, int c) {
+// row i, columns c .. c + 3 of T, times 2^14
+__device__ inline f4 enlarged(const Square &T, int i, int c) {
     f4 p;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) p[j] = c / 16 <= i / 16 ? T[i][c + j] * beta[c + j] * 16.0f : 0.0f;
+    for (int j = 0; j < 4; ++j) p[j] = c / 16 <= i / 16 ? T[i][c + j] * 0x1p14f : 0.0f;
     return p;
 }
-// of 64 decays: e^G_i, then e^(G_last - G_i)
-__device__ inline float decay_of(const double *G, int i) { return expf(float(i < 32 ? G[i] : G[31] - G[i - 32])); }
+// of 96 factors: e^G_i, then e^(G_last - G_i), then beta_i
+__device__ inline float factor_of(const double *G, const float *beta, int i) {
+    return i < 64 ? expf(float(i < 32 ? G[i] : G[31] - G[i - 32])) : beta[i - 64];
+}
 
-// T diag(beta) and P of one group and key head, for its value heads two at a time (both inverses in one wave).
+// T and P of one group and key head, for its value heads two at a time (both inverses in one wave).
 template <int DK>
 __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, DeltaScratch w, int tiles) {
     constexpr int NU = DK / 32, NI = DK / 64;
@@ -443,7 +447,7 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, DeltaSc
                 head_steps(a, r0 + m, hk * of + h0 + hh, m, hh < nh && m < left, G[hh], beta[hh]);
             }
             __syncthreads();
-            if (t < 64 * nh) w.decays[(first + t / 64) * 64 + t % 64] = decay_of(G[t / 64], t % 64);
+            if (t < kFactors * nh) w.factors[first * kFactors + t] = factor_of(G[t / kFactors], beta[t / kFactors], t % kFactors);
             const int i = t / 8, c = t % 8 * 4, place = (c % 16 / 4) * 256 + i % 16 * 16 + c / 16 * 8;
             for (int hh = 0; hh < nh; ++hh)
                 store_operand(w.matrices + (first + hh) * kDeltaMatrices + 4 * kBlock, i, place, mask_and_decay(kk, qk, G[hh], beta[hh], i, c, A[hh]));
@@ -452,7 +456,7 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, DeltaSc
             __syncthreads();
             if (wid < nh) invert_corner(A[wid], lane, T[wid]);
             __syncthreads();
-            for (int hh = 0; hh < nh; ++hh) store_operand(w.matrices + (first + hh) * kDeltaMatrices, i, place, weighted(T[hh], beta[hh], i, c));
+            for (int hh = 0; hh < nh; ++hh) store_operand(w.matrices + (first + hh) * kDeltaMatrices, i, place, enlarged(T[hh], i, c));
             __syncthreads();
         }
         __syncthreads();
@@ -472,12 +476,12 @@ __device__ inline float over_groups(float x) {  // sum over the four lanes of a 
 
 // The walk over a sequence's groups. A workgroup has 16 columns of the state in each of its NW first waves, all rows, as
 // sums of matrix products; nothing of it leaves the wave's registers from group to group. Four more waves bring the
-// next group's K, Q, T diag(beta) and P into LDS as operands meanwhile.
+// next group's K, Q, T and P into LDS as operands meanwhile.
 template <int DK, int NW>
 __global__ __launch_bounds__(512) void delta_walk_kernel(DeltaArgs a, DeltaScratch w, int splits) {
     constexpr int NU = DK / 32, NI = DK / 64;
     constexpr int kK = 0, kQ = kK + 2 * NU * 2 * kBlock, kTurned = kQ + 2 * NU * 2 * kBlock, kM = kTurned + DK / 16 * 2 * kBlock;
-    constexpr int kP = kM + 4 * kBlock, kDecays = kP + 4 * kBlock, kBuffer = kDecays + 256;
+    constexpr int kP = kM + 4 * kBlock, kFactor = kP + 4 * kBlock, kBuffer = kFactor + kFactors * 4;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int of = a.v_heads / a.qk_heads, per = of * splits;
     // workgroups that read the same keys on one XCD (they go to the eight in turns)
@@ -498,7 +502,7 @@ __global__ __launch_bounds__(512) void delta_walk_kernel(DeltaArgs a, DeltaScrat
             f4 x[NI][4];
             f4 inv[NI];
             f4 m0, m1;
-            float decay;
+            float factor;
         };
         auto load = [&](int n, Held &y) {  // (past the last group: rows of zeros, the last one's matrices)
             const size_t group = group0 + min(n, n_groups - 1);
@@ -511,7 +515,7 @@ __global__ __launch_bounds__(512) void delta_walk_kernel(DeltaArgs a, DeltaScrat
             const f4 *src = reinterpret_cast<const f4 *>(w.matrices + (group * a.v_heads + h) * kDeltaMatrices);
             y.m0 = src[i];
             y.m1 = src[i + 256];
-            y.decay = w.decays[(group * a.v_heads + h) * 64 + lane];
+            y.factor = w.factors[(group * a.v_heads + h) * kFactors + i % kFactors];
         };
         // One step: group n from the registers to LDS, and group n + 2 on its way to them. The writes come last: LDS is the
         // walking waves' while they read the first operands of their step.
@@ -521,14 +525,14 @@ __global__ __launch_bounds__(512) void delta_walk_kernel(DeltaArgs a, DeltaScrat
 #pragma unroll
             for (int j = 0; j < NI; ++j) Item<DK>(i, j).convert(y.x[j], y.inv[j], hi[j], lo[j]);
             const f4 m0 = y.m0, m1 = y.m1;
-            const float decay = y.decay;
+            const float factor = y.factor;
             __builtin_amdgcn_sched_barrier(0);
             load(n + 2, y);
             __builtin_amdgcn_sched_barrier(0);
             char *to = buf + kM + i / 64 * kBlock + i % 64 / 16 * 256 + (i % 16 ^ i % 64 / 16) * 16;
             *reinterpret_cast<f4 *>(to) = m0;
             *reinterpret_cast<f4 *>(to + 4 * kBlock) = m1;
-            reinterpret_cast<float *>(buf + kDecays)[lane] = decay;
+            reinterpret_cast<float *>(buf + kFactor)[i % kFactors] = factor;
 #pragma unroll
             for (int j = 0; j < NI; ++j) {
                 const Item<DK> it(i, j);
@@ -612,10 +616,10 @@ __global__ __launch_bounds__(512) void delta_walk_kernel(DeltaArgs a, DeltaScrat
     __syncthreads();
     for (int n = 0; n < n_groups; ++n) {
         const char *buf = lds + n % 2 * kBuffer + lane_at;
-        const float *decays = reinterpret_cast<const float *>(lds + n % 2 * kBuffer + kDecays);
+        const float *factors = reinterpret_cast<const float *>(lds + n % 2 * kBuffer + kFactor);
         // A wave has no other beside it to fill its gaps: operands are read ahead of their products, and Q S, for which
         // nothing waits, runs beside the steps from K S to D.
-        f4 ks[2] = {zero, zero}, qs[2] = {zero, zero}, eg[2], el[2];
+        f4 ks[2] = {zero, zero}, qs[2] = {zero, zero}, eg[2], el[2], beta[2];
         Pair ops[2][2], b[NU], m[2], p[2];
         auto read_rows = [&](int at, int u, Pair (&to)[2]) {  // both token tiles
 #pragma unroll
@@ -637,7 +641,8 @@ __global__ __launch_bounds__(512) void delta_walk_kernel(DeltaArgs a, DeltaScrat
 #pragma unroll
                 for (int ti = 0; ti < 2; ++ti) {
                     m[ti] = operand(buf + kM + ti * 2 * kBlock);
-                    eg[ti] = *reinterpret_cast<const f4 *>(decays + 16 * ti + 4 * g);
+                    eg[ti] = *reinterpret_cast<const f4 *>(factors + 16 * ti + 4 * g);
+                    beta[ti] = *reinterpret_cast<const f4 *>(factors + 64 + 16 * ti + 4 * g);
                 }
                 read_rows(kQ, 0, ops[u % 2]);
             } else {
@@ -645,12 +650,12 @@ __global__ __launch_bounds__(512) void delta_walk_kernel(DeltaArgs a, DeltaScrat
             }
             __builtin_amdgcn_sched_barrier(0);
         }
-        const float all = decays[31];
-        f4 x[2];  // V - e^G K S, times 2^(scale - 4)
+        const float all = factors[31];
+        f4 x[2];  // diag(beta) (V - diag(e^G) K S), times 2^scale
 #pragma unroll
         for (int ti = 0; ti < 2; ++ti)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) x[ti][r] = __builtin_fmaf(eg[ti][r] * -0x1p-8f, ks[ti][r], val[ti][r] * two_to(scale - 4));
+            for (int r = 0; r < 4; ++r) x[ti][r] = beta[ti][r] * __builtin_fmaf(eg[ti][r] * -0x1p-4f, ks[ti][r], val[ti][r] * two_to(scale));
         const Pair xb = split(x[0], x[1]);
         products(ops[0], b[0], qs);
         mix<6, 6>();
@@ -663,13 +668,13 @@ __global__ __launch_bounds__(512) void delta_walk_kernel(DeltaArgs a, DeltaScrat
         }
         load_values(n + 2, ahead);
         __builtin_amdgcn_sched_barrier(0);
-        f4 d[2] = {zero, zero};  // D times 2^scale
+        f4 d[2] = {zero, zero};  // D times 2^(scale + 14)
         products(m, xb, d);
         products(ops[1], b[1], qs);
         bound = __builtin_fmaf(all, bound, sum);
         sum = sizes(val);
         const int next = scale_for(bound + sum);
-        const float turn = two_to(next - scale), out_scale = a.scale * two_to(-(scale + 4));
+        const float turn = two_to(next - scale), out_scale = a.scale * two_to(-(scale + 14));
         scale = next;
 #pragma unroll
         for (int k = 0; k < 2 * NU; ++k) S[k] *= all * turn;
@@ -682,11 +687,12 @@ __global__ __launch_bounds__(512) void delta_walk_kernel(DeltaArgs a, DeltaScrat
         };
         if (NU > 2) read_rows(kQ, 3, ops[1]);
 #pragma unroll
-        for (int ti = 0; ti < 2; ++ti) el[ti] = *reinterpret_cast<const f4 *>(decays + 32 + 16 * ti + 4 * g);
+        for (int ti = 0; ti < 2; ++ti) el[ti] = *reinterpret_cast<const f4 *>(factors + 32 + 16 * ti + 4 * g);
         read_turned(0, kt[0]);
         __builtin_amdgcn_sched_barrier(0);
         if constexpr (NU > 2) products(ops[0], b[2], qs);
-        const Pair db = split(d[0] * (el[0] * (turn * 0x1p-4f)), d[1] * (el[1] * (turn * 0x1p-4f))), dp = split(d[0], d[1]);
+        const Pair db = split(d[0] * (el[0] * (turn * 0x1p-18f)), d[1] * (el[1] * (turn * 0x1p-18f)));
+        const Pair dp = split(d[0] * 0x1p-14f, d[1] * 0x1p-14f);
         mix<6, 10>();
         __builtin_amdgcn_sched_barrier(0);
         f4 o[2];
@@ -734,7 +740,7 @@ __global__ __launch_bounds__(512, 4) void delta_group_kernel(DeltaArgs a) {
     __shared__ __attribute__((aligned(16))) Square squares[4];  // k k', q k', A, T; then the outputs
     static_assert(sizeof(squares) >= 32 * (DV + 4) * 4);
     __shared__ float sums[2][32][NU];
-    __shared__ __attribute__((aligned(16))) float inv[2][32], decays[64];
+    __shared__ __attribute__((aligned(16))) float inv[2][32], factors[kFactors];
     __shared__ double G[32];
     __shared__ float beta[32];
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -775,7 +781,7 @@ __global__ __launch_bounds__(512, 4) void delta_group_kernel(DeltaArgs a) {
         if (wid == 7 && lane < 32) head_steps(a, r0 + lane, h, lane, lane < left, G, beta);
         __syncthreads();
         if (wid == 0) inv[lane / 32][lane % 32] = inverse_length<DK>(sums[lane / 32][lane % 32], a.qk_eps);
-        if (wid == 7) decays[lane] = decay_of(G, lane);
+        if (t >= 512 - kFactors) factors[t - (512 - kFactors)] = factor_of(G, beta, t - (512 - kFactors));
         __syncthreads();
         if (has_item) {
             h4 hi[4], lo[4];
@@ -831,7 +837,7 @@ __global__ __launch_bounds__(512, 4) void delta_group_kernel(DeltaArgs a) {
             }
         }
         __syncthreads();
-        if (t < 256) store_operand(matrices, i, operand_at(i, c), weighted(squares[3], beta, i, c));
+        if (t < 256) store_operand(matrices, i, operand_at(i, c), enlarged(squares[3], i, c));
         __syncthreads();
         float(*const out)[DV + 4] = reinterpret_cast<float(*)[DV + 4]>(squares);
         if (walks) {
@@ -839,22 +845,23 @@ __global__ __launch_bounds__(512, 4) void delta_group_kernel(DeltaArgs a) {
             Pair m[2], p[2];
 #pragma unroll
             for (int ti = 0; ti < 2; ++ti) {
-                eg[ti] = *reinterpret_cast<const f4 *>(decays + 16 * ti + 4 * g);
-                el[ti] = *reinterpret_cast<const f4 *>(decays + 32 + 16 * ti + 4 * g);
+                eg[ti] = *reinterpret_cast<const f4 *>(factors + 16 * ti + 4 * g);
+                el[ti] = *reinterpret_cast<const f4 *>(factors + 32 + 16 * ti + 4 * g);
+                const f4 bt = *reinterpret_cast<const f4 *>(factors + 64 + 16 * ti + 4 * g);
                 m[ti] = operand(matrices + ti * 2 * kBlock + lane_at);
                 p[ti] = operand(matrices + (4 + ti * 2) * kBlock + lane_at);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) y[ti][r] = __builtin_fmaf(eg[ti][r] * -0x1p-8f, ks[ti][r], val[ti][r] * two_to(scale - 4));
+                for (int r = 0; r < 4; ++r) y[ti][r] = bt[r] * __builtin_fmaf(eg[ti][r] * -0x1p-4f, ks[ti][r], val[ti][r] * two_to(scale));
             }
             products(m, split(y[0], y[1]), d);
             f4 o[2] = {qs[0] * eg[0], qs[1] * eg[1]};
-            products(p, split(d[0], d[1]), o);
-            const float f = a.scale * two_to(-(scale + 4)), all = decays[31];
+            products(p, split(d[0] * 0x1p-14f, d[1] * 0x1p-14f), o);
+            const float f = a.scale * two_to(-(scale + 14)), all = factors[31];
 #pragma unroll
             for (int ti = 0; ti < 2; ++ti)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) out[16 * ti + 4 * g + r][col] = o[ti][r] * f;
-            const Pair db = split(d[0] * (el[0] * 0x1p-4f), d[1] * (el[1] * 0x1p-4f));
+            const Pair db = split(d[0] * (el[0] * 0x1p-18f), d[1] * (el[1] * 0x1p-18f));
             bound = __builtin_fmaf(all, bound, sum);
 #pragma unroll
             for (int u = 0; u < NU; ++u) {
@@ -913,7 +920,7 @@ __global__ __launch_bounds__(256) void delta_norm_kernel(DeltaArgs a, int tiles)
 }
 
 template <int DK, int NW> hipError_t launch_walk(const DeltaArgs &a, const DeltaScratch &w, hipStream_t s) {
-    constexpr int kBuffer = ((2 * 2 * (DK / 32) + DK / 16) * 2 + 8) * kBlock + 256;
+    constexpr int kBuffer = ((2 * 2 * (DK / 32) + DK / 16) * 2 + 8) * kBlock + kFactors * 4;
     const int splits = a.value_dim / (16 * NW), per = a.v_heads / a.qk_heads * splits;
     const int units = a.b.n_seqs * a.qk_heads;
     hipLaunchKernelGGL((delta_walk_kernel<DK, NW>), dim3(unsigned((units + 7) / 8) * 8u * unsigned(per)), dim3(512), 2 * kBuffer, s, a, w, splits);
@@ -954,8 +961,8 @@ hipError_t launch_delta(const DeltaArgs &a, void *scratch, size_t scratch_bytes,
         const size_t groups = size_t(delta_groups(a.b.n_rows, a.b.n_seqs));
         DeltaScratch w;
         w.matrices = static_cast<char *>(scratch);
-        w.decays = reinterpret_cast<float *>(w.matrices + groups * a.v_heads * kDeltaMatrices);
-        w.inverse = w.decays + groups * a.v_heads * 64;
+        w.factors = reinterpret_cast<float *>(w.matrices + groups * a.v_heads * kDeltaMatrices);
+        w.inverse = w.factors + groups * a.v_heads * kFactors;
         return a.key_dim == 128 ? launch_groups<128>(a, w, cu_count, s) : launch_groups<64>(a, w, cu_count, s);
     }
     const dim3 grid(unsigned(a.b.n_seqs) * unsigned(a.v_heads));

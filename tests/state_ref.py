@@ -90,7 +90,15 @@ def delta(b, q, k, v, a, bt, rate, dt, scale, eps, pool, z=None, gamma=None, gam
     adds |v| at most, so the errors of the steps add up, each shrunk by the decays after it. One step's error in a
     column is at most C 2^-24 (|S column| + |v|): sums of DK products (DK), unit vectors (DK / 4 of a sum
     of squares, a root, two products), a decay exp(g) that is (|g| + 8) 2^-24 off, operands of 22 bits (16
-    in units of 2^-24), and a few products; C = 1.5 DK + 64 + |g|. An output adds one more such sum."""
+    in units of 2^-24), and a few products; C = 1.5 DK + 64 + |g|. An output adds one more such sum.
+
+    Operands of groups of 32 tokens have a smallest step, too. A column is scaled so that b, what its state's values and the
+    group's sum to in size, is 2^14 or more, and the low part of a pair is a multiple of 2^-24: at most 2^-39 b off; matrices
+    of values up to 1 are at most 2^-39 off. For a token, 2^-39 b of its value, sqrt(DK) 2^-39 b of k.S and
+    2^-39 (the sum of 32 values, each at most b) of T's row are another value for the rule, whose effect does not grow;
+    the state's own update takes factors 2^4 smaller, 2^-35 b. Together less than 2^-33 b a token. An output adds sqrt(DK) 2^-39 b of q.S,
+    and P's row like T's and the 32 values that it meets: less than 2^-32 b. (Columns below 2^-46 count as that.) It
+    shows only in values that are 2^-16 times smaller than others of their column and group."""
     M, HV, DV = v.shape
     DK = q.shape[2]
     out, tol = np.zeros((M, HV, DV)), np.zeros((M, HV, DV))
@@ -98,8 +106,11 @@ def delta(b, q, k, v, a, bt, rate, dt, scale, eps, pool, z=None, gamma=None, gam
     unit = lambda x: x / np.sqrt((x * x).sum(-1, keepdims=True) + eps)  # noqa: E731
     for _, r0, n, i, o in b.sequences():
         S = pool[i].astype(np.float64) if i >= 0 else np.zeros((HV, DK, DV))
-        err = np.zeros((HV, DV))
+        err, held = np.zeros((HV, DV)), np.abs(S).sum(1)
         for r in range(r0, r0 + n):
+            if (r - r0) % 32 == 0:
+                group = np.abs(v[r:min(r + 32, r0 + n)].astype(np.float64)).sum(0)
+                held = np.maximum(held + group, 2.0 ** -46)  # (more than b: without decays)
             kk, qq = (np.repeat(unit(x[r].astype(np.float64)), of, 0) for x in (k, q))
             x = a[r].astype(np.float64) + dt
             g = np.minimum(rate.astype(np.float64) * (np.maximum(x, 0) + np.log1p(np.exp(-np.abs(x)))), 0)
@@ -109,9 +120,9 @@ def delta(b, q, k, v, a, bt, rate, dt, scale, eps, pool, z=None, gamma=None, gam
             S = S * decay[:, None, None]
             d = beta[:, None] * (v[r] - np.einsum("hkv,hk->hv", S, kk))
             S = S + kk[:, :, None] * d[:, None, :]
-            err = err * decay[:, None] + C * size
+            err = err * decay[:, None] + C * size + 2.0 ** -33 * held
             y = np.einsum("hkv,hk->hv", S, qq) * scale
-            e = scale * (err + C * np.linalg.norm(S, axis=1))
+            e = scale * (err + C * np.linalg.norm(S, axis=1) + 2.0 ** -32 * held)
             if gamma is not None:
                 rms = np.sqrt((y * y).mean(1, keepdims=True) + gamma_eps)
                 e = (e + np.abs(y) * np.sqrt((e * e).mean(1, keepdims=True)) / rms) / rms * np.abs(gamma)
