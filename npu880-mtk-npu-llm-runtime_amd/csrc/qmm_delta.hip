@@ -54,7 +54,7 @@ template <int DV, typename F> __device__ inline void write_rows(const DeltaArgs 
 // before it changes: S' q after the step is e^g S' q + (k.q) d, so one pass and one
 // sum over the lanes serve both, and no wave waits for another between tokens.
 template <int DK, int DV>
-__global__ __launch_bounds__(256, 3) void delta_step_kernel(DeltaArgs a) {
+__global__ __launch_bounds__(256, 4) void delta_step_kernel(DeltaArgs a) {
     constexpr int CL = DV / 16, RL = 64 / CL, NG = DK / (4 * RL), NV = (kGroup * DV + 1023) / 1024, HL = 32;  // HL: lanes that hold one row of q or k
     __shared__ float qk[kGroup][2][DK];
     __shared__ float vo[kGroup][DV];  // values, then outputs
@@ -65,13 +65,20 @@ __global__ __launch_bounds__(256, 3) void delta_step_kernel(DeltaArgs a) {
     const StateSeq v = state_seq(a.b, s);
     const int cl = lane % CL, rl = lane / CL, col = wid * (DV / 4) + 4 * cl;
     const int sub = lane % HL, is_k = lane / HL;
-    const float *src = (is_k ? a.k : a.q) + size_t(hk) * DK + 4 * sub;
-    const size_t src_stride = is_k ? a.k_stride : a.q_stride;
-    const size_t place = size_t(h) * DK * DV + col;
     const size_t pool = size_t(a.v_heads) * DK * DV;
+    // Four workgroups of a CU: places are worked out again for every use, and k is read from LDS twice (kept over the tokens they take
+    // the registers of the fourth; 64 sequences of a token 57 us with three, 51 with four).
+    auto now = [](int x) {
+        asm("" : "+v"(x));
+        return x;
+    };
+    auto state = [&](int slot, int at) { return a.state + size_t(slot) * pool + size_t(h) * DK * DV + size_t(4 * (at / CL)) * DV + wid * (DV / 4) + 4 * (at % CL); };
 
     float4 x[kGroup / 4], val[NV];
-    auto load = [&](int t0) {
+    auto load = [&](int t0, int t) {
+        const int sub = t % HL, is_k = t / HL % 2;
+        const float *src = (is_k ? a.k : a.q) + size_t(hk) * DK + 4 * sub;
+        const size_t src_stride = is_k ? a.k_stride : a.q_stride;
 #pragma unroll
         for (int i = 0; i < kGroup / 4; ++i) {
             const int m = t0 + 4 * i + wid;
@@ -85,17 +92,18 @@ __global__ __launch_bounds__(256, 3) void delta_step_kernel(DeltaArgs a) {
             if (m < v.n && e < kGroup * DV) val[i] = load4(a.v + size_t(v.r0 + m) * a.v_stride + size_t(h) * DV + e % DV);
         }
     };
-    if (v.n > 0) load(0);
+    if (v.n > 0) load(0, t);
     float4 S[NG][4];
 #pragma unroll
     for (int g = 0; g < NG; ++g)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             S[g][j] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (v.in >= 0) S[g][j] = load4(a.state + size_t(v.in) * pool + place + size_t(4 * (rl + RL * g) + j) * DV);
+            if (v.in >= 0) S[g][j] = load4(state(v.in, lane) + size_t(4 * RL * g + j) * DV);
         }
     for (int t0 = 0; t0 < v.n; t0 += kGroup) {
         const int nt = min(kGroup, v.n - t0);
+        if (t0 > 0) load(t0, now(t) & 255);
         if (t < nt) {
             sc[t][0] = expf(log_decay(a, v.r0 + t0 + t, h));
             sc[t][1] = step_size(a, v.r0 + t0 + t, h);
@@ -114,19 +122,17 @@ __global__ __launch_bounds__(256, 3) void delta_step_kernel(DeltaArgs a) {
         for (int i = 0; i < NV; ++i)
             if (i * 1024 + 4 * t < kGroup * DV) *reinterpret_cast<float4 *>(&vo[0][0] + i * 1024 + 4 * t) = val[i];
         __syncthreads();
-        if (t0 + kGroup < v.n) load(t0 + kGroup);
         for (int m = 0; m < nt; ++m) {
             const float decay = sc[m][0], beta = sc[m][1], kq = sc[m][2];
             const float4 val = load4(&vo[m][col]);
-            float4 kr[NG];
             float ks[4] = {}, qs[4] = {};
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                kr[g] = load4(&qk[m][1][4 * (rl + RL * g)]);
+                const float4 kr = load4(&qk[m][1][4 * (rl + RL * g)]);
                 const float4 qr = load4(&qk[m][0][4 * (rl + RL * g)]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const float kj = reinterpret_cast<const float *>(&kr[g])[j], qj = reinterpret_cast<const float *>(&qr)[j];
+                    const float kj = reinterpret_cast<const float *>(&kr)[j], qj = reinterpret_cast<const float *>(&qr)[j];
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         const float sv = reinterpret_cast<const float *>(&S[g][j])[c];
@@ -142,27 +148,35 @@ __global__ __launch_bounds__(256, 3) void delta_step_kernel(DeltaArgs a) {
                 d[c] = beta * (reinterpret_cast<const float *>(&val)[c] - old);
                 qs[c] = __builtin_fmaf(kq, d[c], columns_sum<CL>(qs[c]) * decay);
             }
+            const int again = now(m);
 #pragma unroll
-            for (int g = 0; g < NG; ++g)
+            for (int g = 0; g < NG; ++g) {
+                const float4 kr = load4(&qk[again][1][4 * (rl + RL * g)]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         float &sv = reinterpret_cast<float *>(&S[g][j])[c];
-                        sv = __builtin_fmaf(reinterpret_cast<const float *>(&kr[g])[j], d[c], sv * decay);
+                        sv = __builtin_fmaf(reinterpret_cast<const float *>(&kr)[j], d[c], sv * decay);
                     }
+            }
             if (rl == 0) *reinterpret_cast<float4 *>(&vo[m][col]) = make_float4(qs[0], qs[1], qs[2], qs[3]);
         }
         __syncthreads();
-        write_rows<DV>(a, h, v.r0 + t0, nt, t, 256, [&](int m, int e) { return load4(&vo[m][e]); });
+        write_rows<DV>(a, h, v.r0 + t0, nt, now(t) & 255, 256, [&](int m, int e) { return load4(&vo[m][e]); });
         __syncthreads();
     }
     if (v.out >= 0) {
+        float *to = state(v.out, now(lane) & 63);
+        const bool past = size_t(gridDim.x) * (DK * DV * 4) > (32u << 20);
 #pragma unroll
         for (int g = 0; g < NG; ++g)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                *reinterpret_cast<float4 *>(a.state + size_t(v.out) * pool + place + size_t(4 * (rl + RL * g) + j) * DV) = S[g][j];
+            for (int j = 0; j < 4; ++j) {
+                float4 *p = reinterpret_cast<float4 *>(to + size_t(4 * RL * g + j) * DV);
+                if (past) store_past(p, S[g][j]);
+                else *p = S[g][j];
+            }
     }
 }
 
