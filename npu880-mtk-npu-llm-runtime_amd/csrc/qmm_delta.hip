@@ -259,7 +259,12 @@ struct DeltaScratch {
     char *matrices;  // [groups][v_heads]: T, then P: two tiles of 16 rows, each 1 KB hi and 1 KB lo
     float *factors;  // [groups][v_heads][96]: e^G_i, e^(G_last - G_i), beta_i
     float *inverse;  // [groups][qk_heads][64]: 1 / |k_i|, 1 / |q_i|
+    // of sequences that are walked in halves, per sequence and value head: the state after the first one; the second one's end
+    // from a state of zeros; and what it makes of the unit vectors; of the second one's tokens, what they read of those
+    float *middle, *end, *carry, *reads;
 };
+// A sequence's second half begins at this group (its number of groups: it has none).
+__device__ inline int second_half(int n_groups, bool halves) { return halves && n_groups >= kHalfGroups ? (n_groups + 1) / 2 : n_groups; }
 __device__ inline int64_t first_group(const StateSeq &v, int s) { return v.r0 / kChunk + s; }
 
 // Up to 32 rows from `p` on, of which `left` are the sequence's, as a buffer: loads past them give 0 and stores nothing, without a
@@ -491,20 +496,31 @@ __device__ inline float over_groups(float x) {  // sum over the four lanes of a 
 // The walk over a sequence's groups. A workgroup has 16 columns of the state in each of its NW first waves, all rows, as
 // sums of matrix products; nothing of it leaves the wave's registers from group to group. Four more waves bring the
 // next group's K, Q, T and P into LDS as operands meanwhile.
-template <int DK, int NW>
+//
+// HALVES: a sequence of many groups goes in two halves at once, where compute units are left. The rule is linear in the state:
+// what follows from S is what follows from zeros, with the values, and M S without them, M from the unit matrix. So the second half is
+// walked twice, for the values (kind 1) and for M (kind 2), and joined with the first one's last state afterwards.
+template <int DK, int NW, bool HALVES>
 __global__ __launch_bounds__(512) void delta_walk_kernel(DeltaArgs a, DeltaScratch w, int splits) {
     constexpr int NU = DK / 32, NI = DK / 64;
     constexpr int kK = 0, kQ = kK + 2 * NU * 2 * kBlock, kTurned = kQ + 2 * NU * 2 * kBlock, kM = kTurned + DK / 16 * 2 * kBlock;
     constexpr int kP = kM + 4 * kBlock, kFactor = kP + 4 * kBlock, kBuffer = kFactor + kFactors * 4;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    const int of = a.v_heads / a.qk_heads, per = of * splits;
+    const int of = a.v_heads / a.qk_heads, parts = HALVES ? 2 * splits + DK / (16 * NW) : splits, per = of * parts;
     // workgroups that read the same keys on one XCD (they go to the eight in turns)
     const int unit = int(blockIdx.x / 8 / unsigned(per)) * 8 + int(blockIdx.x % 8), part = int(blockIdx.x / 8 % unsigned(per));
     if (unit >= a.b.n_seqs * a.qk_heads) return;
-    const int s = unit / a.qk_heads, hk = unit % a.qk_heads, h = hk * of + part / splits;
-    const StateSeq v = state_seq(a.b, s);
-    const int n_groups = (v.n + kChunk - 1) / kChunk;
-    const size_t group0 = size_t(first_group(v, s));
+    const int s = unit / a.qk_heads, hk = unit % a.qk_heads, h = hk * of + part / parts;
+    StateSeq v = state_seq(a.b, s);
+    const int kind = HALVES ? min(part % parts / splits, 2) : 0;
+    const int all_groups = (v.n + kChunk - 1) / kChunk, middle = second_half(all_groups, HALVES), first = kind ? middle : 0;
+    if (HALVES && kind && middle == all_groups) return;
+    const int n_groups = HALVES ? (kind ? all_groups - middle : middle) : all_groups;
+    const size_t group0 = size_t(first_group(v, s)) + size_t(first), read0 = size_t(v.r0) / 2;
+    if (HALVES) {
+        v.n = kind ? v.n - first * kChunk : min(v.n, middle * kChunk);
+        v.r0 += first * kChunk;
+    }
     const int t = threadIdx.x, lane = t & 63, wid = __builtin_amdgcn_readfirstlane(t >> 6);
 
     if (wid >= NW) {
@@ -575,8 +591,21 @@ __global__ __launch_bounds__(512) void delta_walk_kernel(DeltaArgs a, DeltaScrat
 
     __builtin_amdgcn_s_setprio(2);  // before the waves that bring operands
     const int g = lane / 16, lane_at = g * 256 + (lane % 16 ^ g) * 16;
-    const int col = (part % splits * NW + wid) * 16 + lane % 16, DV = a.value_dim;
-    const size_t place = size_t(h) * DK * DV + col, pool = size_t(a.v_heads) * DK * DV;
+    const int DV = a.value_dim, columns = kind == 2 ? DK : DV;
+    const int col = ((part % parts - kind * splits) * NW + wid) * 16 + lane % 16;
+    const size_t pool = size_t(a.v_heads) * DK * DV, list = size_t(s) * a.v_heads + h;
+    const float *from = v.in >= 0 ? a.state + size_t(v.in) * pool + size_t(h) * DK * DV : nullptr;
+    float *to = v.out >= 0 ? a.state + size_t(v.out) * pool + size_t(h) * DK * DV : nullptr;
+    float *out = a.out + size_t(v.r0) * a.out_stride + size_t(h) * DV;
+    size_t out_stride = a.out_stride;
+    float out_factor = a.scale;
+    if (HALVES && kind) from = nullptr;
+    if (HALVES && (kind || middle < all_groups)) to = kind == 2 ? w.carry + list * DK * DK : (kind ? w.end : w.middle) + list * DK * DV;
+    if (HALVES && kind == 2) {
+        out_stride = size_t(a.v_heads) * DK;
+        out = w.reads + read0 * out_stride + size_t(h) * DK;
+        out_factor = 1.0f;
+    }
     const f4 zero = {0.f, 0.f, 0.f, 0.f};
     f4 S[2 * NU], val[2], ahead[2];     // values of this group and the next
     unsigned v_at[2][4], out_at[2][4];  // bytes from a group's first row to this lane's, of its row tensors
@@ -585,11 +614,11 @@ __global__ __launch_bounds__(512) void delta_walk_kernel(DeltaArgs a, DeltaScrat
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             v_at[ti][r] = (unsigned(16 * ti + 4 * g + r) * unsigned(a.v_stride) + unsigned(col)) * 4u;
-            out_at[ti][r] = (unsigned(16 * ti + 4 * g + r) * unsigned(a.out_stride) + unsigned(col)) * 4u;
+            out_at[ti][r] = (unsigned(16 * ti + 4 * g + r) * unsigned(out_stride) + unsigned(col)) * 4u;
         }
     auto load_values = [&](int n, f4 (&to)[2]) {
         const __amdgpu_buffer_rsrc_t rows =
-            group_rows(a.v + size_t(v.r0 + n * kChunk) * a.v_stride + size_t(h) * DV, a.v_stride, h * DV, v.n - n * kChunk);
+            group_rows(a.v + size_t(v.r0 + n * kChunk) * a.v_stride + size_t(h) * DV, a.v_stride, h * DV, kind == 2 ? 0 : v.n - n * kChunk);
 #pragma unroll
         for (int ti = 0; ti < 2; ++ti)
 #pragma unroll
@@ -608,14 +637,17 @@ __global__ __launch_bounds__(512) void delta_walk_kernel(DeltaArgs a, DeltaScrat
 #pragma unroll
     for (int k = 0; k < 2 * NU; ++k)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) S[k][r] = v.in >= 0 ? a.state[size_t(v.in) * pool + place + size_t(16 * k + 4 * g + r) * DV] : 0.0f;
+        for (int r = 0; r < 4; ++r) {
+            const int row = 16 * k + 4 * g + r;
+            S[k][r] = from ? from[size_t(row) * DV + col] : kind == 2 && row == col ? 1.0f : 0.0f;
+        }
     if (n_groups == 0) {
         __syncthreads();
-        if (v.out >= 0)
+        if (to)
 #pragma unroll
             for (int k = 0; k < 2 * NU; ++k)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) a.state[size_t(v.out) * pool + place + size_t(16 * k + 4 * g + r) * DV] = S[k][r];
+                for (int r = 0; r < 4; ++r) to[size_t(16 * k + 4 * g + r) * DV + col] = S[k][r];
         return;
     }
     float bound = 0.0f, sum = sizes(val);  // of the column's length; of the values' sizes
@@ -688,7 +720,7 @@ __global__ __launch_bounds__(512) void delta_walk_kernel(DeltaArgs a, DeltaScrat
         bound = __builtin_fmaf(all, bound, sum);
         sum = sizes(val);
         const int next = scale_for(bound + sum);
-        const float turn = two_to(next - scale), out_scale = a.scale * two_to(-(scale + 14));
+        const float turn = two_to(next - scale), out_scale = out_factor * two_to(-(scale + 14));
         scale = next;
 #pragma unroll
         for (int k = 0; k < 2 * NU; ++k) S[k] *= all * turn;
@@ -726,7 +758,7 @@ __global__ __launch_bounds__(512) void delta_walk_kernel(DeltaArgs a, DeltaScrat
             if (k == (NU > 2 ? 2 : 0)) products(p, dp, o);
             if (k == 2 * NU - 2) {
                 const __amdgpu_buffer_rsrc_t rows =
-                    group_rows(a.out + size_t(v.r0 + n * kChunk) * a.out_stride + size_t(h) * DV, a.out_stride, h * DV, v.n - n * kChunk);
+                    group_rows(out + size_t(n * kChunk) * out_stride, out_stride, h * columns, v.n - n * kChunk);
 #pragma unroll
                 for (int ti = 0; ti < 2; ++ti)
 #pragma unroll
@@ -736,11 +768,11 @@ __global__ __launch_bounds__(512) void delta_walk_kernel(DeltaArgs a, DeltaScrat
         }
         __syncthreads();
     }
-    if (v.out >= 0) {
+    if (to) {
 #pragma unroll
         for (int k = 0; k < 2 * NU; ++k)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) a.state[size_t(v.out) * pool + place + size_t(16 * k + 4 * g + r) * DV] = S[k][r] * two_to(-scale);
+            for (int r = 0; r < 4; ++r) to[size_t(16 * k + 4 * g + r) * columns + col] = S[k][r] * two_to(-scale);
     }
 }
 
@@ -933,11 +965,95 @@ __global__ __launch_bounds__(256) void delta_norm_kernel(DeltaArgs a, int tiles)
         }
 }
 
-template <int DK, int NW> hipError_t launch_walk(const DeltaArgs &a, const DeltaScratch &w, hipStream_t s) {
+// What a first half left goes to the second half's tokens and last state: O + scale R S and E + M S, with S the state in the middle, R what
+// the tokens read of the unit vectors, O and E what the values gave; 32 rows at a time. Then, and for all other rows, norm and
+// gate. R and M are at most 1 in size and kept 2^14 times, S with a scale for each column, as above.
+template <int DK, int DV>
+__global__ __launch_bounds__(512, 4) void delta_join_kernel(DeltaArgs a, DeltaScratch w, int tiles) {
+    constexpr int NU = DK / 32;
+    __shared__ __attribute__((aligned(16))) char rows[2 * NU * 2 * kBlock];
+    __shared__ __attribute__((aligned(16))) float sum[32][DV + 4];
+    const int t = threadIdx.x, lane = t & 63, wid = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int h = int(blockIdx.x % unsigned(a.v_heads)), st = int(blockIdx.x / unsigned(a.v_heads)), s = st / tiles;
+    const StateSeq v = state_seq(a.b, s);
+    const int n_groups = (v.n + kChunk - 1) / kChunk, middle = second_half(n_groups, true);
+    const int g = lane / 16, lane_at = g * 256 + (lane % 16 ^ g) * 16, col = wid * 16 + lane % 16;
+    const bool multiplies = wid < DV / 16;
+    const size_t list = size_t(s) * a.v_heads + h, read_stride = size_t(a.v_heads) * DK;
+    Pair b[NU];
+    int scale = 0;
+    if (middle < n_groups && multiplies) {
+        f4 S[2 * NU];
+        float bound = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 2 * NU; ++k)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                S[k][r] = w.middle[list * DK * DV + size_t(16 * k + 4 * g + r) * DV + col];
+                bound += fabsf(S[k][r]);
+            }
+        scale = scale_for(over_groups(bound));
+#pragma unroll
+        for (int u = 0; u < NU; ++u) b[u] = split(S[2 * u] * two_to(scale), S[2 * u + 1] * two_to(scale));
+    }
+    const int items = n_groups + (middle < n_groups ? DK / 32 : 0);
+    for (int i = st % tiles; i < items; i += tiles) {
+        const int r0 = v.r0 + i * kChunk, left = min(v.n - i * kChunk, kChunk);
+        float *const out = a.out + size_t(h) * DV;
+        if (i < middle) {
+            if (a.gamma || a.z) write_rows<DV>(a, h, r0, left, t, 512, [&](int m, int e) { return load4(out + size_t(r0 + m) * a.out_stride + e); });
+            continue;
+        }
+        const bool state = i >= n_groups;
+        if (t < 8 * DK / 4) {
+            const Item<DK> it(t, 0);
+            const size_t stride = state ? DK : read_stride;
+            const float *from = state ? w.carry + list * DK * DK + size_t(i - n_groups) * 32 * DK
+                                      : w.reads + (size_t(v.r0) / 2 + size_t(i - middle) * kChunk) * read_stride + size_t(h) * DK;
+            h4 hi[4], lo[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                f4 x = {0.f, 0.f, 0.f, 0.f};
+                if (state || it.token + j < left) x = *reinterpret_cast<const f4 *>(from + size_t(it.token + j) * stride + it.at);
+                split4(x, 0x1p14f, hi[j], lo[j]);
+            }
+            it.store(rows, nullptr, hi, lo);
+        }
+        __syncthreads();
+        if (multiplies) {
+            f4 c[2] = {};
+#pragma unroll
+            for (int u = 0; u < NU; ++u) {
+                Pair op[2];
+#pragma unroll
+                for (int ti = 0; ti < 2; ++ti) op[ti] = operand(rows + (ti * NU + u) * 2 * kBlock + lane_at);
+                products(op, b[u], c);
+            }
+            const float f = (state ? 1.0f : a.scale) * two_to(-(scale + 14));
+#pragma unroll
+            for (int ti = 0; ti < 2; ++ti)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) sum[16 * ti + 4 * g + r][col] = c[ti][r] * f;
+        }
+        __syncthreads();
+        auto plus = [](float4 x, float4 y) { return make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w); };
+        if (!state) {
+            write_rows<DV>(a, h, r0, left, t, 512, [&](int m, int e) { return plus(load4(&sum[m][e]), load4(out + size_t(r0 + m) * a.out_stride + e)); });
+        } else if (v.out >= 0) {
+            const size_t at = size_t(i - n_groups) * 32 * DV;
+            float *to = a.state + (size_t(v.out) * a.v_heads + size_t(h)) * DK * DV + at;
+            for (int e = 4 * t; e < 32 * DV; e += 4 * 512)
+                *reinterpret_cast<float4 *>(to + e) = plus(load4(&sum[e / DV][e % DV]), load4(w.end + list * DK * DV + at + e));
+        }
+        __syncthreads();
+    }
+}
+
+template <int DK, int NW, bool HALVES> hipError_t launch_walk(const DeltaArgs &a, const DeltaScratch &w, hipStream_t s) {
     constexpr int kBuffer = ((2 * 2 * (DK / 32) + DK / 16) * 2 + 8) * kBlock + kFactors * 4;
-    const int splits = a.value_dim / (16 * NW), per = a.v_heads / a.qk_heads * splits;
+    const int splits = a.value_dim / (16 * NW), parts = HALVES ? 2 * splits + DK / (16 * NW) : splits, per = a.v_heads / a.qk_heads * parts;
     const int units = a.b.n_seqs * a.qk_heads;
-    hipLaunchKernelGGL((delta_walk_kernel<DK, NW>), dim3(unsigned((units + 7) / 8) * 8u * unsigned(per)), dim3(512), 2 * kBuffer, s, a, w, splits);
+    hipLaunchKernelGGL((delta_walk_kernel<DK, NW, HALVES>), dim3(unsigned((units + 7) / 8) * 8u * unsigned(per)), dim3(512), 2 * kBuffer, s, a, w, splits);
     return hipGetLastError();
 }
 
@@ -950,7 +1066,17 @@ template <int DK> hipError_t launch_groups(const DeltaArgs &a, const DeltaScratc
     if (e != hipSuccess) return e;
     // Where workgroups of 32 columns find a CU each they are a little faster (a prompt of 8192 and 32 heads: 411 us, with 64
     // columns 423), else those of 64 (six prompts of 4887 tokens in all: 106 us, with 32 columns 144).
-    e = lists * (a.value_dim / 32) <= cu_count ? launch_walk<DK, 2>(a, w, s) : launch_walk<DK, 4>(a, w, s);
+    // Halves where all their workgroups find a CU: a prompt of 32 heads and 640 tokens 50 us, in one 54; of 2048 109 and 141; of
+    // 8192 397 and 559.
+    if (want >= kHalfGroups && lists <= kHalfLists && lists * ((2 * a.value_dim + DK) / 64) <= cu_count) {
+        if ((e = launch_walk<DK, 4, true>(a, w, s)) != hipSuccess) return e;
+        const int turns = int((want + DK / 32 + 3) / 4);  // (each workgroup with about four items, for one reading of the state)
+        const dim3 grid(unsigned(lists) * unsigned(turns));
+        if (a.value_dim == 64) hipLaunchKernelGGL((delta_join_kernel<DK, 64>), grid, dim3(512), 0, s, a, w, turns);
+        else hipLaunchKernelGGL((delta_join_kernel<DK, 128>), grid, dim3(512), 0, s, a, w, turns);
+        return hipGetLastError();
+    }
+    e = lists * (a.value_dim / 32) <= cu_count ? launch_walk<DK, 2, false>(a, w, s) : launch_walk<DK, 4, false>(a, w, s);
     if (e != hipSuccess || (!a.gamma && !a.z)) return e;
     const dim3 grid(unsigned(lists) * unsigned(tiles));
     if (a.value_dim == 64) hipLaunchKernelGGL(delta_norm_kernel<64>, grid, dim3(256), 0, s, a, tiles);
@@ -977,6 +1103,11 @@ hipError_t launch_delta(const DeltaArgs &a, void *scratch, size_t scratch_bytes,
         w.matrices = static_cast<char *>(scratch);
         w.factors = reinterpret_cast<float *>(w.matrices + groups * a.v_heads * kDeltaMatrices);
         w.inverse = w.factors + groups * a.v_heads * kFactors;
+        const size_t half = size_t(min(lists, kHalfLists)) * a.key_dim;
+        w.middle = w.inverse + groups * a.qk_heads * 64;
+        w.end = w.middle + half * a.value_dim;
+        w.carry = w.end + half * a.value_dim;
+        w.reads = w.carry + half * a.key_dim;
         return a.key_dim == 128 ? launch_groups<128>(a, w, cu_count, s) : launch_groups<64>(a, w, cu_count, s);
     }
     const dim3 grid(unsigned(a.b.n_seqs) * unsigned(a.v_heads));

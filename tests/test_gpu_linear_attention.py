@@ -183,3 +183,20 @@ def test_delta_long_many_heads(ctx, DK, DV, of):
 def test_delta_wrong_hints(ctx, hint, ws):
     """Sequences longer than the host knew, and shorter: a choice of launch only."""
     delta_case(ctx, [70, 0, 1, 33, 260], 2, 2, hints=hint, ws=ws, slots=[(0, 0), (1, 1), (2, 2), (3, 4), (5, 5)])
+
+
+@pytest.mark.parametrize("DK,DV", [(64, 64), (64, 128), (128, 64), (128, 128)])
+def test_delta_halves(ctx, DK, DV):
+    """Sequences that are walked in halves beside others that are not: an even and an odd number of groups, a last group of one
+    token, the shortest ones; states in place, new, not kept."""
+    kw = dict(gap=4, extra=3, ws=True, seed=DK + DV)
+    delta_case(ctx, [1025, 0, 481, 480, 1, 700, 33], 1, 2, DK, DV, **kw)
+    delta_case(ctx, [640, 511, 512, 40, 900], 1, 3, DK, DV, gamma=False, slots=[(0, 0), (-1, 2), (3, -1), (4, 4), (5, 6)], **kw)
+    delta_case(ctx, [3000], 2, 2, DK, DV, gate=False, hints=False, **kw)
+
+
+@pytest.mark.parametrize("decay", [(0.0, 1e-6), (0.0, 0.01), (20.0, 200.0)])
+@pytest.mark.parametrize("alike", [0.0, 0.999, 1.0])
+def test_delta_halves_of_all_kinds(ctx, decay, alike):
+    delta_case(ctx, [1600, 560], alike=alike, decay=decay, spread=100.0, ws=True)
+    delta_case(ctx, [1600, 560], alike=alike, decay=decay, spread=1e-3, state_spread=10.0, gamma=False, gate=False, ws=True)
