@@ -340,9 +340,11 @@ template <int DK> __device__ inline float inverse_length(const float (&sums)[DK 
     for (int u = 0; u < DK / 32; ++u) eps += sums[u];
     return inv_root(eps);
 }
-// sums of the log decays of a head and its step sizes, a token per lane of half a wave
+// 2^x, x rounded to fp32 first: |x| 2^-24 off
+__device__ inline float power_of_two(double x) { return __builtin_amdgcn_exp2f(float(x)); }
+// sums of the log decays of a head (of 2: the decays are powers of two, one instruction each) and its step sizes, a token per lane of half a wave
 __device__ inline void head_steps(const DeltaArgs &a, int row, int h, int m, bool on, double *G, float *beta) {
-    double g = on ? double(log_decay(a, row, h)) : 0.0;
+    double g = on ? double(log_decay(a, row, h)) * 1.4426950408889634 : 0.0;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
         const double o = shfl_up(g, d);
@@ -370,15 +372,18 @@ __device__ inline void store_operand(char *matrix, int i, int place, f4 x) {
     *reinterpret_cast<h4 *>(matrix + i / 16 * 2 * kBlock + place) = hi;
     *reinterpret_cast<h4 *>(matrix + i / 16 * 2 * kBlock + place + kBlock) = lo;
 }
-// row i, columns c .. c + 3 of A, and of P times 2^14
+// row i, columns c .. c + 3 of A, and of P times 2^14 (above the diagonal's tiles nothing was written: any value)
 __device__ inline f4 mask_and_decay(const Square &kk, const Square &qk, const double *G, const float *beta, int i, int c, Square &A) {
-    f4 p;
+    const f4 kv = *reinterpret_cast<const f4 *>(&kk[i][c]), qv = *reinterpret_cast<const f4 *>(&qk[i][c]);
+    const double row = G[i];
+    f4 p, x;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const float e = c + j <= i ? expf(float(G[i] - G[c + j])) : 0.0f;
-        A[i][c + j] = c + j < i ? beta[i] * e * kk[i][c + j] : 0.0f;
-        p[j] = c + j <= i ? e * qk[i][c + j] * 0x1p14f : 0.0f;  // (above the diagonal's tiles nothing was written)
+        const float e = power_of_two(row - G[c + j]);
+        x[j] = c + j < i ? beta[i] * e * kv[j] : 0.0f;
+        p[j] = c + j <= i ? e * qv[j] * 0x1p14f : 0.0f;
     }
+    *reinterpret_cast<f4 *>(&A[i][c]) = x;
     return p;
 }
 // The inverse of I + A: its two 16 x 16 triangles by substitution, a column per lane, then T21 = -T22 A21 T11 on the matrix
@@ -406,14 +411,11 @@ __device__ inline void invert_corner(const Square &A, int lane, Square &T) {  //
 }
 // row i, columns c .. c + 3 of T, times 2^14
 __device__ inline f4 enlarged(const Square &T, int i, int c) {
-    f4 p;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) p[j] = c / 16 <= i / 16 ? T[i][c + j] * 0x1p14f : 0.0f;
-    return p;
+    return c / 16 <= i / 16 ? *reinterpret_cast<const f4 *>(&T[i][c]) * 0x1p14f : f4{0.f, 0.f, 0.f, 0.f};
 }
 // of 96 factors: e^G_i, then e^(G_last - G_i), then beta_i
 __device__ inline float factor_of(const double *G, const float *beta, int i) {
-    return i < 64 ? expf(float(i < 32 ? G[i] : G[31] - G[i - 32])) : beta[i - 64];
+    return i < 64 ? power_of_two(i < 32 ? G[i] : G[31] - G[i - 32]) : beta[i - 64];
 }
 
 // T and P of one group and key head, for its value heads two at a time (both inverses in one wave).
@@ -426,7 +428,7 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, DeltaSc
     Square *const A = reinterpret_cast<Square *>(shared), *const T = A + 2;
     __shared__ float sums[2][32][NU];
     __shared__ __attribute__((aligned(16))) float inv[2][32];
-    __shared__ Square kk, qk;
+    __shared__ __attribute__((aligned(16))) Square kk, qk;
     __shared__ double G[2][32];
     __shared__ float beta[2][32];
     const int t = threadIdx.x, lane = t & 63, wid = __builtin_amdgcn_readfirstlane(t >> 6);
