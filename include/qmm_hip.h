@@ -498,9 +498,11 @@ int qmm_short_conv(qmm_context *ctx, const qmm_state_batch *batch, const qmm_con
  *   S <- decay * S;   S <- S + k^ (beta * (v - S' k^))';   o = S' q^
  * on the state S [key_dim][value_dim], and its output is
  *   o, or with gamma  o / sqrt(mean o^2 + gamma_eps) * gamma,  with z times z / (1 + exp(-z)).
- * A rate above 0 counts as 0. Few new rows go through the state one after another;
- * prompts in groups of 32 on the matrix units, their operands as pairs of fp16
- * values that hold 22 bits, where a workspace allows it. */
+ * A rate above 0 counts as 0. Up to 8 new rows go through the state one after another;
+ * more in groups of 32 on the matrix units (strides of q, k, v and out below 2^24
+ * values; else as the few), their operands as pairs of fp16 values: 22 bits, and never
+ * finer than 2^-39 of what the column's values of a group and its state sum to. Long
+ * prompts are faster with a workspace. */
 typedef struct {
     const float *q, *k;   /* device [n_rows][..]: qk_heads heads of key_dim values */
     size_t q_stride, k_stride;

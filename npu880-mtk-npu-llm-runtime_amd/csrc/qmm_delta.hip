@@ -2,7 +2,10 @@
 //
 // Every token of a head, in order, on its state S [DK][DV]:
 //   S <- e^g S;  d = beta (v - S' k);  S <- S + k d';  o = S' q
-// with k and q of unit length. The columns of S are independent of each other.
+// with k and q of unit length. The columns of S are independent of each other. Three ways, by the new rows of a sequence:
+// a token at a time (up to 8), groups of 32 in one launch, groups in three launches (launch_delta has the rule).
+// Bound: a token at a time and one group by the states' way through memory, or the latency of a launch where they are
+// few; prompts by the chain of groups, one product after the other (figures at the kernels, heads of 128).
 #include <hip/hip_runtime.h>
 
 #include "qmm_lanes.h"
@@ -52,7 +55,8 @@ template <int DV, typename F> __device__ inline void write_rows(const DeltaArgs 
 // sequence and head, a wave 16 * CL / 4 columns (4 a lane) of all rows, in
 // registers; a lane has rows 4 (rl + RL g) .. + 3. Both products with S are taken
 // before it changes: S' q after the step is e^g S' q + (k.q) d, so one pass and one
-// sum over the lanes serve both, and no wave waits for another between tokens.
+// sum over the lanes serve both, and no wave waits for another between tokens. 32 heads: one sequence of a token 5.6 us (a launch and one
+// way through memory), 64 sequences 50.9 us (5.4 TB/s of 273 MB); another token adds 0.8 us.
 template <int DK, int DV>
 __global__ __launch_bounds__(256, 4) void delta_step_kernel(DeltaArgs a) {
     constexpr int CL = DV / 16, RL = 64 / CL, NG = DK / (4 * RL), NV = (kGroup * DV + 1023) / 1024, HL = 32;  // HL: lanes that hold one row of q or k
@@ -418,7 +422,9 @@ __device__ inline float factor_of(const double *G, const float *beta, int i) {
     return i < 64 ? power_of_two(i < 32 ? G[i] : G[31] - G[i - 32]) : beta[i - 64];
 }
 
-// T and P of one group and key head, for its value heads two at a time (both inverses in one wave).
+// T and P of one group and key head, for its value heads two at a time (both inverses in one wave). Bound: the chain of nine barriers at
+// three workgroups of a CU (44 KB of LDS): 8192 tokens of 16 key and 32 value heads 58 us, of which loads, conversion and products
+// 31, inverses 6, stores 4.
 template <int DK>
 __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, DeltaScratch w, int tiles) {
     constexpr int NU = DK / 32, NI = DK / 64;
@@ -495,13 +501,30 @@ __device__ inline float over_groups(float x) {  // sum over the four lanes of a 
     return __uint_as_float(q[0]) + __uint_as_float(q[1]);
 }
 
+// The i-th longest of up to 64 sequences: the longest walks begin first (prompts of 951, 677, 403, 129, 1500 and 1225 tokens: 107 us
+// in their order, 97 so). More fill the compute units anyway.
+__device__ inline int by_length(const StateView &b, int i) {
+    if (b.n_seqs > 64) return i;
+    const int lane = threadIdx.x % 64, n = lane < b.n_seqs ? state_seq(b, lane).n : -1;
+    int longer = 0;
+    for (int j = 0; j < b.n_seqs; ++j) {
+        const int other = __builtin_amdgcn_readlane(n, j);
+        longer += other > n || (other == n && j < lane);
+    }
+    return int(__builtin_ctzll(__ballot(longer == i)));
+}
+
 // The walk over a sequence's groups. A workgroup has 16 columns of the state in each of its NW first waves, all rows, as
 // sums of matrix products; nothing of it leaves the wave's registers from group to group. Four more waves bring the
-// next group's K, Q, T and P into LDS as operands meanwhile.
+// next group's K, Q, T and P into LDS as operands meanwhile. Bound: one wave's chain of 84 matrix products and 300 vector instructions a
+// group, none of which can wait for another group's, beside 120 KB of reads and 57 KB of writes of LDS: 1.6 us a group where the
+// products alone take 0.57 (16.2 cycles each). 417 tokens 26.8 us. Measured and not kept: 16 columns a workgroup, operands made by the
+// first kernel (480 us for 8192 tokens against 411), output products in waves of their own, K S of the next group beside this one's.
 //
 // HALVES: a sequence of many groups goes in two halves at once, where compute units are left. The rule is linear in the state:
 // what follows from S is what follows from zeros, with the values, and M S without them, M from the unit matrix. So the second half is
-// walked twice, for the values (kind 1) and for M (kind 2), and joined with the first one's last state afterwards.
+// walked twice, for the values (kind 1) and for M (kind 2), and joined with the first one's last state afterwards. 8192 tokens: 411 us in
+// one, 240 in halves.
 template <int DK, int NW, bool HALVES>
 __global__ __launch_bounds__(512) void delta_walk_kernel(DeltaArgs a, DeltaScratch w, int splits) {
     constexpr int NU = DK / 32, NI = DK / 64;
@@ -512,7 +535,7 @@ __global__ __launch_bounds__(512) void delta_walk_kernel(DeltaArgs a, DeltaScrat
     // workgroups that read the same keys on one XCD (they go to the eight in turns)
     const int unit = int(blockIdx.x / 8 / unsigned(per)) * 8 + int(blockIdx.x % 8), part = int(blockIdx.x / 8 % unsigned(per));
     if (unit >= a.b.n_seqs * a.qk_heads) return;
-    const int s = unit / a.qk_heads, hk = unit % a.qk_heads, h = hk * of + part / parts;
+    const int s = HALVES ? unit / a.qk_heads : by_length(a.b, unit / a.qk_heads), hk = unit % a.qk_heads, h = hk * of + part / parts;
     StateSeq v = state_seq(a.b, s);
     const int kind = HALVES ? min(part % parts / splits, 2) : 0;
     const int all_groups = (v.n + kChunk - 1) / kChunk, middle = second_half(all_groups, HALVES), first = kind ? middle : 0;
@@ -779,7 +802,8 @@ __global__ __launch_bounds__(512) void delta_walk_kernel(DeltaArgs a, DeltaScrat
 }
 
 // Few groups, drafts mostly: all of the above in one workgroup per sequence and head, that makes a group's matrices itself and
-// has all columns of the state (16 a wave), so that the norm needs no launch of its own.
+// has all columns of the state (16 a wave), so that the norm needs no launch of its own. Two workgroups of a CU. 8 sequences of 5 to
+// 16 tokens and 32 heads 15.2 us: launch and loads, then eleven steps between barriers.
 template <int DK, int DV>
 __global__ __launch_bounds__(512, 4) void delta_group_kernel(DeltaArgs a) {
     constexpr int NU = DK / 32, kRows = 2 * NU * 2 * kBlock;
@@ -938,7 +962,8 @@ __global__ __launch_bounds__(512, 4) void delta_group_kernel(DeltaArgs a) {
     }
 }
 
-// The norm and the gate of rows as the walk leaves them, in place: half a wave per row and head
+// The norm and the gate of rows as the walk leaves them, in place: half a wave per row and head. Bound: memory (8192 tokens
+// of 32 heads 77 us, 5.2 TB/s).
 template <int DV>
 __global__ __launch_bounds__(256) void delta_norm_kernel(DeltaArgs a, int tiles) {
     const int lane = threadIdx.x & 31, h = int(blockIdx.x % unsigned(a.v_heads)), st = int(blockIdx.x / unsigned(a.v_heads));
@@ -969,7 +994,8 @@ __global__ __launch_bounds__(256) void delta_norm_kernel(DeltaArgs a, int tiles)
 
 // What a first half left goes to the second half's tokens and last state: O + scale R S and E + M S, with S the state in the middle, R what
 // the tokens read of the unit vectors, O and E what the values gave; 32 rows at a time. Then, and for all other rows, norm and
-// gate. R and M are at most 1 in size and kept 2^14 times, S with a scale for each column, as above.
+// gate. R and M are at most 1 in size and kept 2^14 times, S with a scale for each column, as above. Bound: memory (8192 tokens of 32 heads
+// 100 us, 4.7 TB/s).
 template <int DK, int DV>
 __global__ __launch_bounds__(512, 4) void delta_join_kernel(DeltaArgs a, DeltaScratch w, int tiles) {
     constexpr int NU = DK / 32;
