@@ -14,9 +14,9 @@
 //    the sums in 64 bits; then every candidate's rank is the number of those before
 //    it, by bisection in the beams' lists, which are in order.
 // Bound: memory (the logits are read once) for many rows, else the latency of the
-// two launches. 4 beams over 151936 tokens, 8 kept: 5.8 + 5.8 us; 128 beams of 16 items, 16 kept: 17.9 (3.7 TB/s; 2048 logits in a wave's
-// registers leave five waves of a SIMD to wait for memory) + 8.7. Where the keys are found by their upper half first, a search of 16
-// steps of a ballot instead of 64 (35.1 us with 64).
+// two launches. 4 beams over 151936 tokens, 8 kept: 5.8 + 5.8 us; 128 beams of 16 items, 16 kept: 17.9 (3.7 TB/s: some 500
+// vector instructions a wave, 8.6 us of issue in all, and the scalar ones of its searches between them) + 8.7. Keys are found by
+// their upper half first: a search of 16 ballots, not 64 (35.1 us for both launches with 64, 28.5 so).
 #include <hip/hip_runtime.h>
 
 #include "qmm_lanes.h"

@@ -18,8 +18,10 @@ constexpr int kStepRows = 8;  // new rows up to which a token at a time is faste
 constexpr int kGroup = 8;  // tokens whose inputs are in LDS at a time
 
 __device__ inline float softplus(float x) { return x > 0.0f ? x + log1pf(expf(-x)) : log1pf(expf(x)); }
+// Between -200, whose e^x is 0 in fp32 (sums over tokens keep their small parts, and no infinity meets another), and 0; NaN stays.
 __device__ inline float log_decay(const DeltaArgs &a, int row, int h) {
-    return fminf(a.rate[h] * softplus(a.a[size_t(row) * a.a_stride + h] + a.dt_bias[h]), 0.0f);
+    const float g = a.rate[h] * softplus(a.a[size_t(row) * a.a_stride + h] + a.dt_bias[h]);
+    return g > 0.0f ? 0.0f : g < -200.0f ? -200.0f : g;
 }
 __device__ inline float step_size(const DeltaArgs &a, int row, int h) {
     return 1.0f / (1.0f + expf(-a.beta[size_t(row) * a.b_stride + h]));
@@ -517,8 +519,8 @@ __device__ inline int by_length(const StateView &b, int i) {
 // The walk over a sequence's groups. A workgroup has 16 columns of the state in each of its NW first waves, all rows, as
 // sums of matrix products; nothing of it leaves the wave's registers from group to group. Four more waves bring the
 // next group's K, Q, T and P into LDS as operands meanwhile. Bound: one wave's chain of 84 matrix products and 300 vector instructions a
-// group, none of which can wait for another group's, beside 120 KB of reads and 57 KB of writes of LDS: 1.6 us a group where the
-// products alone take 0.57 (16.2 cycles each). 417 tokens 26.8 us. Measured and not kept: 16 columns a workgroup, operands made by the
+// group, beside 62 KB of LDS reads a wave and 57 KB of writes: 1.6 us a group of 32 columns, 1.65 to 2.0 of 64, where the products alone
+// take 0.57 (16.2 cycles each). 417 tokens 26.8 us. Measured and not kept: 16 columns a workgroup, operands made by the
 // first kernel (480 us for 8192 tokens against 411), output products in waves of their own, K S of the next group beside this one's.
 //
 // HALVES: a sequence of many groups goes in two halves at once, where compute units are left. The rule is linear in the state:
@@ -685,7 +687,8 @@ __global__ __launch_bounds__(512) void delta_walk_kernel(DeltaArgs a, DeltaScrat
 #pragma unroll
     for (int k = 0; k < 2 * NU; ++k) S[k] *= two_to(scale);
     __syncthreads();
-    for (int n = 0; n < n_groups; ++n) {
+    int n = 0;
+    do {
         const char *buf = lds + n % 2 * kBuffer + lane_at;
         const float *factors = reinterpret_cast<const float *>(lds + n % 2 * kBuffer + kFactor);
         // A wave has no other beside it to fill its gaps: operands are read ahead of their products, and Q S, for which
@@ -792,12 +795,15 @@ __global__ __launch_bounds__(512) void delta_walk_kernel(DeltaArgs a, DeltaScrat
             __builtin_amdgcn_sched_barrier(0);
         }
         __syncthreads();
-    }
+    } while (++n < n_groups);
     if (to) {
+        int now = lane;
+        asm("" : "+v"(now));  // (places worked out here, not kept over the walk)
+        float *p = to + size_t(4 * (now / 16 & 3)) * columns + ((part % parts - kind * splits) * NW + wid) * 16 + now % 16;
 #pragma unroll
         for (int k = 0; k < 2 * NU; ++k)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) to[size_t(16 * k + 4 * g + r) * columns + col] = S[k][r] * two_to(-scale);
+            for (int r = 0; r < 4; ++r) p[size_t(16 * k + r) * columns] = S[k][r] * two_to(-scale);
     }
 }
 

@@ -200,3 +200,48 @@ def test_delta_halves(ctx, DK, DV):
 def test_delta_halves_of_all_kinds(ctx, decay, alike):
     delta_case(ctx, [1600, 560], alike=alike, decay=decay, spread=100.0, ws=True)
     delta_case(ctx, [1600, 560], alike=alike, decay=decay, spread=1e-3, state_spread=10.0, gamma=False, gate=False, ws=True)
+
+
+@pytest.mark.parametrize("news", [[3, 1], [30, 9], [200, 40], [700]], ids=str)
+def test_delta_decays_past_fp32(ctx, news):
+    """Log decays that overflow, beside heads that forget little: a state is forgotten, and no infinity meets another."""
+    delta_case(ctx, news, 2, 2, decay=(1e38, 3e38))
+    delta_case(ctx, news, 2, 2, decay=(100.0, 1e7))
+
+
+@pytest.mark.parametrize("news", [[3, 1], [30, 9], [200, 40], [700, 2]], ids=str)
+@pytest.mark.parametrize("which", ["q", "k", "v", "a", "b", "state"])
+def test_delta_no_number_shows(ctx, which, news):
+    """A NaN is in its own head's output of the token and in the state after it; a query's in no state."""
+    rng = np.random.default_rng(3)
+    HK, HV, D, m, n = 2, 4, 64, sum(news), len(news)
+    say(f"delta NaN in {which} news={news}")
+    x = {"q": rng.standard_normal((m, HK, D)), "k": rng.standard_normal((m, HK, D)), "v": rng.standard_normal((m, HV, D)),
+         "a": rng.standard_normal((m, HV)), "b": rng.standard_normal((m, HV)), "state": rng.standard_normal((n, HV, D, D))}
+    x = {i: y.astype(np.float32) for i, y in x.items()}
+    row, h = (0 if which == "state" else 1), 1  # (head 1 reads key head 0)
+    x[which][(0, h, 5, 7) if which == "state" else (row, 0, 5) if which in "qk" else (row, h, 7) if which == "v" else (row, h)] = np.nan
+    up = {i: ctx.upload(y) for i, y in x.items()}
+    up.update(starts=ctx.upload(np.concatenate([[0], np.cumsum(news)]).astype(np.int32)), slots=ctx.upload(np.arange(n, dtype=np.int32)),
+              rate=ctx.upload(np.full(HV, -0.1, np.float32)), dt=ctx.upload(np.zeros(HV, np.float32)), out=ctx.upload(np.zeros((m, HV, D), np.float32)))
+    at = {i: int(u) for i, u in up.items()}
+    batch = qmm_hip.StateBatch(n, m, at["starts"], at["slots"], at["slots"], n, max(news))
+    args = qmm_hip.DeltaArgs(q=at["q"], k=at["k"], q_stride=HK * D, k_stride=HK * D, v=at["v"], v_stride=HV * D, qk_heads=HK, v_heads=HV, key_dim=D,
+                             value_dim=D, a=at["a"], b=at["b"], a_stride=HV, b_stride=HV, rate=at["rate"], dt_bias=at["dt"], scale=1.0, qk_eps=1e-6,
+                             state=at["state"], out=at["out"], out_stride=HV * D)
+    ws = ctx.gated_delta_workspace(batch, args)
+    ctx.gated_delta(batch, args, ws)
+    ctx.sync()
+    out, state = np.isnan(ctx.d2h(up["out"], np.float32, (m, HV, D))), np.isnan(ctx.d2h(up["state"], np.float32, (n, HV, D, D)))
+    ws.free()
+    for u in up.values():
+        ctx.free(u)
+    mine = [0, 1] if which in "qk" else [h]
+    rest = [i for i in range(HV) if i not in mine]
+    column = 7 if which in ("v", "state") else slice(None)
+    assert out[row, mine][:, column].all()
+    if which == "q":
+        assert not state.any() and not out[2:].any() and not out[0].any()
+    else:
+        assert state[0, mine][:, :, column].all()
+    assert not out[:, rest].any() and not state[:, rest].any() and not out[news[0]:].any() and not state[1:].any()

@@ -2,12 +2,16 @@
 without a device: rows and slots, sizes, every refusal (tests/state_caller.cpp);
 null contexts through the library; the oracles against other forms of the same."""
 import os
+import re
+import shutil
 import subprocess
 
 import numpy as np
+import pytest
 
 import qmm_hip
 import state_ref as R
+from test_resources import HIPCC, PKG, _resources
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 
@@ -69,3 +73,37 @@ def test_selection_is_the_sorted_vocabulary():
     t, p, y, _ = R.select(x, s, ended, 7, 30)
     assert [(int(b), int(j)) for b, j in zip(p, t)] == [(o[1], o[3]) for o in order]
     assert np.allclose(y, [-o[0] for o in order], rtol=1e-12)
+
+
+@pytest.mark.skipif(not shutil.which(HIPCC), reason="no hipcc")
+@pytest.mark.parametrize("source", ["qmm_delta.hip", "qmm_state.hip", "qmm_beam.hip"])
+def test_no_scratch(source):
+    """No kernel spills (the walk in halves 32 bytes of a lane, between its start and its loop over groups); a token at a time and
+    one group leave registers for two and more workgroups of a CU."""
+    kernels = _resources(source)
+    assert kernels
+    for name, (waves, scratch) in kernels.items():
+        assert scratch <= (32 if "delta_walk_kernelILi128ELi4ELb1" in name else 0), (name, scratch)
+        if "delta_step" in name or "delta_group" in name:
+            assert waves >= 4, (name, waves)
+
+
+@pytest.mark.skipif(not shutil.which(HIPCC), reason="no hipcc")
+def test_walk_keeps_its_loop_out_of_scratch(tmp_path):
+    flags = subprocess.run(["make", "-s", "-C", PKG, "print-flags"], capture_output=True, text=True, timeout=60, check=True).stdout
+    asm = tmp_path / "delta.s"
+    r = subprocess.run([HIPCC, *flags.split(), "--cuda-device-only", "-S", os.path.join(PKG, "csrc", "qmm_delta.hip"), "-o", str(asm)],
+                       capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+    name, depth, products = "", 0, 0
+    for line in asm.read_text().splitlines():
+        if re.match(r"_Z\S+:", line):
+            name, depth = line.split(":")[0], 0
+        elif line.startswith((".LBB", "; %bb.")):  # a block: the loops it is in follow as comments
+            depth = 0
+        if ";" in line:
+            depth = max([depth] + [int(d) for d in re.findall(r"Depth[= ]+(\d+)", line)])
+        code = line.split(";")[0]
+        products += "delta_walk" in name and depth >= 1 and "v_mfma" in code
+        assert not (depth >= 1 and "scratch_" in code), (name, line)
+    assert products >= 6 * 40
