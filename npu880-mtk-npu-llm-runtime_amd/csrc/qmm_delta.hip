@@ -359,17 +359,20 @@ __device__ inline void head_steps(const DeltaArgs &a, int row, int h, int m, boo
     G[m] = g;
     beta[m] = on ? step_size(a, row, h) : 0.0f;
 }
-// one of the six tiles of k k' (0..2) and q k' (3..5) on and below the diagonal, by a wave
-template <int DK> __device__ inline void tile_of(int task, int lane, const char *k, const char *q, Square &kk, Square &qk) {
+// one of the six tiles of k k' (0..2) and q k' (3..5) on and below the diagonal, by a wave; and its way to LDS
+template <int DK> __device__ inline f4 tile_of(int task, int lane, const char *k, const char *q) {
     constexpr int NU = DK / 32;
-    const int is_q = task / 3, ti = task % 3 != 0, tj = task % 3 == 2;
-    const int at = (lane / 16) * 256 + (lane % 16 ^ lane / 16) * 16;
+    const int ti = task % 3 != 0, tj = task % 3 == 2, at = (lane / 16) * 256 + (lane % 16 ^ lane / 16) * 16;
     f4 c{};
 #pragma unroll
-    for (int u = 0; u < NU; ++u) c = product(operand((is_q ? q : k) + (ti * NU + u) * 2 * kBlock + at), operand(k + (tj * NU + u) * 2 * kBlock + at), c);
-    Square &to = is_q ? qk : kk;
+    for (int u = 0; u < NU; ++u)
+        c = product(operand((task < 3 ? k : q) + (ti * NU + u) * 2 * kBlock + at), operand(k + (tj * NU + u) * 2 * kBlock + at), c);
+    return c * (task < 3 ? 0x1p-8f : 0x1p-18f);
+}
+__device__ inline void store_tile(int task, int lane, f4 c, Square &kk, Square &qk) {
+    Square &to = task < 3 ? kk : qk;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) to[16 * ti + 4 * (lane / 16) + r][16 * tj + lane % 16] = c[r] * (is_q ? 0x1p-18f : 0x1p-8f);
+    for (int r = 0; r < 4; ++r) to[16 * (task % 3 != 0) + 4 * (lane / 16) + r][16 * (task % 3 == 2) + lane % 16] = c[r];
 }
 // four values of a 32 x 32 matrix as operand: `place` is that of row and column (operand_at) in the row's tile
 __device__ inline void store_operand(char *matrix, int i, int place, f4 x) {
@@ -424,19 +427,19 @@ __device__ inline float factor_of(const double *G, const float *beta, int i) {
     return i < 64 ? power_of_two(i < 32 ? G[i] : G[31] - G[i - 32]) : beta[i - 64];
 }
 
-// T and P of one group and key head, for its value heads two at a time (both inverses in one wave). Bound: the chain of nine barriers at
-// three workgroups of a CU (44 KB of LDS): 8192 tokens of 16 key and 32 value heads 58 us, of which loads, conversion and products
-// 31, inverses 6, stores 4.
+// T and P of one group and key head, for its value heads two at a time (both inverses in one wave). Bound: the chain of ten barriers at
+// four workgroups of a CU (35 KB of LDS; with three, k k' and q k' beside the rows, 58 us): 8192 tokens of 16 key and 32 value
+// heads 53 us. Of 58, loads, conversion and products were 31, inverses 6, stores 4.
 template <int DK>
 __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, DeltaScratch w, int tiles) {
     constexpr int NU = DK / 32, NI = DK / 64;
-    constexpr int kRows = 2 * NU * 2 * kBlock, kTriangles = 4 * sizeof(Square);
-    __shared__ __attribute__((aligned(16))) char shared[2 * kRows > kTriangles ? 2 * kRows : kTriangles];
-    char *const rows = shared;  // k and q as operands; after their products A and T of two heads
+    constexpr int kRows = 2 * NU * 2 * kBlock, kSquares = 6 * sizeof(Square);
+    __shared__ __attribute__((aligned(16))) char shared[2 * kRows > kSquares ? 2 * kRows : kSquares];
+    char *const rows = shared;  // k and q as operands; after their products those, and A and T of two heads
     Square *const A = reinterpret_cast<Square *>(shared), *const T = A + 2;
+    Square &kk = A[4], &qk = A[5];
     __shared__ float sums[2][32][NU];
     __shared__ __attribute__((aligned(16))) float inv[2][32];
-    __shared__ __attribute__((aligned(16))) Square kk, qk;
     __shared__ double G[2][32];
     __shared__ float beta[2][32];
     const int t = threadIdx.x, lane = t & 63, wid = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -466,7 +469,12 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, DeltaSc
             it.store(rows + it.is_q * kRows, nullptr, hi, lo);
         }
         __syncthreads();
-        for (int task = wid; task < 6; task += 4) tile_of<DK>(task, lane, rows, rows + kRows, kk, qk);
+        const f4 first = tile_of<DK>(wid, lane, rows, rows + kRows);
+        f4 second{};
+        if (wid < 2) second = tile_of<DK>(wid + 4, lane, rows, rows + kRows);
+        __syncthreads();
+        store_tile(wid, lane, first, kk, qk);
+        if (wid < 2) store_tile(wid + 4, lane, second, kk, qk);
         __syncthreads();
         for (int h0 = 0; h0 < of; h0 += 2) {
             const int nh = min(2, of - h0);
@@ -868,7 +876,7 @@ __global__ __launch_bounds__(512, 4) void delta_group_kernel(DeltaArgs a) {
         }
         __syncthreads();
         if (n + 1 < n_groups) load_rows(t, n + 1);
-        if (wid < 6) tile_of<DK>(wid, lane, rows, rows + 2 * kRows, squares[0], squares[1]);
+        if (wid < 6) store_tile(wid, lane, tile_of<DK>(wid, lane, rows, rows + 2 * kRows), squares[0], squares[1]);
         __syncthreads();
         const int i = t / 8, c = t % 8 * 4;
         if (t < 256) store_operand(matrices + 4 * kBlock, i, operand_at(i, c), mask_and_decay(squares[0], squares[1], G, beta, i, c, squares[2]));
