@@ -1112,7 +1112,8 @@ template <int DK> hipError_t launch_groups(const DeltaArgs &a, const DeltaScratc
     // 8192 397 and 559.
     if (want >= kHalfGroups && lists <= kHalfLists && lists * ((2 * a.value_dim + DK) / 64) <= cu_count) {
         if ((e = launch_walk<DK, 4, true>(a, w, s)) != hipSuccess) return e;
-        const int turns = int((want + DK / 32 + 3) / 4);  // (each workgroup with about four items, for one reading of the state)
+        // (each workgroup with about four items, for one reading of the state; more than four past 2^31 threads)
+        const int turns = int(min((want + DK / 32 + 3) / 4, (int64_t(1) << 22) / lists));
         const dim3 grid(unsigned(lists) * unsigned(turns));
         if (a.value_dim == 64) hipLaunchKernelGGL((delta_join_kernel<DK, 64>), grid, dim3(512), 0, s, a, w, turns);
         else hipLaunchKernelGGL((delta_join_kernel<DK, 128>), grid, dim3(512), 0, s, a, w, turns);

@@ -245,3 +245,11 @@ def test_delta_no_number_shows(ctx, which, news):
     else:
         assert state[0, mine][:, :, column].all()
     assert not out[:, rest].any() and not state[:, rest].any() and not out[news[0]:].any() and not state[1:].any()
+
+
+@pytest.mark.parametrize("n", [2, 63, 64, 65, 130])
+def test_delta_many_sequences(ctx, n):
+    """Sequences in the order of their lengths, up to 64 of them; equal lengths and empty ones among them."""
+    rng = np.random.default_rng(n)
+    news = [int(x) for x in rng.choice([0, 1, 31, 33, 64, 65, 97], n - 1)] + [330]
+    delta_case(ctx, news, 1, 1, 64, 64, seed=n)

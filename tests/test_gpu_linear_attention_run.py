@@ -169,7 +169,8 @@ def test_decoding_with_beams(ctx, copies):
 OUT = ("seq", "att", "past", "S", "token", "parent", "total")
 
 
-@pytest.mark.parametrize("news,hint", [([1] * 6, 1), ([12, 16, 0, 9, 1, 16], 16), ([150, 0, 70, 33, 1, 40], 150)], ids=["tokens", "drafts", "prompts"])
+@pytest.mark.parametrize("news,hint", [([1] * 6, 1), ([12, 16, 0, 9, 1, 16], 16), ([150, 0, 70, 33, 1, 40], 150),
+                                       ([700, 0, 520, 33, 1, 40], 700)], ids=["tokens", "drafts", "prompts", "halves"])
 def test_captured_steps(news, hint):
     """All calls but the projections, captured once and replayed with other rows, lengths, slots and logits, and eager work
     between: the eager calls' bits each time."""
@@ -305,6 +306,28 @@ def test_spoilt_sequence(ctx, what, hint):
     for (a, b), keep in zip(zip(*got), (rows, rows, slots, slots)):
         assert np.array_equal(a[keep].view(np.uint32), b[keep].view(np.uint32))
         assert np.isfinite(a[keep]).all()
+    layer.free()
+
+
+@pytest.mark.parametrize("what", ["mix", "z", "ab", "S", "past"])
+def test_spoilt_sequence_of_halves(ctx, what):
+    """The same where sequences are walked in halves: the middle one's second half."""
+    news, m = [600, 700, 555], 1855
+    layer = Layer(ctx, m, 6, 1, 1, seed=69)
+    rng = np.random.default_rng(70)
+    fill = {n: rng.standard_normal(layer.shape[n]).astype(np.float32) for n in ("past", "S", "mix", "z", "ab")}
+    got = []
+    for bad in (False, True):
+        if bad:
+            fill[what][1 if what in ("S", "past") else slice(600 + 500, 600 + 503)] = np.nan
+        say(f"spoilt {what if bad else 'nothing'} in halves")
+        layer.put(row_start=[0, 600, 1300, 1855], slot_in=[0, 1, 2], slot_out=[3, 4, 5], **fill)
+        layer.attend(3, m, 700)
+        ctx.sync()
+        got.append(layer.get("seq", "att", "past", "S"))
+    rows, slots = np.r_[0:600, 1300:1855], [0, 2, 3, 5]
+    for (a, b), keep in zip(zip(*got), (rows, rows, slots, slots)):
+        assert np.array_equal(a[keep].view(np.uint32), b[keep].view(np.uint32)) and np.isfinite(a[keep]).all()
     layer.free()
 
 
