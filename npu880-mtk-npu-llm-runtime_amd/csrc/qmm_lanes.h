@@ -1,4 +1,4 @@
-// qmm_lanes.h — sums and maxima over lanes in the vector registers' own network; stores past the caches.
+// qmm_lanes.h — sums and maxima over lanes in the vector registers' own network; loads and stores past the caches.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -58,8 +58,12 @@ __device__ inline float silu(float y) {
     return y * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(y * -1.4426950408889634f));
 }
 
-// A store that leaves the caches to others: of large tensors that are read again only after as much else has passed
+// Loads and stores that leave the caches to others: of large tensors that are used again only after as much else has passed
 typedef float Four __attribute__((ext_vector_type(4)));
+template <typename T> __device__ inline T load_past(const T *p) {
+    static_assert(sizeof(T) == sizeof(Four));
+    return __builtin_bit_cast(T, __builtin_nontemporal_load(reinterpret_cast<const Four *>(p)));
+}
 template <typename T> __device__ inline void store_past(T *p, T x) {
     static_assert(sizeof(T) == sizeof(Four));
     __builtin_nontemporal_store(__builtin_bit_cast(Four, x), reinterpret_cast<Four *>(p));

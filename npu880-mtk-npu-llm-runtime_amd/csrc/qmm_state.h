@@ -30,9 +30,9 @@ QMM_HD inline StateSeq state_seq(const StateView &b, int s) {
     return v;
 }
 
-constexpr int kConvRows = 16;  // rows of one workgroup of the convolution
+constexpr int kConvRows = 8;  // rows of one workgroup of the convolution
 
-// The convolution's workgroups a sequence and 1024 channels: one per 16 rows as far as the host knows
+// The convolution's workgroups a sequence and 1024 channels: one per 8 rows as far as the host knows
 // (they take turns where there are more), below 2^24 in all.
 inline int conv_tiles(const StateView &b, int channels, int max_new) {
     const int64_t lists = int64_t(b.n_seqs) * ((channels + 1023) / 1024);

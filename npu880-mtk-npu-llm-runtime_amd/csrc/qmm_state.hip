@@ -3,10 +3,11 @@
 //
 //   y[t][c] = act(bias[c] + sum_i w[c][i] x[t - W + 1 + i][c]),  act(y) = y / (1 + exp(-y))
 //
-// Bound: memory; every input is read once (and W - 1 of 16 rows again, from L2)
-// and every output written once. 8192 channels: 16 sequences of a token 4.5 us (one launch); five prompts of 5581 75 us,
-// 4.9 TB/s. Stores past the caches take 59 us, but the delta rule then reads its inputs from memory: both together lose
-// (6 prompts of 800 tokens 264 us as it is, 272 so). 32 rows a workgroup measured the same (75 us).
+// Bound: memory; every input is read once (and W - 1 of 8 rows again, from the caches)
+// and every output written once. 8192 channels: 16 sequences of a token 4.5 us (one launch), five prompts of 5581 63 us, 5.8 TB/s.
+// Inputs of more than 32 MB are loaded past the caches, in which the outputs then lie for what reads them: 75 us without; 6
+// prompts of 800 tokens with the delta rule behind 237 us and 245. Outputs past them too are faster alone (59 us before
+// this) and slower together (272 us against 264). 16 rows a workgroup: 64 us, and 8 sequences of 16 tokens 1.5 us more.
 #include <hip/hip_runtime.h>
 
 #include "qmm_lanes.h"
@@ -19,10 +20,14 @@ __device__ inline float4 fma4(float4 w, float4 x, float4 y) {
     return make_float4(__builtin_fmaf(w.x, x.x, y.x), __builtin_fmaf(w.y, x.y, y.y), __builtin_fmaf(w.z, x.z, y.z),
                        __builtin_fmaf(w.w, x.w, y.w));
 }
-// A workgroup: 1024 channels (4 a thread) of 16 rows of a sequence. A thread keeps the last W - 1
+template <bool PAST> __device__ inline float4 load4(const float *p) {
+    if (PAST) return load_past(reinterpret_cast<const float4 *>(p));
+    return *reinterpret_cast<const float4 *>(p);
+}
+// A workgroup: 1024 channels (4 a thread) of 8 rows of a sequence. A thread keeps the last W - 1
 // inputs in registers. The first rows' workgroup alone reads and writes the carried inputs (a slot may be
 // both read and written), and it reads them before it writes.
-template <int W>
+template <int W, bool PAST>
 __global__ __launch_bounds__(256) void conv_kernel(ConvArgs a, int tiles, int chunks) {
     const int chunk = int(blockIdx.x % unsigned(chunks)), st = int(blockIdx.x / unsigned(chunks));
     const int s = st / tiles;
@@ -47,27 +52,24 @@ __global__ __launch_bounds__(256) void conv_kernel(ConvArgs a, int tiles, int ch
             if (tile > 0) last[i] = *reinterpret_cast<const float4 *>(x + size_t(p) * a.x_stride);
             else if (v.in >= 0) last[i] = *reinterpret_cast<const float4 *>(carried(v.in, i));
         }
+        float4 in[kConvRows];
 #pragma unroll
-        for (int half = 0; half < kConvRows; half += 8) {
-            float4 in[8];
+        for (int j = 0; j < kConvRows; ++j) {
+            in[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (t0 + j < t1) in[j] = load4<PAST>(x + size_t(t0 + j) * a.x_stride);
+        }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                in[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (t0 + half + j < t1) in[j] = *reinterpret_cast<const float4 *>(x + size_t(t0 + half + j) * a.x_stride);
-            }
+        for (int j = 0; j < kConvRows; ++j) {
+            if (t0 + j >= t1) break;
+            float4 y = bias;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                if (t0 + half + j >= t1) break;
-                float4 y = bias;
+            for (int i = 0; i < W - 1; ++i) y = fma4(w[i], last[i], y);
+            y = fma4(w[W - 1], in[j], y);
+            if (a.silu) y = make_float4(silu(y.x), silu(y.y), silu(y.z), silu(y.w));
+            *reinterpret_cast<float4 *>(out + size_t(t0 + j) * a.out_stride) = y;
 #pragma unroll
-                for (int i = 0; i < W - 1; ++i) y = fma4(w[i], last[i], y);
-                y = fma4(w[W - 1], in[j], y);
-                if (a.silu) y = make_float4(silu(y.x), silu(y.y), silu(y.z), silu(y.w));
-                *reinterpret_cast<float4 *>(out + size_t(t0 + half + j) * a.out_stride) = y;
-#pragma unroll
-                for (int i = 0; i + 1 < W - 1; ++i) last[i] = last[i + 1];
-                last[W - 2] = in[j];
-            }
+            for (int i = 0; i + 1 < W - 1; ++i) last[i] = last[i + 1];
+            last[W - 2] = in[j];
         }
         if (tile == 0 && v.out >= 0) {
             float4 left[W - 1];  // the inputs after the last row, all read before the first is written
@@ -116,9 +118,16 @@ __global__ __launch_bounds__(256) void copy_kernel(CopyArgs a) {
 hipError_t launch_conv(const ConvArgs &a, hipStream_t s) {
     const int chunks = (a.channels + 1023) / 1024, tiles = conv_tiles(a.b, a.channels, a.max_new);
     const dim3 grid(unsigned(a.b.n_seqs) * unsigned(tiles) * unsigned(chunks));
-    if (a.width == 2) hipLaunchKernelGGL(conv_kernel<2>, grid, dim3(256), 0, s, a, tiles, chunks);
-    else if (a.width == 3) hipLaunchKernelGGL(conv_kernel<3>, grid, dim3(256), 0, s, a, tiles, chunks);
-    else hipLaunchKernelGGL(conv_kernel<4>, grid, dim3(256), 0, s, a, tiles, chunks);
+    const bool past = size_t(a.b.n_rows) * size_t(a.channels) * 4 > (32u << 20);
+#define QMM_CONV(W) \
+    do { \
+        if (past) hipLaunchKernelGGL((conv_kernel<W, true>), grid, dim3(256), 0, s, a, tiles, chunks); \
+        else hipLaunchKernelGGL((conv_kernel<W, false>), grid, dim3(256), 0, s, a, tiles, chunks); \
+    } while (0)
+    if (a.width == 2) QMM_CONV(2);
+    else if (a.width == 3) QMM_CONV(3);
+    else QMM_CONV(4);
+#undef QMM_CONV
     return hipGetLastError();
 }
 
