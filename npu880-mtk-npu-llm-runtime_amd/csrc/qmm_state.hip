@@ -4,10 +4,10 @@
 //   y[t][c] = act(bias[c] + sum_i w[c][i] x[t - W + 1 + i][c]),  act(y) = y / (1 + exp(-y))
 //
 // Bound: memory; every input is read once (and W - 1 of 8 rows again, from the caches)
-// and every output written once. 8192 channels: 16 sequences of a token 4.5 us (one launch), five prompts of 5581 63 us, 5.8 TB/s.
-// Inputs of more than 32 MB are loaded past the caches, in which the outputs then lie for what reads them: 75 us without; 6
-// prompts of 800 tokens with the delta rule behind 237 us and 245. Outputs past them too are faster alone (59 us before
-// this) and slower together (272 us against 264). 16 rows a workgroup: 64 us, and 8 sequences of 16 tokens 1.5 us more.
+// and every output written once. 8192 channels: 16 sequences of a token 4.5 us (one launch), five prompts of 5581 73.5 us, 5.0 TB/s.
+// Inputs of more than 32 MB are loaded past the caches, in which the outputs then lie for what reads them: 6 prompts of 800 tokens
+// with the delta rule behind 237 us, 245 without. Outputs past them too are faster alone (64.5 us) and slower together (241).
+// With 16 rows a workgroup 78.5 us, with 4 80.
 #include <hip/hip_runtime.h>
 
 #include "qmm_lanes.h"
