@@ -58,7 +58,7 @@ template <int DV, typename F> __device__ inline void write_rows(const DeltaArgs 
 // registers; a lane has rows 4 (rl + RL g) .. + 3. Both products with S are taken
 // before it changes: S' q after the step is e^g S' q + (k.q) d, so one pass and one
 // sum over the lanes serve both, and no wave waits for another between tokens. 32 heads: one sequence of a token 5.6 us (a launch and one
-// way through memory), 64 sequences 50.9 us (5.4 TB/s of 273 MB); another token adds 0.8 us.
+// way through memory), 64 sequences 49.2 us (5.5 TB/s of 273 MB); another token adds 0.8 us.
 template <int DK, int DV>
 __global__ __launch_bounds__(256, 4) void delta_step_kernel(DeltaArgs a) {
     constexpr int CL = DV / 16, RL = 64 / CL, NG = DK / (4 * RL), NV = (kGroup * DV + 1023) / 1024, HL = 32;  // HL: lanes that hold one row of q or k
@@ -73,7 +73,7 @@ __global__ __launch_bounds__(256, 4) void delta_step_kernel(DeltaArgs a) {
     const int sub = lane % HL, is_k = lane / HL;
     const size_t pool = size_t(a.v_heads) * DK * DV;
     // Four workgroups of a CU: places are worked out again for every use, and k is read from LDS twice (kept over the tokens they take
-    // the registers of the fourth; 64 sequences of a token 57 us with three, 51 with four).
+    // the registers of the fourth, and of 32 sequences 29 us become 23).
     auto now = [](int x) {
         asm("" : "+v"(x));
         return x;
@@ -99,13 +99,16 @@ __global__ __launch_bounds__(256, 4) void delta_step_kernel(DeltaArgs a) {
         }
     };
     if (v.n > 0) load(0, t);
+    // States of more than 32 MB in all are read and written past the caches: 64 sequences 49.2 us, 51 with the stores alone, 57 without
+    const bool past = size_t(gridDim.x) * (DK * DV * 4) > (32u << 20);
     float4 S[NG][4];
 #pragma unroll
     for (int g = 0; g < NG; ++g)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
+            const float4 *p = reinterpret_cast<const float4 *>(state(v.in, lane) + size_t(4 * RL * g + j) * DV);
             S[g][j] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (v.in >= 0) S[g][j] = load4(state(v.in, lane) + size_t(4 * RL * g + j) * DV);
+            if (v.in >= 0) S[g][j] = past ? load_past(p) : *p;
         }
     for (int t0 = 0; t0 < v.n; t0 += kGroup) {
         const int nt = min(kGroup, v.n - t0);
@@ -174,7 +177,6 @@ __global__ __launch_bounds__(256, 4) void delta_step_kernel(DeltaArgs a) {
     }
     if (v.out >= 0) {
         float *to = state(v.out, now(lane) & 63);
-        const bool past = size_t(gridDim.x) * (DK * DV * 4) > (32u << 20);
 #pragma unroll
         for (int g = 0; g < NG; ++g)
 #pragma unroll
@@ -1130,8 +1132,8 @@ template <int DK> hipError_t launch_groups(const DeltaArgs &a, const DeltaScratc
 }  // namespace
 
 hipError_t launch_delta(const DeltaArgs &a, void *scratch, size_t scratch_bytes, int cu_count, hipStream_t s) {
-    // A token at a time (T tokens) or one group of 32, of 1, 8 and 32 sequences of 32 heads: T = 4 7.7, 10.8, 28.6 us;
-    // T = 8 10.7, 14.8, 35.5; T = 12 14.9, 19.6, 44; a group 11.4 to 12, 15.2 to 17, 40 to 47.
+    // A token at a time (T tokens) or one group of 32, of 1, 8 and 32 sequences of 32 heads: T = 4 8.2, 11.2, 22.3 us;
+    // T = 8 11.6, 15.3, 31.0; T = 12 14.9, 19.6, 44; a group 10.9 to 11.5, 15.0 to 16.5, 40 to 46.
     const size_t widest = max(max(a.q_stride, a.k_stride), max(a.v_stride, a.out_stride));
     const int64_t lists = int64_t(a.b.n_seqs) * a.v_heads;
     const bool grouped = a.max_new > kStepRows && widest < (1 << 24) && lists < (1 << 20);  // (32 rows in 32 bits of bytes; threads)
