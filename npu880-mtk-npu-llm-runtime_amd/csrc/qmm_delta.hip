@@ -57,10 +57,14 @@ template <int DV, typename F> __device__ inline void write_rows(const DeltaArgs 
 // sequence and head, a wave 16 * CL / 4 columns (4 a lane) of all rows, in
 // registers; a lane has rows 4 (rl + RL g) .. + 3. Both products with S are taken
 // before it changes: S' q after the step is e^g S' q + (k.q) d, so one pass and one
-// sum over the lanes serve both, and no wave waits for another between tokens. 32 heads: one sequence of a token 5.6 us (a launch and one
-// way through memory), 64 sequences 49.2 us (5.5 TB/s of 273 MB); another token adds 0.8 us.
-template <int DK, int DV>
-__global__ __launch_bounds__(256, 4) void delta_step_kernel(DeltaArgs a) {
+// sum over the lanes serve both, and no wave waits for another between tokens. 32 heads: one sequence of a token 5.5 us (a launch and one
+// way through memory), 64 sequences 49.2 us (5.5 TB/s of 273 MB); another token adds 0.75 us.
+//
+// MANY: more workgroups than three a CU. Then four: places are worked out again for every use, and k is read from LDS twice (kept over
+// the tokens they take the registers of the fourth), and states of more than 32 MB in all go past the caches: 32 sequences of 4 tokens
+// 29 us become 22, 64 of one 57 become 49. For fewer that only costs: one sequence of 8 tokens 10.7 us, so 11.6.
+template <int DK, int DV, bool MANY>
+__global__ __launch_bounds__(256, MANY ? 4 : 3) void delta_step_kernel(DeltaArgs a) {
     constexpr int CL = DV / 16, RL = 64 / CL, NG = DK / (4 * RL), NV = (kGroup * DV + 1023) / 1024, HL = 32;  // HL: lanes that hold one row of q or k
     __shared__ float qk[kGroup][2][DK];
     __shared__ float vo[kGroup][DV];  // values, then outputs
@@ -72,10 +76,8 @@ __global__ __launch_bounds__(256, 4) void delta_step_kernel(DeltaArgs a) {
     const int cl = lane % CL, rl = lane / CL, col = wid * (DV / 4) + 4 * cl;
     const int sub = lane % HL, is_k = lane / HL;
     const size_t pool = size_t(a.v_heads) * DK * DV;
-    // Four workgroups of a CU: places are worked out again for every use, and k is read from LDS twice (kept over the tokens they take
-    // the registers of the fourth, and of 32 sequences 29 us become 23).
     auto now = [](int x) {
-        asm("" : "+v"(x));
+        if (MANY) asm("" : "+v"(x));
         return x;
     };
     auto state = [&](int slot, int at) { return a.state + size_t(slot) * pool + size_t(h) * DK * DV + size_t(4 * (at / CL)) * DV + wid * (DV / 4) + 4 * (at % CL); };
@@ -99,8 +101,7 @@ __global__ __launch_bounds__(256, 4) void delta_step_kernel(DeltaArgs a) {
         }
     };
     if (v.n > 0) load(0, t);
-    // States of more than 32 MB in all are read and written past the caches: 64 sequences 49.2 us, 51 with the stores alone, 57 without
-    const bool past = size_t(gridDim.x) * (DK * DV * 4) > (32u << 20);
+    const bool past = MANY && size_t(gridDim.x) * (DK * DV * 4) > (32u << 20);
     float4 S[NG][4];
 #pragma unroll
     for (int g = 0; g < NG; ++g)
@@ -134,10 +135,12 @@ __global__ __launch_bounds__(256, 4) void delta_step_kernel(DeltaArgs a) {
         for (int m = 0; m < nt; ++m) {
             const float decay = sc[m][0], beta = sc[m][1], kq = sc[m][2];
             const float4 val = load4(&vo[m][col]);
+            float4 kept[NG];
             float ks[4] = {}, qs[4] = {};
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 const float4 kr = load4(&qk[m][1][4 * (rl + RL * g)]);
+                kept[g] = kr;
                 const float4 qr = load4(&qk[m][0][4 * (rl + RL * g)]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -160,7 +163,7 @@ __global__ __launch_bounds__(256, 4) void delta_step_kernel(DeltaArgs a) {
             const int again = now(m);
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                const float4 kr = load4(&qk[again][1][4 * (rl + RL * g)]);
+                const float4 kr = MANY ? load4(&qk[again][1][4 * (rl + RL * g)]) : kept[g];
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -1132,8 +1135,8 @@ template <int DK> hipError_t launch_groups(const DeltaArgs &a, const DeltaScratc
 }  // namespace
 
 hipError_t launch_delta(const DeltaArgs &a, void *scratch, size_t scratch_bytes, int cu_count, hipStream_t s) {
-    // A token at a time (T tokens) or one group of 32, of 1, 8 and 32 sequences of 32 heads: T = 4 8.2, 11.2, 22.3 us;
-    // T = 8 11.6, 15.3, 31.0; T = 12 14.9, 19.6, 44; a group 10.9 to 11.5, 15.0 to 16.5, 40 to 46.
+    // A token at a time (T tokens) or one group of 32, of 1, 8 and 32 sequences of 32 heads: T = 4 7.8, 10.8, 22.3 us;
+    // T = 8 10.8, 14.8, 31.0; T = 12 14.9, 19.6, 44; a group 10.9 to 11.5, 15.0 to 16.5, 40 to 46.
     const size_t widest = max(max(a.q_stride, a.k_stride), max(a.v_stride, a.out_stride));
     const int64_t lists = int64_t(a.b.n_seqs) * a.v_heads;
     const bool grouped = a.max_new > kStepRows && widest < (1 << 24) && lists < (1 << 20);  // (32 rows in 32 bits of bytes; threads)
@@ -1159,7 +1162,8 @@ hipError_t launch_delta(const DeltaArgs &a, void *scratch, size_t scratch_bytes,
 #define QMM_STEP(K, V) \
     do { \
         if (grouped) hipLaunchKernelGGL((delta_group_kernel<K, V>), grid, dim3(512), 0, s, a); \
-        else hipLaunchKernelGGL((delta_step_kernel<K, V>), grid, dim3(256), 0, s, a); \
+        else if (lists > 3 * int64_t(cu_count)) hipLaunchKernelGGL((delta_step_kernel<K, V, true>), grid, dim3(256), 0, s, a); \
+        else hipLaunchKernelGGL((delta_step_kernel<K, V, false>), grid, dim3(256), 0, s, a); \
     } while (0)
     if (a.key_dim == 128) {
         if (a.value_dim == 128) QMM_STEP(128, 128);

@@ -253,3 +253,13 @@ def test_delta_many_sequences(ctx, n):
     rng = np.random.default_rng(n)
     news = [int(x) for x in rng.choice([0, 1, 31, 33, 64, 65, 97], n - 1)] + [330]
     delta_case(ctx, news, 1, 1, 64, 64, seed=n)
+
+
+@pytest.mark.parametrize("hint", [True, 1])
+@pytest.mark.parametrize("DK,DV", [(64, 64), (64, 128), (128, 64), (128, 128)])
+def test_delta_large_batches(ctx, DK, DV, hint):
+    """More workgroups than three a CU, with states of more than 32 MB in all and less; some read no state, some keep none."""
+    rng = np.random.default_rng(DK + 2 * DV)
+    news = [int(n) for n in rng.integers(0, 9 if hint is True else 3, 270)] + ([] if hint is True else [19, 1])
+    slots = [(i if i % 5 else -1, i if i % 7 else -1) for i in range(len(news))]
+    delta_case(ctx, news, 1, 3, DK, DV, slots=slots, hints=hint, seed=DV)
