@@ -835,7 +835,10 @@ __global__ __launch_bounds__(512, 4) void delta_group_kernel(DeltaArgs a) {
     __shared__ double G[32];
     __shared__ float beta[32];
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int s = int(blockIdx.x / unsigned(a.v_heads)), h = int(blockIdx.x % unsigned(a.v_heads));
+    // (24 and 32 sequences of 9 to 192 tokens 100 and 125 us in their order, 75 and 112 longest first; of up to 64 tokens 47 and 44 but 56
+    // and 58, 64 sequences 112 and 122: no order for up to three groups)
+    const int number = int(blockIdx.x / unsigned(a.v_heads)), h = int(blockIdx.x % unsigned(a.v_heads));
+    const int s = a.max_new > 3 * kChunk ? by_length(a.b, number) : number;
     const int hk = h / (a.v_heads / a.qk_heads);
     const StateSeq v = state_seq(a.b, s);
     const int col = wid * 16 + threadIdx.x % 16;
