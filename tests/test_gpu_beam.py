@@ -169,3 +169,16 @@ def test_copies_of_pools_of_several_sizes(ctx):
             assert np.array_equal(ctx.d2h(b, np.uint8, p.shape), p)
     for u in [*bufs, sb, db]:
         ctx.free(u)
+
+
+@pytest.mark.parametrize("V,gap", [(5003, 0), (5001, 0), (5002, 1), (9002, 0), (50257, 0), (2047, 0), (3, 0)])
+def test_beams_alike_at_any_alignment(ctx, V, gap):
+    """Rows of the same bits at the four places that a row may have in 16 B: the same totals, bit for bit, so the lower beam first."""
+    one = _logits(1, V, V)
+    K = min(10, 5 * V)
+    t, p, total = beam_case(ctx, np.repeat(one, 10, 0), None, None, K, 5, gap)
+    assert np.array_equal(p, np.tile(np.arange(5), (2, 2))[:, :K]) and np.array_equal(t[0], t[1])
+    assert len({x.tobytes() for x in total.reshape(-1, 5)}) == K // 5
+    for offset in (1, 2, 3):  # the same item elsewhere
+        again = beam_case(ctx, np.repeat(one, 10, 0), None, None, K, 5, gap, offset)
+        assert all(x.tobytes() == y.tobytes() for x, y in zip(again, (t, p, total)))
