@@ -547,7 +547,7 @@ typedef struct {
     size_t stride;        /* >= vocab; any */
     int vocab;            /* below 2^30 */
     int n_items;
-    int n_beams;          /* 1..64; n_items * n_beams below 2^20 */
+    int n_beams;          /* 1..64; n_items * n_beams below 2^20, times vocab / 2048 below 2^26 */
     const float *score;   /* device [n_items * n_beams], or NULL: zeros */
     const int32_t *ended; /* device [n_items * n_beams], nonzero where ended; or NULL */
     int end_token;        /* with ended: 0..vocab - 1 */

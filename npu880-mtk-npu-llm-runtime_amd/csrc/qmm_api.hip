@@ -1143,7 +1143,6 @@ int qmm_beam_select(qmm_context *ctx, const qmm_beam_args *t, qmm_attn_workspace
     const int64_t rows = int64_t(t->n_items) * t->n_beams;
     if (!ws || ws->bytes < qmm::beam_scratch_bytes(rows, t->vocab, t->n_keep))
         return fail(ctx, QMM_ENOMEM, "no workspace, or one below qmm_beam_workspace_bytes");
-    if (rows * qmm::beam_slices(t->vocab) >= (int64_t(1) << 26)) return fail(ctx, QMM_ESHAPE, "too many logits for one launch");
     qmm::BeamArgs a{};
     a.logits = t->logits;
     a.score = t->score;

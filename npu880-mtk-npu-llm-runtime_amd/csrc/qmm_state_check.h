@@ -5,6 +5,7 @@
 #pragma once
 
 #include "qmm_attn_check.h"
+#include "qmm_state.h"
 
 namespace qmm {
 
@@ -75,6 +76,8 @@ inline Refusal check_beam(const qmm_beam_args *t) {
     if (t->vocab <= 0 || t->vocab >= (1 << 30)) return {QMM_EINVAL, "vocab must be 1..2^30 - 1"};
     if (t->n_items < 0 || t->n_beams < 1 || t->n_beams > kMaxBeams) return {QMM_EINVAL, "n_beams must be 1..64, n_items not negative"};
     if (int64_t(t->n_items) * t->n_beams >= (int64_t(1) << 20)) return {QMM_ESHAPE, "n_items * n_beams must stay below 2^20"};
+    if (int64_t(t->n_items) * t->n_beams * beam_slices(t->vocab) >= (int64_t(1) << 26))
+        return {QMM_ESHAPE, "n_items * n_beams * vocab / 2048 must stay below 2^26"};
     if (t->n_keep < 1 || t->n_keep > kMaxKeep || t->n_keep > int64_t(t->n_beams) * t->vocab)
         return {QMM_EINVAL, "n_keep must be 1..64, at most n_beams * vocab"};
     if (t->stride < size_t(t->vocab)) return {QMM_EINVAL, "row stride below vocab"};

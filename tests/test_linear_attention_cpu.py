@@ -107,3 +107,13 @@ def test_walk_keeps_its_loop_out_of_scratch(tmp_path):
         products += "delta_walk" in name and depth >= 1 and "v_mfma" in code
         assert not (depth >= 1 and "scratch_" in code), (name, line)
     assert products >= 6 * 40
+
+
+def test_limits_and_workspaces(tmp_path):
+    """tests/state_limits.cpp"""
+    exe = str(tmp_path / "state_limits")
+    r = subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-fsanitize=undefined", "-fno-sanitize-recover=all",
+                        os.path.join(HERE, "state_limits.cpp"), "-o", exe], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stderr
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and r.stdout.strip() == "ok", (r.stdout + r.stderr)[-2000:]
