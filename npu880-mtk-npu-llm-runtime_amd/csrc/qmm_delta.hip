@@ -1016,13 +1016,15 @@ __global__ __launch_bounds__(256) void delta_norm_kernel(DeltaArgs a, int tiles)
 
 // What a first half left goes to the second half's tokens and last state: O + scale R S and E + M S, with S the state in the middle, R what
 // the tokens read of the unit vectors, O and E what the values gave; 32 rows at a time. Then, and for all other rows, norm and
-// gate. R and M are at most 1 in size and kept 2^14 times, S with a scale for each column, as above. Bound: memory (8192 tokens of 32 heads
-// 100 us, 4.7 TB/s).
+// gate. S has a scale for each column, as above, and R and M one for each row, from what it sums to: they fall with the decays of the
+// second half, far below 1, and what is left of the state in the middle is to keep its bits. Bound: memory (8192 tokens of 32 heads
+// 100 us, 4.7 TB/s; with scales summed over waves, through LDS and one more barrier, 117).
 template <int DK, int DV>
 __global__ __launch_bounds__(512, 4) void delta_join_kernel(DeltaArgs a, DeltaScratch w, int tiles) {
     constexpr int NU = DK / 32;
     __shared__ __attribute__((aligned(16))) char rows[2 * NU * 2 * kBlock];
     __shared__ __attribute__((aligned(16))) float sum[32][DV + 4];
+    __shared__ float shrink[32];  // what undoes the rows' scales
     const int t = threadIdx.x, lane = t & 63, wid = __builtin_amdgcn_readfirstlane(t >> 6);
     const int h = int(blockIdx.x % unsigned(a.v_heads)), st = int(blockIdx.x / unsigned(a.v_heads)), s = st / tiles;
     const StateSeq v = state_seq(a.b, s);
@@ -1055,19 +1057,29 @@ __global__ __launch_bounds__(512, 4) void delta_join_kernel(DeltaArgs a, DeltaSc
             continue;
         }
         const bool state = i >= n_groups;
-        if (t < 8 * DK / 4) {
-            const Item<DK> it(t, 0);
-            const size_t stride = state ? DK : read_stride;
-            const float *from = state ? w.carry + list * DK * DK + size_t(i - n_groups) * 32 * DK
-                                      : w.reads + (size_t(v.r0) / 2 + size_t(i - middle) * kChunk) * read_stride + size_t(h) * DK;
-            h4 hi[4], lo[4];
+        // DK / 4 lanes a row, so that its scale needs no exchange between waves
+        const size_t stride = state ? DK : read_stride;
+        const float *from = state ? w.carry + list * DK * DK + size_t(i - n_groups) * 32 * DK
+                                  : w.reads + (size_t(v.r0) / 2 + size_t(i - middle) * kChunk) * read_stride + size_t(h) * DK;
+        constexpr int kLanes = DK / 4, kTurns = 32 * kLanes / 512;
+        const int at = t % kLanes * 4, row = t / kLanes;
+        f4 x[kTurns];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                f4 x = {0.f, 0.f, 0.f, 0.f};
-                if (state || it.token + j < left) x = *reinterpret_cast<const f4 *>(from + size_t(it.token + j) * stride + it.at);
-                split4(x, 0x1p14f, hi[j], lo[j]);
-            }
-            it.store(rows, nullptr, hi, lo);
+        for (int j = 0; j < kTurns; ++j) {
+            const int m = row + j * (512 / kLanes);
+            x[j] = f4{0.f, 0.f, 0.f, 0.f};
+            if (state || m < left) x[j] = *reinterpret_cast<const f4 *>(from + size_t(m) * stride + at);
+        }
+#pragma unroll
+        for (int j = 0; j < kTurns; ++j) {
+            const int m = row + j * (512 / kLanes);
+            const int e = scale_for(lanes_sum<kLanes>((fabsf(x[j][0]) + fabsf(x[j][1])) + (fabsf(x[j][2]) + fabsf(x[j][3]))));
+            if (at == 0) shrink[m] = two_to(-e);
+            h4 hi, lo;
+            split4(x[j], two_to(e), hi, lo);
+            char *p = rows + (m / 16 * NU + at / 32) * 2 * kBlock + operand_at(m, at % 32);
+            *reinterpret_cast<h4 *>(p) = hi;
+            *reinterpret_cast<h4 *>(p + kBlock) = lo;
         }
         __syncthreads();
         if (multiplies) {
@@ -1079,11 +1091,11 @@ __global__ __launch_bounds__(512, 4) void delta_join_kernel(DeltaArgs a, DeltaSc
                 for (int ti = 0; ti < 2; ++ti) op[ti] = operand(rows + (ti * NU + u) * 2 * kBlock + lane_at);
                 products(op, b[u], c);
             }
-            const float f = (state ? 1.0f : a.scale) * two_to(-(scale + 14));
+            const float f = (state ? 1.0f : a.scale) * two_to(-scale);
 #pragma unroll
             for (int ti = 0; ti < 2; ++ti)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) sum[16 * ti + 4 * g + r][col] = c[ti][r] * f;
+                for (int r = 0; r < 4; ++r) sum[16 * ti + 4 * g + r][col] = c[ti][r] * f * shrink[16 * ti + 4 * g + r];
         }
         __syncthreads();
         auto plus = [](float4 x, float4 y) { return make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w); };

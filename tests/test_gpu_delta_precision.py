@@ -1,0 +1,119 @@
+"""How many bits the delta rule keeps where a column's values or its state change their size: states that decay over the second
+half of a prompt, small values after large ones, values of any size. The rule in 64 bits; errors are compared with the size that the
+results have there, not with the largest that ever was."""
+import numpy as np
+import pytest
+
+import qmm_hip
+import state_ref as R
+from gpu_util import say
+
+pytestmark = pytest.mark.gpu
+
+
+def run(ctx, news, x, rate, state, ws=True, hint=None, gamma=None, eps=1e-6):
+    """One call on rows x = {q, k, v, a, b} ([rows][heads][..]; scale 1, no bias of the steps), states in place: (rows, states)."""
+    m, HK, DK = x["q"].shape
+    HV, DV = x["v"].shape[1:]
+    n = len(news)
+    up = {i: ctx.upload(np.ascontiguousarray(y, np.float32)) for i, y in x.items()}
+    up.update(starts=ctx.upload(np.concatenate([[0], np.cumsum(news)]).astype(np.int32)), slots=ctx.upload(np.arange(n, dtype=np.int32)),
+              rate=ctx.upload(np.asarray(rate, np.float32)), dt=ctx.upload(np.zeros(HV, np.float32)),
+              out=ctx.upload(np.zeros((m, HV, DV), np.float32)), state=ctx.upload(np.asarray(state, np.float32)))
+    if gamma is not None:
+        up["gamma"] = ctx.upload(np.asarray(gamma, np.float32))
+    at = {i: int(u) for i, u in up.items()}
+    batch = qmm_hip.StateBatch(n, m, at["starts"], at["slots"], at["slots"], n, max(news) if hint is None else hint)
+    args = qmm_hip.DeltaArgs(q=at["q"], k=at["k"], q_stride=HK * DK, k_stride=HK * DK, v=at["v"], v_stride=HV * DV, qk_heads=HK, v_heads=HV,
+                             key_dim=DK, value_dim=DV, a=at["a"], b=at["b"], a_stride=HV, b_stride=HV, rate=at["rate"], dt_bias=at["dt"],
+                             scale=1.0, qk_eps=eps, state=at["state"], gamma=at.get("gamma"), gamma_eps=0.0, out=at["out"],
+                             out_stride=HV * DV)
+    w = ctx.gated_delta_workspace(batch, args) if ws else None
+    ctx.gated_delta(batch, args, w)
+    ctx.sync()
+    got = ctx.d2h(up["out"], np.float32, (m, HV, DV)), ctx.d2h(up["state"], np.float32, state.shape)
+    if w:
+        w.free()
+    for u in up.values():
+        ctx.free(u)
+    return got
+
+
+def exact(news, x, rate, state, gamma=None, eps=1e-6):
+    """The same in 64 bits; and what the state's columns' lengths were after every token [rows][heads][DV]."""
+    x = {i: np.asarray(y, np.float32).astype(np.float64) for i, y in x.items()}
+    of = x["v"].shape[1] // x["q"].shape[1]
+    unit = lambda y: np.repeat(y / np.sqrt((y * y).sum(-1, keepdims=True) + np.float64(np.float32(eps))), of, 1)  # noqa: E731
+    q, k = unit(x["q"]), unit(x["k"])
+    decay = np.exp(np.asarray(rate, np.float32).astype(np.float64) * np.log1p(np.exp(x["a"])))
+    beta = 1 / (1 + np.exp(-x["b"]))
+    S, r = np.asarray(state, np.float32).astype(np.float64), 0
+    out, size = np.zeros(x["v"].shape), np.zeros(x["v"].shape)
+    for s, n in enumerate(news):
+        for r in range(r, r + n):
+            S[s] *= decay[r][:, None, None]
+            S[s] += k[r][:, :, None] * (beta[r][:, None] * (x["v"][r] - (S[s] * k[r][:, :, None]).sum(1)))[:, None]
+            out[r] = (S[s] * q[r][:, :, None]).sum(1)
+            size[r] = np.sqrt((S[s] ** 2).sum(1))
+        r += 1
+    if gamma is not None:
+        out = out / np.sqrt((out ** 2).mean(-1, keepdims=True)) * np.asarray(gamma, np.float32)
+    return out, S, size
+
+
+def rows(m, HK, of, DK, DV, seed):
+    g = np.random.default_rng(seed)
+    return {"q": g.standard_normal((m, HK, DK)), "k": g.standard_normal((m, HK, DK)), "v": g.standard_normal((m, HK * of, DV)),
+            "a": g.standard_normal((m, HK * of)), "b": g.standard_normal((m, HK * of))}, g
+
+
+def rms(x, axis=None):
+    return np.sqrt(np.mean(np.square(x), axis))
+
+
+def mean_error(n):
+    """A bound of the rms error of n tokens' steps, relative to the state: a step has six operands (k twice, S, T, the values, D) that are
+    2^-22 off or less, and sums in fp32, two more; roundings of either sign, so the steps' errors add as squares."""
+    return 8 * 2.0 ** -22 * np.sqrt(n)
+
+
+WAYS = {"halves": dict(), "walk": dict(beside=3), "one launch": dict(ws=False), "tokens": dict(hint=1)}
+
+
+def on_way(ctx, way, news, x, rate, state, **kw):
+    """The call on one of its ways. `beside`: short sequences that take the halves from the long one (there are then too many heads)."""
+    how = dict(WAYS[way])
+    n, m = how.pop("beside", 0), sum(news)
+    if n:
+        HV = x["v"].shape[1]
+        n = 64 // HV + 1
+        x = {i: np.concatenate([y, np.ones((n, *y.shape[1:]))]) for i, y in x.items()}
+        state = np.concatenate([state, np.zeros((n, *state.shape[1:]))])
+    got = run(ctx, news + [1] * n, x, rate, state, **how, **kw)
+    return got[0][:m], got[1][:len(news)]
+
+
+@pytest.mark.parametrize("way", WAYS)
+@pytest.mark.parametrize("gamma", [False, True])
+@pytest.mark.parametrize("lost", [10, 20, 25, 30])
+@pytest.mark.parametrize("DK,DV", [(64, 128), (128, 128), (128, 64)])
+def test_state_decays_over_the_second_half(ctx, DK, DV, lost, gamma, way):
+    """A large state in the middle of a prompt, forgotten by e^-lost to its end, and next to nothing added: what is left of it keeps its
+    bits, in rows and in the state."""
+    say(f"delta precision: decays DK={DK} DV={DV} lost={lost} gamma={gamma} way={way}")
+    n = 640
+    x, g = rows(n, 1, 2, DK, DV, DK + lost)
+    x["a"][:n // 2] = -40.0  # no decay
+    x["a"][n // 2:] = 0.0
+    x["v"][n // 2:] *= 1e-30
+    x["b"] -= 3.0  # (small steps: the first state is there to the end)
+    rate = np.full(2, -lost / (n / 2) / np.log(2.0))
+    state = 300.0 * g.standard_normal((1, 2, DK, DV))
+    w = g.uniform(0.5, 1.5, DV) if gamma else None
+    out, after = on_way(ctx, way, [n], x, rate, state, gamma=w)
+    ref, ref_after, _ = exact([n], x, rate, state, w)
+    for part in (slice(0, n // 2), slice(n // 2, 500), slice(500, 600), slice(600, n)):
+        off = rms((out[part] - ref[part]) / rms(ref[part], -1)[..., None])
+        assert off <= mean_error(n), (part, off, mean_error(n))
+    off = rms((after - ref_after) / rms(ref_after, (2, 3))[..., None, None])
+    assert off <= mean_error(n), (off, mean_error(n))
