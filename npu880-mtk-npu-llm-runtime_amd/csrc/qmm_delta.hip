@@ -506,9 +506,13 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, DeltaSc
 }
 
 __device__ inline float two_to(int e) { return __uint_as_float(uint32_t(e + 127) << 23); }
-// the power of two that takes numbers up to `bound` below 2^15; within 2^-60 .. 2^60, so that two of them
-// have a quotient in fp32 (columns below 2^-46 lose bits under 2^-85)
-__device__ inline int scale_for(float bound) { return min(max(141 - int(__float_as_uint(bound) >> 23 & 255), -60), 60); }
+// The power of two that takes numbers up to `bound` below 2^15, from 2^-32 (2^30 rows of values below 65520 sum to less than 2^46) to
+// 2^94, so that two of them have a quotient in fp32. Columns that sum to less than 2^-80 lose the bits below 2^-119. It is kept less 30:
+// its largest is then 64, the largest constant of an instruction (8192 tokens of 8 heads otherwise 268 us, so 263).
+constexpr int kScale = 30;
+__device__ inline int scale_for(float bound) { return min(max(141 - kScale - int(__float_as_uint(bound) >> 23 & 255), -32 - kScale), 94 - kScale); }
+__device__ inline float grown(int scale) { return two_to(scale + kScale); }
+__device__ inline float shrunk(int scale, int more = 0) { return two_to(-(scale + kScale + more)); }
 __device__ inline float over_groups(float x) {  // sum over the four lanes of a column
     auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     x = __uint_as_float(p[0]) + __uint_as_float(p[1]);
@@ -696,9 +700,9 @@ __global__ __launch_bounds__(512) void delta_walk_kernel(DeltaArgs a, DeltaScrat
 #pragma unroll
         for (int r = 0; r < 4; ++r) bound += fabsf(S[k][r]);
     bound = over_groups(bound);
-    int scale = scale_for(bound + sum);  // S is kept times 2^scale
+    int scale = scale_for(bound + sum);  // S is kept times grown(scale)
 #pragma unroll
-    for (int k = 0; k < 2 * NU; ++k) S[k] *= two_to(scale);
+    for (int k = 0; k < 2 * NU; ++k) S[k] *= grown(scale);
     __syncthreads();
     int n = 0;
     do {
@@ -738,11 +742,11 @@ __global__ __launch_bounds__(512) void delta_walk_kernel(DeltaArgs a, DeltaScrat
             __builtin_amdgcn_sched_barrier(0);
         }
         const float all = factors[31];
-        f4 x[2];  // diag(beta) (V - diag(e^G) K S), times 2^scale
+        f4 x[2];  // diag(beta) (V - diag(e^G) K S), times grown(scale)
 #pragma unroll
         for (int ti = 0; ti < 2; ++ti)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) x[ti][r] = beta[ti][r] * __builtin_fmaf(eg[ti][r] * -0x1p-4f, ks[ti][r], val[ti][r] * two_to(scale));
+            for (int r = 0; r < 4; ++r) x[ti][r] = beta[ti][r] * __builtin_fmaf(eg[ti][r] * -0x1p-4f, ks[ti][r], val[ti][r] * grown(scale));
         const Pair xb = split(x[0], x[1]);
         products(ops[0], b[0], qs);
         mix<6, 6>();
@@ -755,13 +759,13 @@ __global__ __launch_bounds__(512) void delta_walk_kernel(DeltaArgs a, DeltaScrat
         }
         load_values(n + 2, ahead);
         __builtin_amdgcn_sched_barrier(0);
-        f4 d[2] = {zero, zero};  // D times 2^(scale + 14)
+        f4 d[2] = {zero, zero};  // D times 2^14 grown(scale)
         products(m, xb, d);
         products(ops[1], b[1], qs);
         bound = __builtin_fmaf(all, bound, sum);
         sum = sizes(val);
         const int next = scale_for(bound + sum);
-        const float turn = two_to(next - scale), out_scale = out_factor * two_to(-(scale + 14));
+        const float turn = two_to(next - scale), out_scale = out_factor * shrunk(scale, 14);
         scale = next;
 #pragma unroll
         for (int k = 0; k < 2 * NU; ++k) S[k] *= all * turn;
@@ -816,7 +820,7 @@ __global__ __launch_bounds__(512) void delta_walk_kernel(DeltaArgs a, DeltaScrat
 #pragma unroll
         for (int k = 0; k < 2 * NU; ++k)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) p[size_t(16 * k + r) * columns] = S[k][r] * two_to(-scale);
+            for (int r = 0; r < 4; ++r) p[size_t(16 * k + r) * columns] = S[k][r] * shrunk(scale);
     }
 }
 
@@ -855,7 +859,7 @@ __global__ __launch_bounds__(512, 4) void delta_group_kernel(DeltaArgs a) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) S[k][r] = walks && v.in >= 0 ? a.state[size_t(v.in) * pool + place + size_t(16 * k + r) * DV] : 0.0f;
     float bound = 0.0f;
-    int scale = 0;  // S is kept times 2^scale
+    int scale = -kScale;  // S is kept times grown(scale)
     const int n_groups = (v.n + kChunk - 1) / kChunk;
     for (int n = 0; n < n_groups; ++n) {
         const int r0 = v.r0 + n * kChunk, left = v.n - n * kChunk;
@@ -945,12 +949,12 @@ __global__ __launch_bounds__(512, 4) void delta_group_kernel(DeltaArgs a) {
                 m[ti] = operand(matrices + ti * 2 * kBlock + lane_at);
                 p[ti] = operand(matrices + (4 + ti * 2) * kBlock + lane_at);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) y[ti][r] = bt[r] * __builtin_fmaf(eg[ti][r] * -0x1p-4f, ks[ti][r], val[ti][r] * two_to(scale));
+                for (int r = 0; r < 4; ++r) y[ti][r] = bt[r] * __builtin_fmaf(eg[ti][r] * -0x1p-4f, ks[ti][r], val[ti][r] * grown(scale));
             }
             products(m, split(y[0], y[1]), d);
             f4 o[2] = {qs[0] * eg[0], qs[1] * eg[1]};
             products(p, split(d[0] * 0x1p-14f, d[1] * 0x1p-14f), o);
-            const float f = a.scale * two_to(-(scale + 14)), all = factors[31];
+            const float f = a.scale * shrunk(scale, 14), all = factors[31];
 #pragma unroll
             for (int ti = 0; ti < 2; ++ti)
 #pragma unroll
@@ -979,7 +983,7 @@ __global__ __launch_bounds__(512, 4) void delta_group_kernel(DeltaArgs a) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const float y = S[k][r];
-                a.state[size_t(v.out) * pool + place + size_t(16 * k + r) * DV] = n_groups ? y * two_to(-scale) : y;
+                a.state[size_t(v.out) * pool + place + size_t(16 * k + r) * DV] = n_groups ? y * shrunk(scale) : y;
             }
     }
 }
@@ -1046,7 +1050,7 @@ __global__ __launch_bounds__(512, 4) void delta_join_kernel(DeltaArgs a, DeltaSc
             }
         scale = scale_for(over_groups(bound));
 #pragma unroll
-        for (int u = 0; u < NU; ++u) b[u] = split(S[2 * u] * two_to(scale), S[2 * u + 1] * two_to(scale));
+        for (int u = 0; u < NU; ++u) b[u] = split(S[2 * u] * grown(scale), S[2 * u + 1] * grown(scale));
     }
     const int items = n_groups + (middle < n_groups ? DK / 32 : 0);
     for (int i = st % tiles; i < items; i += tiles) {
@@ -1074,9 +1078,9 @@ __global__ __launch_bounds__(512, 4) void delta_join_kernel(DeltaArgs a, DeltaSc
         for (int j = 0; j < kTurns; ++j) {
             const int m = row + j * (512 / kLanes);
             const int e = scale_for(lanes_sum<kLanes>((fabsf(x[j][0]) + fabsf(x[j][1])) + (fabsf(x[j][2]) + fabsf(x[j][3]))));
-            if (at == 0) shrink[m] = two_to(-e);
+            if (at == 0) shrink[m] = shrunk(e);
             h4 hi, lo;
-            split4(x[j], two_to(e), hi, lo);
+            split4(x[j], grown(e), hi, lo);
             char *p = rows + (m / 16 * NU + at / 32) * 2 * kBlock + operand_at(m, at % 32);
             *reinterpret_cast<h4 *>(p) = hi;
             *reinterpret_cast<h4 *>(p + kBlock) = lo;
@@ -1091,7 +1095,7 @@ __global__ __launch_bounds__(512, 4) void delta_join_kernel(DeltaArgs a, DeltaSc
                 for (int ti = 0; ti < 2; ++ti) op[ti] = operand(rows + (ti * NU + u) * 2 * kBlock + lane_at);
                 products(op, b[u], c);
             }
-            const float f = (state ? 1.0f : a.scale) * two_to(-scale);
+            const float f = (state ? 1.0f : a.scale) * shrunk(scale);
 #pragma unroll
             for (int ti = 0; ti < 2; ++ti)
 #pragma unroll

@@ -117,3 +117,51 @@ def test_state_decays_over_the_second_half(ctx, DK, DV, lost, gamma, way):
         assert off <= mean_error(n), (part, off, mean_error(n))
     off = rms((after - ref_after) / rms(ref_after, (2, 3))[..., None, None])
     assert off <= mean_error(n), (off, mean_error(n))
+
+
+@pytest.mark.parametrize("way", WAYS)
+@pytest.mark.parametrize("size", [1e-15, 1e-20, 1e-25, 1e-28])
+@pytest.mark.parametrize("D", [64, 128])
+def test_values_of_any_size(ctx, D, size, way):
+    """Values and states of one size, however small: as far as fp32 has all its bits for what they sum to, none are lost."""
+    say(f"delta precision: size={size} D={D} way={way}")
+    n = 600
+    x, g = rows(n, 1, 2, D, D, D)
+    x["v"] *= size
+    state = size * g.standard_normal((1, 2, D, D))
+    rate = np.array([-0.01, -1.0])
+    out, after = on_way(ctx, way, [n], x, rate, state)
+    ref, ref_after, _ = exact([n], x, rate, state)
+    for h in range(2):
+        assert rms(out[:, h] - ref[:, h]) <= mean_error(n) * rms(ref[:, h])
+        assert rms(after[:, h] - ref_after[:, h]) <= mean_error(n) * rms(ref_after[:, h])
+
+
+@pytest.mark.parametrize("way", WAYS)
+@pytest.mark.parametrize("large,small", [(1e4, 1e-25), (6e4, 1e-20), (1e10, 1e-25)])
+def test_values_change_their_size_at_once(ctx, large, small, way):
+    """Values and a state of one size, all forgotten within a token, and then values of another: no infinity meets a zero. The token
+    is the first of a group, so the state before the group is large, and its operands are never finer than 2^-39 of it: 2^-33 of what the
+    state and the values before sum to, a token of the group (see state_ref.delta), which stays in the state as nothing decays
+    afterwards. A group of zeros between leaves the next ones all their bits. (1e10 is more than the rows may hold: nothing but finite
+    numbers is asked for there.)"""
+    n, D, first = 576, 64, 288
+    for zeros in (0, 32):
+        say(f"delta precision: from {large} to {small} zeros={zeros} way={way}")
+        x, g = rows(n, 1, 1, D, D, 7)
+        x["v"][:first] *= large
+        x["v"][first:] *= small
+        x["v"][first - zeros:first] = 0.0
+        x["a"][:] = -40.0
+        x["a"][first - zeros] = 300.0  # e^-300 once
+        state = large * g.standard_normal((1, 1, D, D))
+        out, after = on_way(ctx, way, [n], x, np.array([-1.0]), state)
+        ref, ref_after, _ = exact([n], x, np.array([-1.0]), state)
+        assert np.isfinite(out).all() and np.isfinite(after).all()
+        if large > 65520:
+            continue
+        assert rms(out[:first - zeros] - ref[:first - zeros]) <= mean_error(n) * rms(ref[:first - zeros])
+        held = 0.0 if zeros else np.abs(x["v"][:first]).sum(0).max() + np.abs(state).sum(2).max()
+        for part in (slice(first, first + 32), slice(first + 32, n)):
+            assert rms(out[part] - ref[part]) <= mean_error(n) * rms(ref[part]) + 32 * 2.0 ** -33 * held, (zeros, part)
+        assert rms(after - ref_after) <= mean_error(n) * rms(ref_after) + 32 * 2.0 ** -33 * held, zeros
