@@ -501,8 +501,10 @@ int qmm_short_conv(qmm_context *ctx, const qmm_state_batch *batch, const qmm_con
  * A rate above 0 counts as 0. Up to 8 new rows go through the state one after another;
  * more in groups of 32 on the matrix units (strides of q, k, v and out below 2^24
  * values; else as the few), their operands as pairs of fp16 values: 22 bits, and never
- * finer than 2^-39 of what the column's values of a group and its state sum to. Long
- * prompts are faster with a workspace. */
+ * finer than 2^-28 of the largest value of the same column in the last 96 rows and in the
+ * state before them (nor than 2^-119). Long prompts are faster with a workspace, and go in
+ * halves where few heads leave room: then not finer either than 2^-28 of the state in the
+ * middle, as far as any part of that is left. */
 typedef struct {
     const float *q, *k;   /* device [n_rows][..]: qk_heads heads of key_dim values */
     size_t q_stride, k_stride;

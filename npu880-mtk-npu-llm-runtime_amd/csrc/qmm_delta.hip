@@ -202,8 +202,8 @@ __global__ __launch_bounds__(256, MANY ? 4 : 3) void delta_step_kernel(DeltaArgs
 // operands are kept large: K, at most 1 in size and of length 1, 2^4 times; Q, T and P, at most 1 in size, 2^14
 // times (their small values meet large ones of D where decays are strong); the scale of a column of S, D
 // and V is a power of two, from a bound of the column that holds for the group (|S column| grows by |v| at most, as a
-// step makes no column longer). What is left of a value is good to 2^-22, or 2^-39 of that bound. beta is no part of T:
-// small ones would lose bits there.
+// step makes no column longer; and it is measured now and then). What is left of a value is good to 2^-22, or 2^-39 of that bound
+// (D in the state's update, 2^-4 times for the keys' 2^4, 2^-36). beta is no part of T: small ones would lose bits there.
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
@@ -520,6 +520,18 @@ __device__ inline float over_groups(float x) {  // sum over the four lanes of a 
     return __uint_as_float(q[0]) + __uint_as_float(q[1]);
 }
 
+__device__ inline float most_over_groups(float x) {
+    auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+    auto q = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
+}
+// A column's length is at most sqrt(DK) of its largest value, and at most what it was, decayed, and what the values added. The second grows
+// with every token where nothing decays, so the walk measures the first after every second group (8192 tokens of 32 heads 387 us, 385
+// without; after each one 391).
+constexpr int kMeasured = 2;
+__device__ inline float larger(float m, float x, float y) { return fmaxf(fmaxf(m, fabsf(x)), fabsf(y)); }
+
 // The i-th longest of up to 64 sequences: the longest walks begin first (prompts of 951, 677, 403, 129, 1500 and 1225 tokens: 107 us
 // in their order, 97 so). More fill the compute units anyway.
 __device__ inline int by_length(const StateView &b, int i) {
@@ -811,6 +823,12 @@ __global__ __launch_bounds__(512) void delta_walk_kernel(DeltaArgs a, DeltaScrat
             }
             __builtin_amdgcn_sched_barrier(0);
         }
+        if (n % kMeasured == kMeasured - 1) {
+            float most = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 2 * NU; ++k) most = larger(larger(most, S[k][0], S[k][1]), S[k][2], S[k][3]);
+            bound = fminf(bound, most_over_groups(most) * ((DK == 128 ? 11.32f : 8.0f) * shrunk(scale)));
+        }
         __syncthreads();
     } while (++n < n_groups);
     if (to) {
@@ -858,7 +876,7 @@ __global__ __launch_bounds__(512, 4) void delta_group_kernel(DeltaArgs a) {
     for (int k = 0; k < 2 * NU; ++k)
 #pragma unroll
         for (int r = 0; r < 4; ++r) S[k][r] = walks && v.in >= 0 ? a.state[size_t(v.in) * pool + place + size_t(16 * k + r) * DV] : 0.0f;
-    float bound = 0.0f;
+    float bound = __builtin_huge_valf();
     int scale = -kScale;  // S is kept times grown(scale)
     const int n_groups = (v.n + kChunk - 1) / kChunk;
     for (int n = 0; n < n_groups; ++n) {
@@ -908,13 +926,12 @@ __global__ __launch_bounds__(512, 4) void delta_group_kernel(DeltaArgs a) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) sum += fabsf(val[ti][r]);
             sum = over_groups(sum);
-            if (n == 0) {
+            float state = 0.0f;
 #pragma unroll
-                for (int k = 0; k < 2 * NU; ++k)
+            for (int k = 0; k < 2 * NU; ++k)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) bound += fabsf(S[k][r]);
-                bound = over_groups(bound);
-            }
+                for (int r = 0; r < 4; ++r) state += fabsf(S[k][r]);
+            bound = fminf(bound, over_groups(state) * shrunk(scale));  // (what the steps add up to, if that is less)
             const int next = scale_for(bound + sum);
             const float turn = two_to(next - scale);
             scale = next;

@@ -165,3 +165,26 @@ def test_values_change_their_size_at_once(ctx, large, small, way):
         for part in (slice(first, first + 32), slice(first + 32, n)):
             assert rms(out[part] - ref[part]) <= mean_error(n) * rms(ref[part]) + 32 * 2.0 ** -33 * held, (zeros, part)
         assert rms(after - ref_after) <= mean_error(n) * rms(ref_after) + 32 * 2.0 ** -33 * held, zeros
+
+
+@pytest.mark.parametrize("way", WAYS)
+@pytest.mark.parametrize("large", [32, 256, 600])
+@pytest.mark.parametrize("D", [64, 128])
+def test_small_values_after_large_ones(ctx, D, large, way):
+    """Nothing decays, but every value is written over within D tokens (unit vectors in turn as keys, steps of 1): once no large one is
+    left, the small ones keep their bits. A row of the state is as its last writing left it."""
+    say(f"delta precision: small after large D={D} large={large} way={way}")
+    n = large + 5 * D + 61
+    x, _ = rows(n, 1, 1, D, D, D + large)
+    x["k"] = np.eye(D)[np.arange(n) % D][:, None]
+    x["b"][:], x["a"][:] = 40.0, -40.0
+    x["v"][:large] *= 6e4
+    x["v"][large:] *= 1e-3
+    state = np.zeros((1, 1, D, D))
+    out, after = on_way(ctx, way, [n], x, np.full(1, -1.0), state, eps=1e-12)
+    ref, ref_after, size = exact([n], x, np.full(1, -1.0), state, eps=1e-12)
+    # a large value's own error, 2^-22 of it and more, goes as it is written over, and what that leaves the next time
+    part = slice(large + 4 * D, n)
+    off = rms(out[part] - ref[part]) / rms(ref[part])
+    assert off <= mean_error(D), (off, mean_error(D))
+    assert rms(after - ref_after) <= mean_error(D) * rms(ref_after)
