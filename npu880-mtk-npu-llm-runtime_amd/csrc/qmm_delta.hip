@@ -1140,7 +1140,7 @@ template <int DK, int NW, bool HALVES> hipError_t launch_walk(const DeltaArgs &a
     return hipGetLastError();
 }
 
-template <int DK> hipError_t launch_groups(const DeltaArgs &a, const DeltaScratch &w, int cu_count, hipStream_t s) {
+template <int DK> hipError_t launch_groups(const DeltaArgs &a, const DeltaScratch &w, bool halves, int cu_count, hipStream_t s) {
     const int64_t lists = int64_t(a.b.n_seqs) * a.v_heads;
     const int64_t want = (int64_t(a.max_new) + kChunk - 1) / kChunk, most = ((int64_t(1) << 24) - 1) / lists;
     const int tiles = int(want < 1 ? 1 : want < most ? want : most);  // (the others in turns)
@@ -1151,7 +1151,7 @@ template <int DK> hipError_t launch_groups(const DeltaArgs &a, const DeltaScratc
     // columns 423), else those of 64 (six prompts of 4887 tokens in all: 106 us, with 32 columns 144).
     // Halves where all their workgroups find a CU: a prompt of 32 heads and 640 tokens 50 us, in one 54; of 2048 109 and 141; of
     // 8192 397 and 559.
-    if (want >= kHalfGroups && lists <= kHalfLists && lists * ((2 * a.value_dim + DK) / 64) <= cu_count) {
+    if (halves && want >= kHalfGroups && lists <= kHalfLists && lists * ((2 * a.value_dim + DK) / 64) <= cu_count) {
         if ((e = launch_walk<DK, 4, true>(a, w, s)) != hipSuccess) return e;
         // (each workgroup with about four items, for one reading of the state; more than four past 2^31 threads)
         const int turns = int(min((want + DK / 32 + 3) / 4, (int64_t(1) << 22) / lists));
@@ -1181,7 +1181,8 @@ hipError_t launch_delta(const DeltaArgs &a, void *scratch, size_t scratch_bytes,
     // and three: 1 sequence of 64 tokens 20.2, 20.9, of 128 36.3, 24.2; 8 of 64 26.1, 36.2, of 192 60.1, 66.4; 32 of 192 175, 249.
     const double steps = double((int64_t(a.max_new) + kChunk - 1) / kChunk);
     const double all = min(steps * a.b.n_seqs, double(a.b.n_rows / kChunk + a.b.n_seqs)) * a.v_heads;
-    if (grouped && 8.4 * steps > 13 + max(1.9 * steps, 0.029 * all) && scratch && scratch_bytes >= delta_scratch_bytes(a)) {
+    if (grouped && 8.4 * steps > 13 + max(1.9 * steps, 0.029 * all) && scratch && scratch_bytes >= delta_group_bytes(a)) {
+        const bool halves = scratch_bytes >= delta_scratch_bytes(a);
         const size_t groups = size_t(delta_groups(a.b.n_rows, a.b.n_seqs));
         DeltaScratch w;
         w.matrices = static_cast<char *>(scratch);
@@ -1192,7 +1193,7 @@ hipError_t launch_delta(const DeltaArgs &a, void *scratch, size_t scratch_bytes,
         w.end = w.middle + half * a.value_dim;
         w.carry = w.end + half * a.value_dim;
         w.reads = w.carry + half * a.key_dim;
-        return a.key_dim == 128 ? launch_groups<128>(a, w, cu_count, s) : launch_groups<64>(a, w, cu_count, s);
+        return a.key_dim == 128 ? launch_groups<128>(a, w, halves, cu_count, s) : launch_groups<64>(a, w, halves, cu_count, s);
     }
     const dim3 grid(unsigned(a.b.n_seqs) * unsigned(a.v_heads));
 #define QMM_STEP(K, V) \

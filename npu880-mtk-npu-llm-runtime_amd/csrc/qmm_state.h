@@ -62,20 +62,26 @@ struct DeltaArgs {
 // Prompts go through the delta rule in groups of 32 tokens. Group i of sequence s has number
 // row_start[s] / 32 + s + i: different for all groups of ascending sequences, and below
 // n_rows / 32 + n_seqs for any starts. Of every group the workspace holds, per value head, two 32 x 32
-// matrices as pairs of fp16 in operand order (8 KB) and 96 factors; per key head 64 inverse lengths. Where few heads (at most
-// kHalfLists) walk long sequences in halves, it also holds three matrices of each and a row of key_dim values for
-// every token and head of a second half.
+// matrices as pairs of fp16 in operand order (8 KB) and 96 factors; per key head 64 inverse lengths.
 constexpr int kChunk = 32;
 constexpr int64_t delta_groups(int n_rows, int n_seqs) { return int64_t(n_rows) / kChunk + n_seqs; }
 constexpr size_t kDeltaMatrices = 8192;
 constexpr int kFactors = 96;
+inline size_t delta_group_bytes(const DeltaArgs &a) {
+    return size_t(delta_groups(a.b.n_rows, a.b.n_seqs)) * (size_t(a.v_heads) * (kDeltaMatrices + kFactors * 4) + size_t(a.qk_heads) * 256) + 256;
+}
+// Where few heads (of all sequences together at most kHalfLists) walk long sequences in halves, it also holds three matrices of each
+// and a row of key_dim values for every token and head of a second half. A workspace serves calls of fewer rows and sequences, too: it
+// has that place (of 32768 rows and 32 heads of 128 as much again as the groups) if one sequence of all rows would use it, and without it
+// the groups are walked in one.
 constexpr int64_t kHalfLists = 64;
 constexpr int kHalfGroups = 16;  // groups of a sequence from which on halves are faster (32 heads, 512 tokens: 47 us either way)
 inline size_t delta_scratch_bytes(const DeltaArgs &a) {
+    const size_t groups = delta_group_bytes(a);
+    if (a.v_heads > kHalfLists || a.b.n_rows <= (kHalfGroups - 1) * kChunk) return groups;
     const int64_t lists = int64_t(a.b.n_seqs) * a.v_heads;
-    const size_t half = size_t(lists < kHalfLists ? lists : kHalfLists) * size_t(a.key_dim) * size_t(2 * a.value_dim + a.key_dim) * 4;
-    return size_t(delta_groups(a.b.n_rows, a.b.n_seqs)) * (size_t(a.v_heads) * (kDeltaMatrices + kFactors * 4) + size_t(a.qk_heads) * 256) + half +
-           size_t(a.b.n_rows / 2) * size_t(a.v_heads) * size_t(a.key_dim) * 4 + 256;
+    return groups + size_t(lists < kHalfLists ? lists : kHalfLists) * size_t(a.key_dim) * size_t(2 * a.value_dim + a.key_dim) * 4 +
+           size_t(a.b.n_rows / 2) * size_t(a.v_heads) * size_t(a.key_dim) * 4;
 }
 
 // The selection's lists: every wave of the first kernel reads 2048 logits of one

@@ -1,5 +1,5 @@
 // What the host decides for the layers with a carried state and the beam search, without a device: a size is given for
-// exactly the calls that are taken. Prints one line per failure and "ok" at the end.
+// exactly the calls that are taken, and covers the smaller ones. Prints one line per failure and "ok" at the end.
 #include <cstdio>
 #include <initializer_list>
 
@@ -26,8 +26,45 @@ static void slices() {
             }
 }
 
+// A workspace serves all calls of no more rows and sequences; the place for second halves is there where one of those would use it,
+// and nowhere else.
+static void workspaces() {
+    auto args = [](int seqs, int rows, int hk, int of, int dk, int dv) {
+        DeltaArgs a{};
+        a.b = StateView{nullptr, nullptr, nullptr, seqs, rows, 0};
+        a.qk_heads = hk;
+        a.v_heads = hk * of;
+        a.key_dim = dk;
+        a.value_dim = dv;
+        return a;
+    };
+    for (int hk : {1, 8, 16, 64, 65})
+        for (int of : {1, 2, 3})
+            for (int dk : {64, 128})
+                for (int dv : {64, 128}) {
+                    size_t last = 0;
+                    for (int seqs : {1, 2, 65, 1000})
+                        for (int rows : {1, 31, 480, 481, 512, 8192, 1 << 20}) {
+                            const DeltaArgs a = args(seqs, rows, hk, of, dk, dv);
+                            const size_t n = delta_scratch_bytes(a), groups = delta_group_bytes(a), lists = size_t(seqs) * a.v_heads;
+                            const size_t half = (lists < 64 ? lists : 64) * dk * (2 * dv + dk) * 4 + size_t(rows / 2) * a.v_heads * dk * 4;
+                            EXPECT(n == groups + (a.v_heads <= 64 && rows > 480 ? half : 0), "%d x %d, %d rows of %d", hk, of, rows, seqs);
+                            EXPECT(groups >= size_t(rows / 32 + seqs) * (a.v_heads * (8192 + 384) + hk * 256), "%d rows of %d", rows, seqs);
+                            for (int s2 : {1, 2, 65, 1000})
+                                for (int r2 : {1, 31, 480, 481, 512, 8192, 1 << 20})
+                                    if (s2 <= seqs && r2 <= rows) {
+                                        const DeltaArgs less = args(s2, r2, hk, of, dk, dv);
+                                        EXPECT(delta_scratch_bytes(less) <= n && delta_group_bytes(less) <= groups, "%d of %d, %d of %d", r2, rows, s2, seqs);
+                                    }
+                            last = n;
+                        }
+                    EXPECT(last > 0, "none");
+                }
+}
+
 int main() {
     slices();
+    workspaces();
     if (!bad) std::printf("ok\n");
     return bad != 0;
 }

@@ -1,6 +1,8 @@
 """How many bits the delta rule keeps where a column's values or its state change their size: states that decay over the second
 half of a prompt, small values after large ones, values of any size. The rule in 64 bits; errors are compared with the size that the
-results have there, not with the largest that ever was."""
+results have there, not with the largest that ever was. And what a workspace without the place for second halves gives."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -12,7 +14,8 @@ pytestmark = pytest.mark.gpu
 
 
 def run(ctx, news, x, rate, state, ws=True, hint=None, gamma=None, eps=1e-6):
-    """One call on rows x = {q, k, v, a, b} ([rows][heads][..]; scale 1, no bias of the steps), states in place: (rows, states)."""
+    """One call on rows x = {q, k, v, a, b} ([rows][heads][..]; scale 1, no bias of the steps), states in place: (rows, states). ws:
+    a workspace of its own; an int: smaller by so many bytes."""
     m, HK, DK = x["q"].shape
     HV, DV = x["v"].shape[1:]
     n = len(news)
@@ -29,6 +32,11 @@ def run(ctx, news, x, rate, state, ws=True, hint=None, gamma=None, eps=1e-6):
                              scale=1.0, qk_eps=eps, state=at["state"], gamma=at.get("gamma"), gamma_eps=0.0, out=at["out"],
                              out_stride=HV * DV)
     w = ctx.gated_delta_workspace(batch, args) if ws else None
+    if w and ws is not True:
+        w.free()
+        h = C.c_void_p()
+        ctx._call("qmm_attention_workspace_create", ctx._h, ctx.lib.qmm_gated_delta_workspace_bytes(ctx._h, C.byref(batch), C.byref(args)) - ws, C.byref(h))
+        w = qmm_hip._Handle(ctx, h.value, "qmm_attention_workspace_destroy")
     ctx.gated_delta(batch, args, w)
     ctx.sync()
     got = ctx.d2h(up["out"], np.float32, (m, HV, DV)), ctx.d2h(up["state"], np.float32, state.shape)
@@ -188,3 +196,18 @@ def test_small_values_after_large_ones(ctx, D, large, way):
     off = rms(out[part] - ref[part]) / rms(ref[part])
     assert off <= mean_error(D), (off, mean_error(D))
     assert rms(after - ref_after) <= mean_error(D) * rms(ref_after)
+
+
+@pytest.mark.parametrize("DK,DV", [(64, 64), (128, 128)])
+def test_workspace_without_room_for_halves(ctx, DK, DV):
+    """One that holds the groups still makes three launches of a long prompt: the bits of the walk in one, which short sequences
+    beside it leave."""
+    say(f"delta: workspace without halves D={DK},{DV}")
+    n = 700
+    x, g = rows(n, 1, 2, DK, DV, DK)
+    state, rate = g.standard_normal((1, 2, DK, DV)), np.array([-0.1, -1.0])
+    out, after = run(ctx, [n], x, rate, state, ws=1024)
+    for a, b in zip((out, after), on_way(ctx, "walk", [n], x, rate, state)):
+        assert np.array_equal(a.view(np.uint32), b.view(np.uint32))
+    for a, b in zip((out, after), on_way(ctx, "halves", [n], x, rate, state)):
+        assert rms(a - b) <= 2 * mean_error(n) * rms(b)
