@@ -470,8 +470,8 @@ typedef struct {
     const int32_t *slot_in;   /* device [n_seqs], or NULL */
     const int32_t *slot_out;  /* device [n_seqs], or NULL */
     int n_slots;
-    int max_new;              /* the most new rows of a sequence, as far as the host knows (0: not known): a choice of
-                                 launch, no result but by the order of sums */
+    int max_new;              /* the most new rows of a sequence, as far as the host knows (0: not known, n_rows count):
+                                 a choice of launch, which in the delta rule is one of arithmetic, too (see there) */
 } qmm_state_batch;
 
 /* out = act(bias + sum over i < width of weight[c][i] * x_{t - width + 1 + i}[c]),
@@ -498,13 +498,18 @@ int qmm_short_conv(qmm_context *ctx, const qmm_state_batch *batch, const qmm_con
  *   S <- decay * S;   S <- S + k^ (beta * (v - S' k^))';   o = S' q^
  * on the state S [key_dim][value_dim], and its output is
  *   o, or with gamma  o / sqrt(mean o^2 + gamma_eps) * gamma,  with z times z / (1 + exp(-z)).
- * A rate above 0 counts as 0. Up to 8 new rows go through the state one after another;
- * more in groups of 32 on the matrix units (strides of q, k, v and out below 2^24
- * values; else as the few), their operands as pairs of fp16 values: 22 bits, and never
- * finer than 2^-28 of the largest value of the same column in the last 96 rows and in the
- * state before them (nor than 2^-119). Long prompts are faster with a workspace, and go in
- * halves where few heads leave room: then not finer either than 2^-28 of the state in the
- * middle, as far as any part of that is left. */
+ * A rate above 0 counts as 0.
+ * The call's longest sequence, as max_new says (n_rows where that is 0), decides for all
+ * of them. With up to 8 new rows they go through the state one after another, in fp32
+ * (also where a sequence has more than it says, and with strides of q, k, v or out of
+ * 2^24 values or n_seqs * v_heads of 2^20 and more). Else in groups of 32 on the matrix
+ * units, operands as pairs of fp16 values: 22 bits, and never finer than 2^-28 of the
+ * largest value of the same column in the last 96 rows and in the state before them (nor
+ * than 2^-119). So batches that only decode say max_new = 1 (without, 32 sequences of 32
+ * heads take 43 us, with it 23), and a sequence's last bits follow the longest one
+ * beside it. Long prompts are faster with a workspace, and go in halves where few heads
+ * leave room: then not finer either than 2^-28 of the state in the middle, as far as any
+ * part of that is left. */
 typedef struct {
     const float *q, *k;   /* device [n_rows][..]: qk_heads heads of key_dim values */
     size_t q_stride, k_stride;
@@ -528,8 +533,8 @@ typedef struct {
 /* Bytes of a workspace (qmm_attention_workspace_create; its rules, and one made
  * for the attention serves here too) for calls of these heads with no more
  * sequences and rows; 0: arguments that the call refuses (qmm_last_error). A
- * smaller one, or NULL, makes prompts slower, and no result other than by the
- * order of sums. */
+ * smaller one, or NULL, makes prompts slower, and no result other than by roundings
+ * (one launch, three, or halves: the same operands in another order). */
 size_t qmm_gated_delta_workspace_bytes(qmm_context *ctx, const qmm_state_batch *batch, const qmm_delta_args *args);
 int qmm_gated_delta(qmm_context *ctx, const qmm_state_batch *batch, const qmm_delta_args *args, qmm_attn_workspace *ws);
 
@@ -538,12 +543,14 @@ int qmm_gated_delta(qmm_context *ctx, const qmm_state_batch *batch, const qmm_de
  * n_beams beams. Beam b continued by token j has
  *   total = score[b] + logits[b][j] - log(sum over i of exp(logits[b][i]));
  * an ended beam has one continuation, end_token, at its own score, and its
- * logits are not read. Order: the larger total (64 bits); among equal ones the
- * lower beam, then the larger logit, then the lower token. A logit or score that
- * is NaN or +infinite counts as -infinite (a token that is ruled out); all
- * continuations of a beam without a finite one have a total of -infinite, and
- * come last, by beam and token. What the LM head wrote as logits_out is read in
- * place. */
+ * logits are not read. Order: the larger total; among equal ones the lower beam,
+ * then the larger logit, then the lower token. Totals are added in 64 bits, but the
+ * exponentials and their sums over 2048 logits are fp32: totals of two beams that are
+ * nearer than 40 * 2^-24 may change places, the same way in every call, and beams of
+ * the same logits and scores have equal ones. A logit or score that is NaN or
+ * +infinite counts as -infinite (a token that is ruled out); all continuations of a
+ * beam without a finite one have a total of -infinite, and come last, by beam and
+ * token. What the LM head wrote as logits_out is read in place. */
 typedef struct {
     const float *logits;  /* device [n_items * n_beams][stride] */
     size_t stride;        /* >= vocab; any */

@@ -2,8 +2,8 @@
 //
 // Every token of a head, in order, on its state S [DK][DV]:
 //   S <- e^g S;  d = beta (v - S' k);  S <- S + k d';  o = S' q
-// with k and q of unit length. The columns of S are independent of each other. Three ways, by the new rows of a sequence:
-// a token at a time (up to 8), groups of 32 in one launch, groups in three launches (launch_delta has the rule).
+// with k and q of unit length. The columns of S are independent of each other. Three ways, one for all sequences of a call, by the
+// new rows of the longest: a token at a time (up to 8), groups of 32 in one launch, groups in three (launch_delta has the rule).
 // Bound: a token at a time and one group by the states' way through memory, or the latency of a launch where they are
 // few; prompts by the chain of groups, one product after the other (figures at the kernels, heads of 128).
 #include <hip/hip_runtime.h>
@@ -334,8 +334,8 @@ __device__ inline double shfl_up(double x, int d) {
 
 constexpr int kRow = 36;  // floats of a row of a 32 x 32 matrix in LDS
 typedef float Square[32][kRow];
-// The pieces of T and P of one group.
-// squares of an item's rows, summed over the eight lanes that share them, to sums[kind][token][of 32 values]
+
+// The pieces of T and P of one group: squares of an item's rows, summed over the eight lanes that share them, to sums[kind][token][of 32 values]
 template <int DK> __device__ inline void row_squares(const Item<DK> &it, const f4 x[4], float (*sums)[32][DK / 32]) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -1148,7 +1148,7 @@ template <int DK> hipError_t launch_groups(const DeltaArgs &a, const DeltaScratc
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     // Where workgroups of 32 columns find a CU each they are a little faster (a prompt of 8192 and 32 heads: 411 us, with 64
-    // columns 423), else those of 64 (six prompts of 4887 tokens in all: 106 us, with 32 columns 144).
+    // columns 423), else those of 64 (six prompts of 4885 tokens in all: 106 us, with 32 columns 144).
     // Halves where all their workgroups find a CU: a prompt of 32 heads and 640 tokens 50 us, in one 54; of 2048 109 and 141; of
     // 8192 397 and 559.
     if (halves && want >= kHalfGroups && lists <= kHalfLists && lists * ((2 * a.value_dim + DK) / 64) <= cu_count) {

@@ -211,3 +211,23 @@ def test_workspace_without_room_for_halves(ctx, DK, DV):
         assert np.array_equal(a.view(np.uint32), b.view(np.uint32))
     for a, b in zip((out, after), on_way(ctx, "halves", [n], x, rate, state)):
         assert rms(a - b) <= 2 * mean_error(n) * rms(b)
+
+
+@pytest.mark.parametrize("hint", [1, 8, 9, 40])
+def test_a_sequence_follows_the_hint_and_not_its_neighbours(ctx, hint):
+    """max_new decides how all of a call's sequences are computed; under the same one a sequence has the same bits alone."""
+    say(f"delta: neighbours hint={hint}")
+    news, D = [1, 0, 5, 8, 30, 64, 1], 64
+    x, g = rows(sum(news), 1, 2, D, D, 11)
+    state, rate = g.standard_normal((len(news), 2, D, D)), np.array([-0.1, -1.0])
+    out, after = run(ctx, news, x, rate, state, ws=False, hint=hint)
+    r = 0
+    for i, n in enumerate(news):
+        if n:
+            alone, alone_after = run(ctx, [n], {k: y[r:r + n] for k, y in x.items()}, rate, state[i:i + 1], ws=False, hint=hint if hint < 9 or n > 8 else 0)
+            if hint < 9 or n > 8:
+                assert np.array_equal(alone.view(np.uint32), out[r:r + n].view(np.uint32))
+                assert np.array_equal(alone_after.view(np.uint32), after[i:i + 1].view(np.uint32))
+            else:  # (alone the host knows that the rows are few)
+                assert rms(alone - out[r:r + n]) <= 2 * mean_error(n) * rms(alone)
+        r += n
