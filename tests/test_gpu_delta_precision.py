@@ -231,3 +231,23 @@ def test_a_sequence_follows_the_hint_and_not_its_neighbours(ctx, hint):
             else:  # (alone the host knows that the rows are few)
                 assert rms(alone - out[r:r + n]) <= 2 * mean_error(n) * rms(alone)
         r += n
+
+
+@pytest.mark.parametrize("way", WAYS)
+@pytest.mark.parametrize("alike", [0.0, 0.9, 1.0])
+@pytest.mark.parametrize("decay", [1e-6, 0.01, 1.0])
+def test_mean_error_of_long_prompts(ctx, decay, alike, way):
+    """The rms error of a long prompt's rows, also of its last ones, and of its state: a worst case for each token adds up to
+    a third of the values there, a lost low part of one operand (2^-11) to a hundredth and less."""
+    say(f"delta precision: mean error decay={decay} alike={alike} way={way}")
+    n, D = 1600, 64
+    x, g = rows(n, 1, 2, D, D, 5)
+    x["k"] = alike * g.standard_normal(D) + (1 - alike) * x["k"]
+    state, rate = g.standard_normal((1, 2, D, D)), np.array([-decay, -decay / 3])
+    out, after = on_way(ctx, way, [n], x, rate, state)
+    ref, ref_after, _ = exact([n], x, rate, state)
+    for h in range(2):
+        for part in (slice(0, 400), slice(400, 1200), slice(1200, 1590), slice(1590, n)):
+            off = rms(out[part, h] - ref[part, h]) / rms(ref[part, h])
+            assert off <= mean_error(n), (h, part, off)
+        assert rms(after[0, h] - ref_after[0, h]) <= mean_error(n) * rms(ref_after[0, h]), h
