@@ -13,10 +13,10 @@
 //  - a workgroup per item: a wave per beam joins the beam's lists the same way and
 //    the sums in 64 bits; then every candidate's rank is the number of those before
 //    it, by bisection in the beams' lists, which are in order.
-// Bound: memory (the logits are read once) for many rows, else the latency of the
-// two launches. 4 beams over 151936 tokens, 8 kept: 5.8 + 5.8 us; 128 beams of 16 items, 16 kept: 17.9 (3.7 TB/s: some 500
-// vector instructions a wave, 8.6 us of issue in all, and the scalar ones of its searches between them) + 8.7. Keys are found by
-// their upper half first: a search of 16 ballots, not 64 (35.1 us for both launches with 64, 28.5 so).
+// Bound: memory (the logits are read once) for many rows, else the latency of the two launches. 4 beams over 151936
+// tokens, 8 kept: 5.8 + 5.8 us; 128 beams of 16 items, 16 kept: 17.9 (3.7 TB/s: some 500 vector instructions a wave,
+// 8.6 us of issue in all, and the scalar ones of its searches between them) + 8.7. Keys are found by their upper half
+// first: a search of 16 ballots, not 64 (35.1 us for both launches with 64, 28.5 so).
 #include <hip/hip_runtime.h>
 
 #include "qmm_lanes.h"
@@ -41,8 +41,8 @@ __device__ inline void wave_sync() {
     __builtin_amdgcn_wave_barrier();
 }
 
-// The largest T of the bits `from` .. `to` - 1 (the lower ones 0, those above as in T) that at least n of the lanes where
-// `on` have at or above.
+// The largest T of the bits `from` .. `to` - 1 (the lower ones 0, those above as in T) that at least n of the lanes
+// where `on` have at or above.
 __device__ inline uint32_t nth_bits(uint32_t x, bool on, int n, uint32_t T, int from, int to) {
 #pragma unroll 1
     for (int bit = to - 1; bit >= from; --bit) {
@@ -104,9 +104,10 @@ __global__ __launch_bounds__(256) void beam_slice_kernel(BeamArgs a, int slices)
     const float *x = a.logits + size_t(row) * a.stride + first;
     uint64_t *list = found + wid * a.n_keep * kPerLane;
     float v[kPerLane];
-    // Place of this lane's value i: 4 neighbours, one load, at whatever 4-B address the row begins (16-B loads need no more). The
-    // same for all rows: beams alike add their exponentials in one order and get the same bits, so that the lower one comes first.
-    // 6 rows of 50257 logits without a gap, whose addresses differ: 12.3 us (13.0 with a load a value where a row was not 16-B aligned).
+    // Place of this lane's value i: 4 neighbours, one load, at whatever 4-B address the row begins (16-B loads need no
+    // more). The same for all rows: beams alike add their exponentials in one order and get the same bits, so that the
+    // lower one comes first. 6 rows of 50257 logits without a gap, whose addresses differ: 12.3 us (13.0 with a load a
+    // value where a row was not 16-B aligned).
     typedef float AnyFour __attribute__((ext_vector_type(4), aligned(4)));
     auto place = [&](int i) { return (i / 4) * 256 + 4 * lane + i % 4; };
 #pragma unroll

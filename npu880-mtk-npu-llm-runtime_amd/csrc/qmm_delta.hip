@@ -2,10 +2,11 @@
 //
 // Every token of a head, in order, on its state S [DK][DV]:
 //   S <- e^g S;  d = beta (v - S' k);  S <- S + k d';  o = S' q
-// with k and q of unit length. The columns of S are independent of each other. Three ways, one for all sequences of a call, by the
-// new rows of the longest: a token at a time (up to 8), groups of 32 in one launch, groups in three (launch_delta has the rule).
-// Bound: a token at a time and one group by the states' way through memory, or the latency of a launch where they are
-// few; prompts by the chain of groups, one product after the other (figures at the kernels, heads of 128).
+// with k and q of unit length. The columns of S are independent of each other. Three ways, one for all sequences of a
+// call, by the new rows of the longest: a token at a time (up to 8), groups of 32 in one launch, groups in three
+// (launch_delta has the rule). Bound: a token at a time and one group by the states' way through memory, or the latency
+// of a launch where they are few; prompts by the chain of groups, one product after the other (figures at the kernels,
+// heads of 128).
 #include <hip/hip_runtime.h>
 
 #include "qmm_lanes.h"
@@ -14,11 +15,12 @@
 namespace qmm {
 namespace {
 
-constexpr int kStepRows = 8;  // new rows up to which a token at a time is faster than a group of 32
+constexpr int kStepRows = 8;  // new rows up to which a token at a time is as fast as a group of 32 (heads of 128 and of 64)
 constexpr int kGroup = 8;  // tokens whose inputs are in LDS at a time
 
 __device__ inline float softplus(float x) { return x > 0.0f ? x + log1pf(expf(-x)) : log1pf(expf(x)); }
-// Between -200, whose e^x is 0 in fp32 (sums over tokens keep their small parts, and no infinity meets another), and 0; NaN stays.
+// Between -200, whose e^x is 0 in fp32 (sums over tokens keep their small parts, and no infinity meets another), and 0;
+// NaN stays.
 __device__ inline float log_decay(const DeltaArgs &a, int row, int h) {
     const float g = a.rate[h] * softplus(a.a[size_t(row) * a.a_stride + h] + a.dt_bias[h]);
     return g > 0.0f ? 0.0f : g < -200.0f ? -200.0f : g;
@@ -53,19 +55,20 @@ template <int DV, typename F> __device__ inline void write_rows(const DeltaArgs 
     }
 }
 
-// One token after another through the state, for few new rows: a workgroup per
-// sequence and head, a wave 16 * CL / 4 columns (4 a lane) of all rows, in
-// registers; a lane has rows 4 (rl + RL g) .. + 3. Both products with S are taken
-// before it changes: S' q after the step is e^g S' q + (k.q) d, so one pass and one
-// sum over the lanes serve both, and no wave waits for another between tokens. 32 heads: one sequence of a token 5.5 us (a launch and one
-// way through memory), 64 sequences 49.2 us (5.5 TB/s of 273 MB); another token adds 0.75 us.
+// One token after another through the state, for few new rows: a workgroup per sequence and head, a wave 16 * CL / 4
+// columns (4 a lane) of all rows, in registers; a lane has rows 4 (rl + RL g) .. + 3. Both products with S are taken
+// before it changes: S' q after the step is e^g S' q + (k.q) d, so one pass and one sum over the lanes serve both, and
+// no wave waits for another between tokens. 32 heads: one sequence of a token 5.5 us (a launch and one way through
+// memory), 64 sequences 49.2 us (5.5 TB/s of 273 MB); another token adds 0.75 us.
 //
-// MANY: more workgroups than three a CU. Then four: places are worked out again for every use, and k is read from LDS twice (kept over
-// the tokens they take the registers of the fourth), and states of more than 32 MB in all go past the caches: 32 sequences of 4 tokens
-// 29 us become 22, 64 of one 57 become 49. For fewer that only costs: one sequence of 8 tokens 10.7 us, so 11.6.
+// MANY: more workgroups than three a CU. Then four: places are worked out again for every use, and k is read from LDS
+// twice (kept over the tokens they take the registers of the fourth), and states of more than 32 MB in all go past the
+// caches: 32 sequences of 4 tokens 29 us become 22, 64 of one 57 become 49. For fewer that only costs: one sequence of
+// 8 tokens 10.7 us, so 11.6.
 template <int DK, int DV, bool MANY>
 __global__ __launch_bounds__(256, MANY ? 4 : 3) void delta_step_kernel(DeltaArgs a) {
-    constexpr int CL = DV / 16, RL = 64 / CL, NG = DK / (4 * RL), NV = (kGroup * DV + 1023) / 1024, HL = 32;  // HL: lanes that hold one row of q or k
+    constexpr int CL = DV / 16, RL = 64 / CL, NG = DK / (4 * RL), NV = (kGroup * DV + 1023) / 1024;
+    constexpr int HL = 32;  // lanes that hold one row of q or k
     __shared__ float qk[kGroup][2][DK];
     __shared__ float vo[kGroup][DV];  // values, then outputs
     __shared__ float sc[kGroup][4];   // decay, beta, k.q
@@ -80,7 +83,9 @@ __global__ __launch_bounds__(256, MANY ? 4 : 3) void delta_step_kernel(DeltaArgs
         if (MANY) asm("" : "+v"(x));
         return x;
     };
-    auto state = [&](int slot, int at) { return a.state + size_t(slot) * pool + size_t(h) * DK * DV + size_t(4 * (at / CL)) * DV + wid * (DV / 4) + 4 * (at % CL); };
+    auto state = [&](int slot, int at) {
+        return a.state + size_t(slot) * pool + size_t(h) * DK * DV + size_t(4 * (at / CL)) * DV + wid * (DV / 4) + 4 * (at % CL);
+    };
 
     float4 x[kGroup / 4], val[NV];
     auto load = [&](int t0, int t) {
@@ -196,22 +201,22 @@ __global__ __launch_bounds__(256, MANY ? 4 : 3) void delta_step_kernel(DeltaArgs
 // S the state before it:
 //   A_ij = beta_i e^(G_i - G_j) k_i.k_j  (j < i),   T = (I + A)^-1,   P_ij = e^(G_i - G_j) q_i.k_j  (j <= i)
 //   D = T diag(beta) (V - diag(e^G) K S),   O = diag(e^G) Q S + P D,   S <- e^(G_last) S + K' diag(e^(G_last - G)) D
-// The first kernel makes T and P of every group at once; the second walks a
-// sequence's groups. All products but the inverse run on the matrix units in fp16, each operand as a
-// pair hi + lo of 22 bits (three products: hi hi, hi lo, lo hi), sums in fp32. A low part is a multiple of 2^-24, so
-// operands are kept large: K, at most 1 in size and of length 1, 2^4 times; Q, T and P, at most 1 in size, 2^14
-// times (their small values meet large ones of D where decays are strong); the scale of a column of S, D
-// and V is a power of two, from a bound of the column that holds for the group (|S column| grows by |v| at most, as a
-// step makes no column longer; and it is measured now and then). What is left of a value is good to 2^-22, or 2^-39 of that bound
-// (D in the state's update, 2^-4 times for the keys' 2^4, 2^-36). beta is no part of T: small ones would lose bits there.
+// The first kernel makes T and P of every group at once; the second walks a sequence's groups. All products but the
+// inverse run on the matrix units in fp16, each operand as a pair hi + lo of 22 bits (three products: hi hi, hi lo, lo
+// hi), sums in fp32. A low part is a multiple of 2^-24, so operands are kept large: K, at most 1 in size and of length
+// 1, 2^4 times; Q, T and P, at most 1 in size, 2^14 times (their small values meet large ones of D where decays are
+// strong); the scale of a column of S, D and V is a power of two, from a bound of the column that holds for the group
+// (|S column| grows by |v| at most, as a step makes no column longer; and it is measured now and then). What is left of
+// a value is good to 2^-22, or 2^-39 of that bound (D in the state's update, 2^-4 times for the keys' 2^4, 2^-36). beta
+// is no part of T: small ones would lose bits there.
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 
-// An operand of 16 rows and 32 columns k in LDS, 1 KB: lane (row r, group g of lanes) reads the 16 B of place 16 g + (r ^ g),
-// columns 4 g .. + 3 and 16 + 4 g .. + 3. That is the order in which a group of lanes holds the rows of two tiles
-// of a product, so a product's result is the next product's right operand as it stands. (r ^ g, not r: pieces of
-// 8 B of four columns, written by the lanes of four rows and all g at once, then lie on all banks.)
+// An operand of 16 rows and 32 columns k in LDS, 1 KB: lane (row r, group g of lanes) reads the 16 B of place 16 g + (r
+// ^ g), columns 4 g .. + 3 and 16 + 4 g .. + 3. That is the order in which a group of lanes holds the rows of two tiles
+// of a product, so a product's result is the next product's right operand as it stands. (r ^ g, not r: pieces of 8 B of
+// four columns, written by the lanes of four rows and all g at once, then lie on all banks.)
 constexpr int kBlock = 1024;
 __device__ inline int operand_at(int row, int col) {  // of the aligned 4 columns from `col` (of 32)
     const int g = col % 16 / 4;
@@ -257,7 +262,8 @@ __device__ inline void products(const Pair (&op)[2], const Pair &b, f4 (&c)[2]) 
 #pragma unroll
         for (int i = 0; i < 2; ++i) c[i] = mfma(part < 2 ? op[i].hi : op[i].lo, part == 1 ? b.lo : b.hi, c[i]);
 }
-// the order of what stands since the last barrier of the scheduler: N times one matrix product and K vector instructions
+// the order of what stands since the last barrier of the scheduler: N times one matrix product and K vector
+// instructions
 template <int N, int K> __device__ inline void mix() {
     if constexpr (N > 0) {
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
@@ -270,16 +276,18 @@ struct DeltaScratch {
     char *matrices;  // [groups][v_heads]: T, then P: two tiles of 16 rows, each 1 KB hi and 1 KB lo
     float *factors;  // [groups][v_heads][96]: e^G_i, e^(G_last - G_i), beta_i
     float *inverse;  // [groups][qk_heads][64]: 1 / |k_i|, 1 / |q_i|
-    // of sequences that are walked in halves, per sequence and value head: the state after the first one; the second one's end
-    // from a state of zeros; and what it makes of the unit vectors; of the second one's tokens, what they read of those
+    // of sequences that are walked in halves, per sequence and value head: the state after the first one; the second
+    // one's end from a state of zeros; and what it makes of the unit vectors; of the second one's tokens, what they
+    // read of those
     float *middle, *end, *carry, *reads;
 };
 // A sequence's second half begins at this group (its number of groups: it has none).
 __device__ inline int second_half(int n_groups, bool halves) { return halves && n_groups >= kHalfGroups ? (n_groups + 1) / 2 : n_groups; }
 __device__ inline int64_t first_group(const StateSeq &v, int s) { return v.r0 / kChunk + s; }
 
-// Up to 32 rows from `p` on, of which `left` are the sequence's, as a buffer: loads past them give 0 and stores nothing, without a
-// branch. p: row 0 of one head, `before` values into its row; stride below 2^24 values, so that all offsets fit.
+// Up to 32 rows from `p` on, of which `left` are the sequence's, as a buffer: loads past them give 0 and stores
+// nothing, without a branch. p: row 0 of one head, `before` values into its row; stride below 2^24 values, so that all
+// offsets fit.
 __device__ inline __amdgpu_buffer_rsrc_t group_rows(const float *p, size_t stride, int before, int left) {
     const uint32_t rows = uint32_t(min(max(left, 0), kChunk));
     const uint32_t bytes = (rows * uint32_t(stride) - (rows ? uint32_t(before) : 0u)) * 4u;
@@ -302,10 +310,11 @@ template <int DK> struct Item {
         const __amdgpu_buffer_rsrc_t rows = group_rows((is_q ? a.q : a.k) + size_t(r0) * stride + size_t(hk) * DK, stride, hk * DK, left);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            x[j] = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(rows, (unsigned(token + j) * unsigned(stride) + unsigned(at)) * 4u, 0, 0));
+            x[j] = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(
+                                              rows, (unsigned(token + j) * unsigned(stride) + unsigned(at)) * 4u, 0, 0));
     }
-    // times 2^4 (k) or 2^14 (q) / length as left operand, rows the tokens (tiles of 16, each DK / 32 blocks of hi and lo) and, where
-    // `turned`, rows the values (tiles of 16, each one block)
+    // times 2^4 (k) or 2^14 (q) / length as left operand, rows the tokens (tiles of 16, each DK / 32 blocks of hi and
+    // lo) and, where `turned`, rows the values (tiles of 16, each one block)
     __device__ void convert(const f4 x[4], f4 inv, h4 hi[4], h4 lo[4]) const {
 #pragma unroll
         for (int j = 0; j < 4; ++j) split4(x[j], inv[j] * (is_q ? 0x1p14f : 0x1p4f), hi[j], lo[j]);
@@ -335,7 +344,8 @@ __device__ inline double shfl_up(double x, int d) {
 constexpr int kRow = 36;  // floats of a row of a 32 x 32 matrix in LDS
 typedef float Square[32][kRow];
 
-// The pieces of T and P of one group: squares of an item's rows, summed over the eight lanes that share them, to sums[kind][token][of 32 values]
+// The pieces of T and P of one group: squares of an item's rows, summed over the eight lanes that share them, to
+// sums[kind][token][of 32 values]
 template <int DK> __device__ inline void row_squares(const Item<DK> &it, const f4 x[4], float (*sums)[32][DK / 32]) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -353,7 +363,8 @@ template <int DK> __device__ inline float inverse_length(const float (&sums)[DK 
 }
 // 2^x, x rounded to fp32 first: |x| 2^-24 off
 __device__ inline float power_of_two(double x) { return __builtin_amdgcn_exp2f(float(x)); }
-// sums of the log decays of a head (of 2: the decays are powers of two, one instruction each) and its step sizes, a token per lane of half a wave
+// sums of the log decays of a head (of 2: the decays are powers of two, one instruction each) and its step sizes, a
+// token per lane of half a wave
 __device__ inline void head_steps(const DeltaArgs &a, int row, int h, int m, bool on, double *G, float *beta) {
     double g = on ? double(log_decay(a, row, h)) * 1.4426950408889634 : 0.0;
 #pragma unroll
@@ -400,8 +411,8 @@ __device__ inline f4 mask_and_decay(const Square &kk, const Square &qk, const do
     *reinterpret_cast<f4 *>(&A[i][c]) = x;
     return p;
 }
-// The inverse of I + A: its two 16 x 16 triangles by substitution, a column per lane, then T21 = -T22 A21 T11 on the matrix
-// units in fp32.
+// The inverse of I + A: its two 16 x 16 triangles by substitution, a column per lane, then T21 = -T22 A21 T11 on the
+// matrix units in fp32.
 __device__ inline void invert_half(const Square &A, int b, int col, Square &T) {
     float x[16];
 #pragma unroll
@@ -432,9 +443,9 @@ __device__ inline float factor_of(const double *G, const float *beta, int i) {
     return i < 64 ? power_of_two(i < 32 ? G[i] : G[31] - G[i - 32]) : beta[i - 64];
 }
 
-// T and P of one group and key head, for its value heads two at a time (both inverses in one wave). Bound: the chain of ten barriers at
-// four workgroups of a CU (35 KB of LDS; with three, k k' and q k' beside the rows, 58 us): 8192 tokens of 16 key and 32 value
-// heads 53 us. Of 58, loads, conversion and products were 31, inverses 6, stores 4.
+// T and P of one group and key head, for its value heads two at a time (both inverses in one wave). Bound: the chain of
+// ten barriers at four workgroups of a CU (35 KB of LDS; with three, k k' and q k' beside the rows, 58 us): 8192 tokens
+// of 16 key and 32 value heads 53 us. Of 58, loads, conversion and products were 31, inverses 6, stores 4.
 template <int DK>
 __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, DeltaScratch w, int tiles) {
     constexpr int NU = DK / 32, NI = DK / 64;
@@ -492,7 +503,8 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, DeltaSc
             if (t < kFactors * nh) w.factors[first * kFactors + t] = factor_of(G[t / kFactors], beta[t / kFactors], t % kFactors);
             const int i = t / 8, c = t % 8 * 4, place = (c % 16 / 4) * 256 + i % 16 * 16 + c / 16 * 8;
             for (int hh = 0; hh < nh; ++hh)
-                store_operand(w.matrices + (first + hh) * kDeltaMatrices + 4 * kBlock, i, place, mask_and_decay(kk, qk, G[hh], beta[hh], i, c, A[hh]));
+                store_operand(w.matrices + (first + hh) * kDeltaMatrices + 4 * kBlock, i, place,
+                              mask_and_decay(kk, qk, G[hh], beta[hh], i, c, A[hh]));
             __syncthreads();
             if (wid == 0 && lane / 32 < nh) invert_half(A[lane / 32], lane / 16 % 2 * 16, lane % 16, T[lane / 32]);
             __syncthreads();
@@ -506,11 +518,14 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, DeltaSc
 }
 
 __device__ inline float two_to(int e) { return __uint_as_float(uint32_t(e + 127) << 23); }
-// The power of two that takes numbers up to `bound` below 2^15, from 2^-32 (2^30 rows of values below 65520 sum to less than 2^46) to
-// 2^94, so that two of them have a quotient in fp32. Columns that sum to less than 2^-80 lose the bits below 2^-119. It is kept less 30:
-// its largest is then 64, the largest constant of an instruction (8192 tokens of 8 heads otherwise 268 us, so 263).
+// The power of two that takes numbers up to `bound` below 2^15, from 2^-32 (2^30 rows of values below 65520 sum to less
+// than 2^46) to 2^94, so that two of them have a quotient in fp32. Columns that sum to less than 2^-80 lose the bits
+// below 2^-119. It is kept less 30: its largest is then 64, the largest constant of an instruction (8192 tokens of 8
+// heads otherwise 268 us, so 263).
 constexpr int kScale = 30;
-__device__ inline int scale_for(float bound) { return min(max(141 - kScale - int(__float_as_uint(bound) >> 23 & 255), -32 - kScale), 94 - kScale); }
+__device__ inline int scale_for(float bound) {
+    return min(max(141 - kScale - int(__float_as_uint(bound) >> 23 & 255), -32 - kScale), 94 - kScale);
+}
 __device__ inline float grown(int scale) { return two_to(scale + kScale); }
 __device__ inline float shrunk(int scale, int more = 0) { return two_to(-(scale + kScale + more)); }
 __device__ inline float over_groups(float x) {  // sum over the four lanes of a column
@@ -526,14 +541,15 @@ __device__ inline float most_over_groups(float x) {
     auto q = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
 }
-// A column's length is at most sqrt(DK) of its largest value, and at most what it was, decayed, and what the values added. The second grows
-// with every token where nothing decays, so the walk measures the first after every second group (8192 tokens of 32 heads 387 us, 385
-// without; after each one 391).
+// A column's length is at most sqrt(DK) of its largest value, and at most what it was, decayed, and what the values
+// added. The second grows with every token where nothing decays, so the walk measures the first after every second
+// group (8192 tokens of 32 heads 387 us, 385 without; after each one 391).
 constexpr int kMeasured = 2;
 __device__ inline float larger(float m, float x, float y) { return fmaxf(fmaxf(m, fabsf(x)), fabsf(y)); }
 
-// The i-th longest of up to 64 sequences: the longest walks begin first (prompts of 951, 677, 403, 129, 1500 and 1225 tokens: 107 us
-// in their order, 97 so). More fill the compute units anyway.
+// The i-th longest of up to 64 sequences, a lane each: the longest walks begin first (prompts of 951, 677, 403, 129,
+// 1500 and 1225 tokens: 107 us in their order, 97 so). More than a wave can rank keep their order (2000 tokens behind
+// 64 of 100 in all 490 us, in front of them 415).
 __device__ inline int by_length(const StateView &b, int i) {
     if (b.n_seqs > 64) return i;
     const int lane = threadIdx.x % 64, n = lane < b.n_seqs ? state_seq(b, lane).n : -1;
@@ -545,17 +561,18 @@ __device__ inline int by_length(const StateView &b, int i) {
     return int(__builtin_ctzll(__ballot(longer == i)));
 }
 
-// The walk over a sequence's groups. A workgroup has 16 columns of the state in each of its NW first waves, all rows, as
-// sums of matrix products; nothing of it leaves the wave's registers from group to group. Four more waves bring the
-// next group's K, Q, T and P into LDS as operands meanwhile. Bound: one wave's chain of 84 matrix products and 300 vector instructions a
-// group, beside 62 KB of LDS reads a wave and 57 KB of writes: 1.6 us a group of 32 columns, 1.65 to 2.0 of 64, where the products alone
-// take 0.57 (16.2 cycles each). 417 tokens 26.8 us. Measured and not kept: 16 columns a workgroup, operands made by the
-// first kernel (480 us for 8192 tokens against 411), output products in waves of their own, K S of the next group beside this one's.
+// The walk over a sequence's groups. A workgroup has 16 columns of the state in each of its NW first waves, all rows,
+// as sums of matrix products; nothing of it leaves the wave's registers from group to group. Four more waves bring the
+// next group's K, Q, T and P into LDS as operands meanwhile. Bound: one wave's chain of 84 matrix products and 300
+// vector instructions a group, beside 62 KB of LDS reads a wave and 57 KB of writes: 1.6 us a group of 32 columns, 1.65
+// to 2.0 of 64, where the products alone take 0.57 (16.2 cycles each). 417 tokens 26.8 us. Measured and not kept: 16
+// columns a workgroup, operands made by the first kernel (480 us for 8192 tokens against 411), output products in waves
+// of their own, K S of the next group beside this one's.
 //
-// HALVES: a sequence of many groups goes in two halves at once, where compute units are left. The rule is linear in the state:
-// what follows from S is what follows from zeros, with the values, and M S without them, M from the unit matrix. So the second half is
-// walked twice, for the values (kind 1) and for M (kind 2), and joined with the first one's last state afterwards. 8192 tokens: 411 us in
-// one, 240 in halves.
+// HALVES: a sequence of many groups goes in two halves at once, where compute units are left. The rule is linear in the
+// state: what follows from S is what follows from zeros, with the values, and M S without them, M from the unit matrix.
+// So the second half is walked twice, for the values (kind 1) and for M (kind 2), and joined with the first one's last
+// state afterwards. 8192 tokens: 411 us in one, 240 in halves.
 template <int DK, int NW, bool HALVES>
 __global__ __launch_bounds__(512) void delta_walk_kernel(DeltaArgs a, DeltaScratch w, int splits) {
     constexpr int NU = DK / 32, NI = DK / 64;
@@ -603,8 +620,8 @@ __global__ __launch_bounds__(512) void delta_walk_kernel(DeltaArgs a, DeltaScrat
             y.m1 = src[i + 256];
             y.factor = w.factors[(group * a.v_heads + h) * kFactors + i % kFactors];
         };
-        // One step: group n from the registers to LDS, and group n + 2 on its way to them. The writes come last: LDS is the
-        // walking waves' while they read the first operands of their step.
+        // One step: group n from the registers to LDS, and group n + 2 on its way to them. The writes come last: LDS is
+        // the walking waves' while they read the first operands of their step.
         auto pass = [&](int n, Held &y) {
             char *buf = lds + n % 2 * kBuffer;
             h4 hi[NI][4], lo[NI][4];
@@ -674,7 +691,8 @@ __global__ __launch_bounds__(512) void delta_walk_kernel(DeltaArgs a, DeltaScrat
         }
     auto load_values = [&](int n, f4 (&to)[2]) {
         const __amdgpu_buffer_rsrc_t rows =
-            group_rows(a.v + size_t(v.r0 + n * kChunk) * a.v_stride + size_t(h) * DV, a.v_stride, h * DV, kind == 2 ? 0 : v.n - n * kChunk);
+            group_rows(a.v + size_t(v.r0 + n * kChunk) * a.v_stride + size_t(h) * DV, a.v_stride, h * DV,
+                       kind == 2 ? 0 : v.n - n * kChunk);
 #pragma unroll
         for (int ti = 0; ti < 2; ++ti)
 #pragma unroll
@@ -758,7 +776,8 @@ __global__ __launch_bounds__(512) void delta_walk_kernel(DeltaArgs a, DeltaScrat
 #pragma unroll
         for (int ti = 0; ti < 2; ++ti)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) x[ti][r] = beta[ti][r] * __builtin_fmaf(eg[ti][r] * -0x1p-4f, ks[ti][r], val[ti][r] * grown(scale));
+            for (int r = 0; r < 4; ++r)
+                x[ti][r] = beta[ti][r] * __builtin_fmaf(eg[ti][r] * -0x1p-4f, ks[ti][r], val[ti][r] * grown(scale));
         const Pair xb = split(x[0], x[1]);
         products(ops[0], b[0], qs);
         mix<6, 6>();
@@ -819,7 +838,8 @@ __global__ __launch_bounds__(512) void delta_walk_kernel(DeltaArgs a, DeltaScrat
 #pragma unroll
                 for (int ti = 0; ti < 2; ++ti)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(o[ti][r] * out_scale), rows, out_at[ti][r], 0, 0);
+                    for (int r = 0; r < 4; ++r)
+                        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(o[ti][r] * out_scale), rows, out_at[ti][r], 0, 0);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -842,9 +862,9 @@ __global__ __launch_bounds__(512) void delta_walk_kernel(DeltaArgs a, DeltaScrat
     }
 }
 
-// Few groups, drafts mostly: all of the above in one workgroup per sequence and head, that makes a group's matrices itself and
-// has all columns of the state (16 a wave), so that the norm needs no launch of its own. Two workgroups of a CU. 8 sequences of 5 to
-// 16 tokens and 32 heads 15.2 us: launch and loads, then eleven steps between barriers.
+// Few groups, drafts mostly: all of the above in one workgroup per sequence and head, that makes a group's matrices
+// itself and has all columns of the state (16 a wave), so that the norm needs no launch of its own. Two workgroups of a
+// CU. 8 sequences of 5 to 16 tokens and 32 heads 15.2 us: launch and loads, then eleven steps between barriers.
 template <int DK, int DV>
 __global__ __launch_bounds__(512, 4) void delta_group_kernel(DeltaArgs a) {
     constexpr int NU = DK / 32, kRows = 2 * NU * 2 * kBlock;
@@ -857,8 +877,8 @@ __global__ __launch_bounds__(512, 4) void delta_group_kernel(DeltaArgs a) {
     __shared__ double G[32];
     __shared__ float beta[32];
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    // (24 and 32 sequences of 9 to 192 tokens 100 and 125 us in their order, 75 and 112 longest first; of up to 64 tokens 47 and 44 but 56
-    // and 58, 64 sequences 112 and 122: no order for up to three groups)
+    // (24 and 32 sequences of 9 to 192 tokens 100 and 125 us in their order, 75 and 112 longest first; of up to 64
+    // tokens 47 and 44 but 56 and 58, 64 sequences 112 and 122: no order for up to three groups)
     const int number = int(blockIdx.x / unsigned(a.v_heads)), h = int(blockIdx.x % unsigned(a.v_heads));
     const int s = a.max_new > 3 * kChunk ? by_length(a.b, number) : number;
     const int hk = h / (a.v_heads / a.qk_heads);
@@ -891,7 +911,8 @@ __global__ __launch_bounds__(512, 4) void delta_group_kernel(DeltaArgs a) {
         for (int ti = 0; ti < 2; ++ti)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-                val[ti][r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(v_rows, (unsigned(16 * ti + 4 * g + r) * unsigned(a.v_stride) + unsigned(walks ? col : 0)) * 4u, 0, 0));
+                val[ti][r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
+                    v_rows, (unsigned(16 * ti + 4 * g + r) * unsigned(a.v_stride) + unsigned(walks ? col : 0)) * 4u, 0, 0));
         const Item<DK> it(t % 256, wid / 4);
         if (has_item) row_squares<DK>(it, x, sums);
         if (wid == 7 && lane < 32) head_steps(a, r0 + lane, h, lane, lane < left, G, beta);
@@ -909,7 +930,8 @@ __global__ __launch_bounds__(512, 4) void delta_group_kernel(DeltaArgs a) {
         if (wid < 6) store_tile(wid, lane, tile_of<DK>(wid, lane, rows, rows + 2 * kRows), squares[0], squares[1]);
         __syncthreads();
         const int i = t / 8, c = t % 8 * 4;
-        if (t < 256) store_operand(matrices + 4 * kBlock, i, operand_at(i, c), mask_and_decay(squares[0], squares[1], G, beta, i, c, squares[2]));
+        if (t < 256)
+            store_operand(matrices + 4 * kBlock, i, operand_at(i, c), mask_and_decay(squares[0], squares[1], G, beta, i, c, squares[2]));
         __syncthreads();
         if (wid == 7) {  // (the others have products to make meanwhile)
             if (lane < 32) invert_half(squares[2], lane / 16 * 16, lane % 16, squares[3]);
@@ -1005,8 +1027,8 @@ __global__ __launch_bounds__(512, 4) void delta_group_kernel(DeltaArgs a) {
     }
 }
 
-// The norm and the gate of rows as the walk leaves them, in place: half a wave per row and head. Bound: memory (8192 tokens
-// of 32 heads 77 us, 5.2 TB/s).
+// The norm and the gate of rows as the walk leaves them, in place: half a wave per row and head. Bound: memory (8192
+// tokens of 32 heads 77 us, 5.2 TB/s).
 template <int DV>
 __global__ __launch_bounds__(256) void delta_norm_kernel(DeltaArgs a, int tiles) {
     const int lane = threadIdx.x & 31, h = int(blockIdx.x % unsigned(a.v_heads)), st = int(blockIdx.x / unsigned(a.v_heads));
@@ -1035,11 +1057,12 @@ __global__ __launch_bounds__(256) void delta_norm_kernel(DeltaArgs a, int tiles)
         }
 }
 
-// What a first half left goes to the second half's tokens and last state: O + scale R S and E + M S, with S the state in the middle, R what
-// the tokens read of the unit vectors, O and E what the values gave; 32 rows at a time. Then, and for all other rows, norm and
-// gate. S has a scale for each column, as above, and R and M one for each row, from what it sums to: they fall with the decays of the
-// second half, far below 1, and what is left of the state in the middle is to keep its bits. Bound: memory (8192 tokens of 32 heads
-// 100 us, 4.7 TB/s; with scales summed over waves, through LDS and one more barrier, 117).
+// What a first half left goes to the second half's tokens and last state: O + scale R S and E + M S, with S the state
+// in the middle, R what the tokens read of the unit vectors, O and E what the values gave; 32 rows at a time. Then, and
+// for all other rows, norm and gate. S has a scale for each column, as above, and R and M one for each row, from what
+// it sums to: they fall with the decays of the second half, far below 1, and what is left of the state in the middle is
+// to keep its bits. Bound: memory (8192 tokens of 32 heads 100 us, 4.7 TB/s; with scales summed over waves, through LDS
+// and one more barrier, 117).
 template <int DK, int DV>
 __global__ __launch_bounds__(512, 4) void delta_join_kernel(DeltaArgs a, DeltaScratch w, int tiles) {
     constexpr int NU = DK / 32;
@@ -1074,7 +1097,8 @@ __global__ __launch_bounds__(512, 4) void delta_join_kernel(DeltaArgs a, DeltaSc
         const int r0 = v.r0 + i * kChunk, left = min(v.n - i * kChunk, kChunk);
         float *const out = a.out + size_t(h) * DV;
         if (i < middle) {
-            if (a.gamma || a.z) write_rows<DV>(a, h, r0, left, t, 512, [&](int m, int e) { return load4(out + size_t(r0 + m) * a.out_stride + e); });
+            if (a.gamma || a.z)
+                write_rows<DV>(a, h, r0, left, t, 512, [&](int m, int e) { return load4(out + size_t(r0 + m) * a.out_stride + e); });
             continue;
         }
         const bool state = i >= n_groups;
@@ -1121,7 +1145,9 @@ __global__ __launch_bounds__(512, 4) void delta_join_kernel(DeltaArgs a, DeltaSc
         __syncthreads();
         auto plus = [](float4 x, float4 y) { return make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w); };
         if (!state) {
-            write_rows<DV>(a, h, r0, left, t, 512, [&](int m, int e) { return plus(load4(&sum[m][e]), load4(out + size_t(r0 + m) * a.out_stride + e)); });
+            write_rows<DV>(a, h, r0, left, t, 512, [&](int m, int e) {
+                return plus(load4(&sum[m][e]), load4(out + size_t(r0 + m) * a.out_stride + e));
+            });
         } else if (v.out >= 0) {
             const size_t at = size_t(i - n_groups) * 32 * DV;
             float *to = a.state + (size_t(v.out) * a.v_heads + size_t(h)) * DK * DV + at;
@@ -1134,9 +1160,11 @@ __global__ __launch_bounds__(512, 4) void delta_join_kernel(DeltaArgs a, DeltaSc
 
 template <int DK, int NW, bool HALVES> hipError_t launch_walk(const DeltaArgs &a, const DeltaScratch &w, hipStream_t s) {
     constexpr int kBuffer = ((2 * 2 * (DK / 32) + DK / 16) * 2 + 8) * kBlock + kFactors * 4;
-    const int splits = a.value_dim / (16 * NW), parts = HALVES ? 2 * splits + DK / (16 * NW) : splits, per = a.v_heads / a.qk_heads * parts;
+    const int splits = a.value_dim / (16 * NW), parts = HALVES ? 2 * splits + DK / (16 * NW) : splits;
+    const int per = a.v_heads / a.qk_heads * parts;
     const int units = a.b.n_seqs * a.qk_heads;
-    hipLaunchKernelGGL((delta_walk_kernel<DK, NW, HALVES>), dim3(unsigned((units + 7) / 8) * 8u * unsigned(per)), dim3(512), 2 * kBuffer, s, a, w, splits);
+    const dim3 grid(unsigned((units + 7) / 8) * 8u * unsigned(per));
+    hipLaunchKernelGGL((delta_walk_kernel<DK, NW, HALVES>), grid, dim3(512), 2 * kBuffer, s, a, w, splits);
     return hipGetLastError();
 }
 
@@ -1144,13 +1172,14 @@ template <int DK> hipError_t launch_groups(const DeltaArgs &a, const DeltaScratc
     const int64_t lists = int64_t(a.b.n_seqs) * a.v_heads;
     const int64_t want = (int64_t(a.max_new) + kChunk - 1) / kChunk, most = ((int64_t(1) << 24) - 1) / lists;
     const int tiles = int(want < 1 ? 1 : want < most ? want : most);  // (the others in turns)
-    hipLaunchKernelGGL(delta_prepare_kernel<DK>, dim3(unsigned(a.b.n_seqs) * unsigned(tiles) * unsigned(a.qk_heads)), dim3(256), 0, s, a, w, tiles);
+    const dim3 all_groups(unsigned(a.b.n_seqs) * unsigned(tiles) * unsigned(a.qk_heads));
+    hipLaunchKernelGGL(delta_prepare_kernel<DK>, all_groups, dim3(256), 0, s, a, w, tiles);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    // Where workgroups of 32 columns find a CU each they are a little faster (a prompt of 8192 and 32 heads: 411 us, with 64
-    // columns 423), else those of 64 (six prompts of 4885 tokens in all: 106 us, with 32 columns 144).
-    // Halves where all their workgroups find a CU: a prompt of 32 heads and 640 tokens 50 us, in one 54; of 2048 109 and 141; of
-    // 8192 397 and 559.
+    // Where workgroups of 32 columns find a CU each they are a little faster (a prompt of 8192 and 32 heads: 411 us,
+    // with 64 columns 423), else those of 64 (six prompts of 4885 tokens in all: 106 us, with 32 columns 144). Halves
+    // where all their workgroups find a CU: a prompt of 32 heads and 640 tokens 50 us, in one 54; of 2048 109 and 141;
+    // of 8192 397 and 559.
     if (halves && want >= kHalfGroups && lists <= kHalfLists && lists * ((2 * a.value_dim + DK) / 64) <= cu_count) {
         if ((e = launch_walk<DK, 4, true>(a, w, s)) != hipSuccess) return e;
         // (each workgroup with about four items, for one reading of the state; more than four past 2^31 threads)
@@ -1176,9 +1205,11 @@ hipError_t launch_delta(const DeltaArgs &a, void *scratch, size_t scratch_bytes,
     const size_t widest = max(max(a.q_stride, a.k_stride), max(a.v_stride, a.out_stride));
     const int64_t lists = int64_t(a.b.n_seqs) * a.v_heads;
     const bool grouped = a.max_new > kStepRows && widest < (1 << 24) && lists < (1 << 20);  // (32 rows in 32 bits of bytes; threads)
-    // All in one launch takes about 4 us and 8.4 for each group of the longest sequence; three launches 17 us and the longer of
-    // 1.9 for each of its groups and 0.029 for each group of any head (one launch has 0.025 of that). Measured, one launch
-    // and three: 1 sequence of 64 tokens 20.2, 20.9, of 128 36.3, 24.2; 8 of 64 26.1, 36.2, of 192 60.1, 66.4; 32 of 192 175, 249.
+    // All in one launch takes about 4 us and 8.4 for each group of the longest sequence; three launches 17 us and the
+    // longer of 1.9 for each of its groups and 0.029 for each group of any head (one launch has 0.025 of that).
+    // Measured, one launch and three: 1 sequence of 64 tokens 19.1, 20.4, of 128 36.7, 24.1; 8 of 64 25.2, 37.2, of 192
+    // 64, 69.5; 32 of 192 171, 252. Fitted to heads of 128. Of 64 it is 14.2, 19.0; 26.2, 20.8; 17.2, 23.7; 43.5, 34.6;
+    // 114, 126.
     const double steps = double((int64_t(a.max_new) + kChunk - 1) / kChunk);
     const double all = min(steps * a.b.n_seqs, double(a.b.n_rows / kChunk + a.b.n_seqs)) * a.v_heads;
     if (grouped && 8.4 * steps > 13 + max(1.9 * steps, 0.029 * all) && scratch && scratch_bytes >= delta_group_bytes(a)) {

@@ -70,10 +70,10 @@ constexpr int kFactors = 96;
 inline size_t delta_group_bytes(const DeltaArgs &a) {
     return size_t(delta_groups(a.b.n_rows, a.b.n_seqs)) * (size_t(a.v_heads) * (kDeltaMatrices + kFactors * 4) + size_t(a.qk_heads) * 256) + 256;
 }
-// Where few heads (of all sequences together at most kHalfLists) walk long sequences in halves, it also holds three matrices of each
-// and a row of key_dim values for every token and head of a second half. A workspace serves calls of fewer rows and sequences, too: it
-// has that place (of 32768 rows and 32 heads of 128 as much again as the groups) if one sequence of all rows would use it, and without it
-// the groups are walked in one.
+// Where few heads (of all sequences together at most kHalfLists) walk long sequences in halves, it also holds three
+// matrices of each and a row of key_dim values for every token and head of a second half. A workspace serves calls of
+// fewer rows and sequences, too: it has that place (of 32768 rows and 32 heads of 128 as much again as the groups) if
+// one sequence of all rows would use it, and without it the groups are walked in one.
 constexpr int64_t kHalfLists = 64;
 constexpr int kHalfGroups = 16;  // groups of a sequence from which on halves are faster (32 heads, 512 tokens: 47 us either way)
 inline size_t delta_scratch_bytes(const DeltaArgs &a) {

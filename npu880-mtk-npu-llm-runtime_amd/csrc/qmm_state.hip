@@ -3,11 +3,11 @@
 //
 //   y[t][c] = act(bias[c] + sum_i w[c][i] x[t - W + 1 + i][c]),  act(y) = y / (1 + exp(-y))
 //
-// Bound: memory; every input is read once (and W - 1 of 8 rows again, from the caches)
-// and every output written once. 8192 channels: 16 sequences of a token 4.5 us (one launch), five prompts of 5581 73.5 us, 5.0 TB/s.
-// Inputs of more than 32 MB are loaded past the caches, in which the outputs then lie for what reads them: 6 prompts of 800 tokens
-// with the delta rule behind 237 us, 245 without. Outputs past them too are faster alone (64.5 us) and slower together (241).
-// With 16 rows a workgroup 78.5 us, with 4 80.
+// Bound: memory; every input is read once (and W - 1 of 8 rows again, from the caches) and every output written once.
+// 8192 channels: 16 sequences of a token 4.5 us (one launch), five prompts of 5581 73.5 us, 5.0 TB/s. Inputs of more
+// than 32 MB are loaded past the caches, in which the outputs then lie for what reads them: 6 prompts of 800 tokens
+// with the delta rule behind 237 us, 245 without. Outputs past them too are faster alone (64.5 us) and slower together
+// (241). With 16 rows a workgroup 78.5 us, with 4 80.
 #include <hip/hip_runtime.h>
 
 #include "qmm_lanes.h"
@@ -86,8 +86,8 @@ __global__ __launch_bounds__(256) void conv_kernel(ConvArgs a, int tiles, int ch
     }
 }
 
-// 16 KB of one pair's slot in one pool a workgroup: four 16-B loads of a thread under way. Bound: memory, 6.1 to 6.6 TB/s at
-// 200 MB (stores past the caches: 7 more of 51 us here, but lost again where the copies are read next).
+// 16 KB of one pair's slot in one pool a workgroup: four 16-B loads of a thread under way. Bound: memory, 6.1 to 6.6
+// TB/s at 200 MB (stores past the caches: 7 more of 51 us here, but lost again where the copies are read next).
 constexpr int kCopyChunk = 16384;
 __global__ __launch_bounds__(256) void copy_kernel(CopyArgs a) {
     const auto pool = a.pool[blockIdx.z];
