@@ -508,9 +508,9 @@ int qmm_short_conv(qmm_context *ctx, const qmm_state_batch *batch, const qmm_con
  * than 2^-119). So batches that only decode say max_new = 1 (without, 32 sequences of 32
  * heads take 43 us, with it 23), and a sequence's last bits follow the longest one
  * beside it. A program that wants fp32 throughout says 1 for its prompts, too (417 rows
- * 405 us, in groups 42). Long prompts are faster with a workspace, and go in halves where few heads
- * leave room: then not finer either than 2^-28 of the state in the middle, as far as any
- * part of that is left. */
+ * 405 us, in groups 42). Long prompts are faster with a workspace, and go in halves where
+ * few heads leave room: then not finer either than 2^-28 of the state in the middle, as
+ * far as any part of that is left. */
 typedef struct {
     const float *q, *k;   /* device [n_rows][..]: qk_heads heads of key_dim values */
     size_t q_stride, k_stride;
